@@ -1,0 +1,519 @@
+"""The position rotation of queries and keys, alone and in the pass of their norms, and the operators that serve the layer from
+pages, as timed cases with their plain forms.
+
+A case is a dict of plain values.  ``op`` names the operator:
+
+  rotary    ``rotary``: B, T, H, D, R rotated elements, interleaved or halves, positions from ``first`` on; with ``grad`` forward and backward
+  qk_norm   ``qk_norm_rotary``: the same for queries and keys together, behind their RMS norms; weights per head or shared by the heads
+  slots     ``page_slots`` for ``tokens`` new tokens of B requests, behind ``page_release`` of the finished ones where there are any
+  append    ``paged_append`` of T tokens, some of which have no slot
+  attend    ``paged_forgetting_attention``: one new token for each of B requests that hold between ``shortest`` and ``longest`` tokens
+
+``draw_seed`` fixes what the amount of work depends on (how long each request is); everything else comes from the seed of ``prepare``.
+"""
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+_DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+_EPS = 1e-5
+
+
+def _ft():
+    pkg = str(Path.cwd() / "forgetting-transformer_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    import forgetting_transformer
+    return forgetting_transformer
+
+
+def _rotary(name, B, T, H, D, R, *, dtype="bf16", interleaved=False, head_first=False, first=0, grad=False):
+    return dict(name=name, op="rotary", B=B, T=T, H=H, D=D, R=R, dtype=dtype, interleaved=interleaved, head_first=head_first, first=first, grad=grad)
+
+
+def _qk_norm(name, B, T, H, D, R, *, dtype="bf16", interleaved=False, head_first=False, first=0, grad=False, shared=False):
+    return dict(_rotary(name, B, T, H, D, R, dtype=dtype, interleaved=interleaved, head_first=head_first, first=first, grad=grad), op="qk_norm",
+                shared=shared)
+
+
+def _slots(name, B, tokens, longest, page, *, finished=False, draw_seed=0):
+    return dict(name=name, op="slots", B=B, tokens=tokens, longest=longest, page=page, finished=finished, draw_seed=draw_seed)
+
+
+def _append(name, T, H, D, page, *, dtype="bf16", skipped=0):
+    return dict(name=name, op="append", T=T, H=H, D=D, page=page, dtype=dtype, skipped=skipped)
+
+
+def _attend(name, B, H, D, page, shortest, longest, *, dtype="bf16", draw_seed=0):
+    return dict(name=name, op="attend", B=B, H=H, D=D, page=page, shortest=shortest, longest=longest, dtype=dtype, draw_seed=draw_seed)
+
+
+def listed():
+    return [
+        # queries or keys of one training step, whole heads rotated
+        _rotary("rotate_step", 2, 2048, 12, 64, 64, grad=True),
+        # a ragged fp16 batch far into a long context, a quarter of each head rotated, neighbouring pairs, head-first views
+        _rotary("rotate_part_far", 3, 777, 5, 128, 32, dtype="fp16", interleaved=True, head_first=True, first=100000),
+        # one new token for each of sixteen sequences that are generated together: the smallest call
+        _qk_norm("norm_rotate_tokens", 16, 1, 16, 128, 128, first=1500),
+        # a training step of the layer at head dim 64
+        _qk_norm("norm_rotate_step", 2, 2048, 12, 64, 64, grad=True),
+        # long-context training, one row of weights for all heads: the largest tensors the layer takes
+        _qk_norm("norm_rotate_long", 4, 16384, 16, 128, 128, grad=True, shared=True),
+        # every one of 256 requests brings its next token
+        _slots("slots_tokens", 256, 256, 8192, 16, draw_seed=1),
+        # some requests have finished and give their pages back, others bring prompts
+        _slots("slots_prompts", 64, 16384, 16384, 64, finished=True, draw_seed=2),
+        # the next tokens of 48 requests into the pages of one layer
+        _append("append_tokens", 48, 12, 64, 16, dtype="fp16"),
+        # prompts into the pages of one layer, some tokens refused
+        _append("append_prompts", 16384, 16, 128, 64, skipped=100),
+        # a single user generates from a short cache
+        _attend("paged_single", 1, 12, 64, 16, 1500, 1500),
+        # 48 requests of very different lengths, some of them idle
+        _attend("paged_ragged", 48, 12, 64, 16, 0, 8192, dtype="fp16", draw_seed=3),
+        # a large batch generates from long caches
+        _attend("paged_long", 16, 16, 128, 64, 24576, 32768, draw_seed=4),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+_MAX_STEP = 4 * 16384 * 16 * 128       # elements of a tensor of norm_rotate_long
+_MAX_CACHE = 16 * 16 * 32768 * 128     # elements of the keys of paged_long
+_HEADS = [1, 2, 3, 5, 8, 12, 12, 16, 16, 32]
+
+
+def draw(rng):
+    op = rng.choice(["rotary", "qk_norm", "qk_norm", "slots", "append", "attend", "attend"])
+    D = rng.choice([16, 32, 64, 64, 128, 128])
+    H, dtype = rng.choice(_HEADS), rng.choice(["bf16", "bf16", "fp16"])
+    page, draw_seed = rng.choice([16, 16, 32, 64, 128]), rng.randrange(1 << 20)
+    if op in ("rotary", "qk_norm"):
+        interleaved = rng.random() < 0.4
+        R = rng.choice([D, D, max(16, D // 2), max(16, D // 4)])
+        if interleaved and rng.random() < 0.3:
+            R = rng.randrange(2, D + 1, 2)
+        B, T = _log_int(rng, 1, 64), 1 if rng.random() < 0.25 else _log_int(rng, 2, 16384)
+        while B > 1 and B * T * H * D > _MAX_STEP:
+            B -= 1
+        args = dict(dtype=dtype, interleaved=interleaved, head_first=rng.random() < 0.4, first=rng.choice([0, 0, _log_int(rng, 1, 1000000)]),
+                    grad=T > 1 and rng.random() < 0.6)
+        case = _rotary("", B, T, H, D, R, **args) if op == "rotary" else _qk_norm("", B, T, H, D, R, shared=rng.random() < 0.4, **args)
+    elif op == "slots":
+        B = _log_int(rng, 1, 512)
+        tokens = B if rng.random() < 0.5 else _log_int(rng, max(B, 16), 16384)
+        case = _slots("", B, tokens, _log_int(rng, 64, 16384), page, finished=rng.random() < 0.5, draw_seed=draw_seed)
+    elif op == "append":
+        T = _log_int(rng, 1, 16384)
+        while T * H * D > 16384 * 16 * 128:
+            T = T // 2 + 1
+        case = _append("", T, H, D, page, dtype=dtype, skipped=rng.choice([0, 0, T // 5]))
+    else:
+        longest = _log_int(rng, 16, 32768)
+        shortest = rng.choice([0, 1, longest // 2, longest])
+        B = _log_int(rng, 1, 64)
+        while B > 1 and B * H * longest * D > _MAX_CACHE:
+            B -= 1
+        case = _attend("", B, H, D, page, min(shortest, longest), longest, dtype=dtype, draw_seed=draw_seed)
+    del case["name"]
+    return case
+
+
+def _request_lengths(case):
+    """Cached tokens of each request: spread over the logarithm from the shortest to the longest."""
+    rng = random.Random(case["draw_seed"])
+    lo, hi = case["shortest"], case["longest"]
+    n = [min(hi, max(lo, _log_int(rng, max(lo, 1), hi) if lo or rng.random() > 0.1 else 0)) for _ in range(case["B"])]
+    n[rng.randrange(case["B"])] = hi
+    return n
+
+
+def _new_tokens(case):
+    """New tokens of each request and which requests have finished; a finished one brings none."""
+    rng = random.Random(case["draw_seed"])
+    B = case["B"]
+    done = [case["finished"] and rng.random() < 0.25 for _ in range(B)]
+    done[rng.randrange(B)] = False
+    live = [b for b in range(B) if not done[b]]
+    if case["tokens"] == B:                       # generation: one each (a finished one's goes to another)
+        n = [0 if d else 1 for d in done]
+        n[live[0]] += B - len(live)
+    else:                                         # prompts: uneven shares of the tokens
+        share = [0.0 if d else rng.random() ** 3 + 1e-3 for d in done]
+        n = [int(case["tokens"] * s / sum(share)) for s in share]
+        n[live[0]] += case["tokens"] - sum(n)
+    return n, done
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    op = case["op"]
+    st = dict(case=case)
+
+    def rnd(*shape, dtype=torch.float32):
+        return torch.randn(*shape, generator=gen, device=dev, dtype=dtype)
+
+    def ints(values):
+        return torch.tensor(values, dtype=torch.int32, device=dev)
+
+    def perm(n):
+        return torch.randperm(n, generator=gen, device=dev)
+
+    if op in ("rotary", "qk_norm"):
+        B, T, H, D, R = (case[n] for n in "BTHDR")
+        dt = _DTYPES[case["dtype"]]
+        shape = (B, H, T, D) if case["head_first"] else (B, T, H, D)
+        st["inv_freq"] = 10000.0 ** (-torch.arange(0, R, 2, dtype=torch.float64, device=dev) / R)
+        # a row's tokens follow each other from a position of its own
+        start = case["first"] + torch.randint(0, 64, (B, 1), generator=gen, device=dev)
+        st["positions"] = start + torch.arange(T, device=dev)
+        names = ["x"] if op == "rotary" else ["q", "k"]
+        for n in names:
+            st[n] = rnd(*shape, dtype=dt)
+        if op == "qk_norm":
+            for n in ("q_weight", "k_weight"):
+                st[n] = torch.rand(D if case["shared"] else H * D, generator=gen, device=dev) + 0.5
+            names += ["q_weight", "k_weight"]
+        if case["grad"]:
+            for n in names:
+                st[n].requires_grad_()
+            st["leaves"] = [st[n] for n in names]
+            st["douts"] = [rnd(*shape, dtype=dt) for _ in range(1 if op == "rotary" else 2)]
+    elif op == "slots":
+        B, S = case["B"], case["page"]
+        new, done = _new_tokens(case)
+        width = (case["longest"] + max(new) + S - 1) // S
+        held = torch.randint(1, case["longest"] + 1, (B,), generator=gen, device=dev, dtype=torch.int32)
+        used = (held + S - 1) // S
+        pool = B * width + B
+        pages = perm(pool).to(torch.int32)
+        table = pages[:B * width].reshape(B, width).clone()
+        free = torch.zeros(pool, dtype=torch.int32, device=dev)
+        unused = (torch.arange(width, device=dev)[None] >= used[:, None]).reshape(-1)
+        order = torch.argsort((~unused).to(torch.int32), stable=True)     # pages that no request holds first
+        free[:B * width] = pages[:B * width][order]
+        st.update(lengths=held, new=ints(new), block_table=torch.where(unused.reshape(B, width), -1, table), free_pages=free,
+                  free_count=unused.sum(dtype=torch.int32).reshape(1))
+        if case["finished"]:
+            st["done"] = torch.tensor(done, device=dev)
+    elif op == "append":
+        T, H, D, S = case["T"], case["H"], case["D"], case["page"]
+        dt = _DTYPES[case["dtype"]]
+        pool = (T + S - 1) // S + 8
+        st.update(k=rnd(T, H, D, dtype=dt), v=rnd(T, H, D, dtype=dt), log_fgate=torch.nn.functional.logsigmoid(rnd(T, H) + 2.0),
+                  k_pages=rnd(pool, H, S, D, dtype=dt), v_pages=rnd(pool, H, S, D, dtype=dt), log_fgate_pages=-rnd(pool, H, S).abs())
+        # pages in any order, the rows of a page one after the other
+        slots = (perm(pool)[:, None] * S + torch.arange(S, device=dev)).reshape(-1)[:T].clone()
+        if case["skipped"]:
+            slots[perm(T)[:case["skipped"]]] = -1
+        st["slots"] = slots
+    else:
+        B, H, D, S = case["B"], case["H"], case["D"], case["page"]
+        dt = _DTYPES[case["dtype"]]
+        lens = _request_lengths(case)
+        width = (max(lens) + S - 1) // S + 1
+        counts = [(n + S - 1) // S for n in lens]
+        pool = sum(counts) + 3
+        ids = perm(pool).to(torch.int32)
+        table = torch.zeros(B, width, dtype=torch.int32, device=dev)
+        at = 0
+        for b, c in enumerate(counts):
+            table[b, :c] = ids[at:at + c]
+            at += c
+        st.update(q=rnd(B, H, D, dtype=dt), k_pages=rnd(pool, H, S, D, dtype=dt), v_pages=rnd(pool, H, S, D, dtype=dt),
+                  log_fgate_pages=torch.nn.functional.logsigmoid(rnd(pool, H, S) + 3.0), block_table=table, lengths=ints(lens))
+    return st
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the operators through the framework, and in their plain form
+# ---------------------------------------------------------------------------------------------------------------
+def run(st):
+    op = st["case"]["op"]
+    if own:
+        return {"rotary": _own_rotary, "qk_norm": _own_qk_norm, "slots": _own_slots, "append": _own_append, "attend": _own_attend}[op](st)
+    with torch.no_grad():
+        return {"rotary": _plain_rotary, "qk_norm": _plain_qk_norm, "slots": _plain_slots, "append": _plain_append, "attend": _plain_attend}[op](st)
+
+
+def _own_rotary(st):
+    c = st["case"]
+    y = _ft().rotary(st["x"], st["inv_freq"], positions=st["positions"], interleaved=c["interleaved"], head_first=c["head_first"])
+    return [y.detach(), *torch.autograd.grad([y], st["leaves"], st["douts"])] if c["grad"] else [y]
+
+
+def _own_qk_norm(st):
+    c = st["case"]
+    q, k = _ft().qk_norm_rotary(st["q"], st["k"], st["q_weight"], st["k_weight"], st["inv_freq"], positions=st["positions"],
+                                interleaved=c["interleaved"], eps=_EPS, head_first=c["head_first"])
+    return [q.detach(), k.detach(), *torch.autograd.grad([q, k], st["leaves"], st["douts"])] if c["grad"] else [q, k]
+
+
+def _own_slots(st):
+    ft, S = _ft(), st["case"]["page"]
+    lengths, free_count = st["lengths"], st["free_count"]
+    if "done" in st:
+        lengths, free_count = ft.page_release(lengths, st["done"], st["block_table"], st["free_pages"], free_count, page_size=S)
+    s = ft.page_slots(lengths, st["new"], st["block_table"], st["free_pages"], free_count, page_size=S, max_tokens=st["case"]["tokens"])
+    return [s.slots, s.positions, s.requests, s.lengths, s.free_count, s.granted, st["block_table"]]
+
+
+def _own_append(st):
+    _ft().paged_append(st["k"], st["v"], st["log_fgate"], st["k_pages"], st["v_pages"], st["log_fgate_pages"], st["slots"])
+    return [st["k_pages"], st["v_pages"], st["log_fgate_pages"]]
+
+
+def _own_attend(st):
+    return [_ft().paged_forgetting_attention(st["q"], st["k_pages"], st["v_pages"], st["log_fgate_pages"], st["block_table"], st["lengths"])]
+
+
+def _angles(st):
+    """cos and sin of the tokens' angles, 32 bits from 64-bit angles, broadcast over the heads."""
+    c = st["case"]
+    a = st["positions"].double()[..., None] * st["inv_freq"]            # (B, T, R/2)
+    a = a[:, None] if c["head_first"] else a[:, :, None]
+    return a.cos().float(), a.sin().float()
+
+
+def _turn(x, cos, sin, R, interleaved):
+    """The first R elements of the last axis turned by the angles, the others as they are (32 bits)."""
+    y = x.clone()
+    a, b = (x[..., 0:R:2], x[..., 1:R:2]) if interleaved else (x[..., :R // 2], x[..., R // 2:R])
+    ya, yb = a * cos - b * sin, a * sin + b * cos
+    if interleaved:
+        y[..., 0:R:2], y[..., 1:R:2] = ya, yb
+    else:
+        y[..., :R // 2], y[..., R // 2:R] = ya, yb
+    return y
+
+
+def _plain_rotary(st):
+    c = st["case"]
+    cos, sin = _angles(st)
+    out = [_turn(st["x"].float(), cos, sin, c["R"], c["interleaved"]).to(st["x"].dtype)]
+    if c["grad"]:
+        out.append(_turn(st["douts"][0].float(), cos, -sin, c["R"], c["interleaved"]).to(st["x"].dtype))
+    return out
+
+
+def _plain_qk_norm(st):
+    c = st["case"]
+    H, D = c["H"], c["D"]
+    cos, sin = _angles(st)
+    outs, dxs, dws = [], [], []
+    for i, n in enumerate("qk"):
+        x, w = st[n].float(), st[n + "_weight"]
+        rows = w.expand(H, D) if c["shared"] else w.reshape(H, D)
+        w4 = rows[:, None] if c["head_first"] else rows                   # against (..., H, T, D) or (..., T, H, D)
+        rstd = torch.rsqrt((x * x).mean(-1, keepdim=True) + _EPS)
+        xhat = x * rstd
+        outs.append(_turn(xhat * w4, cos, sin, c["R"], c["interleaved"]).to(st[n].dtype))
+        if c["grad"]:
+            dn = _turn(st["douts"][i].float(), cos, -sin, c["R"], c["interleaved"])
+            dw = (dn * xhat).sum((0, 2) if c["head_first"] else (0, 1), dtype=torch.float64)
+            dws.append((dw.sum(0) if c["shared"] else dw.reshape(-1)).float())
+            dn = dn * w4
+            dxs.append((rstd * (dn - xhat * (dn * xhat).mean(-1, keepdim=True))).to(st[n].dtype))
+    return outs + dxs + dws
+
+
+def _plain_slots(st):
+    S, T = st["case"]["page"], st["case"]["tokens"]
+    lengths, new, table, free = st["lengths"].long(), st["new"].long(), st["block_table"], st["free_pages"]
+    count, width = st["free_count"].long(), table.shape[1]
+    cols = torch.arange(width, device=table.device)
+    if "done" in st:
+        back = torch.where(st["done"], (lengths + S - 1) // S, 0)
+        at = count + back.cumsum(0) - back
+        dest = torch.where(cols < back[:, None], at[:, None] + cols, free.numel())
+        padded = torch.cat([free, free.new_zeros(1)])
+        padded[dest.reshape(-1)] = table.reshape(-1)
+        free.copy_(padded[:-1])
+        count = count + back.sum()
+        lengths = torch.where(st["done"], 0, lengths)
+    end = new.cumsum(0)
+    held = (lengths + S - 1) // S
+    need = (lengths + new + S - 1) // S - held
+    fits = (held + need <= width) & (end <= T)
+    taken = torch.where(fits, need, 0).cumsum(0)
+    ok = fits & ((need == 0) | (taken <= count))
+    first = count - 1 - (taken - need)                                    # place of a request's first new page in the stack
+    fresh = free[(first[:, None] - (cols - held[:, None])).clamp(0, free.numel() - 1)]
+    takes = ok[:, None] & (cols >= held[:, None]) & (cols < (held + need)[:, None])
+    table.copy_(torch.where(takes, fresh, table))
+    t = torch.arange(T, device=table.device)
+    b = torch.searchsorted(end, t, right=True).clamp(max=len(new) - 1)
+    real = t < end[-1]
+    pos = lengths[b] + t - (end - new)[b]
+    page = table[b, (pos // S).clamp(0, width - 1)].long()
+    granted = real & ok[b]
+    return [torch.where(granted, page * S + pos % S, -1), torch.where(real, pos, 0), torch.where(granted, b, -1).int(),
+            torch.where(ok, lengths + new, lengths).int(), (count - torch.where(ok & (need > 0), taken, 0).max()).int(), ok, table]
+
+
+def _plain_append(st):
+    S = st["case"]["page"]
+    keep = st["slots"] >= 0
+    at = st["slots"].clamp(min=0)
+    for n, pages in (("k", "k_pages"), ("v", "v_pages"), ("log_fgate", "log_fgate_pages")):
+        p = st[pages]
+        flat = torch.cat([p.transpose(1, 2).reshape(-1, *p.shape[1:2], *p.shape[3:]), st[n][:1]])   # a spare row takes what has no slot
+        flat[torch.where(keep, at, len(flat) - 1)] = st[n]
+        p.copy_(flat[:-1].reshape(p.shape[0], S, *flat.shape[1:]).transpose(1, 2))
+    return [st["k_pages"], st["v_pages"], st["log_fgate_pages"]]
+
+
+def _plain_attend(st):
+    B, H, D, S = (st["case"][n] for n in ("B", "H", "D", "page"))
+    table, lengths = st["block_table"].long(), st["lengths"].long()
+    N = table.shape[1] * S
+    valid = (torch.arange(N, device=table.device) < lengths[:, None])[:, None]                    # (B, 1, N)
+    gates = st["log_fgate_pages"][table].transpose(1, 2).reshape(B, H, N).double() * valid
+    behind = (gates.flip(-1).cumsum(-1).flip(-1) - gates).float()                                 # of the keys behind each key
+    k = st["k_pages"][table].transpose(1, 2).reshape(B, H, N, D).float()
+    s = (k * st["q"].float()[:, :, None]).sum(-1) / math.sqrt(D) + behind
+    del k
+    s = s.masked_fill(~valid, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    p = (s - torch.where(top == -math.inf, 0.0, top)).exp()
+    total = p.sum(-1, keepdim=True)
+    v = st["v_pages"][table].transpose(1, 2).reshape(B, H, N, D).float()
+    return [((v * p[..., None]).sum(-2) / torch.where(total == 0, 1.0, total)).to(st["q"].dtype)]
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the definitions in 64 bits
+# ---------------------------------------------------------------------------------------------------------------
+def exact(case, seed):
+    st = prepare(case, seed)
+    return {"rotary": _exact_heads, "qk_norm": _exact_heads, "slots": _exact_slots, "append": _exact_append, "attend": _exact_attend}[case["op"]](st)
+
+
+def _exact_heads(st):
+    """Each pair a complex number times e^(i theta); gradients by 64-bit automatic differentiation, batch row by batch row."""
+    c = st["case"]
+    B, H, D, R = (c[n] for n in "BHDR")
+    names = ["x"] if c["op"] == "rotary" else ["q", "k"]
+    outs, dxs, dws = [], [], []
+    for i, n in enumerate(names):
+        w = st[n + "_weight"].detach().double().requires_grad_() if c["op"] == "qk_norm" else None
+        ys, gs, dw = [], [], 0
+        for b in range(B):
+            x = st[n].detach()[b].double().requires_grad_()
+            y = x.transpose(0, 1) if c["head_first"] else x               # (T, H, D)
+            if w is not None:
+                y = y / (y.square().mean(-1, keepdim=True) + _EPS).sqrt() * (w if c["shared"] else w.view(H, D))
+            z = y[..., :R].unflatten(-1, (R // 2, 2)) if c["interleaved"] else y[..., :R].unflatten(-1, (2, R // 2)).transpose(-1, -2)
+            theta = torch.outer(st["positions"][b].double(), st["inv_freq"])
+            turned = torch.view_as_real(torch.view_as_complex(z.contiguous()) * torch.polar(torch.ones_like(theta), theta)[:, None])
+            turned = turned.flatten(-2) if c["interleaved"] else turned.transpose(-1, -2).flatten(-2)
+            y = torch.cat([turned, y[..., R:]], -1)
+            y = y.transpose(0, 1) if c["head_first"] else y
+            ys.append(y.detach())
+            if c["grad"]:
+                g = torch.autograd.grad(y, [x] if w is None else [x, w], st["douts"][i][b].double())
+                gs.append(g[0])
+                if w is not None:
+                    dw = dw + g[1]
+        outs.append(torch.stack(ys))
+        if c["grad"]:
+            dxs.append(torch.stack(gs))
+            if w is not None:
+                dws.append(dw)
+    return outs + dxs + dws
+
+
+def _exact_slots(st):
+    """The same bookkeeping request by request, with lists."""
+    S, T = st["case"]["page"], st["case"]["tokens"]
+    lengths, new, table = (st[n].tolist() for n in ("lengths", "new", "block_table"))
+    stack, pool = st["free_pages"].tolist()[:int(st["free_count"])], st["free_pages"].numel()
+    if "done" in st:
+        for b, d in enumerate(st["done"].tolist()):
+            if d:
+                stack += table[b][:-(-lengths[b] // S)]
+                lengths[b] = 0
+    assert len(stack) <= pool
+    slots, positions, requests, granted = [], [], [], []
+    full = False
+    for b, n in enumerate(new):
+        want = -(-(lengths[b] + n) // S) - -(-lengths[b] // S)
+        ok = len(positions) + n <= T and -(-(lengths[b] + n) // S) <= len(table[b])
+        if ok and want:
+            full = full or want > len(stack)
+            ok = not full
+        if ok:
+            old = -(-lengths[b] // S)
+            for j in range(want):
+                table[b][old + j] = stack.pop()
+        for i in range(min(n, T - len(positions))):
+            at = lengths[b] + i
+            slots.append(table[b][at // S] * S + at % S if ok else -1)
+            positions.append(at)
+            requests.append(b if ok else -1)
+        lengths[b] += n if ok else 0
+        granted.append(ok)
+    rest = T - len(slots)
+    dev = st["lengths"].device
+    return [torch.tensor(v, device=dev) for v in (slots + [-1] * rest, positions + [0] * rest, requests + [-1] * rest, lengths, [len(stack)],
+                                                  granted, table)]
+
+
+def _exact_append(st):
+    """What each slot of the pool holds afterwards: the token that names it, or what it held."""
+    S = st["case"]["page"]
+    out = []
+    P = st["k_pages"].shape[0]
+    token = torch.full((P * S,), -1, device=st["slots"].device)
+    has = st["slots"] >= 0
+    token[st["slots"][has]] = torch.arange(len(has), device=has.device)[has]
+    token = token.view(P, 1, S)
+    for n, pages in (("k", "k_pages"), ("v", "v_pages"), ("log_fgate", "log_fgate_pages")):
+        held, new = st[pages].double(), st[n].double()
+        rows = new[token.clamp(min=0)[:, 0]].transpose(1, 2)              # (P, H, S[, D])
+        out.append(torch.where((token < 0)[..., None] if held.dim() == 4 else token < 0, held, rows))
+    return out
+
+
+def _exact_attend(st):
+    """Request by request over the keys that it holds."""
+    D, S = st["case"]["D"], st["case"]["page"]
+    out = torch.zeros_like(st["q"], dtype=torch.float64)
+    for b, n in enumerate(st["lengths"].tolist()):
+        if n == 0:
+            continue
+        ids = st["block_table"][b, :(n + S - 1) // S].long()
+        k, v, g = (st[p][ids].double().transpose(0, 1).flatten(1, 2)[:, :n] for p in ("k_pages", "v_pages", "log_fgate_pages"))
+        c = g.cumsum(-1)
+        s = torch.matmul(k, st["q"][b].double()[:, :, None])[..., 0] * D ** -0.5 + (c[:, -1:] - c)
+        out[b] = torch.matmul(torch.softmax(s, -1)[:, None], v)[:, 0]
+    return [out]
+
+
+def work(case):
+    op = case["op"]
+    if op in ("rotary", "qk_norm"):
+        B, T, H, D, R = (case[n] for n in "BTHDR")
+        n = B * T * H * D * (1 if op == "rotary" else 2)
+        passes = 2 + (2 if op == "rotary" else 3) * case["grad"]          # x in, y out; dy (and x) in, dx out
+        norm = 0 if op == "rotary" else 4 + 10 * case["grad"]             # a multiplication or addition per element each
+        return {"bytes": 2 * n * passes + 8 * B * T, "flops": n * norm + 3 * n * R // D * (2 if case["grad"] else 1)}
+    if op == "slots":
+        B, S = case["B"], case["page"]
+        pages = B * (case["longest"] // 2) // S // 4 if case["finished"] else 0
+        return {"bytes": 20 * case["tokens"] + 13 * B + 8 * (case["tokens"] // S) + 8 * pages, "flops": 4 * case["tokens"]}
+    if op == "append":
+        T, H, D = case["T"] - case["skipped"], case["H"], case["D"]
+        return {"bytes": 2 * T * H * (4 * D + 4) + 8 * case["T"], "flops": 0}
+    B, H, D, S = (case[n] for n in ("B", "H", "D", "page"))
+    keys = sum(_request_lengths(case))
+    return {"bytes": keys * H * (4 * D + 4) + 4 * B * H * D + 4 * (keys // S), "flops": 4 * keys * H * D}
