@@ -240,6 +240,88 @@ int make_norm_gate(const fox_norm_gate_args* a, fox::NormGateK& k, bool bwd) {
   return FOX_OK;
 }
 
+int check_head_dim(int D) {
+  if (D != 16 && D != 32 && D != 64 && D != 128) return fail(FOX_E_ARG, "head dim must be one of 16, 32, 64, 128 (got %d)", D);
+  return FOX_OK;
+}
+int check_dtype16(int dtype) {
+  if (dtype != FOX_DTYPE_BF16 && dtype != FOX_DTYPE_FP16) return fail(FOX_E_ARG, "dtype must be FOX_DTYPE_BF16 or FOX_DTYPE_FP16 (got %d)", dtype);
+  return FOX_OK;
+}
+
+int make_rotary(const fox_rotary_args* a, fox::RotaryK& k, bool bwd) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  if (a->sides != 1 && a->sides != 2) return fail(FOX_E_ARG, "sides must be 1 or 2 (got %d)", a->sides);
+  FOX_TRY(check_head_dim(a->D));
+  FOX_TRY(check_dtype16(a->dtype));
+  if (a->B <= 0 || a->T <= 0 || (int64_t)a->B * a->T > 0x7fffffffLL) return fail(FOX_E_ARG, "B and T must be positive and B * T below 2^31 (got %d, %d)", a->B, a->T);
+  const int step = a->interleaved ? 2 : 16;
+  if (a->rotary_dim <= 0 || a->rotary_dim > a->D || a->rotary_dim % step)
+    return fail(FOX_E_ARG, "rotary_dim must be a multiple of %d up to the head dim (got %d)", step, a->rotary_dim);
+  if (!a->inv_freq) return fail(FOX_E_ARG, "inv_freq must not be NULL");
+  const bool norm = a->side[0].weight != nullptr;
+  if (norm && a->weight_stride_h != 0 && a->weight_stride_h != a->D) return fail(FOX_E_ARG, "weight_stride_h must be 0 or the head dim");
+  k = fox::RotaryK{};
+  int64_t heads = 0;
+  for (int i = 0; i < a->sides; ++i) {
+    const fox_rotary_side& s = a->side[i];
+    if (s.H <= 0 || s.H > 65535) return fail(FOX_E_ARG, "the heads must be positive and at most 65535 (got %d)", s.H);
+    if ((s.weight != nullptr) != norm) return fail(FOX_E_ARG, "weights must be given for both sides or for neither");
+    if (!bwd || norm) FOX_TRY(check_view(&s.x, "x"));
+    FOX_TRY(check_view(&s.y, "y"));
+    if (bwd) FOX_TRY(check_view(&s.dx, "dx"));
+    if (norm && ((uintptr_t)s.weight & 15)) return fail(FOX_E_ALIGN, "weight must be 16-byte aligned");
+    k.side[i].H = s.H;
+    k.side[i].w = s.weight;
+    if (bwd && norm) k.side[i].x = to_view(s.x);
+    k.side[i].in = to_view(bwd ? s.y : s.x);
+    k.side[i].out = to_view(bwd ? s.dx : s.y);
+    heads += s.H;
+  }
+  if (bwd && norm) {
+    if (!a->dweight || !a->workspace) return fail(FOX_E_ARG, "dweight and workspace must not be NULL");
+    if ((uintptr_t)a->workspace & 15) return fail(FOX_E_ALIGN, "workspace must be 16-byte aligned");
+  }
+  k.inv_freq = a->inv_freq;
+  k.positions = a->positions;
+  k.p_sb = a->position_stride_b; k.p_st = a->position_stride_t; k.first = a->first_position;
+  k.w_sh = a->weight_stride_h;
+  k.dw = a->dweight; k.dw_partial = a->workspace;
+  k.N = a->B * a->T; k.T = a->T; k.R = a->rotary_dim;
+  k.sign = bwd ? -1 : 1;
+  k.eps = a->eps;
+  return FOX_OK;
+}
+
+// log2 of a page's tokens
+int page_shift(int page_size, int* shift) {
+  if (page_size < 8 || page_size > 4096 || (page_size & (page_size - 1))) return fail(FOX_E_ARG, "page_size must be a power of two from 8 to 4096 (got %d)", page_size);
+  *shift = __builtin_ctz((unsigned)page_size);
+  return FOX_OK;
+}
+int make_pages(const fox_pages& p, fox::PagesK& k) {
+  FOX_TRY(check_head_dim(p.D));
+  FOX_TRY(check_dtype16(p.dtype));
+  if (p.P <= 0 || p.H <= 0) return fail(FOX_E_ARG, "pages and heads must be positive (got %d, %d)", p.P, p.H);
+  FOX_TRY(page_shift(p.page_size, &k.shift));
+  FOX_TRY(check_view(&p.k, "k pages"));
+  FOX_TRY(check_view(&p.v, "v pages"));
+  if (!p.g) return fail(FOX_E_ARG, "the pages of the log gates must not be NULL");
+  k.k = to_view(p.k); k.v = to_view(p.v);
+  k.g = p.g; k.g_sp = p.g_stride_p; k.g_sh = p.g_stride_h; k.g_ss = p.g_stride_t;
+  k.P = p.P;
+  return FOX_OK;
+}
+int check_table(int B, int W, int P) {
+  if (B <= 0 || W <= 0 || P <= 0) return fail(FOX_E_ARG, "requests, pages of a request and pages of the pool must be positive (got %d, %d, %d)", B, W, P);
+  if (B > fox::kPageRequests) return fail(FOX_E_ARG, "at most %d requests (got %d)", fox::kPageRequests, B);
+  return FOX_OK;
+}
+int check_room(int W, int page_size) {
+  if ((int64_t)W * page_size > (1 << 30)) return fail(FOX_E_ARG, "a request's pages must hold at most 2^30 tokens (got %d pages of %d)", W, page_size);
+  return FOX_OK;
+}
+
 // What the forward does with a shape: the key splits its size asks for (only with scratch to hold their partial results), and whether
 // it runs as the paired kernel, which takes the place of the splits.
 struct FwdPlan {
@@ -384,8 +466,8 @@ extern "C" {
 // 0.2.x: fox_bwd_args and the scan entry points differ from 0.1.0; 0.2.1 adds fox_set_stream_min_kv_bytes and fox_probe_mfma, 0.2.2
 // fox_attn_decode, fox_cache_append, fox_qk_norm_threshold and fox_attn_fwd_plan, 0.2.3 fox_attn_fwd_gates, fox_attn_fwd_takes_gates,
 // fox_auto_threshold_scan, fox_attn_decode_counted and fox_attn_bwd_logits, 0.2.4 fox_attn_bwd_one_launch,
-// fox_auto_threshold_scan_one_launch and fox_attn_decode_counters
-int fox_version(void) { return 204; }
+// fox_auto_threshold_scan_one_launch and fox_attn_decode_counters, 0.2.5 the rotation (fox_rotary_*) and the pages (fox_page_*, fox_paged_*)
+int fox_version(void) { return 205; }
 
 const char* fox_last_error(void) { return g_err; }
 
@@ -452,6 +534,121 @@ int fox_norm_gate_workspace_bytes(int64_t rows, int32_t G, int32_t D, int64_t* b
   if (rows <= 0 || G <= 0 || (D != 16 && D != 32 && D != 64 && D != 128)) return fail(FOX_E_ARG, "rows and G must be positive and D one of 16, 32, 64, 128");
   *bytes = fox::norm_gate_workspace_rows(rows) * G * D * (int64_t)sizeof(float);
   return FOX_OK;
+}
+
+int fox_rotary_fwd(const fox_rotary_args* args, void* stream) {
+  fox::RotaryK k;
+  FOX_TRY(make_rotary(args, k, false));
+  return check_hip(fox::launch_rotary(k, args->D, args->dtype, k.side[0].w != nullptr, args->interleaved != 0, false, (hipStream_t)stream), "fox_rotary_fwd");
+}
+
+int fox_rotary_bwd(const fox_rotary_args* args, void* stream) {
+  fox::RotaryK k;
+  FOX_TRY(make_rotary(args, k, true));
+  const bool norm = k.side[0].w != nullptr;   // without one the gradient is the rotation the other way
+  return check_hip(fox::launch_rotary(k, args->D, args->dtype, norm, args->interleaved != 0, norm, (hipStream_t)stream), "fox_rotary_bwd");
+}
+
+int fox_rotary_workspace_bytes(int64_t tokens, int32_t heads, int32_t D, int32_t shared_weight, int64_t* bytes) {
+  if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
+  FOX_TRY(check_head_dim(D));
+  if (tokens <= 0 || tokens > 0x7fffffffLL || heads <= 0 || heads > 2 * 65535) return fail(FOX_E_ARG, "tokens and heads must be positive");
+  *bytes = fox::rotary_workspace_floats(tokens, heads, D, shared_weight != 0) * (int64_t)sizeof(float);
+  return FOX_OK;
+}
+
+int fox_page_slots(const fox_page_slots_args* a, void* stream) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  FOX_TRY(check_table(a->B, a->W, a->P));
+  fox::PageSlotsK k{};
+  FOX_TRY(page_shift(a->page_size, &k.shift));
+  FOX_TRY(check_room(a->W, a->page_size));
+  if (a->max_tokens < 0) return fail(FOX_E_ARG, "max_tokens must not be negative");
+  if (!a->lengths || !a->new_tokens || !a->block_table || !a->free_pages || !a->free_count || !a->lengths_out || !a->free_count_out || !a->granted ||
+      (a->max_tokens > 0 && (!a->slots || !a->positions || !a->requests || !a->keys)))
+    return fail(FOX_E_ARG, "fox_page_slots: no pointer may be NULL");
+  if ((a->lengths_out == a->lengths) != (a->free_count_out == a->free_count))
+    return fail(FOX_E_ARG, "lengths_out and free_count_out must both be in place or neither");
+  k.lengths = a->lengths; k.new_tokens = a->new_tokens;
+  k.table = a->block_table; k.table_sb = a->block_table_stride;
+  k.free_pages = a->free_pages; k.free_count = a->free_count;
+  k.slots = a->slots; k.positions = a->positions; k.requests = a->requests; k.keys = a->keys;
+  k.lengths_out = a->lengths_out; k.free_out = a->free_count_out; k.granted = a->granted;
+  k.B = a->B; k.W = a->W; k.P = a->P; k.T = a->max_tokens;
+  return check_hip(fox::launch_page_slots(k, (hipStream_t)stream), "fox_page_slots");
+}
+
+int fox_page_release(const fox_page_release_args* a, void* stream) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  FOX_TRY(check_table(a->B, a->W, a->P));
+  fox::PageReleaseK k{};
+  FOX_TRY(page_shift(a->page_size, &k.shift));
+  FOX_TRY(check_room(a->W, a->page_size));
+  if (!a->lengths || !a->done || !a->block_table || !a->free_pages || !a->free_count || !a->lengths_out || !a->free_count_out)
+    return fail(FOX_E_ARG, "fox_page_release: no pointer may be NULL");
+  k.lengths = a->lengths; k.done = a->done;
+  k.table = a->block_table; k.table_sb = a->block_table_stride;
+  k.free_pages = a->free_pages; k.free_count = a->free_count;
+  k.lengths_out = a->lengths_out; k.free_out = a->free_count_out;
+  k.B = a->B; k.W = a->W; k.P = a->P;
+  return check_hip(fox::launch_page_release(k, (hipStream_t)stream), "fox_page_release");
+}
+
+int fox_paged_append(const fox_paged_append_args* a, void* stream) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  fox::PagedAppendK k{};
+  FOX_TRY(make_pages(a->pages, k.pages));
+  if (a->T <= 0 || (int64_t)a->T * a->pages.H > 0x7fffffffLL) return fail(FOX_E_ARG, "T must be positive and T * H below 2^31 (got %d)", a->T);
+  FOX_TRY(check_view(&a->k, "k"));
+  FOX_TRY(check_view(&a->v, "v"));
+  if (!a->g || !a->slots) return fail(FOX_E_ARG, "g and slots must not be NULL");
+  k.k = (const uint16_t*)a->k.ptr; k.k_st = a->k.stride_t; k.k_sh = a->k.stride_h;
+  k.v = (const uint16_t*)a->v.ptr; k.v_st = a->v.stride_t; k.v_sh = a->v.stride_h;
+  k.g = a->g; k.g_st = a->g_stride_t; k.g_sh = a->g_stride_h;
+  k.slots = a->slots;
+  k.H = a->pages.H;
+  k.total = (int64_t)a->T * k.H * (a->pages.D / 8);
+  k.by_heads = fox::divisor(k.H);
+  return check_hip(fox::launch_paged_append(k, a->pages.D, (hipStream_t)stream), "fox_paged_append");
+}
+
+int fox_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int64_t max_keys, int64_t* bytes) {
+  if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
+  FOX_TRY(check_head_dim(D));
+  if (B <= 0 || H <= 0 || (int64_t)B * H > (1 << 24) || max_keys <= 0 || max_keys > (1 << 30)) return fail(FOX_E_ARG, "B, H and max_keys must be positive, B * H at most 2^24, max_keys at most 2^30");
+  *bytes = fox::paged_decode_rows(B, H, (int)max_keys, D) * (int64_t)(D * sizeof(float) + sizeof(fox::DecodePartial));
+  return FOX_OK;
+}
+
+int fox_paged_decode(const fox_paged_decode_args* a, void* stream) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  fox::PagedDecodeK k{};
+  FOX_TRY(make_pages(a->pages, k.pages));
+  const int H = a->pages.H, D = a->pages.D;
+  if (a->B <= 0 || a->requests_in_table <= 0 || a->W <= 0) return fail(FOX_E_ARG, "rows, requests and pages of a request must be positive (got %d, %d, %d)", a->B, a->requests_in_table, a->W);
+  if (!a->requests && a->B > a->requests_in_table) return fail(FOX_E_ARG, "%d rows but %d requests in the table", a->B, a->requests_in_table);
+  FOX_TRY(check_room(a->W, a->pages.page_size));
+  if (a->max_length < 0) return fail(FOX_E_ARG, "max_length must not be negative");
+  if (!a->block_table || !a->lengths) return fail(FOX_E_ARG, "block_table and lengths must not be NULL");
+  FOX_TRY(check_view(&a->q, "q"));
+  FOX_TRY(check_view(&a->o, "o"));
+  const int room = a->W * a->pages.page_size;
+  k.max_keys = a->max_length > 0 && a->max_length < room ? a->max_length : room;
+  int64_t bytes = 0;
+  FOX_TRY(fox_paged_decode_workspace_bytes(a->B, H, D, k.max_keys, &bytes));
+  if (bytes > 0 && (!a->workspace || a->workspace_bytes < bytes)) return fail(FOX_E_ARG, "workspace holds %lld bytes, %lld are needed", a->workspace ? (long long)a->workspace_bytes : 0ll, (long long)bytes);
+  if ((uintptr_t)a->workspace & 15) return fail(FOX_E_ALIGN, "workspace must be 16-byte aligned");
+  k.q = (const uint16_t*)a->q.ptr; k.q_sb = a->q.stride_b; k.q_sh = a->q.stride_h;
+  k.o = (uint16_t*)a->o.ptr; k.o_sb = a->o.stride_b; k.o_sh = a->o.stride_h;
+  k.table = a->block_table; k.table_sb = a->block_table_stride;
+  k.lengths = a->lengths; k.requests = a->requests;
+  k.B = a->B; k.H = H; k.R = a->requests_in_table; k.W = a->W;
+  k.sm_scale = a->sm_scale;
+  k.by_heads = fox::divisor(H);
+  k.pieces = fox::paged_decode_pieces(a->B, H, k.max_keys, D);
+  k.ws_o = (float*)a->workspace;
+  k.ws_p = (fox::DecodePartial*)((char*)a->workspace + fox::paged_decode_rows(a->B, H, k.max_keys, D) * (int64_t)(D * sizeof(float)));
+  return check_hip(fox::launch_paged_decode(k, D, a->pages.dtype, (hipStream_t)stream), "fox_paged_decode");
 }
 
 int fox_token_shift_fwd(const fox_shift_args* args, void* stream) {

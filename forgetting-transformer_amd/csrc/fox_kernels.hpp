@@ -166,6 +166,89 @@ struct NormGateK {
   int cols, rows_per_lane;   // how the backward is cut (norm_bwd_plan), set by the launcher
 };
 
+// Rotation of q and k behind their norms, or of one tensor alone (fox_rotary.hip).  A side is (B, T, H, D) 16-bit; the second may have no heads.
+struct RotarySide {
+  View x;           // backward of the norm: its input
+  View in, out;     // forward: x and y, backward: dy and dx
+  const float* w;   // null without a norm
+  int H;
+};
+struct RotaryK {
+  RotarySide side[2];
+  const double* inv_freq;    // R / 2
+  const int64_t* positions;  // element strides below; null: first, first + 1, ..
+  int64_t p_sb, p_st, first;
+  int64_t w_sh;              // weights of a head and the next: D, or 0 for one row of weights for all
+  float* dw;                 // backward: of q's weights, then of k's
+  float* dw_partial;
+  int N, T, R;               // N = B * T tokens
+  int sign;                  // -1: the other way round
+  float eps;
+  int cols, lanes, rows, tile, tiles;   // how the call is cut (rotary_plan), set by the launcher with the divisors
+  Divisor by_T, by_half, by_cols;
+};
+constexpr int kRotaryRows = 4;                          // tokens a thread holds at once
+template <int D> constexpr int kRotaryTile = 2048 / D;  // tokens whose angles a workgroup holds, at most: 8 KiB
+
+// Pool of pages (fox_paged.hip): pages of 2^shift tokens, (P, H, S, D) keys and values as views with the stride between pages in sb, (P, H, S) log gates.
+struct PagesK {
+  View k, v;
+  float* g;
+  int64_t g_sp, g_sh, g_ss;
+  int P, shift;
+};
+struct PageSlotsK {
+  const int32_t *lengths, *new_tokens;   // (B)
+  int32_t* table;                        // (B, W), stride below
+  int64_t table_sb;
+  const int32_t* free_pages;             // (P), the first *free_count of them are free
+  const int32_t* free_count;
+  int64_t *slots, *positions;            // (T)
+  int32_t *requests, *keys;              // (T)
+  int32_t *lengths_out, *free_out;
+  uint8_t* granted;                      // (B)
+  int B, W, P, T, shift;
+  bool tokens, state;                    // what this launch writes: the tokens' values and the pages of the table; the others
+};
+struct PageReleaseK {
+  const int32_t* lengths;
+  const uint8_t* done;
+  const int32_t* table;
+  int64_t table_sb;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t *lengths_out, *free_out;
+  int B, W, P, shift;
+};
+constexpr int kPageRequests = 4096;      // requests of a page_slots or page_release, at most: what their LDS holds
+struct PagedAppendK {
+  PagesK pages;
+  const uint16_t *k, *v;
+  int64_t k_st, k_sh, v_st, v_sh;
+  const float* g;
+  int64_t g_st, g_sh;
+  const int64_t* slots;
+  int H;
+  int64_t total;                         // 16-byte pieces of k
+  Divisor by_heads;
+};
+// One new token per row against the pages of its request (paged_decode_kernel).
+struct PagedDecodeK {
+  PagesK pages;
+  const uint16_t* q;
+  uint16_t* o;
+  int64_t q_sb, q_sh, o_sb, o_sh;
+  const int32_t* table;                  // (R, W)
+  int64_t table_sb;
+  const int32_t *lengths, *requests;     // (B); requests null: row b of the table
+  int B, H, R, W, max_keys;              // keys of a request, at most
+  int pieces;                            // of all requests and heads together, about
+  float sm_scale;
+  Divisor by_heads;
+  float* ws_o;                           // (rows, D) partial accumulators and
+  DecodePartial* ws_p;                   // their sums, a row per piece: paged_decode_rows
+};
+
 // Tile sizes (see fox_tile_config in the public header)
 constexpr int kXcds = 8, kCus = 256;
 constexpr int kFwdBM = 128;
@@ -294,6 +377,16 @@ hipError_t launch_decode_gates(const DecodeK& a, int D, int dtype, hipStream_t s
 hipError_t launch_cache_append(const CacheAppendK& a, hipStream_t s);
 hipError_t launch_norm_gate(const NormGateK& a, int D, int dtype, bool bwd, int act, hipStream_t s);  // act: FOX_ACT_*
 int64_t norm_gate_workspace_rows(int64_t rows);
+hipError_t launch_reduce_rows(float* src, float* dst, int64_t rows, int width, hipStream_t s);   // fox_norm_gate.hip
+int64_t reduce_rows_floats(int64_t rows, int64_t width);
+hipError_t launch_rotary(const RotaryK& a, int D, int dtype, bool norm, bool interleaved, bool bwd, hipStream_t s);   // bwd: of the norm and the rotation
+hipError_t launch_page_slots(const PageSlotsK& a, hipStream_t s);
+hipError_t launch_page_release(const PageReleaseK& a, hipStream_t s);
+hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s);
+hipError_t launch_paged_decode(const PagedDecodeK& a, int D, int dtype, hipStream_t s);
+int paged_decode_pieces(int B, int H, int max_keys, int D);
+int64_t paged_decode_rows(int B, int H, int max_keys, int D);   // of workspace; 0: no request is split
+int64_t rotary_workspace_floats(int64_t tokens, int heads, int D, bool shared);
 hipError_t launch_shift_fwd(const ShiftK& a, int D, int dtype, hipStream_t s);
 hipError_t launch_shift_bwd(const ShiftK& a, int D, int dtype, hipStream_t s);
 hipError_t launch_cumsum_fwd(const float* g, int64_t sb, int64_t sh, int64_t sn, const int64_t* seq_start, float* c, int B,

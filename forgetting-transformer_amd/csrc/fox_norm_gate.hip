@@ -252,6 +252,21 @@ int64_t norm_gate_workspace_rows(int64_t rows) {
   return strips + (strips + 31) / 32;
 }
 
+// dst[j] = sum of the `rows` rows of `width` floats at src, behind which the sums of groups of rows have room (reduce_rows_floats in all).
+hipError_t launch_reduce_rows(float* src, float* dst, int64_t rows, int width, hipStream_t s) {
+  const int64_t groups = (rows + kReduceRows - 1) / kReduceRows;
+  const dim3 columns((unsigned)((width + 63) / 64));
+  if (groups == 1) {
+    hipLaunchKernelGGL(reduce_rows_kernel, columns, dim3(1024), 0, s, src, dst, rows, width, (int)rows);
+    return hipGetLastError();
+  }
+  float* stage = src + rows * width;
+  hipLaunchKernelGGL(reduce_rows_kernel, dim3(columns.x, (unsigned)groups), dim3(1024), 0, s, src, stage, rows, width, kReduceRows);
+  hipLaunchKernelGGL(reduce_rows_kernel, columns, dim3(1024), 0, s, stage, dst, groups, width, (int)groups);
+  return hipGetLastError();
+}
+int64_t reduce_rows_floats(int64_t rows, int64_t width) { return (rows + (rows > kReduceRows ? (rows + kReduceRows - 1) / kReduceRows : 0)) * width; }
+
 template <typename Tr, int D>
 static hipError_t norm_gate_d(const NormGateK& a, bool bwd, int act, hipStream_t s) {
   constexpr int CH = D / 8;
@@ -272,17 +287,8 @@ static hipError_t norm_gate_d(const NormGateK& a, bool bwd, int act, hipStream_t
   if (act == kActSwish) hipLaunchKernelGGL((norm_gate_bwd_kernel<Tr, D, kActSwish>), grid, block, 0, s, k);
   else if (act == kActNone) hipLaunchKernelGGL((norm_gate_bwd_kernel<Tr, D, kActNone>), grid, block, 0, s, k);
   else hipLaunchKernelGGL((norm_gate_bwd_kernel<Tr, D, kActSigmoid>), grid, block, 0, s, k);
-  const int width = a.G * D;
-  const int64_t groups = (p.strips + kReduceRows - 1) / kReduceRows;
-  const dim3 columns((unsigned)((width + 63) / 64));
-  if (groups == 1) {
-    hipLaunchKernelGGL(reduce_rows_kernel, columns, dim3(1024), 0, s, a.dw_partial, a.dw, p.strips, width, (int)p.strips);
-    return hipGetLastError();
-  }
-  float* stage = a.dw_partial + p.strips * width;  // second part of the workspace
-  hipLaunchKernelGGL(reduce_rows_kernel, dim3(columns.x, (unsigned)groups), dim3(1024), 0, s, a.dw_partial, stage, p.strips, width, kReduceRows);
-  hipLaunchKernelGGL(reduce_rows_kernel, columns, dim3(1024), 0, s, stage, a.dw, groups, width, (int)groups);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess ? e : launch_reduce_rows(a.dw_partial, a.dw, p.strips, a.G * D, s);
 }
 
 template <typename Tr>

@@ -1,0 +1,342 @@
+// Position rotation of queries and keys for gfx950, alone or in the pass of their per-head RMS norms:
+//   n[t,h,:] = x[t,h,:] * rstd[t,h] * w[h,:],  rstd = 1 / sqrt(mean_d x^2 + eps)        (without weights n = x)
+//   theta[t,i] = position[t] * inv_freq[i],  (a, b) = the i-th pair of the first R elements of n[t,h,:]
+//   y = (a cos theta - b sin theta, a sin theta + b cos theta),  the rest of the head as it is.
+// A pair is (i, i + R/2), or (2i, 2i+1) interleaved.  The rotation is orthogonal, so its gradient is the rotation by
+// -theta; behind it the norm's backward, with dn the gradient turned back,
+//   dw[h,:] = sum_t dn * xhat,  dx = rstd * (dn * w - xhat * mean_d(dn * w * xhat)),  xhat = x * rstd.
+// The backward forms rstd again from the x that it reads anyway.
+//
+// All are streams over HBM.  A lane holds sixteen elements of a head, two 16-byte vectors chosen so that both halves of
+// every pair are in the lane: vectors c and c + R/16 of the rotated part (2c and 2c+1 interleaved, and beyond the rotated
+// part).  Row sums are DPP adds over the D/16 lanes of a head.  The angles are the same for all heads of a token: a workgroup
+// forms them once per token, in 64 bits up to the fraction of a turn (a position of 2^20 would leave 32-bit angles 4 digits),
+// and keeps cosine and sine in LDS.  A thread owns one column (tensor, head, sixteen elements) and walks tokens, so the
+// weights are loaded once and their gradient stays in registers; partial gradients leave once per workgroup and are added in a fixed order.
+#include "fox_common.hpp"
+#include "fox_kernels.hpp"
+
+namespace fox {
+
+namespace {
+
+template <typename Tr>
+__device__ __forceinline__ void unpack8r(const u32x4& v, float* f) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[2 * e] = Tr::lo(v[e]);
+    f[2 * e + 1] = Tr::hi(v[e]);
+  }
+}
+template <typename Tr>
+__device__ __forceinline__ u32x4 pack8r(const float* f) {
+  u32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = Tr::pack2(f[2 * e], f[2 * e + 1]);
+  return r;
+}
+
+// A thread's column: which tensor, head and vectors.
+template <int D, bool INTERLEAVED>
+struct Column {
+  static constexpr int L = D / 16;   // lanes per head
+  int side, h, c, v0, v1;
+  __device__ __forceinline__ Column(const RotaryK& a, int col) {
+    const int q_cols = a.side[0].H * L;
+    side = col >= q_cols;
+    const int in = col - (side ? q_cols : 0);
+    h = in / L;
+    c = in % L;
+    const int half_vectors = a.R / 16;
+    const bool apart = !INTERLEAVED && c < half_vectors;
+    v0 = apart ? c : 2 * c;
+    v1 = apart ? c + half_vectors : 2 * c + 1;
+  }
+};
+
+// cos and sin of the tile's tokens, pair by pair.  Executed by the whole workgroup.
+template <int D>
+__device__ __forceinline__ void make_angles(const RotaryK& a, int64_t n0, int tokens, float2 (*cs)[D / 2]) {
+  const int half = a.R / 2;
+  for (int i = threadIdx.x; i < tokens * half; i += blockDim.x) {
+    const int tok = divide(i, a.by_half), pair = i - tok * half;
+    const int64_t n = n0 + tok;
+    if (n < a.N) {
+      const int b = divide((int)n, a.by_T), t = (int)n - b * a.T;
+      const int64_t pos = a.positions ? a.positions[b * a.p_sb + t * a.p_st] : a.first + t;
+      double turns = (double)pos * a.inv_freq[pair] * 0.15915494309189535;   // 1 / (2 pi)
+      turns -= rint(turns);
+      float s, c;
+      sincospif(2.0f * (float)turns, &s, &c);
+      cs[tok][pair] = float2{c, a.sign < 0 ? -s : s};
+    }
+  }
+}
+
+// The lane's sixteen elements turned by the angles of its eight pairs; pairs outside the rotated part stay as they are
+// (not turned by zero: an infinite element would make its neighbour NaN).
+template <bool INTERLEAVED>
+__device__ __forceinline__ void turn(float (&f)[16], const float2* cs, int first_pair, int half) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int ia = INTERLEAVED ? 2 * e : e, ib = INTERLEAVED ? 2 * e + 1 : 8 + e;
+    if (first_pair + e < half) {
+      const float2 t = cs[first_pair + e];
+      const float x = f[ia], y = f[ib];
+      f[ia] = x * t.x - y * t.y;
+      f[ib] = x * t.y + y * t.x;
+    }
+  }
+}
+
+template <int L>
+__device__ __forceinline__ float head_sum(float x) {
+  if constexpr (L > 1) return row_sum<L>(x);
+  return x;
+}
+
+}  // namespace
+
+template <typename Tr, int D, bool NORM, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
+  constexpr int L = D / 16;
+  __shared__ float2 cs[kRotaryTile<D>][D / 2];
+  const int tid = threadIdx.x;
+  const int rl = a.cols > 256 ? 0 : divide(tid, a.by_cols);
+  const int col = a.cols > 256 ? blockIdx.y * 256 + tid : tid - rl * a.cols;
+  const bool live = rl < a.lanes && col < a.cols;
+  const Column<D, INTERLEAVED> at(a, live ? col : 0);
+  const View in = at.side ? a.side[1].in : a.side[0].in, out = at.side ? a.side[1].out : a.side[0].out;
+  const int64_t n0 = (int64_t)blockIdx.x * a.tile;
+  float w[16];
+  if constexpr (NORM) {
+    const float* wp = (at.side ? a.side[1].w : a.side[0].w) + at.h * a.w_sh;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = wp[at.v0 * 8 + e];
+      w[8 + e] = wp[at.v1 * 8 + e];
+    }
+  }
+  u32x4 x0[kRotaryRows], x1[kRotaryRows];
+  int64_t to[kRotaryRows];
+#pragma unroll
+  for (int u = 0; u < kRotaryRows; ++u) {   // tokens past the end read the last one and are not stored
+    const int n = (int)min(n0 + rl + (int64_t)u * a.lanes, (int64_t)a.N - 1);
+    const int b = divide(n, a.by_T), t = n - b * a.T;
+    const uint16_t* p = in.ptr + b * in.sb + t * in.st + at.h * in.sh;
+    to[u] = b * out.sb + t * out.st + at.h * out.sh;
+    if (u == 0 || u < a.rows) {
+      x0[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v0 * 8));
+      x1[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v1 * 8));
+    }
+  }
+  make_angles<D>(a, n0, a.tile, cs);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kRotaryRows; ++u) {
+    if (u > 0 && u >= a.rows) break;
+    const int tok = rl + u * a.lanes;
+    float f[16];
+    unpack8r<Tr>(x0[u], f);
+    unpack8r<Tr>(x1[u], f + 8);
+    if constexpr (NORM) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
+      const float rstd = 1.0f / sqrtf(head_sum<L>(ss) / D + a.eps);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[e] = f[e] * rstd * w[e];
+    }
+    if (live && n0 + tok < a.N) {
+      turn<INTERLEAVED>(f, cs[tok], at.c * 8, a.R / 2);
+      uint16_t* p = const_cast<uint16_t*>(out.ptr) + to[u];
+      *reinterpret_cast<u32x4*>(p + at.v0 * 8) = pack8r<Tr>(f);
+      *reinterpret_cast<u32x4*>(p + at.v1 * 8) = pack8r<Tr>(f + 8);
+    }
+  }
+}
+
+// Gradient of the norm and the rotation behind it.  A workgroup walks a strip of `tiles` tiles of tokens.
+template <typename Tr, int D, bool INTERLEAVED>
+__global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
+  constexpr int L = D / 16;
+  __shared__ float2 cs[2][kRotaryTile<D>][D / 2];   // the next tile's angles are made while others still read this one's
+  __shared__ __align__(16) float dw_s[256 * 16];
+  const int tid = threadIdx.x;
+  const int rl = a.cols > 256 ? 0 : divide(tid, a.by_cols);
+  const int col = a.cols > 256 ? blockIdx.y * 256 + tid : tid - rl * a.cols;
+  const bool live = rl < a.lanes && col < a.cols;
+  const Column<D, INTERLEAVED> at(a, live ? col : 0);
+  const View xv = at.side ? a.side[1].x : a.side[0].x, in = at.side ? a.side[1].in : a.side[0].in;
+  const View out = at.side ? a.side[1].out : a.side[0].out;
+  float w[16], dw[16];
+  {
+    const float* wp = (at.side ? a.side[1].w : a.side[0].w) + at.h * a.w_sh;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = wp[at.v0 * 8 + e];
+      w[8 + e] = wp[at.v1 * 8 + e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) dw[e] = 0.f;
+
+  for (int i = 0; i < a.tiles; ++i) {
+    const int64_t n0 = ((int64_t)blockIdx.x * a.tiles + i) * a.tile;
+    if (n0 >= a.N) break;   // (the same for the whole workgroup)
+    u32x4 x0[kRotaryRows], x1[kRotaryRows], g0[kRotaryRows], g1[kRotaryRows];
+    int64_t to[kRotaryRows];
+#pragma unroll
+    for (int u = 0; u < kRotaryRows; ++u) {
+      const int n = (int)min(n0 + rl + (int64_t)u * a.lanes, (int64_t)a.N - 1);
+      const int b = divide(n, a.by_T), t = n - b * a.T;
+      const uint16_t* p = xv.ptr + b * xv.sb + t * xv.st + at.h * xv.sh;
+      const uint16_t* g = in.ptr + b * in.sb + t * in.st + at.h * in.sh;
+      to[u] = b * out.sb + t * out.st + at.h * out.sh;
+      x0[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v0 * 8));
+      x1[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v1 * 8));
+      g0[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(g + at.v0 * 8));
+      g1[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(g + at.v1 * 8));
+    }
+    make_angles<D>(a, n0, a.tile, cs[i & 1]);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kRotaryRows; ++u) {
+      const int tok = rl + u * a.lanes;
+      const bool here = live && n0 + tok < a.N;
+      float x[16], g[16];
+      unpack8r<Tr>(x0[u], x);
+      unpack8r<Tr>(x1[u], x + 8);
+      unpack8r<Tr>(g0[u], g);
+      unpack8r<Tr>(g1[u], g + 8);
+      turn<INTERLEAVED>(g, cs[i & 1][here ? tok : 0], at.c * 8, a.R / 2);
+      float ss = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        ss += x[e] * x[e];
+        s1 += g[e] * w[e] * x[e];
+      }
+      const float rstd = 1.0f / sqrtf(head_sum<L>(ss) / D + a.eps);
+      const float c1 = head_sum<L>(s1) * rstd * (1.0f / D);
+      if (here) {
+        float dx[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float xhat = x[e] * rstd;
+          dw[e] += g[e] * xhat;
+          dx[e] = (g[e] * w[e] - xhat * c1) * rstd;
+        }
+        uint16_t* p = const_cast<uint16_t*>(out.ptr) + to[u];
+        *reinterpret_cast<u32x4*>(p + at.v0 * 8) = pack8r<Tr>(dx);
+        *reinterpret_cast<u32x4*>(p + at.v1 * 8) = pack8r<Tr>(dx + 8);
+      }
+    }
+  }
+
+  // the workgroup's sums in element order: row lanes, and with shared weights heads, one after the other
+  const int cols = a.cols > 256 ? min(256, a.cols - (int)blockIdx.y * 256) : a.cols, col0 = a.cols > 256 ? blockIdx.y * 256 : 0;
+  if (live) {
+    float* p = dw_s + rl * cols * 16 + (col - col0) / L * D;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[at.v0 * 8 + e] = dw[e];
+      p[at.v1 * 8 + e] = dw[8 + e];
+    }
+  }
+  __syncthreads();
+  const int width = cols * 16;
+  if (a.w_sh != 0) {
+    float* dst = a.dw_partial + (int64_t)blockIdx.x * a.cols * 16 + col0 * 16;
+    for (int j = tid; j < width; j += blockDim.x) {
+      float sum = dw_s[j];
+      for (int r = 1; r < a.lanes; ++r) sum += dw_s[r * width + j];
+      dst[j] = sum;
+    }
+  } else {
+    float* dst = a.dw_partial + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * D;
+    const int q_elems = min(max(a.side[0].H * D - col0 * 16, 0), width);   // of this workgroup's columns
+    for (int j = tid; j < 2 * D; j += blockDim.x) {
+      const int k0 = j < D ? j : q_elems + j - D, k1 = j < D ? q_elems : width;
+      float sum = 0.f;
+      for (int r = 0; r < a.lanes; ++r)
+        for (int k = k0; k < k1; k += D) sum += dw_s[r * width + k];
+      dst[j] = sum;
+    }
+  }
+}
+
+namespace {
+// How a call over `tokens` tokens is cut: columns, row lanes of a workgroup, tokens a thread holds, tokens a tile, tiles a workgroup.
+struct RotaryPlan {
+  int cols, chunks, lanes, rows, tile, tiles;
+  int64_t strips;
+};
+RotaryPlan rotary_plan(int64_t tokens, int heads, int D, bool bwd) {
+  RotaryPlan p;
+  const int most = 2048 / D / kRotaryRows;   // what the angles in LDS have room for (kRotaryTile)
+  p.cols = heads * (D / 16);
+  p.chunks = (p.cols + 255) / 256;
+  p.lanes = p.cols > 256 ? 1 : 256 / p.cols;
+  if (p.lanes > most) p.lanes = most;
+  // four tokens a thread and tile, fewer where a forward would not make four workgroups a CU
+  const int64_t rows = tokens * p.chunks / ((int64_t)p.lanes * 4 * kCus);
+  p.rows = bwd || rows > kRotaryRows ? kRotaryRows : rows < 1 ? 1 : (int)rows;
+  p.tile = p.lanes * p.rows;
+  const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? tiles * p.chunks / (4 * kCus) : 1;
+  p.tiles = (int)(per < 1 ? 1 : per);
+  p.strips = (tiles + p.tiles - 1) / p.tiles;
+  return p;
+}
+}  // namespace
+
+int64_t rotary_workspace_floats(int64_t tokens, int heads, int D, bool shared) {
+  const RotaryPlan p = rotary_plan(tokens, heads, D, true);
+  const int64_t width = shared ? 2 * D : (int64_t)heads * D;
+  return reduce_rows_floats(shared ? p.strips * p.chunks : p.strips, width);
+}
+
+template <typename Tr, int D>
+static hipError_t launch_rotary_d(const RotaryK& args, bool norm, bool interleaved, bool bwd, hipStream_t s) {
+  RotaryK a = args;
+  const int heads = a.side[0].H + a.side[1].H;
+  const RotaryPlan p = rotary_plan(a.N, heads, D, bwd);
+  a.cols = p.cols;
+  a.lanes = p.lanes;
+  a.rows = p.rows;
+  a.tile = p.tile;
+  a.tiles = p.tiles;
+  a.by_T = divisor(a.T);
+  a.by_half = divisor(a.R / 2);
+  a.by_cols = divisor(p.cols);
+  const dim3 grid((unsigned)p.strips, (unsigned)p.chunks), block(p.cols > 256 ? 256u : (unsigned)((p.cols * p.lanes + 63) / 64 * 64));
+  if (!bwd) {
+    if (norm && interleaved) hipLaunchKernelGGL((rotary_kernel<Tr, D, true, true>), grid, block, 0, s, a);
+    else if (norm) hipLaunchKernelGGL((rotary_kernel<Tr, D, true, false>), grid, block, 0, s, a);
+    else if (interleaved) hipLaunchKernelGGL((rotary_kernel<Tr, D, false, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<Tr, D, false, false>), grid, block, 0, s, a);
+    return hipGetLastError();
+  }
+  if (interleaved) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<Tr, D, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<Tr, D, false>), grid, block, 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const bool shared = a.w_sh == 0;
+  return launch_reduce_rows(a.dw_partial, a.dw, shared ? p.strips * p.chunks : p.strips, shared ? 2 * D : heads * D, s);
+}
+
+template <typename Tr>
+static hipError_t launch_rotary_t(const RotaryK& a, int D, bool norm, bool interleaved, bool bwd, hipStream_t s) {
+  switch (D) {
+    case 16: return launch_rotary_d<Tr, 16>(a, norm, interleaved, bwd, s);
+    case 32: return launch_rotary_d<Tr, 32>(a, norm, interleaved, bwd, s);
+    case 64: return launch_rotary_d<Tr, 64>(a, norm, interleaved, bwd, s);
+    case 128: return launch_rotary_d<Tr, 128>(a, norm, interleaved, bwd, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_rotary(const RotaryK& a, int D, int dtype, bool norm, bool interleaved, bool bwd, hipStream_t s) {
+  return dtype == 0 ? launch_rotary_t<Bf16>(a, D, norm, interleaved, bwd, s) : launch_rotary_t<Fp16>(a, D, norm, interleaved, bwd, s);
+}
+
+}  // namespace fox

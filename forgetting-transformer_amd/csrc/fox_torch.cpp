@@ -521,6 +521,162 @@ struct ShiftNode : public torch::autograd::Function<ShiftNode> {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
+// position rotation, alone and behind the norms of queries and keys
+// ---------------------------------------------------------------------------------------------------------------
+struct Rotary {      // what the calls share
+  bool head_first = false, interleaved = false;
+  Tensor inv_freq;   // double, contiguous
+  Tensor positions;  // int64, undefined: first, first + 1, ..
+  int64_t first = 0;
+
+  fox_rotary_args args(const Tensor& x) const {
+    fox_rotary_args a{};
+    a.sides = 1;
+    a.B = (int32_t)x.size(0);
+    a.T = (int32_t)x.size(head_first ? 2 : 1);
+    a.D = (int32_t)x.size(3);
+    a.dtype = dtype_code(x);
+    a.rotary_dim = (int32_t)(2 * inv_freq.size(0));
+    a.interleaved = interleaved;
+    a.inv_freq = inv_freq.const_data_ptr<double>();
+    a.first_position = first;
+    if (positions.defined()) {   // (T), (B, T), (B, 1) or (1, T)
+      const bool two = positions.dim() == 2;
+      a.positions = positions.const_data_ptr<int64_t>();
+      a.position_stride_b = two && positions.size(0) > 1 ? positions.stride(0) : 0;
+      a.position_stride_t = positions.size(-1) > 1 ? positions.stride(-1) : 0;
+    }
+    return a;
+  }
+  void save(torch::autograd::AutogradContext* ctx) const {
+    ctx->saved_data["hf"] = head_first;
+    ctx->saved_data["inter"] = interleaved;
+    ctx->saved_data["first"] = first;
+  }
+  static Rotary load(torch::autograd::AutogradContext* ctx, const Tensor& inv_freq, const Tensor& positions) {
+    Rotary r;
+    r.head_first = ctx->saved_data["hf"].toBool();
+    r.interleaved = ctx->saved_data["inter"].toBool();
+    r.first = ctx->saved_data["first"].toInt();
+    r.inv_freq = packed(inv_freq);
+    r.positions = positions;
+    return r;
+  }
+};
+
+// x turned by the angles of its tokens, or back
+Tensor run_rotary(const Rotary& r, const Tensor& x, bool back) {
+  Tensor y = at::empty_like(x);
+  if (x.numel() == 0) return y;
+  fox_rotary_args a = r.args(x);
+  fox_rotary_side& s = a.side[0];
+  s.H = (int32_t)x.size(r.head_first ? 1 : 2);
+  (back ? s.y : s.x) = view_of(x, r.head_first);
+  (back ? s.dx : s.y) = view_of(y, r.head_first);
+  check(back ? fox_rotary_bwd(&a, stream_of(x)) : fox_rotary_fwd(&a, stream_of(x)), back ? "fox_rotary_bwd" : "fox_rotary_fwd");
+  return y;
+}
+
+// As the kernels take it, copied where it is not (contiguous() would hand a tensor back that merely starts at an odd address).
+Tensor aligned(const Tensor& t) { return vectors_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+struct RotaryNode : public torch::autograd::Function<RotaryNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& inv_freq, const std::optional<Tensor>& positions, const Rotary* r, bool back) {
+    ctx->save_for_backward({inv_freq, positions.value_or(Tensor())});
+    r->save(ctx);
+    ctx->saved_data["back"] = back;
+    return run_rotary(*r, x, back);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    if (!grads[0].defined()) return variable_list(5);
+    const c10::DeviceGuard guard(grads[0].device());
+    const Rotary r = Rotary::load(ctx, s[0], s[1]);
+    const bool back = !ctx->saved_data["back"].toBool();
+    const Tensor dy = aligned(grads[0]);
+    // (linear: its gradient has one of its own)
+    const Tensor dx = at::GradMode::is_enabled() ? RotaryNode::apply(dy, r.inv_freq, some_tensor(r.positions), &r, back) : run_rotary(r, dy, back);
+    return {dx, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+  static std::optional<Tensor> some_tensor(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+};
+
+// fox_rotary_args of queries and keys with their norms; the views are the caller's to fill
+fox_rotary_args qk_args(const Rotary& r, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, bool shared, double eps) {
+  fox_rotary_args a = r.args(q);
+  a.sides = 2;
+  a.side[0].H = (int32_t)q.size(r.head_first ? 1 : 2);
+  a.side[1].H = (int32_t)k.size(r.head_first ? 1 : 2);
+  a.side[0].weight = wq.const_data_ptr<float>();
+  a.side[1].weight = wk.const_data_ptr<float>();
+  a.weight_stride_h = shared ? 0 : a.D;
+  a.eps = (float)eps;
+  return a;
+}
+
+struct QkNormRotaryNode : public torch::autograd::Function<QkNormRotaryNode> {
+  static variable_list run(const Rotary& r, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, bool shared, double eps) {
+    Tensor yq = at::empty_like(q), yk = at::empty_like(k);
+    if (q.numel() == 0) return {yq, yk};
+    fox_rotary_args a = qk_args(r, q, k, wq, wk, shared, eps);
+    a.side[0].x = view_of(q, r.head_first);
+    a.side[1].x = view_of(k, r.head_first);
+    a.side[0].y = view_of(yq, r.head_first);
+    a.side[1].y = view_of(yk, r.head_first);
+    check(fox_rotary_fwd(&a, stream_of(q)), "fox_rotary_fwd");
+    return {yq, yk};
+  }
+  // The kernels read the weights as aligned fp32 rows.
+  static Tensor weights(const Tensor& w) {
+    Tensor t = w.detach().to(at::kFloat).contiguous();
+    return reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15 ? t.clone() : t;
+  }
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& inv_freq,
+                               const std::optional<Tensor>& positions, const Rotary* r, bool shared, double eps) {
+    const Tensor wq32 = weights(wq), wk32 = weights(wk);
+    ctx->save_for_backward({q, k, wq32, wk32, inv_freq, positions.value_or(Tensor())});
+    r->save(ctx);
+    ctx->saved_data["shared"] = shared;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["wqtype"] = (int64_t)wq.scalar_type();
+    ctx->saved_data["wktype"] = (int64_t)wk.scalar_type();
+    return run(*r, q, k, wq32, wk32, shared, eps);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    if (!grads[0].defined() && !grads[1].defined()) return variable_list(9);
+    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rotary has no second derivative (create_graph)");
+    const Tensor q = aligned(s[0]), k = aligned(s[1]), wq = weights(s[2]), wk = weights(s[3]);
+    const c10::DeviceGuard guard(q.device());
+    const Rotary r = Rotary::load(ctx, s[4], s[5]);
+    const bool shared = ctx->saved_data["shared"].toBool();
+    const Tensor dyq = grads[0].defined() ? aligned(grads[0]) : at::zeros_like(q), dyk = grads[1].defined() ? aligned(grads[1]) : at::zeros_like(k);
+    Tensor dq = at::empty_like(q), dk = at::empty_like(k);
+    const int64_t nq = wq.numel(), nk = wk.numel();
+    Tensor dw = q.numel() == 0 ? at::zeros({nq + nk}, wq.options()) : at::empty({nq + nk}, wq.options());
+    if (q.numel() > 0) {
+      fox_rotary_args a = qk_args(r, q, k, wq, wk, shared, ctx->saved_data["eps"].toDouble());
+      int64_t bytes = 0;
+      check(fox_rotary_workspace_bytes((int64_t)a.B * a.T, a.side[0].H + a.side[1].H, a.D, shared, &bytes), "fox_rotary_workspace_bytes");
+      Tensor ws = empty_bytes_like(q, bytes);
+      a.side[0].x = view_of(q, r.head_first);
+      a.side[1].x = view_of(k, r.head_first);
+      a.side[0].y = view_of(dyq, r.head_first);
+      a.side[1].y = view_of(dyk, r.head_first);
+      a.side[0].dx = view_of(dq, r.head_first);
+      a.side[1].dx = view_of(dk, r.head_first);
+      a.dweight = dw.mutable_data_ptr<float>();
+      a.workspace = (float*)ws.mutable_data_ptr();
+      check(fox_rotary_bwd(&a, stream_of(q)), "fox_rotary_bwd");
+    }
+    return {dq, dk, dw.narrow(0, 0, nq).to((at::ScalarType)ctx->saved_data["wqtype"].toInt()),
+            dw.narrow(0, nq, nk).to((at::ScalarType)ctx->saved_data["wktype"].toInt()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------------------
 // Python entry points (METH_FASTCALL: the arguments come as a plain array).  Each returns None when the call is not one it
 // handles.  The interpreter lock is free while they allocate, launch and build the graph: a launch may wait for room in a
 // queue, and threads that drive other streams or devices must not wait with it (the argument array keeps its objects alive).
@@ -834,6 +990,357 @@ PyObject* py_cache_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A (B, T, H, D) or (B, H, T, D) tensor the rotation's kernels take as it is.
+bool rotary_ok(const Tensor* x) {
+  return x && x->dim() == 4 && on_current_gpu(*x) && sixteen_bit(*x) && head_dim_ok(x->size(3)) && vectors_ok(*x);
+}
+
+// Fills `r` from the arguments both entry points share, for an x that rotary_ok() took; false: not a call for the native path.
+bool parse_rotary(Rotary& r, const Tensor& x, PyObject* inv_freq, PyObject* positions, PyObject* interleaved, PyObject* head_first) {
+  if (!flag(interleaved, r.interleaved) || !flag(head_first, r.head_first)) return false;
+  const Tensor* f = tensor_of(inv_freq);
+  if (!f || f->dim() != 1 || f->scalar_type() != at::kDouble || f->device() != x.device() || !f->is_contiguous() || f->requires_grad()) return false;
+  const int64_t R = 2 * f->size(0), B = x.size(0), T = x.size(r.head_first ? 2 : 1);
+  if (R < 2 || R > x.size(3) || (!r.interleaved && R % 16) || B * T > INT32_MAX || x.size(r.head_first ? 1 : 2) > 65535) return false;
+  r.inv_freq = *f;
+  if (positions == Py_None) return true;
+  if (PyLong_Check(positions) && !PyBool_Check(positions)) {
+    r.first = PyLong_AsLongLong(positions);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      return false;
+    }
+    return true;
+  }
+  const Tensor* p = tensor_of(positions);
+  if (!p || p->scalar_type() != at::kLong || p->device() != x.device() || (p->dim() != 1 && p->dim() != 2)) return false;
+  if (p->size(-1) != T && p->size(-1) != 1) return false;
+  if (p->dim() == 1 && p->size(0) != T) return false;
+  if (p->dim() == 2 && p->size(0) != B && p->size(0) != 1) return false;
+  r.positions = *p;
+  return true;
+}
+
+// rotary(x, inv_freq, positions, interleaved, head_first)
+PyObject* py_rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 5, "rotary takes 5 arguments");
+  const Tensor* x = tensor_of(o[0]);
+  Rotary r;
+  if (!rotary_ok(x) || !parse_rotary(r, *x, o[1], o[2], o[3], o[4])) return none();
+  Tensor y;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    if (needs_graph({x})) {
+      y = RotaryNode::apply(*x, r.inv_freq, some(r.positions), &r, false);
+    } else {
+      const at::NoGradGuard no_grad;
+      y = run_rotary(r, *x, false);
+    }
+  }
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, positions, interleaved, eps, head_first) -> (q, k)
+PyObject* py_qk_norm_rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 9, "qk_norm_rotary takes 9 arguments");
+  const Tensor *q = tensor_of(o[0]), *k = tensor_of(o[1]), *wq = tensor_of(o[2]), *wk = tensor_of(o[3]);
+  Rotary r;
+  if (!rotary_ok(q) || !rotary_ok(k) || !wq || !wk || !parse_rotary(r, *q, o[4], o[5], o[6], o[8])) return none();
+  const int ih = r.head_first ? 1 : 2, it = r.head_first ? 2 : 1;
+  const int64_t D = q->size(3), Hq = q->size(ih), Hk = k->size(ih);
+  if (k->scalar_type() != q->scalar_type() || k->device() != q->device() || k->size(0) != q->size(0) || k->size(it) != q->size(it) || k->size(3) != D ||
+      Hq < 1 || Hk < 1 || Hk > 65535)
+    return none();
+  for (const Tensor* w : {wq, wk})
+    if (w->dim() != 1 || w->device() != q->device() || !w->is_floating_point()) return none();
+  // weights of one head serve all of them; both sides alike
+  const bool shared = wq->size(0) == D && wk->size(0) == D && (Hq > 1 || Hk > 1);
+  if (!shared && (wq->size(0) != Hq * D || wk->size(0) != Hk * D)) return none();
+  const double eps = PyFloat_AsDouble(o[7]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  variable_list y;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    if (needs_graph({q, k, wq, wk})) {
+      y = QkNormRotaryNode::apply(*q, *k, *wq, *wk, r.inv_freq, some(r.positions), &r, shared, eps);
+    } else {
+      const at::NoGradGuard no_grad;
+      y = QkNormRotaryNode::run(r, *q, *k, QkNormRotaryNode::weights(*wq), QkNormRotaryNode::weights(*wk), shared, eps);
+    }
+  }
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) return nullptr;
+  for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(y[i]));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// serving from pages (no gradients)
+// ---------------------------------------------------------------------------------------------------------------
+bool int32_ok(const Tensor* t, const Tensor& like, int64_t dim) {
+  return t && t->dim() == dim && t->scalar_type() == at::kInt && t->device() == like.device() && (dim == 1 ? t->is_contiguous() : t->stride(1) == 1);
+}
+// Written in place: a leaf of a graph may not be, nor an inference tensor outside inference mode.
+bool writable(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) < 1) return false;   // rows that lie on each other
+  return !(at::GradMode::is_enabled() && t.requires_grad()) && (!t.is_inference() || c10::InferenceMode::is_enabled());
+}
+void wrote(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+bool shares_storage(const Tensor& a, const Tensor& b) { return a.storage().is_alias_of(b.storage()); }
+
+// The integer arguments of page_slots and page_release: lengths (B), block_table (B, W), free_pages (P), free_count (1).
+bool page_state_ok(const Tensor* lengths, const Tensor* table, const Tensor* free_pages, const Tensor* free_count) {
+  if (!lengths || !on_current_gpu(*lengths) || !int32_ok(lengths, *lengths, 1) || !int32_ok(table, *lengths, 2) || !int32_ok(free_pages, *lengths, 1) ||
+      !int32_ok(free_count, *lengths, 1))
+    return false;
+  const Tensor* all[4] = {lengths, table, free_pages, free_count};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      if (shares_storage(*all[i], *all[j])) {   // parts of one buffer are fine while they do not overlap
+        const auto span = [](const Tensor& t) {
+          const char* p = (const char*)t.const_data_ptr();
+          const int64_t n = t.dim() == 2 ? (t.size(0) - 1) * t.stride(0) + t.size(1) : t.numel();
+          return std::pair<const char*, const char*>(p, p + 4 * n);
+        };
+        const auto a = span(*all[i]), b = span(*all[j]);
+        if (a.first < b.second && b.first < a.second) return false;
+      }
+  const int64_t B = lengths->size(0), W = table->size(1), P = free_pages->size(0);
+  return B > 0 && B <= 4096 && table->size(0) == B && W > 0 && W <= INT32_MAX && P > 0 && P <= INT32_MAX && free_count->size(0) == 1 &&
+         (B == 1 || table->stride(0) >= W);
+}
+
+// page_slots(lengths, new_tokens, block_table, free_pages, free_count, page_size, max_tokens, in_place)
+// -> (slots, positions, requests, keys, lengths, free_count, granted)
+PyObject* py_page_slots(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 8, "page_slots takes 8 arguments");
+  const Tensor *lengths = tensor_of(o[0]), *fresh = tensor_of(o[1]), *table = tensor_of(o[2]), *pages = tensor_of(o[3]), *count = tensor_of(o[4]);
+  if (!page_state_ok(lengths, table, pages, count) || !int32_ok(fresh, *lengths, 1) || fresh->sizes() != lengths->sizes()) return none();
+  const int64_t S = PyLong_AsLongLong(o[5]), T = PyLong_AsLongLong(o[6]);
+  bool in_place = false;
+  if (PyErr_Occurred() || !flag(o[7], in_place)) {
+    PyErr_Clear();
+    return none();
+  }
+  if (T < 0 || T > INT32_MAX || S < 1 || S > INT32_MAX || !writable(*table) || (in_place && (!writable(*lengths) || !writable(*count) || shares_storage(*fresh, *lengths))))
+    return none();
+  Tensor out[7];
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const at::NoGradGuard no_grad;
+    for (int i = 0; i < 4; ++i) out[i] = at::empty({T}, lengths->options().dtype(i < 2 ? at::kLong : at::kInt));
+    out[4] = in_place ? *lengths : at::empty_like(*lengths);
+    out[5] = in_place ? *count : at::empty_like(*count);
+    out[6] = at::empty(lengths->sizes(), lengths->options().dtype(at::kBool));
+    fox_page_slots_args a{};
+    a.B = (int32_t)lengths->size(0);
+    a.W = (int32_t)table->size(1);
+    a.P = (int32_t)pages->size(0);
+    a.page_size = (int32_t)S;
+    a.max_tokens = (int32_t)T;
+    a.lengths = lengths->const_data_ptr<int32_t>();
+    a.new_tokens = fresh->const_data_ptr<int32_t>();
+    a.block_table = table->mutable_data_ptr<int32_t>();
+    a.block_table_stride = table->stride(0);
+    a.free_pages = pages->const_data_ptr<int32_t>();
+    a.free_count = count->const_data_ptr<int32_t>();
+    a.slots = out[0].mutable_data_ptr<int64_t>();
+    a.positions = out[1].mutable_data_ptr<int64_t>();
+    a.requests = out[2].mutable_data_ptr<int32_t>();
+    a.keys = out[3].mutable_data_ptr<int32_t>();
+    a.lengths_out = out[4].mutable_data_ptr<int32_t>();
+    a.free_count_out = out[5].mutable_data_ptr<int32_t>();
+    a.granted = (uint8_t*)out[6].mutable_data_ptr();
+    check(fox_page_slots(&a, stream_of(*lengths)), "fox_page_slots");
+  }
+  wrote(*table);
+  if (in_place) {
+    wrote(*lengths);
+    wrote(*count);
+  }
+  PyObject* result = PyTuple_New(7);
+  if (!result) return nullptr;
+  for (int i = 0; i < 7; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(out[i]));
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+// page_release(lengths, done, block_table, free_pages, free_count, page_size, in_place) -> (lengths, free_count)
+PyObject* py_page_release(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 7, "page_release takes 7 arguments");
+  const Tensor *lengths = tensor_of(o[0]), *done = tensor_of(o[1]), *table = tensor_of(o[2]), *pages = tensor_of(o[3]), *count = tensor_of(o[4]);
+  if (!page_state_ok(lengths, table, pages, count) || !done || done->scalar_type() != at::kBool || done->device() != lengths->device() ||
+      done->sizes() != lengths->sizes() || !done->is_contiguous())
+    return none();
+  const int64_t S = PyLong_AsLongLong(o[5]);
+  bool in_place = false;
+  if (PyErr_Occurred() || !flag(o[6], in_place)) {
+    PyErr_Clear();
+    return none();
+  }
+  if (S < 1 || S > INT32_MAX || !writable(*pages) || (in_place && (!writable(*lengths) || !writable(*count)))) return none();
+  Tensor out[2];
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const at::NoGradGuard no_grad;
+    out[0] = in_place ? *lengths : at::empty_like(*lengths);
+    out[1] = in_place ? *count : at::empty_like(*count);
+    fox_page_release_args a{};
+    a.B = (int32_t)lengths->size(0);
+    a.W = (int32_t)table->size(1);
+    a.P = (int32_t)pages->size(0);
+    a.page_size = (int32_t)S;
+    a.lengths = lengths->const_data_ptr<int32_t>();
+    a.done = (const uint8_t*)done->const_data_ptr();
+    a.block_table = table->const_data_ptr<int32_t>();
+    a.block_table_stride = table->stride(0);
+    a.free_pages = pages->mutable_data_ptr<int32_t>();
+    a.free_count = count->const_data_ptr<int32_t>();
+    a.lengths_out = out[0].mutable_data_ptr<int32_t>();
+    a.free_count_out = out[1].mutable_data_ptr<int32_t>();
+    check(fox_page_release(&a, stream_of(*lengths)), "fox_page_release");
+  }
+  wrote(*pages);
+  if (in_place) {
+    wrote(*lengths);
+    wrote(*count);
+  }
+  PyObject* result = PyTuple_New(2);
+  if (!result) return nullptr;
+  for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(out[i]));
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+// Pages of keys, values (P, H, S, D) and log gates (P, H, S).
+bool pages_ok(const Tensor* k, const Tensor* v, const Tensor* g, fox_pages& p) {
+  if (!k || !v || !g || k->dim() != 4 || g->dim() != 3 || k->numel() == 0 || !on_current_gpu(*k) || !sixteen_bit(*k) || v->scalar_type() != k->scalar_type() ||
+      g->scalar_type() != at::kFloat || v->device() != k->device() || g->device() != k->device() || v->sizes() != k->sizes() ||
+      g->sizes() != k->sizes().slice(0, 3) || !vectors_ok(*k) || !vectors_ok(*v) || !head_dim_ok(k->size(3)))
+    return false;
+  for (int i = 0; i < 3; ++i)
+    if (k->size(i) > INT32_MAX) return false;
+  p = fox_pages{};
+  p.P = (int32_t)k->size(0);
+  p.H = (int32_t)k->size(1);
+  p.page_size = (int32_t)k->size(2);
+  p.D = (int32_t)k->size(3);
+  p.dtype = dtype_code(*k);
+  p.k = view_of(*k, true);
+  p.v = view_of(*v, true);
+  p.g = const_cast<float*>(g->const_data_ptr<float>());
+  p.g_stride_p = g->stride(0);
+  p.g_stride_h = g->stride(1);
+  p.g_stride_t = g->stride(2);
+  return true;
+}
+// A (T, H, D) tensor of tokens; only token and head strides count.
+fox_view token_view(const Tensor& t) { return fox_view{t.data_ptr(), t.stride(0), t.stride(1), t.stride(0)}; }
+bool tokens_ok(const Tensor* t, const fox_pages& p, const Tensor& pages) {
+  return t && t->dim() == 3 && t->scalar_type() == pages.scalar_type() && t->device() == pages.device() && t->size(1) == p.H && t->size(2) == p.D &&
+         t->size(0) <= INT32_MAX && vectors_ok(*t);
+}
+
+// paged_append(k, v, log_fgate, k_pages, v_pages, log_fgate_pages, slots) -> True
+PyObject* py_paged_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 7, "paged_append takes 7 arguments");
+  const Tensor *k = tensor_of(o[0]), *v = tensor_of(o[1]), *g = tensor_of(o[2]), *kp = tensor_of(o[3]), *vp = tensor_of(o[4]), *gp = tensor_of(o[5]),
+               *slots = tensor_of(o[6]);
+  fox_paged_append_args a{};
+  if (!pages_ok(kp, vp, gp, a.pages) || !tokens_ok(k, a.pages, *kp) || !tokens_ok(v, a.pages, *kp) || v->size(0) != k->size(0)) return none();
+  const int64_t T = k->size(0);
+  if (!g || g->dim() != 2 || g->scalar_type() != at::kFloat || g->device() != kp->device() || g->size(0) != T || g->size(1) != a.pages.H) return none();
+  if (!slots || slots->dim() != 1 || slots->size(0) != T || slots->scalar_type() != at::kLong || slots->device() != kp->device() || !slots->is_contiguous()) return none();
+  if (needs_graph({k, v, g}) || !writable(*kp) || !writable(*vp) || !writable(*gp)) return none();
+  const Tensor* to[3] = {kp, vp, gp};
+  const Tensor* from[3] = {k, v, g};
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j)
+      if (shares_storage(*to[i], *from[j])) return none();
+  if (T > 0) {
+    const pybind11::gil_scoped_release no_gil;
+    a.T = (int32_t)T;
+    a.k = token_view(*k);
+    a.v = token_view(*v);
+    a.g = g->const_data_ptr<float>();
+    a.g_stride_t = g->stride(0);
+    a.g_stride_h = g->stride(1);
+    a.slots = slots->const_data_ptr<int64_t>();
+    check(fox_paged_append(&a, stream_of(*k)), "fox_paged_append");
+  }
+  for (const Tensor* t : to) wrote(*t);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_pages, v_pages, log_fgate_pages, block_table, lengths, requests, sm_scale, max_length)
+PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 9, "paged_attention takes 9 arguments");
+  const Tensor *q = tensor_of(o[0]), *kp = tensor_of(o[1]), *vp = tensor_of(o[2]), *gp = tensor_of(o[3]), *table = tensor_of(o[4]), *lengths = tensor_of(o[5]);
+  fox_paged_decode_args a{};
+  if (!pages_ok(kp, vp, gp, a.pages) || !tokens_ok(q, a.pages, *kp) || !int32_ok(table, *kp, 2) || !int32_ok(lengths, *kp, 1)) return none();
+  const int64_t B = q->size(0), W = table->size(1), S = a.pages.page_size;
+  if (lengths->size(0) != B || table->size(0) < 1 || W < 1 || table->size(0) > INT32_MAX || W * S > (1 << 30) || B * a.pages.H > (1 << 24)) return none();
+  const Tensor* requests = nullptr;
+  if (o[6] != Py_None) {
+    requests = tensor_of(o[6]);
+    if (!int32_ok(requests, *kp, 1) || requests->size(0) != B) return none();
+  } else if (table->size(0) != B) {
+    return none();
+  }
+  double scale = 1.0 / std::sqrt((double)a.pages.D);
+  if (o[7] != Py_None) scale = PyFloat_AsDouble(o[7]);
+  int64_t most = 0;
+  if (o[8] != Py_None) most = PyLong_AsLongLong(o[8]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  if ((o[8] != Py_None && most < 1) || needs_graph({q, kp, vp, gp})) return none();
+  Tensor out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const at::NoGradGuard no_grad;
+    out = at::empty_like(*q);
+    if (B > 0) {
+      a.B = (int32_t)B;
+      a.requests_in_table = (int32_t)table->size(0);
+      a.W = (int32_t)W;
+      a.max_length = (int32_t)(most > W * S ? 0 : most);
+      a.q = token_view(*q);
+      a.o = token_view(out);
+      a.block_table = table->const_data_ptr<int32_t>();
+      a.block_table_stride = table->stride(0);
+      a.lengths = lengths->const_data_ptr<int32_t>();
+      a.requests = requests ? requests->const_data_ptr<int32_t>() : nullptr;
+      a.sm_scale = (float)scale;
+      check(fox_paged_decode_workspace_bytes(a.B, a.pages.H, a.pages.D, a.max_length ? a.max_length : W * S, &a.workspace_bytes), "fox_paged_decode_workspace_bytes");
+      Tensor ws;
+      if (a.workspace_bytes > 0) {
+        ws = empty_bytes_like(*q, a.workspace_bytes);
+        a.workspace = ws.mutable_data_ptr();
+      }
+      check(fox_paged_decode(&a, stream_of(*q)), "fox_paged_decode");
+    }
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // record_bounds(list or None)
 PyObject* py_record_bounds(PyObject*, PyObject* list) {
   if (list != Py_None && !PyList_Check(list)) {
@@ -855,6 +1362,12 @@ PyMethodDef methods[] = {
     {"attention", (PyCFunction)(void (*)(void))py_attention, METH_FASTCALL, nullptr},
     {"attention_norm_gate", (PyCFunction)(void (*)(void))py_attention_norm_gate, METH_FASTCALL, nullptr},
     {"norm", (PyCFunction)(void (*)(void))py_norm, METH_FASTCALL, nullptr},
+    {"rotary", (PyCFunction)(void (*)(void))py_rotary, METH_FASTCALL, nullptr},
+    {"qk_norm_rotary", (PyCFunction)(void (*)(void))py_qk_norm_rotary, METH_FASTCALL, nullptr},
+    {"page_slots", (PyCFunction)(void (*)(void))py_page_slots, METH_FASTCALL, nullptr},
+    {"page_release", (PyCFunction)(void (*)(void))py_page_release, METH_FASTCALL, nullptr},
+    {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
     {"token_shift", (PyCFunction)(void (*)(void))py_token_shift, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fox_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

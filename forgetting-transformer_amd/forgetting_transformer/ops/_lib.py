@@ -121,6 +121,57 @@ class Gates(C.Structure):
     ]
 
 
+class RotarySide(C.Structure):
+    _fields_ = [("H", C.c_int32), ("x", View), ("y", View), ("dx", View), ("weight", C.c_void_p)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("sides", C.c_int32), ("B", C.c_int32), ("T", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32),
+        ("rotary_dim", C.c_int32), ("interleaved", C.c_int32),
+        ("side", RotarySide * 2),
+        ("weight_stride_h", C.c_int64),
+        ("eps", C.c_float),
+        ("inv_freq", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("position_stride_b", C.c_int64), ("position_stride_t", C.c_int64), ("first_position", C.c_int64),
+        ("dweight", C.c_void_p),
+        ("workspace", C.c_void_p),
+    ]
+
+
+class Pages(C.Structure):
+    _fields_ = [
+        ("P", C.c_int32), ("H", C.c_int32), ("page_size", C.c_int32), ("D", C.c_int32), ("dtype", C.c_int32),
+        ("k", View), ("v", View),
+        ("g", C.c_void_p),
+        ("g_stride_p", C.c_int64), ("g_stride_h", C.c_int64), ("g_stride_t", C.c_int64),
+    ]
+
+
+class PageSlotsArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "W", "P", "page_size", "max_tokens")] + [
+        ("lengths", C.c_void_p), ("new_tokens", C.c_void_p), ("block_table", C.c_void_p), ("block_table_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("free_pages", "free_count", "slots", "positions", "requests", "keys", "lengths_out", "free_count_out", "granted")]
+
+
+class PageReleaseArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "W", "P", "page_size")] + [
+        ("lengths", C.c_void_p), ("done", C.c_void_p), ("block_table", C.c_void_p), ("block_table_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("free_pages", "free_count", "lengths_out", "free_count_out")]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [("pages", Pages), ("T", C.c_int32), ("k", View), ("v", View), ("g", C.c_void_p), ("g_stride_t", C.c_int64),
+                ("g_stride_h", C.c_int64), ("slots", C.c_void_p)]
+
+
+class PagedDecodeArgs(C.Structure):
+    _fields_ = [("pages", Pages), ("B", C.c_int32), ("requests_in_table", C.c_int32), ("W", C.c_int32), ("max_length", C.c_int32),
+                ("q", View), ("o", View), ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("lengths", C.c_void_p),
+                ("requests", C.c_void_p), ("sm_scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 # every symbol include/fox_attn.h declares: name -> (restype, argtypes)
 SIGNATURES = {
     "fox_version": (C.c_int, []),
@@ -165,6 +216,14 @@ SIGNATURES = {
     "fox_norm_gate_fwd": (C.c_int, [C.POINTER(NormGateArgs), C.c_void_p]),
     "fox_norm_gate_bwd": (C.c_int, [C.POINTER(NormGateArgs), C.c_void_p]),
     "fox_norm_gate_workspace_bytes": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
+    "fox_rotary_fwd": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
+    "fox_rotary_bwd": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
+    "fox_rotary_workspace_bytes": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
+    "fox_page_slots": (C.c_int, [C.POINTER(PageSlotsArgs), C.c_void_p]),
+    "fox_page_release": (C.c_int, [C.POINTER(PageReleaseArgs), C.c_void_p]),
+    "fox_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "fox_paged_decode": (C.c_int, [C.POINTER(PagedDecodeArgs), C.c_void_p]),
+    "fox_paged_decode_workspace_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.POINTER(C.c_int64)]),
     "fox_token_shift_fwd": (C.c_int, [C.POINTER(ShiftArgs), C.c_void_p]),
     "fox_token_shift_bwd": (C.c_int, [C.POINTER(ShiftArgs), C.c_void_p]),
 }

@@ -419,6 +419,130 @@ int fox_auto_threshold_scan(const fox_dims* dims, const fox_view* q, const fox_v
 /* Whether fox_auto_threshold_scan takes one launch for this shape. */
 int fox_auto_threshold_scan_one_launch(const fox_dims* dims, int32_t* yes);
 
+/*
+ * Position rotation of queries and keys, alone or behind their per-head RMS norms in one pass.  No kernel of the reference's layer does the
+ * two together; its rotation is model/forgetting_transformer/rotary.py:22-153, its norm layernorm.py:183-254.
+ *   n = x (no weight), or x * rstd * weight per head, rstd = 1/sqrt(mean_d x^2 + eps)
+ *   theta[b,t,i] = position[b,t] * inv_freq[i], i < rotary_dim / 2, in 64 bits
+ *   (a, b) -> (a cos theta - b sin theta, a sin theta + b cos theta) for the pairs (i, i + rotary_dim/2) of every head, or (2i, 2i+1) interleaved;
+ *   the other elements of the head stay as they are; everything in fp32, rounded once.
+ * A side is one 16-bit (B, T, H, D) tensor with views like q (stride_t the token's, stride_h the head's) and a head count of its own; two sides
+ * (queries and keys) share B, T, D and the positions, one side alone has sides = 1.  The weights are fp32, `weight_stride_h` = D apart for the
+ * heads or 0 where one row of D serves them all, on both sides or on neither.  D is one of 16, 32, 64, 128; rotary_dim is positive, at most D, even when interleaved and a
+ * multiple of 16 otherwise.  positions: int64 with element strides, or NULL for first_position, first_position + 1, ...
+ */
+typedef struct fox_rotary_side {
+  int32_t H;
+  fox_view x;             /* forward: input.  Backward: the forward's input (ignored without a norm) */
+  fox_view y;             /* forward: written.  Backward: gradient of the output, read */
+  fox_view dx;            /* backward only, written */
+  const float* weight;    /* NULL: no norm */
+} fox_rotary_side;
+
+typedef struct fox_rotary_args {
+  int32_t sides, B, T, D, dtype;
+  int32_t rotary_dim, interleaved;
+  fox_rotary_side side[2];
+  int64_t weight_stride_h;
+  float eps;
+  const double* inv_freq;     /* rotary_dim / 2 */
+  const int64_t* positions;
+  int64_t position_stride_b, position_stride_t, first_position;
+  float* dweight;             /* backward of the norms, written: of side 0 (H * D, or D shared), then of side 1 */
+  float* workspace;           /* backward of the norms: fox_rotary_workspace_bytes() bytes, 16-byte aligned */
+} fox_rotary_args;
+
+int fox_rotary_fwd(const fox_rotary_args* args, void* stream);
+/* dx of every side and, behind norms, dweight; the partial weight gradients are added in a fixed order. */
+int fox_rotary_bwd(const fox_rotary_args* args, void* stream);
+/* Scratch of the backward of the norms for B * T tokens and the heads of both sides together. */
+int fox_rotary_workspace_bytes(int64_t tokens, int32_t heads, int32_t D, int32_t shared_weight, int64_t* bytes);
+
+/*
+ * Serving from a pool of pages; the dense cache of the reference's layer is fgate_cache.py:5-203.  The pool holds P pages of page_size (a power of two, 8 to 4096) tokens: keys and
+ * values (P, H, page_size, D) and fp32 log forget gates (P, H, page_size).  block_table (requests, W) int32 names every request's pages in order: token i of a request is in
+ * slot page * page_size + i % page_size of the page block_table[request][i / page_size].  The free pages are a stack, free_pages[0 .. *free_count).
+ */
+typedef struct fox_pages {
+  int32_t P, H, page_size, D;
+  int32_t dtype;
+  fox_view k, v;              /* stride_b: from page to page, stride_t: from token to token inside one */
+  float* g;
+  int64_t g_stride_p, g_stride_h, g_stride_t;
+} fox_pages;
+
+/*
+ * Pages and slots of a step's new tokens, max_tokens of them, those of one request after those of the one before it: request b brings new_tokens[b] to the lengths[b]
+ * that it has cached.  slots, positions, requests and keys (max_tokens each) get every token's slot, its position in its request, the request and the tokens of it up to this one; new pages come from the top of the stack in
+ * request order and go into block_table.  A request is refused, whole, if its tokens end behind max_tokens, if it would need more than W pages, or if the stack
+ * does not hold its pages and those of the requests in front of it: its tokens get slot -1, request -1 and 0 keys, its length stays and granted[b] is 0.  Places behind the last token get slot -1,
+ * position 0, request -1, 0 keys.  lengths_out and free_count_out may be lengths and free_count (both, or neither).  At most 4096 requests.
+ */
+typedef struct fox_page_slots_args {
+  int32_t B, W, P, page_size, max_tokens;
+  const int32_t* lengths;
+  const int32_t* new_tokens;
+  int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* free_pages;  /* P places */
+  const int32_t* free_count;
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* requests;
+  int32_t* keys;
+  int32_t* lengths_out;
+  int32_t* free_count_out;
+  uint8_t* granted;
+} fox_page_slots_args;
+int fox_page_slots(const fox_page_slots_args* args, void* stream);
+
+/* The pages of the requests with done[b] != 0 go back onto the stack, in request order, and their lengths become 0. */
+typedef struct fox_page_release_args {
+  int32_t B, W, P, page_size;
+  const int32_t* lengths;
+  const uint8_t* done;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* lengths_out;
+  int32_t* free_count_out;
+} fox_page_release_args;
+int fox_page_release(const fox_page_release_args* args, void* stream);
+
+/* Keys, values (T, H, D) and log gates (T, H) of T tokens into their slots.  A token whose slot is not in the pool is left out; slots have to be distinct.  The stride_b of k and v is not used. */
+typedef struct fox_paged_append_args {
+  fox_pages pages;
+  int32_t T;
+  fox_view k, v;
+  const float* g;
+  int64_t g_stride_t, g_stride_h;
+  const int64_t* slots;
+} fox_paged_append_args;
+int fox_paged_append(const fox_paged_append_args* args, void* stream);
+
+/*
+ * One token per row b against the first lengths[b] keys of its request:
+ *   o[b,h,:] = sum_j p_j v_j / sum_j p_j,  p_j = exp(sm_scale q.k_j + sum of the log gates behind j, up to key lengths[b] - 1).
+ * The request of row b is requests[b], or b where that is NULL; a row without keys, or whose request is not in the table, gets zeros.  Keys on pages that the table does not name (entries outside
+ * 0 .. P - 1) are left out, their log gates count as 0.  max_length bounds the lengths (longer ones are cut to it); 0 = what the table holds.
+ * workspace holds fox_paged_decode_workspace_bytes() bytes, 16-byte aligned.
+ */
+typedef struct fox_paged_decode_args {
+  fox_pages pages;
+  int32_t B, requests_in_table, W, max_length;
+  fox_view q, o;              /* (B, H, D): stride_t is not used */
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* lengths;
+  const int32_t* requests;    /* or NULL */
+  float sm_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} fox_paged_decode_args;
+int fox_paged_decode(const fox_paged_decode_args* args, void* stream);
+int fox_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int64_t max_keys, int64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
