@@ -254,7 +254,7 @@ int make_rotary(const fox_rotary_args* a, fox::RotaryK& k, bool bwd) {
   if (a->sides != 1 && a->sides != 2) return fail(FOX_E_ARG, "sides must be 1 or 2 (got %d)", a->sides);
   FOX_TRY(check_head_dim(a->D));
   FOX_TRY(check_dtype16(a->dtype));
-  if (a->B <= 0 || a->T <= 0 || (int64_t)a->B * a->T > 0x7fffffffLL) return fail(FOX_E_ARG, "B and T must be positive and B * T below 2^31 (got %d, %d)", a->B, a->T);
+  if (a->B <= 0 || a->T <= 0 || (int64_t)a->B * a->T > (1 << 30)) return fail(FOX_E_ARG, "B and T must be positive and B * T at most 2^30 (got %d, %d)", a->B, a->T);
   const int step = a->interleaved ? 2 : 16;
   if (a->rotary_dim <= 0 || a->rotary_dim > a->D || a->rotary_dim % step)
     return fail(FOX_E_ARG, "rotary_dim must be a multiple of %d up to the head dim (got %d)", step, a->rotary_dim);
@@ -552,7 +552,7 @@ int fox_rotary_bwd(const fox_rotary_args* args, void* stream) {
 int fox_rotary_workspace_bytes(int64_t tokens, int32_t heads, int32_t D, int32_t shared_weight, int64_t* bytes) {
   if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
   FOX_TRY(check_head_dim(D));
-  if (tokens <= 0 || tokens > 0x7fffffffLL || heads <= 0 || heads > 2 * 65535) return fail(FOX_E_ARG, "tokens and heads must be positive");
+  if (tokens <= 0 || tokens > (1 << 30) || heads <= 0 || heads > 2 * 65535) return fail(FOX_E_ARG, "tokens and heads must be positive");
   *bytes = fox::rotary_workspace_floats(tokens, heads, D, shared_weight != 0) * (int64_t)sizeof(float);
   return FOX_OK;
 }

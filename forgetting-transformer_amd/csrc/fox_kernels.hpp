@@ -184,11 +184,11 @@ struct RotaryK {
   int N, T, R;               // N = B * T tokens
   int sign;                  // -1: the other way round
   float eps;
-  int cols, lanes, rows, tile, tiles;   // how the call is cut (rotary_plan), set by the launcher with the divisors
+  int cols, lanes, tile, tiles;   // how the call is cut (rotary_plan), set by the launcher with the divisors
   Divisor by_T, by_half, by_cols;
 };
-constexpr int kRotaryRows = 4;                          // tokens a thread holds at once
-template <int D> constexpr int kRotaryTile = 2048 / D;  // tokens whose angles a workgroup holds, at most: 8 KiB
+constexpr int kRotaryRows = 4;                          // tokens of a thread and tile
+template <int D> constexpr int kRotaryLanes = 512 / D;  // tokens a workgroup works on side by side, at most: their angles take 2 KiB of LDS
 
 // Pool of pages (fox_paged.hip): pages of 2^shift tokens, (P, H, S, D) keys and values as views with the stride between pages in sb, (P, H, S) log gates.
 struct PagesK {

@@ -365,17 +365,16 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const PagedDecodeK a)
       if (j >= KPB || end - 1 - j < first || page < 0) gx[s] = 0.f;
     }
     u32x4 kx[U], vx[U];
-    int64_t v_at[U];
     uint32_t ok = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int n0 = end - KPB + u * KPL + r, n = max(n0, first), page = page_of(n);   // keys left of the run read its first row and are masked below
       ok |= (uint32_t)(n0 >= first && page >= 0) << u;
-      kx[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + max(page, 0) * pg.k.sb + (n & in_page) * pg.k.st));
-      v_at[u] = max(page, 0) * pg.v.sb + (n & in_page) * pg.v.st;
+      const int64_t from = max(page, 0);
+      const int row = n & in_page;
+      kx[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + from * pg.k.sb + row * pg.k.st));
+      vx[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vp + from * pg.v.sb + row * pg.v.st));
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) vx[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vp + v_at[u]));
     if (__ballot(ok != (1u << U) - 1)) {   // what is masked may hold anything, NaN among it
 #pragma unroll
       for (int u = 0; u < U; ++u)

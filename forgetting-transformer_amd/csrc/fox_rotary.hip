@@ -13,6 +13,10 @@
 // forms them once per token, in 64 bits up to the fraction of a turn (a position of 2^20 would leave 32-bit angles 4 digits),
 // and keeps cosine and sine in LDS.  A thread owns one column (tensor, head, sixteen elements) and walks tokens, so the
 // weights are loaded once and their gradient stays in registers; partial gradients leave once per workgroup and are added in a fixed order.
+//
+// Rows are read through the caches, in which what the projections wrote a moment ago may still be, and written past them.  Norm and rotation, bf16 H16 D128, us by
+// loads / stores, both non-temporal, only the loads, neither, only the stores (as it is): forward B4 T512 10.1, 9.8, 8.6, 7.9, T1024 14.9, 15.2, 13.6, 12.4, T4096 48.8, 45.6, 47.1,
+// 48.8, T16384 179, 202, 178, 183; backward T512 24.7, 22.8, 21.6, 21.3, T4096 81.8, 74.6, 84.2, 68.5, T16384 315, 328, 332, 317 (5.9 and 5.1 TB/s).
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
 
@@ -74,18 +78,18 @@ __device__ __forceinline__ void make_angles(const RotaryK& a, int64_t n0, int to
 }
 
 // The lane's sixteen elements turned by the angles of its eight pairs; pairs outside the rotated part stay as they are
-// (not turned by zero: an infinite element would make its neighbour NaN).
+// (not turned by zero: an infinite element would make its neighbour NaN).  Halves: all of the lane's pairs or none.
 template <bool INTERLEAVED>
 __device__ __forceinline__ void turn(float (&f)[16], const float2* cs, int first_pair, int half) {
+  if (first_pair >= half) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int ia = INTERLEAVED ? 2 * e : e, ib = INTERLEAVED ? 2 * e + 1 : 8 + e;
-    if (first_pair + e < half) {
-      const float2 t = cs[first_pair + e];
-      const float x = f[ia], y = f[ib];
-      f[ia] = x * t.x - y * t.y;
-      f[ib] = x * t.y + y * t.x;
-    }
+    const float2 t = cs[first_pair + e];
+    const float x = f[ia], y = f[ib], a = x * t.x - y * t.y, b = x * t.y + y * t.x;
+    const bool in = !INTERLEAVED || first_pair + e < half;
+    f[ia] = in ? a : x;
+    f[ib] = in ? b : y;
   }
 }
 
@@ -94,13 +98,15 @@ __device__ __forceinline__ float head_sum(float x) {
   if constexpr (L > 1) return row_sum<L>(x);
   return x;
 }
+// 1 / sqrt(x) to an ulp, where 1.0f / sqrtf(x) is some thirty instructions (x is a mean square and eps)
+__device__ __forceinline__ float rsqrt_ulp(float x) { return __builtin_amdgcn_rsqf(x); }
 
 }  // namespace
 
-template <typename Tr, int D, bool NORM, bool INTERLEAVED>
+template <typename Tr, int D, bool NORM, bool INTERLEAVED, int ROWS>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
   constexpr int L = D / 16;
-  __shared__ float2 cs[kRotaryTile<D>][D / 2];
+  __shared__ float2 cs[ROWS * kRotaryLanes<D>][D / 2];
   const int tid = threadIdx.x;
   const int rl = a.cols > 256 ? 0 : divide(tid, a.by_cols);
   const int col = a.cols > 256 ? blockIdx.y * 256 + tid : tid - rl * a.cols;
@@ -117,24 +123,21 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
       w[8 + e] = wp[at.v1 * 8 + e];
     }
   }
-  u32x4 x0[kRotaryRows], x1[kRotaryRows];
-  int64_t to[kRotaryRows];
+  u32x4 x0[ROWS], x1[ROWS];
+  int64_t to[ROWS];
 #pragma unroll
-  for (int u = 0; u < kRotaryRows; ++u) {   // tokens past the end read the last one and are not stored
+  for (int u = 0; u < ROWS; ++u) {   // tokens past the end read the last one and are not stored
     const int n = (int)min(n0 + rl + (int64_t)u * a.lanes, (int64_t)a.N - 1);
     const int b = divide(n, a.by_T), t = n - b * a.T;
     const uint16_t* p = in.ptr + b * in.sb + t * in.st + at.h * in.sh;
     to[u] = b * out.sb + t * out.st + at.h * out.sh;
-    if (u == 0 || u < a.rows) {
-      x0[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v0 * 8));
-      x1[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v1 * 8));
-    }
+    x0[u] = *reinterpret_cast<const u32x4*>(p + at.v0 * 8);
+    x1[u] = *reinterpret_cast<const u32x4*>(p + at.v1 * 8);
   }
   make_angles<D>(a, n0, a.tile, cs);
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kRotaryRows; ++u) {
-    if (u > 0 && u >= a.rows) break;
+  for (int u = 0; u < ROWS; ++u) {
     const int tok = rl + u * a.lanes;
     float f[16];
     unpack8r<Tr>(x0[u], f);
@@ -143,24 +146,25 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
-      const float rstd = 1.0f / sqrtf(head_sum<L>(ss) / D + a.eps);
+      const float rstd = rsqrt_ulp(head_sum<L>(ss) * (1.0f / D) + a.eps);
 #pragma unroll
       for (int e = 0; e < 16; ++e) f[e] = f[e] * rstd * w[e];
     }
     if (live && n0 + tok < a.N) {
       turn<INTERLEAVED>(f, cs[tok], at.c * 8, a.R / 2);
       uint16_t* p = const_cast<uint16_t*>(out.ptr) + to[u];
-      *reinterpret_cast<u32x4*>(p + at.v0 * 8) = pack8r<Tr>(f);
-      *reinterpret_cast<u32x4*>(p + at.v1 * 8) = pack8r<Tr>(f + 8);
+      __builtin_nontemporal_store(pack8r<Tr>(f), reinterpret_cast<u32x4*>(p + at.v0 * 8));
+      __builtin_nontemporal_store(pack8r<Tr>(f + 8), reinterpret_cast<u32x4*>(p + at.v1 * 8));
     }
   }
 }
 
-// Gradient of the norm and the rotation behind it.  A workgroup walks a strip of `tiles` tiles of tokens.
+// Gradient of the norm and the rotation behind it.  A workgroup walks a strip of `tiles` tiles, kRotaryRows tokens of a thread each: a barrier and new angles
+// per tile, and always the rows of the next token on their way while those of one are used.
 template <typename Tr, int D, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
+__global__ __launch_bounds__(256, 3) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
   constexpr int L = D / 16;
-  __shared__ float2 cs[2][kRotaryTile<D>][D / 2];   // the next tile's angles are made while others still read this one's
+  __shared__ float2 cs[2][kRotaryRows * kRotaryLanes<D>][D / 2];
   __shared__ __align__(16) float dw_s[256 * 16];
   const int tid = threadIdx.x;
   const int rl = a.cols > 256 ? 0 : divide(tid, a.by_cols);
@@ -181,56 +185,66 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(const RotaryK a
 #pragma unroll
   for (int e = 0; e < 16; ++e) dw[e] = 0.f;
 
-  for (int i = 0; i < a.tiles; ++i) {
-    const int64_t n0 = ((int64_t)blockIdx.x * a.tiles + i) * a.tile;
-    if (n0 >= a.N) break;   // (the same for the whole workgroup)
-    u32x4 x0[kRotaryRows], x1[kRotaryRows], g0[kRotaryRows], g1[kRotaryRows];
-    int64_t to[kRotaryRows];
+  struct Row {
+    u32x4 x0, x1, g0, g1;
+  };
+  auto load = [&](Row& r, int n) {   // tokens past the end read the last one and count for nothing
+    n = min(n, a.N - 1);
+    const int b = divide(n, a.by_T), t = n - b * a.T;
+    const uint16_t* p = xv.ptr + b * xv.sb + t * xv.st + at.h * xv.sh;
+    const uint16_t* g = in.ptr + b * in.sb + t * in.st + at.h * in.sh;
+    r.x0 = *reinterpret_cast<const u32x4*>(p + at.v0 * 8);
+    r.x1 = *reinterpret_cast<const u32x4*>(p + at.v1 * 8);
+    r.g0 = *reinterpret_cast<const u32x4*>(g + at.v0 * 8);
+    r.g1 = *reinterpret_cast<const u32x4*>(g + at.v1 * 8);
+  };
+  auto use = [&](const Row& r, int n, const float2* angles) {
+    float x[16], g[16];
+    unpack8r<Tr>(r.x0, x);
+    unpack8r<Tr>(r.x1, x + 8);
+    unpack8r<Tr>(r.g0, g);
+    unpack8r<Tr>(r.g1, g + 8);
+    turn<INTERLEAVED>(g, angles, at.c * 8, a.R / 2);
+    float ss = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int u = 0; u < kRotaryRows; ++u) {
-      const int n = (int)min(n0 + rl + (int64_t)u * a.lanes, (int64_t)a.N - 1);
-      const int b = divide(n, a.by_T), t = n - b * a.T;
-      const uint16_t* p = xv.ptr + b * xv.sb + t * xv.st + at.h * xv.sh;
-      const uint16_t* g = in.ptr + b * in.sb + t * in.st + at.h * in.sh;
-      to[u] = b * out.sb + t * out.st + at.h * out.sh;
-      x0[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v0 * 8));
-      x1[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + at.v1 * 8));
-      g0[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(g + at.v0 * 8));
-      g1[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(g + at.v1 * 8));
+    for (int e = 0; e < 16; ++e) {
+      ss += x[e] * x[e];
+      s1 += g[e] * w[e] * x[e];
     }
-    make_angles<D>(a, n0, a.tile, cs[i & 1]);
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kRotaryRows; ++u) {
-      const int tok = rl + u * a.lanes;
-      const bool here = live && n0 + tok < a.N;
-      float x[16], g[16];
-      unpack8r<Tr>(x0[u], x);
-      unpack8r<Tr>(x1[u], x + 8);
-      unpack8r<Tr>(g0[u], g);
-      unpack8r<Tr>(g1[u], g + 8);
-      turn<INTERLEAVED>(g, cs[i & 1][here ? tok : 0], at.c * 8, a.R / 2);
-      float ss = 0.f, s1 = 0.f;
+    const float rstd = rsqrt_ulp(head_sum<L>(ss) * (1.0f / D) + a.eps);
+    const float c1 = head_sum<L>(s1) * rstd * (1.0f / D);
+    if (live && n < a.N) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        ss += x[e] * x[e];
-        s1 += g[e] * w[e] * x[e];
+        const float xhat = x[e] * rstd;
+        dw[e] += g[e] * xhat;
+        g[e] = (g[e] * w[e] - xhat * c1) * rstd;
       }
-      const float rstd = 1.0f / sqrtf(head_sum<L>(ss) / D + a.eps);
-      const float c1 = head_sum<L>(s1) * rstd * (1.0f / D);
-      if (here) {
-        float dx[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float xhat = x[e] * rstd;
-          dw[e] += g[e] * xhat;
-          dx[e] = (g[e] * w[e] - xhat * c1) * rstd;
-        }
-        uint16_t* p = const_cast<uint16_t*>(out.ptr) + to[u];
-        *reinterpret_cast<u32x4*>(p + at.v0 * 8) = pack8r<Tr>(dx);
-        *reinterpret_cast<u32x4*>(p + at.v1 * 8) = pack8r<Tr>(dx + 8);
-      }
+      const int b = divide(n, a.by_T), t = n - b * a.T;
+      uint16_t* p = const_cast<uint16_t*>(out.ptr) + b * out.sb + t * out.st + at.h * out.sh;
+      __builtin_nontemporal_store(pack8r<Tr>(g), reinterpret_cast<u32x4*>(p + at.v0 * 8));
+      __builtin_nontemporal_store(pack8r<Tr>(g + 8), reinterpret_cast<u32x4*>(p + at.v1 * 8));
     }
+  };
+
+  const int start = blockIdx.x * a.tiles * a.tile, stop = min(start + a.tiles * a.tile, a.N);   // (N is at most 2^30)
+  Row even, odd;
+  load(even, start + rl);
+  make_angles<D>(a, start, a.tile, cs[0]);
+  __syncthreads();
+  int buf = 0;
+  for (int n0 = start; n0 < stop; n0 += a.tile, buf ^= 1) {   // (the same steps in the whole workgroup)
+    if (n0 + a.tile < stop) make_angles<D>(a, n0 + a.tile, a.tile, cs[buf ^ 1]);
+#pragma unroll
+    for (int u = 0; u < kRotaryRows; u += 2) {
+      const int tok = rl + u * a.lanes;
+      const float2* angles = cs[buf][live ? tok : 0];
+      load(odd, n0 + tok + a.lanes);
+      use(even, n0 + tok, angles);
+      load(even, n0 + tok + 2 * a.lanes);   // (of the next tile behind this one's last)
+      use(odd, n0 + tok + a.lanes, cs[buf][live ? tok + a.lanes : 0]);
+    }
+    __syncthreads();
   }
 
   // the workgroup's sums in element order: row lanes, and with shared weights heads, one after the other
@@ -266,25 +280,24 @@ __global__ __launch_bounds__(256) void qk_norm_rotary_bwd_kernel(const RotaryK a
 }
 
 namespace {
-// How a call over `tokens` tokens is cut: columns, row lanes of a workgroup, tokens a thread holds, tokens a tile, tiles a workgroup.
+// How a call over `tokens` tokens is cut: columns, workgroups' worth of them, row lanes of a workgroup, tokens a thread holds, tokens a tile, tiles a workgroup.
 struct RotaryPlan {
   int cols, chunks, lanes, rows, tile, tiles;
   int64_t strips;
 };
 RotaryPlan rotary_plan(int64_t tokens, int heads, int D, bool bwd) {
   RotaryPlan p;
-  const int most = 2048 / D / kRotaryRows;   // what the angles in LDS have room for (kRotaryTile)
   p.cols = heads * (D / 16);
   p.chunks = (p.cols + 255) / 256;
   p.lanes = p.cols > 256 ? 1 : 256 / p.cols;
-  if (p.lanes > most) p.lanes = most;
-  // four tokens a thread and tile, fewer where a forward would not make four workgroups a CU
-  const int64_t rows = tokens * p.chunks / ((int64_t)p.lanes * 4 * kCus);
-  p.rows = bwd || rows > kRotaryRows ? kRotaryRows : rows < 1 ? 1 : (int)rows;
+  if (p.lanes > 512 / D) p.lanes = 512 / D;   // kRotaryLanes
+  // forward: four tokens a thread where that still makes four workgroups a CU
+  p.rows = bwd || tokens * p.chunks >= (int64_t)p.lanes * kRotaryRows * 4 * kCus ? kRotaryRows : 1;
   p.tile = p.lanes * p.rows;
-  const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? tiles * p.chunks / (4 * kCus) : 1;
-  p.tiles = (int)(per < 1 ? 1 : per);
-  p.strips = (tiles + p.tiles - 1) / p.tiles;
+  // backward: strips for three workgroups a CU, what its registers leave room for
+  const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? (tiles * p.chunks + 3 * kCus - 1) / (3 * kCus) : 1;
+  p.tiles = (int)per;
+  p.strips = (tiles + per - 1) / per;
   return p;
 }
 }  // namespace
@@ -302,7 +315,6 @@ static hipError_t launch_rotary_d(const RotaryK& args, bool norm, bool interleav
   const RotaryPlan p = rotary_plan(a.N, heads, D, bwd);
   a.cols = p.cols;
   a.lanes = p.lanes;
-  a.rows = p.rows;
   a.tile = p.tile;
   a.tiles = p.tiles;
   a.by_T = divisor(a.T);
@@ -310,10 +322,16 @@ static hipError_t launch_rotary_d(const RotaryK& args, bool norm, bool interleav
   a.by_cols = divisor(p.cols);
   const dim3 grid((unsigned)p.strips, (unsigned)p.chunks), block(p.cols > 256 ? 256u : (unsigned)((p.cols * p.lanes + 63) / 64 * 64));
   if (!bwd) {
-    if (norm && interleaved) hipLaunchKernelGGL((rotary_kernel<Tr, D, true, true>), grid, block, 0, s, a);
-    else if (norm) hipLaunchKernelGGL((rotary_kernel<Tr, D, true, false>), grid, block, 0, s, a);
-    else if (interleaved) hipLaunchKernelGGL((rotary_kernel<Tr, D, false, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((rotary_kernel<Tr, D, false, false>), grid, block, 0, s, a);
+    auto launch = [&](auto n, auto i) {
+      if (p.rows == 1) hipLaunchKernelGGL((rotary_kernel<Tr, D, decltype(n)::value, decltype(i)::value, 1>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((rotary_kernel<Tr, D, decltype(n)::value, decltype(i)::value, kRotaryRows>), grid, block, 0, s, a);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    if (norm && interleaved) launch(yes, yes);
+    else if (norm) launch(yes, no);
+    else if (interleaved) launch(no, yes);
+    else launch(no, no);
     return hipGetLastError();
   }
   if (interleaved) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<Tr, D, true>), grid, block, 0, s, a);

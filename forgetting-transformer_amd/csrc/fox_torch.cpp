@@ -580,6 +580,14 @@ Tensor run_rotary(const Rotary& r, const Tensor& x, bool back) {
 // As the kernels take it, copied where it is not (contiguous() would hand a tensor back that merely starts at an odd address).
 Tensor aligned(const Tensor& t) { return vectors_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+// A contiguous tensor in a part of another's memory, for results that come from one allocation (a view through the dispatcher takes longer than an allocation).
+Tensor part_of(const Tensor& whole, int64_t byte, at::IntArrayRef sizes, at::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(byte / (int64_t)c10::elementSize(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 struct RotaryNode : public torch::autograd::Function<RotaryNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& inv_freq, const std::optional<Tensor>& positions, const Rotary* r, bool back) {
     ctx->save_for_backward({inv_freq, positions.value_or(Tensor())});
@@ -628,6 +636,7 @@ struct QkNormRotaryNode : public torch::autograd::Function<QkNormRotaryNode> {
   }
   // The kernels read the weights as aligned fp32 rows.
   static Tensor weights(const Tensor& w) {
+    if (w.scalar_type() == at::kFloat && w.is_contiguous() && !(reinterpret_cast<uintptr_t>(w.const_data_ptr()) & 15)) return w;
     Tensor t = w.detach().to(at::kFloat).contiguous();
     return reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15 ? t.clone() : t;
   }
@@ -671,8 +680,11 @@ struct QkNormRotaryNode : public torch::autograd::Function<QkNormRotaryNode> {
       a.workspace = (float*)ws.mutable_data_ptr();
       check(fox_rotary_bwd(&a, stream_of(q)), "fox_rotary_bwd");
     }
-    return {dq, dk, dw.narrow(0, 0, nq).to((at::ScalarType)ctx->saved_data["wqtype"].toInt()),
-            dw.narrow(0, nq, nk).to((at::ScalarType)ctx->saved_data["wktype"].toInt()), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto tq = (at::ScalarType)ctx->saved_data["wqtype"].toInt(), tk = (at::ScalarType)ctx->saved_data["wktype"].toInt();
+    Tensor dwq = part_of(dw, 0, {nq}, at::kFloat), dwk = part_of(dw, 4 * nq, {nk}, at::kFloat);
+    if (tq != at::kFloat) dwq = dwq.to(tq);
+    if (tk != at::kFloat) dwk = dwk.to(tk);
+    return {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -1001,7 +1013,7 @@ bool parse_rotary(Rotary& r, const Tensor& x, PyObject* inv_freq, PyObject* posi
   const Tensor* f = tensor_of(inv_freq);
   if (!f || f->dim() != 1 || f->scalar_type() != at::kDouble || f->device() != x.device() || !f->is_contiguous() || f->requires_grad()) return false;
   const int64_t R = 2 * f->size(0), B = x.size(0), T = x.size(r.head_first ? 2 : 1);
-  if (R < 2 || R > x.size(3) || (!r.interleaved && R % 16) || B * T > INT32_MAX || x.size(r.head_first ? 1 : 2) > 65535) return false;
+  if (R < 2 || R > x.size(3) || (!r.interleaved && R % 16) || B * T > (1 << 30) || x.size(r.head_first ? 1 : 2) > 65535) return false;
   r.inv_freq = *f;
   if (positions == Py_None) return true;
   if (PyLong_Check(positions) && !PyBool_Check(positions)) {
@@ -1139,10 +1151,15 @@ PyObject* py_page_slots(PyObject*, PyObject* const* o, Py_ssize_t n) {
   {
     const pybind11::gil_scoped_release no_gil;
     const at::NoGradGuard no_grad;
-    for (int i = 0; i < 4; ++i) out[i] = at::empty({T}, lengths->options().dtype(i < 2 ? at::kLong : at::kInt));
-    out[4] = in_place ? *lengths : at::empty_like(*lengths);
-    out[5] = in_place ? *count : at::empty_like(*count);
-    out[6] = at::empty(lengths->sizes(), lengths->options().dtype(at::kBool));
+    const int64_t B = lengths->size(0);
+    const auto up = [](int64_t bytes) { return (bytes + 15) / 16 * 16; };
+    const int64_t longs = up(8 * T), ints = up(4 * T), state = up(4 * B);
+    Tensor all = empty_bytes_like(*lengths, 2 * longs + 2 * ints + state + 16 + up(B));   // one allocation
+    for (int i = 0; i < 4; ++i) out[i] = part_of(all, i < 2 ? i * longs : 2 * longs + (i - 2) * ints, {T}, i < 2 ? at::kLong : at::kInt);
+    const int64_t at_state = 2 * longs + 2 * ints;
+    out[4] = in_place ? *lengths : part_of(all, at_state, {B}, at::kInt);
+    out[5] = in_place ? *count : part_of(all, at_state + state, {1}, at::kInt);
+    out[6] = part_of(all, at_state + state + 16, {B}, at::kBool);
     fox_page_slots_args a{};
     a.B = (int32_t)lengths->size(0);
     a.W = (int32_t)table->size(1);
@@ -1195,8 +1212,11 @@ PyObject* py_page_release(PyObject*, PyObject* const* o, Py_ssize_t n) {
   {
     const pybind11::gil_scoped_release no_gil;
     const at::NoGradGuard no_grad;
-    out[0] = in_place ? *lengths : at::empty_like(*lengths);
-    out[1] = in_place ? *count : at::empty_like(*count);
+    const int64_t B = lengths->size(0), state = (4 * B + 15) / 16 * 16;
+    Tensor all;
+    if (!in_place) all = empty_bytes_like(*lengths, state + 16);
+    out[0] = in_place ? *lengths : part_of(all, 0, {B}, at::kInt);
+    out[1] = in_place ? *count : part_of(all, state, {1}, at::kInt);
     fox_page_release_args a{};
     a.B = (int32_t)lengths->size(0);
     a.W = (int32_t)table->size(1);

@@ -69,6 +69,7 @@ def _check_heads(t: torch.Tensor, name: str) -> torch.Tensor:
 def _check_angles(x, inv_freq, positions, interleaved, head_first):
     """Frequencies and positions as the kernels take them."""
     B, T = x.shape[0], x.shape[2 if head_first else 1]
+    assert B * T <= 1 << 30 and x.shape[1 if head_first else 2] <= 65535, "at most 2**30 tokens of 65535 heads"
     assert inv_freq.dim() == 1 and inv_freq.is_floating_point(), "inv_freq must be a floating (rotary_dim / 2,) tensor"
     assert not inv_freq.requires_grad, "the frequencies have no gradient"
     R, step = 2 * inv_freq.shape[0], 2 if interleaved else 16
