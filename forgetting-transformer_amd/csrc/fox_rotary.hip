@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
 // Gradient of the norm and the rotation behind it.  A workgroup walks a strip of `tiles` tiles, kRotaryRows tokens of a thread each: a barrier and new angles
 // per tile, and always the rows of the next token on their way while those of one are used.
 template <typename Tr, int D, bool INTERLEAVED>
-__global__ __launch_bounds__(256, 3) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
+__global__ __launch_bounds__(256, 2) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
   constexpr int L = D / 16;
   __shared__ float2 cs[2][kRotaryRows * kRotaryLanes<D>][D / 2];
   __shared__ __align__(16) float dw_s[256 * 16];
@@ -294,8 +294,8 @@ RotaryPlan rotary_plan(int64_t tokens, int heads, int D, bool bwd) {
   // forward: four tokens a thread where that still makes four workgroups a CU
   p.rows = bwd || tokens * p.chunks >= (int64_t)p.lanes * kRotaryRows * 4 * kCus ? kRotaryRows : 1;
   p.tile = p.lanes * p.rows;
-  // backward: strips for three workgroups a CU, what its registers leave room for
-  const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? (tiles * p.chunks + 3 * kCus - 1) / (3 * kCus) : 1;
+  // backward: strips for two workgroups a CU, at once; as many partial weight gradients as one launch adds
+  const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? (tiles * p.chunks + 2 * kCus - 1) / (2 * kCus) : 1;
   p.tiles = (int)per;
   p.strips = (tiles + per - 1) / per;
   return p;
