@@ -616,7 +616,8 @@ int fox_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int64_t ma
   if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
   FOX_TRY(check_head_dim(D));
   if (B <= 0 || H <= 0 || (int64_t)B * H > (1 << 24) || max_keys <= 0 || max_keys > (1 << 30)) return fail(FOX_E_ARG, "B, H and max_keys must be positive, B * H at most 2^24, max_keys at most 2^30");
-  *bytes = fox::paged_decode_rows(B, H, (int)max_keys, D) * (int64_t)(D * sizeof(float) + sizeof(fox::DecodePartial));
+  const int64_t rows = fox::paged_decode_rows(B, H, (int)max_keys, D);
+  *bytes = rows ? rows * (int64_t)(D * sizeof(float) + sizeof(fox::DecodePartial)) + B * (int64_t)sizeof(fox::PagedRow) : 0;
   return FOX_OK;
 }
 
@@ -645,9 +646,11 @@ int fox_paged_decode(const fox_paged_decode_args* a, void* stream) {
   k.B = a->B; k.H = H; k.R = a->requests_in_table; k.W = a->W;
   k.sm_scale = a->sm_scale;
   k.by_heads = fox::divisor(H);
-  k.pieces = fox::paged_decode_pieces(a->B, H, k.max_keys, D);
-  k.ws_o = (float*)a->workspace;
-  k.ws_p = (fox::DecodePartial*)((char*)a->workspace + fox::paged_decode_rows(a->B, H, k.max_keys, D) * (int64_t)(D * sizeof(float)));
+  if (const int64_t rows = fox::paged_decode_rows(a->B, H, k.max_keys, D)) {
+    k.ws_o = (float*)a->workspace;
+    k.ws_p = (fox::DecodePartial*)(k.ws_o + rows * D);
+    k.ws_row = (fox::PagedRow*)(k.ws_p + rows);
+  }
   return check_hip(fox::launch_paged_decode(k, D, a->pages.dtype, (hipStream_t)stream), "fox_paged_decode");
 }
 

@@ -232,6 +232,9 @@ struct PagedAppendK {
   int64_t total;                         // 16-byte pieces of k
   Divisor by_heads;
 };
+struct PagedRow {                        // of a row: its first piece among all of one head, and how many it has
+  int32_t first, pieces;
+};
 // One new token per row against the pages of its request (paged_decode_kernel).
 struct PagedDecodeK {
   PagesK pages;
@@ -242,11 +245,12 @@ struct PagedDecodeK {
   int64_t table_sb;
   const int32_t *lengths, *requests;     // (B); requests null: row b of the table
   int B, H, R, W, max_keys;              // keys of a request, at most
-  int pieces;                            // of all requests and heads together, about
   float sm_scale;
   Divisor by_heads;
   float* ws_o;                           // (rows, D) partial accumulators and
   DecodePartial* ws_p;                   // their sums, a row per piece: paged_decode_rows
+  PagedRow* ws_row;                      // (B); null where nothing is split
+  double per_piece;                      // 1 / the pieces of all rows and heads together, about; set by the launcher
 };
 
 // Tile sizes (see fox_tile_config in the public header)
@@ -384,7 +388,6 @@ hipError_t launch_page_slots(const PageSlotsK& a, hipStream_t s);
 hipError_t launch_page_release(const PageReleaseK& a, hipStream_t s);
 hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s);
 hipError_t launch_paged_decode(const PagedDecodeK& a, int D, int dtype, hipStream_t s);
-int paged_decode_pieces(int B, int H, int max_keys, int D);
 int64_t paged_decode_rows(int B, int H, int max_keys, int D);   // of workspace; 0: no request is split
 int64_t rotary_workspace_floats(int64_t tokens, int heads, int D, bool shared);
 hipError_t launch_shift_fwd(const ShiftK& a, int D, int dtype, hipStream_t s);

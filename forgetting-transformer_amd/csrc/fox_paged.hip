@@ -215,7 +215,7 @@ hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s) {
 // so every gate is read once.
 //
 // How long the requests are only the device knows.  Every wave works out the same plan from the lengths: batches of four waves' loads, at
-// most `pieces` pieces of c batches over all requests and heads together, so that requests of very different lengths still give the
+// most kPagedPieces pieces of c batches over all requests and heads together, so that requests of very different lengths still give the
 // workgroups the same share; a workgroup past the last piece ends.
 //
 // A lane holds the table's entry for one of 64 consecutive pages and takes a row's page from the lane that has it; the entries are read again every 64 pages.
@@ -263,23 +263,37 @@ __device__ __forceinline__ PagedShare share_of(const PagedDecodeK& a, int b, int
   return s;
 }
 
-// Batches a piece so that all rows and heads together make about a.pieces of them.  Executed by whole waves.
+// Batches a piece.  All rows and heads together make at most about kPagedPieces of them; short rows stay whole where splitting them brings no more than a merge and starts of
+// workgroups.  Both ways in us, from the batches that each of the 1024 workgroups that run at once gets (`load`): 10 for the bytes of one batch each at 6.5 TB/s or 1.8 for each
+// of a run's round trips, 3 for every 1024 workgroups that start, 1.5 for the merge, 3 a batch for the longest rows' tail.  Pages of 16, us, split / as it is now: D 64, 512 requests and heads of
+// 300 keys 14.6 / 12.0, 1024 of them 25.4 / 19.0, 512 of 700 23.6 / 20.4, D 128, 512 of 150 to 300 18.7 / 16.1, 1024 of 300 39.7 / 32.4.  Executed by whole waves.
 template <int D>
 __device__ __forceinline__ int batches_per_piece(const PagedDecodeK& a, int lane) {
-  double nb = 0;
-  for (int b = lane; b < a.B; b += 64) nb += (keys_of(a, b) + paged_batch(D) - 1) / paged_batch(D);
-  const double total = of_lane(wave_scan(nb), 63) * a.H;
-  return (int)ceil(total / a.pieces);
+  double sum = 0;
+  int most = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const int nb = (keys_of(a, b) + paged_batch(D) - 1) / paged_batch(D);
+    sum += nb;
+    most = max(most, nb);
+  }
+  const double total = of_lane(wave_scan(sum), 63);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+  const int c = max((int)ceil(total * a.H * a.per_piece), 1);
+  if (most <= c || most > 8) return c;
+  const float load = (float)total * a.H / 1024.f, rows = (float)a.B * a.H / 1024.f, full = (float)total / ((float)a.B * most);
+  const float split = fmaxf(10.f * load, 1.8f * c) + 3.f * fmaxf(load / c, 1.f) + 1.5f;
+  const float whole = fmaxf(10.f * load, 1.8f * most) + 3.f * fmaxf(rows, 1.f) + 3.f * (most - 1) * (1.f - full);
+  return __builtin_amdgcn_readfirstlane(whole < split ? most : c);
 }
 
 struct PagedPiece {
   int b, piece, first;   // row, its piece, and the row's first piece among all (of one head)
   PagedShare share;
 };
-// The row that piece number p (of one head) belongs to, or the row `row` where that is not negative.  b < 0: there is none.  The result is
-// the same in all lanes.
+// The row that piece number p (of one head) belongs to; b < 0: there is none.  The result is the same in all lanes, and in all workgroups, which run this same code.
 template <int D>
-__device__ __forceinline__ PagedPiece find_piece(const PagedDecodeK& a, int p, int row, int lane) {
+__device__ __forceinline__ PagedPiece find_piece(const PagedDecodeK& a, int p, int lane) {
   const int per_piece = batches_per_piece<D>(a, lane);
   int before = 0;
   PagedPiece r;
@@ -287,7 +301,7 @@ __device__ __forceinline__ PagedPiece find_piece(const PagedDecodeK& a, int p, i
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const PagedShare s = share_of<D>(a, b0 + lane, per_piece);
     const int pieces = b0 + lane < a.B ? s.pieces : 0, end = before + (int)wave_scan(pieces), first = end - pieces;
-    const uint64_t hit = __ballot(row >= 0 ? b0 + lane == row : pieces > 0 && first <= p && p < end);
+    const uint64_t hit = __ballot(first <= p && p < end);
     if (hit) {
       const int from = __ffsll((unsigned long long)hit) - 1;
       r.b = b0 + from;
@@ -320,8 +334,9 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const PagedDecodeK a)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ch = lane % LPR, r = lane / LPR;
   const int number = divide(blockIdx.x, a.by_heads), h = blockIdx.x - number * a.H;
-  const PagedPiece at = find_piece<D>(a, number, -1, lane);
+  const PagedPiece at = find_piece<D>(a, number, lane);
   if (at.b < 0) return;   // (the same in all waves)
+  if (a.ws_row && at.piece == 0 && h == 0 && tid == 0) a.ws_row[at.b] = PagedRow{at.first, at.share.pieces};   // for the merge
   const int b = at.b;
   const PagesK& pg = a.pages;
   const int32_t* table = a.table + (a.requests ? a.requests[b] : b) * a.table_sb;
@@ -364,16 +379,23 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const PagedDecodeK a)
       gx[s] = gp[max(page, 0) * pg.g_sp + (n & in_page) * pg.g_ss];
       if (j >= KPB || end - 1 - j < first || page < 0) gx[s] = 0.f;
     }
+    // The fences keep one row's addresses in registers at a time: 119 to 127 registers, four workgroups a CU (131 to 135 and three at head dims 32 and 64 without them, 36 shapes geomean 1.036 of the time; all rows' pages asked
+    // for first, since a page takes as long as an LDS read).
     u32x4 kx[U], vx[U];
     uint32_t ok = 0;
+    int pages[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) pages[u] = page_of(max(end - KPB + u * KPL + r, first));   // keys left of the run read its first row and are masked below
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int n0 = end - KPB + u * KPL + r, n = max(n0, first), page = page_of(n);   // keys left of the run read its first row and are masked below
-      ok |= (uint32_t)(n0 >= first && page >= 0) << u;
-      const int64_t from = max(page, 0);
-      const int row = n & in_page;
+      const int n0 = end - KPB + u * KPL + r;
+      ok |= (uint32_t)(n0 >= first && pages[u] >= 0) << u;
+      const int64_t from = max(pages[u], 0);
+      const int row = max(n0, first) & in_page;
       kx[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp + from * pg.k.sb + row * pg.k.st));
       vx[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(vp + from * pg.v.sb + row * pg.v.st));
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (__ballot(ok != (1u << U) - 1)) {   // what is masked may hold anything, NaN among it
 #pragma unroll
@@ -472,8 +494,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedDecodeK a) 
   __shared__ float l_tot;
   __shared__ __align__(16) float part[GROUPS][D];
   const int tid = threadIdx.x, b = divide(blockIdx.x, a.by_heads), h = blockIdx.x - b * a.H;
-  const PagedPiece at = find_piece<D>(a, 0, b, tid & 63);
-  const int pieces = at.share.pieces;
+  const PagedRow at = a.ws_row[b];   // (written there, not worked out again: another kernel's arithmetic need not round alike)
+  const int pieces = at.pieces;
   if (pieces <= 1) return;   // written where it was computed
   const int grp = tid / TPR, d = (tid % TPR) * 4;
   const int64_t row0 = (int64_t)at.first * a.H + h;
@@ -513,8 +535,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedDecodeK a) 
   *reinterpret_cast<u32x2*>(a.o + b * a.o_sb + h * a.o_sh + d) = w;
 }
 
-// Pieces of all rows and heads together: about eight workgroups a CU.
-int paged_decode_pieces(int B, int H, int max_keys, int D) { return 8 * kCus; }
+// Pieces of all rows and heads together, about: eight workgroups a CU.  4, 6, 12 and 16 instead of 8: geomean of 36 shapes 1.014, 1.010, 1.004, 1.011 of the time.
+constexpr int kPagedPieces = 8 * kCus;
 
 static int64_t most_pieces(int max_keys, int D) {   // of a row
   const int64_t batches = ((int64_t)max_keys + paged_batch(D) - 1) / paged_batch(D);
@@ -522,13 +544,15 @@ static int64_t most_pieces(int max_keys, int D) {   // of a row
 }
 // Workgroups: no row makes more pieces than its share of `pieces` and one for what is left over.
 static int64_t paged_decode_workgroups(int B, int H, int max_keys, int D) {
-  const int64_t by_row = (int64_t)B * H * most_pieces(max_keys, D), shared = paged_decode_pieces(B, H, max_keys, D) + (int64_t)B * H;
+  const int64_t by_row = (int64_t)B * H * most_pieces(max_keys, D), shared = kPagedPieces + (int64_t)B * H;
   return by_row < shared ? by_row : shared;
 }
 int64_t paged_decode_rows(int B, int H, int max_keys, int D) { return most_pieces(max_keys, D) > 1 ? paged_decode_workgroups(B, H, max_keys, D) : 0; }
 
 template <typename Tr, int D>
-static hipError_t launch_paged_decode_d(const PagedDecodeK& a, hipStream_t s) {
+static hipError_t launch_paged_decode_d(const PagedDecodeK& args, hipStream_t s) {
+  PagedDecodeK a = args;
+  a.per_piece = 1.0 / kPagedPieces;
   hipLaunchKernelGGL((paged_decode_kernel<Tr, D>), dim3((unsigned)paged_decode_workgroups(a.B, a.H, a.max_keys, D)), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || most_pieces(a.max_keys, D) <= 1) return e;
