@@ -617,7 +617,7 @@ int fox_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int64_t ma
   FOX_TRY(check_head_dim(D));
   if (B <= 0 || H <= 0 || (int64_t)B * H > (1 << 24) || max_keys <= 0 || max_keys > (1 << 30)) return fail(FOX_E_ARG, "B, H and max_keys must be positive, B * H at most 2^24, max_keys at most 2^30");
   const int64_t rows = fox::paged_decode_rows(B, H, (int)max_keys, D);
-  *bytes = rows ? rows * (int64_t)(D * sizeof(float) + sizeof(fox::DecodePartial)) + B * (int64_t)sizeof(fox::PagedRow) : 0;
+  *bytes = rows ? rows * (int64_t)(D * sizeof(float) + sizeof(fox::DecodePartial)) + (B + 1) * (int64_t)sizeof(fox::PagedRow) : 0;
   return FOX_OK;
 }
 

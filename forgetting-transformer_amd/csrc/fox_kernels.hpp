@@ -249,7 +249,8 @@ struct PagedDecodeK {
   Divisor by_heads;
   float* ws_o;                           // (rows, D) partial accumulators and
   DecodePartial* ws_p;                   // their sums, a row per piece: paged_decode_rows
-  PagedRow* ws_row;                      // (B); null where nothing is split
+  PagedRow* ws_row;                      // (B + 1); null where no row can be more than one piece
+  bool planned;                          // ws_row is filled by a launch in front, set by the launcher
   double per_piece;                      // 1 / the pieces of all rows and heads together, about; set by the launcher
 };
 

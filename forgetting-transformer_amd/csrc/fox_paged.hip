@@ -216,7 +216,7 @@ hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s) {
 //
 // How long the requests are only the device knows.  Every wave works out the same plan from the lengths: batches of four waves' loads, at
 // most kPagedPieces pieces of c batches over all requests and heads together, so that requests of very different lengths still give the
-// workgroups the same share; a workgroup past the last piece ends.
+// workgroups the same share; a workgroup past the last piece ends.  For many rows a launch in front makes the plan once.
 //
 // A lane holds the table's entry for one of 64 consecutive pages and takes a row's page from the lane that has it; the entries are read again every 64 pages.
 // Entries outside the pool name no page: their keys are left out and their gates count as 0.
@@ -266,25 +266,33 @@ __device__ __forceinline__ PagedShare share_of(const PagedDecodeK& a, int b, int
 // Batches a piece.  All rows and heads together make at most about kPagedPieces of them; short rows stay whole where splitting them brings no more than a merge and starts of
 // workgroups.  Both ways in us, from the batches that each of the 1024 workgroups that run at once gets (`load`): 10 for the bytes of one batch each at 6.5 TB/s or 1.8 for each
 // of a run's round trips, 3 for every 1024 workgroups that start, 1.5 for the merge, 3 a batch for the longest rows' tail.  Pages of 16, us, split / as it is now: D 64, 512 requests and heads of
-// 300 keys 14.6 / 12.0, 1024 of them 25.4 / 19.0, 512 of 700 23.6 / 20.4, D 128, 512 of 150 to 300 18.7 / 16.1, 1024 of 300 39.7 / 32.4.  Executed by whole waves.
+// 300 keys 14.6 / 12.0, 1024 of them 25.4 / 19.0, 512 of 700 23.6 / 20.4, D 128, 512 of 150 to 300 18.7 / 16.1, 1024 of 300 39.7 / 32.4.
 template <int D>
-__device__ __forceinline__ int batches_per_piece(const PagedDecodeK& a, int lane) {
-  double sum = 0;
-  int most = 0;
-  for (int b = lane; b < a.B; b += 64) {
-    const int nb = (keys_of(a, b) + paged_batch(D) - 1) / paged_batch(D);
-    sum += nb;
-    most = max(most, nb);
-  }
-  const double total = of_lane(wave_scan(sum), 63);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+__device__ __forceinline__ int choose_batches(const PagedDecodeK& a, double total, int most) {
   const int c = max((int)ceil(total * a.H * a.per_piece), 1);
   if (most <= c || most > 8) return c;
   const float load = (float)total * a.H / 1024.f, rows = (float)a.B * a.H / 1024.f, full = (float)total / ((float)a.B * most);
   const float split = fmaxf(10.f * load, 1.8f * c) + 3.f * fmaxf(load / c, 1.f) + 1.5f;
   const float whole = fmaxf(10.f * load, 1.8f * most) + 3.f * fmaxf(rows, 1.f) + 3.f * (most - 1) * (1.f - full);
-  return __builtin_amdgcn_readfirstlane(whole < split ? most : c);
+  return whole < split ? most : c;
+}
+template <int D>
+__device__ __forceinline__ int batches_of(const PagedDecodeK& a, int b) {
+  return (keys_of(a, b) + paged_batch(D) - 1) / paged_batch(D);
+}
+// The same from the lengths themselves.  Executed by whole waves.
+template <int D>
+__device__ __forceinline__ int batches_per_piece(const PagedDecodeK& a, int lane) {
+  double sum = 0;
+  int most = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const int nb = batches_of<D>(a, b);
+    sum += nb;
+    most = max(most, nb);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+  return __builtin_amdgcn_readfirstlane(choose_batches<D>(a, of_lane(wave_scan(sum), 63), most));
 }
 
 struct PagedPiece {
@@ -294,10 +302,35 @@ struct PagedPiece {
 // The row that piece number p (of one head) belongs to; b < 0: there is none.  The result is the same in all lanes, and in all workgroups, which run this same code.
 template <int D>
 __device__ __forceinline__ PagedPiece find_piece(const PagedDecodeK& a, int p, int lane) {
-  const int per_piece = batches_per_piece<D>(a, lane);
-  int before = 0;
   PagedPiece r;
   r.b = -1;
+  if (!a.ws_row) {   // no row can be more than one piece
+    if (p >= a.B) return r;
+    r.b = r.first = p;
+    r.piece = 0;
+    r.share = PagedShare{keys_of(a, p), 1, 1};
+    return r;
+  }
+  if (a.planned) {   // the rows' first pieces are there, sorted: 64 of them compared at a time
+    const PagedRow all = a.ws_row[a.B];
+    if (p >= all.first) return r;
+    int lo = 0, n = a.B;
+    while (n > 1) {
+      const int step = (n + 63) / 64, at = lane * step;
+      const uint64_t before = __ballot(at < n && a.ws_row[lo + min(at, n - 1)].first <= p);   // (the first always is)
+      const int k = (__popcll(before) - 1) * step;
+      lo += k;
+      n = min(step, n - k);
+    }
+    const PagedRow row = a.ws_row[lo];
+    r.b = lo;
+    r.first = row.first;
+    r.piece = p - row.first;
+    r.share = share_of<D>(a, lo, all.pieces);
+    return r;
+  }
+  const int per_piece = batches_per_piece<D>(a, lane);
+  int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const PagedShare s = share_of<D>(a, b0 + lane, per_piece);
     const int pieces = b0 + lane < a.B ? s.pieces : 0, end = before + (int)wave_scan(pieces), first = end - pieces;
@@ -319,6 +352,34 @@ __device__ __forceinline__ PagedPiece find_piece(const PagedDecodeK& a, int p, i
 
 }  // namespace
 
+// The plan of many rows in a launch of its own: every row's pieces, and behind them the number of all pieces and the batches a piece.
+template <int D>
+__global__ __launch_bounds__(1024) void paged_plan_kernel(const PagedDecodeK a) {
+  __shared__ double waves[16];
+  __shared__ int longest;
+  const int tid = threadIdx.x;
+  if (tid == 0) longest = 0;
+  double total = 0, all;
+  int most = 0;
+  for (int b = tid; b < a.B; b += 1024) {
+    const int nb = batches_of<D>(a, b);
+    total += nb;
+    most = max(most, nb);
+  }
+  block_scan(total, waves, &total);   // (its barriers lie between the zero and the maxima)
+  atomicMax(&longest, most);
+  __syncthreads();
+  const int per_piece = choose_batches<D>(a, total, longest);
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 1024) {
+    const int b = b0 + tid, pieces = b < a.B ? share_of<D>(a, b, per_piece).pieces : 0;
+    const int end = before + (int)block_scan(pieces, waves, &all);
+    if (b < a.B) a.ws_row[b] = PagedRow{end - pieces, pieces};
+    before += (int)all;
+  }
+  if (tid == 0) a.ws_row[a.B] = PagedRow{before, per_piece};
+}
+
 template <typename Tr, int D>
 __global__ __launch_bounds__(256) void paged_decode_kernel(const PagedDecodeK a) {
   constexpr int LPR = D / 8;      // lanes per key row
@@ -336,7 +397,7 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const PagedDecodeK a)
   const int number = divide(blockIdx.x, a.by_heads), h = blockIdx.x - number * a.H;
   const PagedPiece at = find_piece<D>(a, number, lane);
   if (at.b < 0) return;   // (the same in all waves)
-  if (a.ws_row && at.piece == 0 && h == 0 && tid == 0) a.ws_row[at.b] = PagedRow{at.first, at.share.pieces};   // for the merge
+  if (a.ws_row && !a.planned && at.piece == 0 && h == 0 && tid == 0) a.ws_row[at.b] = PagedRow{at.first, at.share.pieces};   // for the merge
   const int b = at.b;
   const PagesK& pg = a.pages;
   const int32_t* table = a.table + (a.requests ? a.requests[b] : b) * a.table_sb;
@@ -553,6 +614,10 @@ template <typename Tr, int D>
 static hipError_t launch_paged_decode_d(const PagedDecodeK& args, hipStream_t s) {
   PagedDecodeK a = args;
   a.per_piece = 1.0 / kPagedPieces;
+  // Up to 255 rows every wave works the plan out from the lengths, 64 at a time, which a launch of its own would not make up for (300 keys, H8 D64, us, waves / launch: 256 rows 41.0 / 40.4, 384
+  // 64.5 / 55.6, 1024 216 / 142; 64 rows take 12.2).
+  a.planned = a.ws_row && a.B >= 256;
+  if (a.planned) hipLaunchKernelGGL(paged_plan_kernel<D>, dim3(1), dim3(1024), 0, s, a);
   hipLaunchKernelGGL((paged_decode_kernel<Tr, D>), dim3((unsigned)paged_decode_workgroups(a.B, a.H, a.max_keys, D)), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || most_pieces(a.max_keys, D) <= 1) return e;

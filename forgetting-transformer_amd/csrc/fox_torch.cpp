@@ -1110,23 +1110,28 @@ void wrote(const Tensor& t) {
 }
 bool shares_storage(const Tensor& a, const Tensor& b) { return a.storage().is_alias_of(b.storage()); }
 
-// The integer arguments of page_slots and page_release: lengths (B), block_table (B, W), free_pages (P), free_count (1).
-bool page_state_ok(const Tensor* lengths, const Tensor* table, const Tensor* free_pages, const Tensor* free_count) {
+// Whether two tensors' memory overlaps (by the span from the first to the last element).
+bool overlaps(const Tensor& a, const Tensor& b) {
+  if (!shares_storage(a, b) || a.numel() == 0 || b.numel() == 0) return false;
+  const auto end = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return (const char*)t.const_data_ptr() + (last + 1) * (int64_t)t.element_size();
+  };
+  return (const char*)a.const_data_ptr() < end(b) && (const char*)b.const_data_ptr() < end(a);
+}
+
+// The integer arguments of page_slots and page_release: lengths (B), block_table (B, W), free_pages (P), free_count (1), none in another's memory,
+// nor `other`, which the calls read, in that of those that they write.
+bool page_state_ok(const Tensor* lengths, const Tensor* table, const Tensor* free_pages, const Tensor* free_count, const Tensor* other, bool in_place) {
   if (!lengths || !on_current_gpu(*lengths) || !int32_ok(lengths, *lengths, 1) || !int32_ok(table, *lengths, 2) || !int32_ok(free_pages, *lengths, 1) ||
-      !int32_ok(free_count, *lengths, 1))
+      !int32_ok(free_count, *lengths, 1) || !other || other->device() != lengths->device() || other->sizes() != lengths->sizes() || !other->is_contiguous())
     return false;
   const Tensor* all[4] = {lengths, table, free_pages, free_count};
   for (int i = 0; i < 4; ++i)
     for (int j = 0; j < i; ++j)
-      if (shares_storage(*all[i], *all[j])) {   // parts of one buffer are fine while they do not overlap
-        const auto span = [](const Tensor& t) {
-          const char* p = (const char*)t.const_data_ptr();
-          const int64_t n = t.dim() == 2 ? (t.size(0) - 1) * t.stride(0) + t.size(1) : t.numel();
-          return std::pair<const char*, const char*>(p, p + 4 * n);
-        };
-        const auto a = span(*all[i]), b = span(*all[j]);
-        if (a.first < b.second && b.first < a.second) return false;
-      }
+      if (overlaps(*all[i], *all[j])) return false;
+  if (overlaps(*other, *table) || overlaps(*other, *free_pages) || (in_place && (overlaps(*other, *lengths) || overlaps(*other, *free_count)))) return false;
   const int64_t B = lengths->size(0), W = table->size(1), P = free_pages->size(0);
   return B > 0 && B <= 4096 && table->size(0) == B && W > 0 && W <= INT32_MAX && P > 0 && P <= INT32_MAX && free_count->size(0) == 1 &&
          (B == 1 || table->stride(0) >= W);
@@ -1138,15 +1143,14 @@ PyObject* py_page_slots(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK(n == 8, "page_slots takes 8 arguments");
   const Tensor *lengths = tensor_of(o[0]), *fresh = tensor_of(o[1]), *table = tensor_of(o[2]), *pages = tensor_of(o[3]), *count = tensor_of(o[4]);
-  if (!page_state_ok(lengths, table, pages, count) || !int32_ok(fresh, *lengths, 1) || fresh->sizes() != lengths->sizes()) return none();
   const int64_t S = PyLong_AsLongLong(o[5]), T = PyLong_AsLongLong(o[6]);
   bool in_place = false;
   if (PyErr_Occurred() || !flag(o[7], in_place)) {
     PyErr_Clear();
     return none();
   }
-  if (T < 0 || T > INT32_MAX || S < 1 || S > INT32_MAX || !writable(*table) || (in_place && (!writable(*lengths) || !writable(*count) || shares_storage(*fresh, *lengths))))
-    return none();
+  if (!page_state_ok(lengths, table, pages, count, fresh, in_place) || fresh->scalar_type() != at::kInt) return none();
+  if (T < 0 || T > INT32_MAX || S < 1 || S > INT32_MAX || !writable(*table) || (in_place && (!writable(*lengths) || !writable(*count)))) return none();
   Tensor out[7];
   {
     const pybind11::gil_scoped_release no_gil;
@@ -1198,15 +1202,13 @@ PyObject* py_page_release(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK(n == 7, "page_release takes 7 arguments");
   const Tensor *lengths = tensor_of(o[0]), *done = tensor_of(o[1]), *table = tensor_of(o[2]), *pages = tensor_of(o[3]), *count = tensor_of(o[4]);
-  if (!page_state_ok(lengths, table, pages, count) || !done || done->scalar_type() != at::kBool || done->device() != lengths->device() ||
-      done->sizes() != lengths->sizes() || !done->is_contiguous())
-    return none();
   const int64_t S = PyLong_AsLongLong(o[5]);
   bool in_place = false;
   if (PyErr_Occurred() || !flag(o[6], in_place)) {
     PyErr_Clear();
     return none();
   }
+  if (!page_state_ok(lengths, table, pages, count, done, in_place) || done->scalar_type() != at::kBool) return none();
   if (S < 1 || S > INT32_MAX || !writable(*pages) || (in_place && (!writable(*lengths) || !writable(*count)))) return none();
   Tensor out[2];
   {
@@ -1287,9 +1289,13 @@ PyObject* py_paged_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (needs_graph({k, v, g}) || !writable(*kp) || !writable(*vp) || !writable(*gp)) return none();
   const Tensor* to[3] = {kp, vp, gp};
   const Tensor* from[3] = {k, v, g};
-  for (int i = 0; i < 3; ++i)
+  // (pages of keys and values may lie between each other, but are not the same)
+  if (kp->const_data_ptr() == vp->const_data_ptr()) return none();
+  for (int i = 0; i < 3; ++i) {
+    if (overlaps(*to[i], *slots)) return none();
     for (int j = 0; j < 3; ++j)
-      if (shares_storage(*to[i], *from[j])) return none();
+      if (overlaps(*to[i], *from[j])) return none();
+  }
   if (T > 0) {
     const pybind11::gil_scoped_release no_gil;
     a.T = (int32_t)T;

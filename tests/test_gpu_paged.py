@@ -142,6 +142,23 @@ def test_paged_append(T, H, D, S, P, dtype, inside):
     paged_append(k[:0], v[:0], f[:0], kp, vp, fp, slots[:0])
 
 
+def test_keys_and_values_in_one_pool():
+    """Pages of keys and values between each other, (P, 2, H, S, D), as two views."""
+    from forgetting_transformer import paged_append, paged_forgetting_attention
+    P, H, S, D, T = 6, 3, 16, 64, 70
+    kv = torch.zeros(P, 2, H, S, D, dtype=torch.bfloat16, device="cuda")
+    f = torch.zeros(P, H, S, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(T, H, D, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    g = -torch.rand(T, H, generator=gen, device="cuda")
+    paged_append(k, v, g, kv[:, 0], kv[:, 1], f, torch.arange(T, device="cuda"))
+    apart = [torch.zeros(P, H, S, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)] + [torch.zeros_like(f)]
+    paged_append(k, v, g, *apart, torch.arange(T, device="cuda"))
+    assert torch.equal(kv[:, 0], apart[0]) and torch.equal(kv[:, 1], apart[1]) and torch.equal(f, apart[2])
+    table, n = on_gpu([list(range(P))]), on_gpu([T])
+    assert torch.equal(paged_forgetting_attention(k[:1], kv[:, 0], kv[:, 1], f, table, n), paged_forgetting_attention(k[:1], *apart, table, n))
+
+
 def attention_reference(q, kp, vp, fp, table, lengths, requests, scale):
     P, H, S, D = kp.shape
     out = torch.zeros_like(q, dtype=torch.float64)
@@ -179,7 +196,7 @@ CASES = [  # B, H, D, S, W, lengths, dtype, heads inside
     (2, 12, 64, 16, 100, [1500, 1], torch.bfloat16, False), (2, 4, 128, 64, 40, [2560, 2499], torch.float16, True), (5, 2, 16, 16, 200, [3200, 0, 7, 1024, 1025], torch.float16, False),
     (1, 2, 128, 4096, 3, [9001], torch.bfloat16, False), (70, 2, 32, 32, 30, None, torch.bfloat16, False), (130, 1, 64, 8, 90, None, torch.float16, True),
     (1, 1, 128, 32, 700, [22400], torch.bfloat16, False), (6, 16, 128, 256, 4, None, torch.bfloat16, False), (300, 3, 16, 8, 40, None, torch.bfloat16, False),
-    (2, 2, 32, 8, 3000, [24000, 200], torch.bfloat16, False)]
+    (2, 2, 32, 8, 3000, [24000, 200], torch.bfloat16, False), (1100, 2, 64, 16, 40, None, torch.bfloat16, False), (256, 1, 128, 16, 100, None, torch.float16, True)]
 
 
 @pytest.mark.parametrize("B,H,D,S,W,lengths,dtype,inside", CASES)
@@ -293,7 +310,7 @@ def test_refusals_on_the_gpu():
         a = {**dict(k=k, f=f, slots=slots), **bad}
         with pytest.raises(AssertionError):
             paged_append(a["k"], k, a["f"], kp, vp, fp, a["slots"])
-    for bad in ((kp[0].transpose(0, 1)[:3], k, kp), (k, k, kp[:1].expand(4, 2, 16, 64)), (k.clone().requires_grad_(), k, kp)):   # reads what it writes; pages that lie on each other; a graph
+    for bad in ((kp[0].transpose(0, 1)[:3], k, kp), (k, k, kp[:1].expand(4, 2, 16, 64)), (k.clone().requires_grad_(), k, kp), (k, k, vp)):   # reads what it writes; pages that lie on each other; a graph; keys and values in one place
         with pytest.raises(RuntimeError, match="does not take"):
             paged_append(bad[0], bad[1], f, bad[2], vp, fp, slots)
     free, count = on_gpu([0, 1, 2, 3]), on_gpu([4])
@@ -301,6 +318,9 @@ def test_refusals_on_the_gpu():
         page_slots(lengths, lengths, table, free, free[:1], page_size=16, max_tokens=4)                    # the stack and its count in one place
     with pytest.raises(RuntimeError, match="does not take"):
         page_slots(lengths, lengths, table, free, count, page_size=16, max_tokens=4, in_place=True)        # reads the new tokens where it writes the lengths
+    mixed = on_gpu([[7, 0, 1], [8, 2, 3]])
+    with pytest.raises(RuntimeError, match="does not take"):
+        page_slots(lengths, mixed.view(-1)[:2], mixed[:, :2], free, count, page_size=16, max_tokens=4)     # reads the new tokens where it writes the table
     with pytest.raises(AssertionError):
         page_slots(lengths, lengths, table[:, :1].expand(2, 2), free, count, page_size=16, max_tokens=4)
 
