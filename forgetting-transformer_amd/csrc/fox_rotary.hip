@@ -71,7 +71,7 @@ __device__ __forceinline__ void make_angles(const RotaryK& a, int64_t n0, int to
       const double turns = (double)pos * a.inv_freq[pair] * 0.15915494309189535;   // 1 / (2 pi)
       // the hardware's sine and cosine of a fraction of a turn, off by at most 1.25e-7 over 2^22 of them (the library's, off by 5e-8, are some sixty
       // instructions, which calls with few heads notice: B8 T16000 H1 D64 17.5 / 15.0 us, B8 T8000 H2 D128 19.0 / 16.5)
-      const float t = (float)(turns - rint(turns)), c = __builtin_amdgcn_cosf(t), s = __builtin_amdgcn_sinf(t);
+      const float part = (float)(turns - rint(turns)), c = __builtin_amdgcn_cosf(part), s = __builtin_amdgcn_sinf(part);
       cs[tok][pair] = float2{c, a.sign < 0 ? -s : s};
     }
   }
