@@ -290,7 +290,9 @@ RotaryPlan rotary_plan(int64_t tokens, int heads, int D, bool bwd) {
   p.cols = heads * (D / 16);
   p.chunks = (p.cols + 255) / 256;
   p.lanes = p.cols > 256 ? 1 : 256 / p.cols;
-  if (p.lanes > 512 / D) p.lanes = 512 / D;   // kRotaryLanes
+  // as many as LDS holds the angles of: two workgroups a CU in the backward.  A quarter of them, us: few heads leave workgroups of one or two waves (norm and rotation with
+  // gradients B8 T4096 H1 D128 43.2 / 28.9, rotation B8 T16000 H1 D64 15.1 / 11.9, B8 T8000 H2 D128 16.3 / 15.0; B33 T9954 H3 D32 29.4 / 31.7, more heads the same)
+  if (p.lanes > 2048 / D) p.lanes = 2048 / D;   // kRotaryLanes
   // forward: four tokens a thread where that still makes four workgroups a CU
   p.rows = bwd || tokens * p.chunks >= (int64_t)p.lanes * kRotaryRows * 4 * kCus ? kRotaryRows : 1;
   p.tile = p.lanes * p.rows;
