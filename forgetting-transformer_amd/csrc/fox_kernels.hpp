@@ -185,7 +185,8 @@ struct RotaryK {
   int sign;                  // -1: the other way round
   float eps;
   int cols, lanes, tile, tiles;   // how the call is cut (rotary_plan), set by the launcher with the divisors
-  Divisor by_T, by_half, by_cols;
+  Divisor by_T, by_half, by_cols, by_lanes;
+  bool tokens_first;
 };
 constexpr int kRotaryRows = 4;                          // tokens of a thread and tile
 template <int D> constexpr int kRotaryLanes = 2048 / D; // tokens a workgroup works on side by side, at most: their angles take 8 KiB of LDS

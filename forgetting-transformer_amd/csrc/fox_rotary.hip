@@ -58,6 +58,25 @@ struct Column {
   }
 };
 
+// A thread's row lane and column.  In memory order, so that a wave reads whole lines: the lanes of a head, then the heads of a token or, where a head's tokens lie next to each
+// other, the tokens of a head.  Norm and rotation with gradients of (B, H, T, D) memory, B4 H16, us, heads / tokens first: T8192 D32 163 / 98, D16 63.4 / 46.5, D64 140 / 141 (two tokens a workgroup).
+template <int D>
+__device__ __forceinline__ void place(const RotaryK& a, int& rl, int& col) {
+  constexpr int L = D / 16;
+  const int tid = threadIdx.x;
+  if (a.cols > 256) {
+    rl = 0;
+    col = blockIdx.y * 256 + tid;
+  } else if (a.tokens_first) {
+    const int unit = tid / L, head = divide(unit, a.by_lanes);
+    rl = unit - head * a.lanes;
+    col = head * L + tid % L;
+  } else {
+    rl = divide(tid, a.by_cols);
+    col = tid - rl * a.cols;
+  }
+}
+
 // cos and sin of the tile's tokens, pair by pair.  Executed by the whole workgroup.
 template <int D>
 __device__ __forceinline__ void make_angles(const RotaryK& a, int64_t n0, int tokens, float2 (*cs)[D / 2]) {
@@ -108,8 +127,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
   constexpr int L = D / 16;
   __shared__ float2 cs[ROWS * kRotaryLanes<D>][D / 2];
   const int tid = threadIdx.x;
-  const int rl = a.cols > 256 ? 0 : divide(tid, a.by_cols);
-  const int col = a.cols > 256 ? blockIdx.y * 256 + tid : tid - rl * a.cols;
+  int rl, col;
+  place<D>(a, rl, col);
   const bool live = rl < a.lanes && col < a.cols;
   const Column<D, INTERLEAVED> at(a, live ? col : 0);
   const View in = at.side ? a.side[1].in : a.side[0].in, out = at.side ? a.side[1].out : a.side[0].out;
@@ -167,8 +186,8 @@ __global__ __launch_bounds__(256, 2) void qk_norm_rotary_bwd_kernel(const Rotary
   __shared__ float2 cs[2][kRotaryRows * kRotaryLanes<D>][D / 2];
   __shared__ __align__(16) float dw_s[256 * 16];
   const int tid = threadIdx.x;
-  const int rl = a.cols > 256 ? 0 : divide(tid, a.by_cols);
-  const int col = a.cols > 256 ? blockIdx.y * 256 + tid : tid - rl * a.cols;
+  int rl, col;
+  place<D>(a, rl, col);
   const bool live = rl < a.lanes && col < a.cols;
   const Column<D, INTERLEAVED> at(a, live ? col : 0);
   const View xv = at.side ? a.side[1].x : a.side[0].x, in = at.side ? a.side[1].in : a.side[0].in;
@@ -322,6 +341,8 @@ static hipError_t launch_rotary_d(const RotaryK& args, bool norm, bool interleav
   a.by_T = divisor(a.T);
   a.by_half = divisor(a.R / 2);
   a.by_cols = divisor(p.cols);
+  a.by_lanes = divisor(p.lanes);
+  a.tokens_first = a.side[0].in.st < a.side[0].in.sh;
   const dim3 grid((unsigned)p.strips, (unsigned)p.chunks), block(p.cols > 256 ? 256u : (unsigned)((p.cols * p.lanes + 63) / 64 * 64));
   if (!bwd) {
     auto launch = [&](auto n, auto i) {
