@@ -11,16 +11,26 @@ namespace fox {
 
 namespace {
 
-// Sum of x over the threads 0 .. own of a workgroup of 1024, exact for integers below 2^53; *all gets the total.  Every thread calls it.
-__device__ __forceinline__ double block_scan(double x, double (&waves)[16], double* all) {
+// Sums of x and y over the threads 0 .. own of a workgroup of 1024, exact for integers below 2^53.  Every thread calls it.
+struct Sums {
+  double x, y, all_x, all_y;   // up to this thread, of all
+};
+__device__ __forceinline__ Sums block_scan(double x, double y, double (&waves)[2][16]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   x = wave_scan(x);
+  y = wave_scan(y);
   __syncthreads();   // (the sums of an earlier call have been read)
-  if (lane == 63) waves[wave] = x;
+  if (lane == 63) {
+    waves[0][wave] = x;
+    waves[1][wave] = y;
+  }
   __syncthreads();
-  const double sums = wave_scan(lane < 16 ? waves[lane] : 0.0);
-  *all = of_lane(sums, 15);
-  return wave == 0 ? x : x + of_lane(sums, wave - 1);
+  const double wx = wave_scan(lane < 16 ? waves[0][lane] : 0.0), wy = wave_scan(lane < 16 ? waves[1][lane] : 0.0);
+  if (wave > 0) {
+    x += of_lane(wx, wave - 1);
+    y += of_lane(wy, wave - 1);
+  }
+  return Sums{x, y, of_lane(wx, 15), of_lane(wy, 15)};
 }
 
 struct Request {   // of a page_slots, in LDS
@@ -33,15 +43,19 @@ struct Request {   // of a page_slots, in LDS
 
 }  // namespace
 
-// Every workgroup scans the requests (16 bytes each, from the L2) and serves 1024 tokens; the first one writes the requests' new state.  Bound by
-// latency: the state's round trip, two scans, a binary search in LDS and the round trip of the page.
+// Every workgroup scans the requests (8 bytes each, from the L2) and serves 1024 tokens; the first one writes the requests' new state.  Bound by
+// latency: the state's round trip, a scan, a binary search in LDS and the round trip of the page; 3.6 us for 4 requests' tokens, 4.1 for 256, where a copy of as much takes 2.2.
 __global__ __launch_bounds__(1024) void page_slots_kernel(const PageSlotsK a) {
   __shared__ Request req[kPageRequests];
-  __shared__ double waves[16];
+  __shared__ double waves[2][16];
+  __shared__ int used_s;
   const int tid = threadIdx.x, S = 1 << a.shift;
+  const bool state = a.state && blockIdx.x == 0;
   const int count = min(max(*a.free_count, 0), a.P);
   const int64_t room = (int64_t)a.W << a.shift;
   double tokens = 0, pages = 0;   // of the requests before this chunk
+  int used = 0;                   // pages handed out, up to this thread's last
+  if (tid == 0) used_s = 0;
   for (int b0 = 0; b0 < a.B; b0 += 1024) {
     const int b = b0 + tid;
     int len = 0, fresh = 0;
@@ -49,40 +63,30 @@ __global__ __launch_bounds__(1024) void page_slots_kernel(const PageSlotsK a) {
       len = (int)min((int64_t)max(a.lengths[b], 0), room);
       fresh = max(a.new_tokens[b], 0);
     }
-    double all;
-    const double end = tokens + block_scan(fresh, waves, &all);
-    tokens += all;
     const int held = (int)(((int64_t)len + S - 1) >> a.shift);
     const int64_t wanted = ((int64_t)len + fresh + S - 1) >> a.shift, need = wanted - held;
-    const bool fits = wanted <= a.W && end <= a.T;
-    const double taken = pages + block_scan(fits ? (double)need : 0.0, waves, &all);
-    pages += all;
+    // A request that fits no row of the table takes no pages.  One whose tokens end behind the last place takes none either, but all behind it end there as well, so that nobody
+    // who is served counts on it.
+    const Sums sum = block_scan(fresh, wanted <= a.W ? (double)need : 0.0, waves);
+    const double end = tokens + sum.x, taken = pages + sum.y;
+    tokens += sum.all_x;
+    pages += sum.all_y;
     // pages in request order while they last: beyond the first that cannot be served the sums only grow
-    const bool ok = fits && (need == 0 || taken <= count);
+    const bool ok = wanted <= a.W && end <= a.T && (need == 0 || taken <= count);
+    if (ok && need > 0) used = (int)taken;
     if (b < a.B) {
       const int32_t e = (int32_t)min(end, 2147483647.0);
       req[b] = Request{e, (int32_t)min(end - fresh, 2147483647.0), len, ok ? held : -1 - held, ok ? (int32_t)(count - 1 - (taken - need)) : 0};
-    }
-    if (a.state && blockIdx.x == 0) {
-      if (b < a.B) {
+      if (state) {
         a.lengths_out[b] = ok ? len + fresh : len;
         a.granted[b] = ok;
       }
-      // what is left below the last page handed out
-      double used = ok && need > 0 ? taken : 0;
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) used = fmax(used, __shfl_xor(used, off));
-      __syncthreads();
-      if ((tid & 63) == 0) waves[tid >> 6] = used;
-      __syncthreads();
-      if (tid == 0) {
-        for (int w = 1; w < 16; ++w) used = fmax(used, waves[w]);
-        if (b0 == 0 || used > 0) *a.free_out = count - (int)used;
-      }
     }
   }
-  if (!a.tokens) return;
+  if (state && used > 0) atomicMax(&used_s, used);   // (the barriers of the scan lie behind the zero)
   __syncthreads();
+  if (state && tid == 0) *a.free_out = count - used_s;   // what is left below the last page handed out
+  if (!a.tokens) return;
   for (int64_t t = (int64_t)blockIdx.x * 1024 + tid; t < a.T; t += (int64_t)gridDim.x * 1024) {
     int lo = 0, hi = a.B;   // the first request whose tokens end behind t
     while (lo < hi) {
@@ -133,10 +137,11 @@ hipError_t launch_page_slots(const PageSlotsK& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// The pages of finished requests back on the stack, request by request.
+// The pages of finished requests back on the stack, request by request, a wave each (a page a thread, which looks its request up as page_slots_kernel's tokens do: a quarter of 512
+// requests with 62 pages each 7.9 us, so 6.6).
 __global__ __launch_bounds__(1024) void page_release_kernel(const PageReleaseK a) {
   __shared__ int32_t place[kPageRequests], held_s[kPageRequests];
-  __shared__ double waves[16];
+  __shared__ double waves[2][16];
   const int tid = threadIdx.x, lane = tid & 63, S = 1 << a.shift;
   const int count = min(max(*a.free_count, 0), a.P);
   double pages = count;
@@ -149,14 +154,13 @@ __global__ __launch_bounds__(1024) void page_release_kernel(const PageReleaseK a
       done = a.done[b] != 0;
     }
     const int held = done ? (int)(((int64_t)len + S - 1) >> a.shift) : 0;
-    double all;
-    const double end = pages + block_scan(held, waves, &all);
-    pages += all;
+    const Sums sum = block_scan(held, 0, waves);
     if (b < a.B) {
-      place[b] = (int32_t)min(end - held, (double)a.P);
+      place[b] = (int32_t)min(pages + sum.x - held, (double)a.P);
       held_s[b] = held;
       a.lengths_out[b] = done ? 0 : len;
     }
+    pages += sum.all_x;
   }
   __syncthreads();
   if (tid == 0) *a.free_out = (int)min(pages, (double)a.P);
@@ -269,7 +273,7 @@ __device__ __forceinline__ PagedShare share_of(const PagedDecodeK& a, int b, int
 // 300 keys 14.6 / 12.0, 1024 of them 25.4 / 19.0, 512 of 700 23.6 / 20.4, D 128, 512 of 150 to 300 18.7 / 16.1, 1024 of 300 39.7 / 32.4.
 template <int D>
 __device__ __forceinline__ int choose_batches(const PagedDecodeK& a, double total, int most) {
-  const int c = max((int)ceil(total * a.H * a.per_piece), 1);
+  const int c = max((int)fmin(ceil(total * a.H * a.per_piece), 1 << 24), 1);   // (no row has more batches)
   if (most <= c || most > 8) return c;
   const float load = (float)total * a.H / 1024.f, rows = (float)a.B * a.H / 1024.f, full = (float)total / ((float)a.B * most);
   const float split = fmaxf(10.f * load, 1.8f * c) + 3.f * fmaxf(load / c, 1.f) + 1.5f;
@@ -355,27 +359,28 @@ __device__ __forceinline__ PagedPiece find_piece(const PagedDecodeK& a, int p, i
 // The plan of many rows in a launch of its own: every row's pieces, and behind them the number of all pieces and the batches a piece.
 template <int D>
 __global__ __launch_bounds__(1024) void paged_plan_kernel(const PagedDecodeK a) {
-  __shared__ double waves[16];
+  __shared__ double waves[2][16];
   __shared__ int longest;
   const int tid = threadIdx.x;
   if (tid == 0) longest = 0;
-  double total = 0, all;
+  double total = 0;
   int most = 0;
   for (int b = tid; b < a.B; b += 1024) {
     const int nb = batches_of<D>(a, b);
     total += nb;
     most = max(most, nb);
   }
-  block_scan(total, waves, &total);   // (its barriers lie between the zero and the maxima)
+  total = block_scan(total, 0, waves).all_x;   // (its barriers lie between the zero and the maxima)
   atomicMax(&longest, most);
   __syncthreads();
   const int per_piece = choose_batches<D>(a, total, longest);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 1024) {
     const int b = b0 + tid, pieces = b < a.B ? share_of<D>(a, b, per_piece).pieces : 0;
-    const int end = before + (int)block_scan(pieces, waves, &all);
+    const Sums sum = block_scan(pieces, 0, waves);
+    const int end = before + (int)sum.x;
     if (b < a.B) a.ws_row[b] = PagedRow{end - pieces, pieces};
-    before += (int)all;
+    before += (int)sum.all_x;
   }
   if (tid == 0) a.ws_row[a.B] = PagedRow{before, per_piece};
 }

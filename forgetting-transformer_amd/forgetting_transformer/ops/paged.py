@@ -9,6 +9,7 @@ path, and none of them has a gradient.
 """
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -34,6 +35,7 @@ class PageSlots(NamedTuple):
 
 
 def _check_page_size(page_size: int) -> None:
+    page_size = operator.index(page_size)
     assert 8 <= page_size <= 4096 and page_size & (page_size - 1) == 0, f"page_size must be a power of two from 8 to 4096, got {page_size}"
 
 
@@ -79,7 +81,7 @@ def page_slots(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
         _check_state(lengths, block_table, free_pages, free_count, page_size)
         _ints(new_tokens, 1, "new_tokens", lengths.device)
         assert new_tokens.shape == lengths.shape, "new_tokens must have an element for every length"
-        assert 0 <= max_tokens < 1 << 31, "max_tokens must not be negative"
+        assert 0 <= operator.index(max_tokens) < 1 << 31, "max_tokens must not be negative"
         with torch.cuda.device(lengths.device):
             out = ext.page_slots(lengths, new_tokens.contiguous(), block_table, free_pages, free_count, page_size, max_tokens, in_place)
         if out is None:
