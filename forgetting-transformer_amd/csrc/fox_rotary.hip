@@ -16,7 +16,8 @@
 //
 // Rows are read through the caches, in which what the projections wrote a moment ago may still be, and written past them.  Norm and rotation, bf16 H16 D128, us by
 // loads / stores, both non-temporal, only the loads, neither, only the stores (as it is): forward B4 T512 10.1, 9.8, 8.6, 7.9, T1024 14.9, 15.2, 13.6, 12.4, T4096 48.8, 45.6, 47.1,
-// 48.8, T16384 179, 202, 178, 183; backward T512 24.7, 22.8, 21.6, 21.3, T4096 81.8, 74.6, 84.2, 68.5, T16384 315, 328, 332, 317 (5.9 and 5.1 TB/s).
+// 48.8, T16384 179, 202, 178, 183; backward T512 24.7, 22.8, 21.6, 21.3, T4096 81.8, 74.6, 84.2, 68.5, T16384 315, 328, 332, 317.
+// Now 181 and 305 us at T16384 (5.9 and 5.3 TB/s; a copy runs at 5.2).
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
 
