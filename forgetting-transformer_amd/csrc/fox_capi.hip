@@ -598,7 +598,7 @@ int fox_paged_append(const fox_paged_append_args* a, void* stream) {
   if (!a) return fail(FOX_E_ARG, "args is NULL");
   fox::PagedAppendK k{};
   FOX_TRY(make_pages(a->pages, k.pages));
-  if (a->T <= 0 || (int64_t)a->T * a->pages.H > 0x7fffffffLL) return fail(FOX_E_ARG, "T must be positive and T * H below 2^31 (got %d)", a->T);
+  if (a->T <= 0) return fail(FOX_E_ARG, "T must be positive (got %d)", a->T);
   FOX_TRY(check_view(&a->k, "k"));
   FOX_TRY(check_view(&a->v, "v"));
   if (!a->g || !a->slots) return fail(FOX_E_ARG, "g and slots must not be NULL");
@@ -608,6 +608,7 @@ int fox_paged_append(const fox_paged_append_args* a, void* stream) {
   k.slots = a->slots;
   k.H = a->pages.H;
   k.total = (int64_t)a->T * k.H * (a->pages.D / 8);
+  if (k.total > 0x7fffffffLL) return fail(FOX_E_ARG, "too many tokens for one call");   // (a thread each)
   k.by_heads = fox::divisor(k.H);
   return check_hip(fox::launch_paged_append(k, a->pages.D, (hipStream_t)stream), "fox_paged_append");
 }
@@ -615,7 +616,7 @@ int fox_paged_append(const fox_paged_append_args* a, void* stream) {
 int fox_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int64_t max_keys, int64_t* bytes) {
   if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
   FOX_TRY(check_head_dim(D));
-  if (B <= 0 || H <= 0 || (int64_t)B * H > (1 << 24) || max_keys <= 0 || max_keys > (1 << 30)) return fail(FOX_E_ARG, "B, H and max_keys must be positive, B * H at most 2^24, max_keys at most 2^30");
+  if (B <= 0 || H <= 0 || (int64_t)B * H > (1 << 23) || max_keys <= 0 || max_keys > (1 << 30)) return fail(FOX_E_ARG, "B, H and max_keys must be positive, B * H at most 2^23, max_keys at most 2^30");
   const int64_t rows = fox::paged_decode_rows(B, H, (int)max_keys, D);
   *bytes = rows ? rows * (int64_t)(D * sizeof(float) + sizeof(fox::DecodePartial)) + (B + 1) * (int64_t)sizeof(fox::PagedRow) : 0;
   return FOX_OK;

@@ -177,7 +177,9 @@ hipError_t launch_page_release(const PageReleaseK& a, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // New tokens' keys, values and log gates into their slots: one 16-byte piece of k and the same piece of v per thread, the thread with a row's
-// first piece also moves its gate.  A plain stream (16384 tokens of H16 D128 53 us, 5.1 TB/s; 48 tokens 2.5 us); slots outside the pool are left out.
+// first piece also moves its gate.  A plain stream, read through the caches (the projections have just written it) and written past them (the attention reads all of the cache before it
+// comes back to these rows): H16 D128, us, loads non-temporal / stores too / neither / the stores only, as it is: 2048 tokens 9.0 / 8.2 / 7.7 / 7.2, 8192 25.7 / 27.1 / 28.0 / 24.2, 16384
+// 53.2 / 51.4 / 52.6 / 51.0 (5.3 TB/s); 48 tokens 2.5.  Slots outside the pool are left out.
 template <int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendK a) {
   constexpr int CH = D / 8;
@@ -185,15 +187,15 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendK a)
   if (idx >= a.total) return;
   const int ch = (int)(idx % CH), row = (int)(idx / CH), t = divide(row, a.by_heads), h = row - t * a.H;
   const int64_t slot = a.slots[t];
-  const u32x4 kx = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.k + t * a.k_st + h * a.k_sh + ch * 8));
-  const u32x4 vx = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.v + t * a.v_st + h * a.v_sh + ch * 8));
+  const u32x4 kx = *reinterpret_cast<const u32x4*>(a.k + t * a.k_st + h * a.k_sh + ch * 8);
+  const u32x4 vx = *reinterpret_cast<const u32x4*>(a.v + t * a.v_st + h * a.v_sh + ch * 8);
   float gx = 0.f;
   if (ch == 0) gx = a.g[t * a.g_st + h * a.g_sh];
   if (slot < 0 || slot >= (int64_t)a.pages.P << a.pages.shift) return;
   const int64_t page = slot >> a.pages.shift, at = slot & ((1 << a.pages.shift) - 1);
   const View &k = a.pages.k, &v = a.pages.v;
-  *reinterpret_cast<u32x4*>(const_cast<uint16_t*>(k.ptr) + page * k.sb + h * k.sh + at * k.st + ch * 8) = kx;
-  *reinterpret_cast<u32x4*>(const_cast<uint16_t*>(v.ptr) + page * v.sb + h * v.sh + at * v.st + ch * 8) = vx;
+  __builtin_nontemporal_store(kx, reinterpret_cast<u32x4*>(const_cast<uint16_t*>(k.ptr) + page * k.sb + h * k.sh + at * k.st + ch * 8));
+  __builtin_nontemporal_store(vx, reinterpret_cast<u32x4*>(const_cast<uint16_t*>(v.ptr) + page * v.sb + h * v.sh + at * v.st + ch * 8));
   if (ch == 0) a.pages.g[page * a.pages.g_sp + h * a.pages.g_sh + at * a.pages.g_ss] = gx;
 }
 

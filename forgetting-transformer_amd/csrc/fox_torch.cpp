@@ -1284,6 +1284,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   fox_paged_append_args a{};
   if (!pages_ok(kp, vp, gp, a.pages) || !tokens_ok(k, a.pages, *kp) || !tokens_ok(v, a.pages, *kp) || v->size(0) != k->size(0)) return none();
   const int64_t T = k->size(0);
+  if (T * a.pages.H * (a.pages.D / 8) > INT32_MAX) return none();
   if (!g || g->dim() != 2 || g->scalar_type() != at::kFloat || g->device() != kp->device() || g->size(0) != T || g->size(1) != a.pages.H) return none();
   if (!slots || slots->dim() != 1 || slots->size(0) != T || slots->scalar_type() != at::kLong || slots->device() != kp->device() || !slots->is_contiguous()) return none();
   if (needs_graph({k, v, g}) || !writable(*kp) || !writable(*vp) || !writable(*gp)) return none();
@@ -1320,7 +1321,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   fox_paged_decode_args a{};
   if (!pages_ok(kp, vp, gp, a.pages) || !tokens_ok(q, a.pages, *kp) || !int32_ok(table, *kp, 2) || !int32_ok(lengths, *kp, 1)) return none();
   const int64_t B = q->size(0), W = table->size(1), S = a.pages.page_size;
-  if (lengths->size(0) != B || table->size(0) < 1 || W < 1 || table->size(0) > INT32_MAX || W * S > (1 << 30) || B * a.pages.H > (1 << 24)) return none();
+  if (lengths->size(0) != B || table->size(0) < 1 || W < 1 || table->size(0) > INT32_MAX || W * S > (1 << 30) || B * a.pages.H > (1 << 23)) return none();
   const Tensor* requests = nullptr;
   if (o[6] != Py_None) {
     requests = tensor_of(o[6]);

@@ -141,6 +141,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, log_fgate: torch.Tensor, k_pa
     _check_pages(k_pages, v_pages, log_fgate_pages)
     k, v = _check_tokens(k, k_pages, "k"), _check_tokens(v, k_pages, "v")
     assert k.shape == v.shape, "k and v must have the same shape"
+    assert k.numel() // 8 < 1 << 31, "too many tokens for one call"
     assert log_fgate.dtype == torch.float32 and log_fgate.shape == k.shape[:2] and log_fgate.device == k.device, "log_fgate must be float32 (tokens, H)"
     assert slots.dtype == torch.int64 and slots.shape == k.shape[:1] and slots.device == k.device, "slots must be int64, one for every token"
     with torch.cuda.device(k.device):
@@ -175,7 +176,7 @@ def paged_forgetting_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: 
         assert requests.shape == (B,), "requests must have an element for every row of q"
         requests = requests.contiguous()
     assert block_table.shape[0] > 0 and 0 < block_table.shape[1] * k_pages.shape[2] <= 1 << 30, "block_table must hold between 1 and 2**30 tokens a request"
-    assert B * k_pages.shape[1] <= 1 << 24, "at most 2**24 rows and heads"
+    assert B * k_pages.shape[1] <= 1 << 23, "at most 2**23 rows and heads"
     assert max_length is None or max_length > 0, "max_length must be positive"
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
     with torch.cuda.device(q.device):

@@ -109,7 +109,7 @@ def test_page_c_abi_checks():
     n = C.c_int64(-1)
     assert lib.fox_paged_decode_workspace_bytes(4, 2, 64, 256, C.byref(n)) == 0 and n.value == 0      # nobody has more than one piece
     assert lib.fox_paged_decode_workspace_bytes(4, 2, 64, 4096, C.byref(n)) == 0 and n.value > 0
-    assert lib.fox_paged_decode_workspace_bytes(4, 2, 64, (1 << 30) + 1, C.byref(n)) == -1 and lib.fox_paged_decode_workspace_bytes(1 << 13, 1 << 13, 64, 64, C.byref(n)) == -1
+    assert lib.fox_paged_decode_workspace_bytes(4, 2, 64, (1 << 30) + 1, C.byref(n)) == -1 and lib.fox_paged_decode_workspace_bytes(1 << 12, 1 << 12, 64, 64, C.byref(n)) == -1
     assert lib.fox_paged_append(None, None) == -1 and lib.fox_paged_decode(None, None) == -1 and lib.fox_page_slots(None, None) == -1 and lib.fox_page_release(None, None) == -1
 
 
