@@ -422,3 +422,79 @@ def test_a_captured_step_replays():
         torch.randn(1 << 20, device="cuda").sum().item()
         assert torch.equal(out, want)
     assert torch.equal(a.lengths, b.lengths) and torch.equal(a.block_table, b.block_table) and torch.equal(a.free_count, b.free_count)
+
+
+def test_lengths_cut_by_max_length():
+    from forgetting_transformer import paged_forgetting_attention
+    kp, vp, fp, gen = pool(40, 2, 16, 64, torch.float16, 5)
+    table = on_gpu([list(range(20)), list(range(20, 40))])
+    q = torch.randn(2, 2, 64, generator=gen, device="cuda").half()
+    for most in (1, 17, 200, 320, 4000):
+        a = paged_forgetting_attention(q, kp, vp, fp, table, on_gpu([320, 100]), max_length=most)
+        want = attention_reference(q, kp, vp, fp, table.tolist(), [min(320, most), min(100, most)], None, 64 ** -0.5)
+        check_attention(a, want, vp, torch.float16)
+
+
+def test_steps_in_inference_mode():
+    """A cache made and used in inference mode, and one made outside that a step in inference mode writes to."""
+    import forgetting_transformer as ft
+    freq = ft.rotary_frequencies(32, device="cuda")
+
+    def make():
+        return ft.PagedFgateCache(1, 2, 32, num_pages=8, max_requests=3, max_length=40, page_size=8)
+
+    def steps(c):
+        g = torch.Generator(device="cuda").manual_seed(0)
+        out = []
+        for n in ([5, 0, 9], [1, 1, 1], [0, 2, 1]):
+            s = c.schedule(on_gpu(n), sum(n))
+            q, k, v = (torch.randn(1, sum(n), 2, 32, generator=g, device="cuda").bfloat16() for _ in range(3))
+            q, k = ft.qk_norm_rotary(q, k, torch.ones(32, device="cuda"), torch.ones(32, device="cuda"), freq, positions=s.positions[None])
+            c.update(k[0], v[0], -torch.rand(sum(n), 2, generator=g, device="cuda"), 0)
+            out.append(c.attend(q[0], 0))
+        c.release(torch.tensor([True, False, True], device="cuda"))
+        return out + [c.lengths.clone(), c.free_count.clone()]
+
+    want = steps(make())
+    outside = make()
+    with torch.inference_mode():
+        inside = steps(make())
+        mixed = steps(outside)
+    for got in (inside, mixed):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_c_entries():
+    """The C entry points on raw pointers: rows that are fewer than the table's requests, and the state of the pages written in place."""
+    import ctypes as C
+    from forgetting_transformer import paged_forgetting_attention
+    from forgetting_transformer.ops import _lib
+    lib = _lib.load()
+    kp, vp, fp, gen = pool(12, 2, 16, 64, torch.bfloat16, 6)
+    view = lambda t: _lib.View(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    pages = _lib.Pages(12, 2, 16, 64, 0, view(kp), view(vp), fp.data_ptr(), *fp.stride())
+    table, lengths = on_gpu([[0, 1, 2, 3], [4, 5, 6, 7], [8, 9, 10, 11]]), on_gpu([50, 3, 0])
+    q = torch.randn(2, 2, 64, generator=gen, device="cuda").bfloat16()
+    out = torch.full_like(q, 7.0)
+    flat = lambda t: _lib.View(t.data_ptr(), t.stride(0), t.stride(1), 8)
+    n = C.c_int64()
+    assert lib.fox_paged_decode_workspace_bytes(2, 2, 64, 64, C.byref(n)) == 0
+    ws = torch.empty(max(n.value, 16), dtype=torch.uint8, device="cuda")
+    args = _lib.PagedDecodeArgs(pages, 2, 3, 4, 0, flat(q), flat(out), table.data_ptr(), 4, lengths.data_ptr(), None, 0.125, ws.data_ptr(), n.value)
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    _lib.check(lib.fox_paged_decode(C.byref(args), stream), "fox_paged_decode")
+    assert torch.equal(out, paged_forgetting_attention(q, kp, vp, fp, table[:2], lengths[:2]))
+
+    free, count, new = on_gpu([9, 8, 7, 6, 5]), on_gpu([5]), on_gpu([20, 0, 4000])
+    state = on_gpu([10, 5, 0])
+    T = 1500                                                              # more than a workgroup's tokens: the state has a launch of its own
+    slots, pos = (torch.empty(T, dtype=torch.int64, device="cuda") for _ in range(2))
+    req, keys = (torch.empty(T, dtype=torch.int32, device="cuda") for _ in range(2))
+    granted = torch.empty(3, dtype=torch.bool, device="cuda")
+    small = table.clone()
+    a = _lib.PageSlotsArgs(3, 4, 5, 16, T, state.data_ptr(), new.data_ptr(), small.data_ptr(), 4, free.data_ptr(), count.data_ptr(), slots.data_ptr(), pos.data_ptr(),
+                           req.data_ptr(), keys.data_ptr(), state.data_ptr(), count.data_ptr(), granted.data_ptr())
+    _lib.check(lib.fox_page_slots(C.byref(a), stream), "fox_page_slots")
+    assert state.tolist() == [30, 5, 0] and count.tolist() == [4] and granted.tolist() == [True, True, False]
+    assert slots.tolist()[:20] == [10 + i if i < 6 else 5 * 16 + i - 6 for i in range(20)] and set(slots.tolist()[20:]) == {-1}
+    assert small.tolist()[0] == [0, 5, 2, 3] and keys.tolist()[:20] == list(range(11, 31)) and req.tolist()[20:] == [-1] * 1480

@@ -286,3 +286,29 @@ def test_streams_and_graph_replay():
             torch.cuda.synchronize()
             torch.randn(1 << 20, device="cuda").sum().item()
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_c_entry():
+    """One side alone through the C entry, on strided views, from a position on; forward and back."""
+    import ctypes as C
+    from forgetting_transformer import rotary, rotary_frequencies
+    from forgetting_transformer.ops import _lib
+    lib = _lib.load()
+    x = torch.randn(2, 30, 5, 64, device="cuda").bfloat16()
+    mem = torch.zeros(2, 5, 40, 72, dtype=torch.bfloat16, device="cuda")
+    y = mem[:, :, 3:33, :64].transpose(1, 2)
+    freq = rotary_frequencies(32, device="cuda")
+    view = lambda t: _lib.View(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
+    none = _lib.View(None, 0, 0, 0)
+
+    def args(a, b, dx):
+        side = _lib.RotarySide(5, a, b, dx, None)
+        return _lib.RotaryArgs(1, 2, 30, 64, 0, 32, 0, (_lib.RotarySide * 2)(side, _lib.RotarySide()), 0, 0.0, freq.data_ptr(), None, 0, 0, 11, None, None)
+
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    _lib.check(lib.fox_rotary_fwd(C.byref(args(view(x), view(y), none)), stream), "fox_rotary_fwd")
+    assert torch.equal(y, rotary(x, freq, positions=11))
+    back = torch.empty_like(x)
+    _lib.check(lib.fox_rotary_bwd(C.byref(args(none, view(y), view(back))), stream), "fox_rotary_bwd")
+    assert torch.equal(back, rotary(y.contiguous(), freq, positions=-torch.arange(11, 41, device="cuda")))
+    assert mem.abs().sum() == y.abs().sum()                              # nothing beside the view
