@@ -188,8 +188,9 @@ struct RotaryK {
   Divisor by_T, by_half, by_cols, by_lanes;
   bool tokens_first;
 };
-constexpr int kRotaryRows = 4;                          // tokens of a thread and tile
-template <int D> constexpr int kRotaryLanes = 2048 / D; // tokens a workgroup works on side by side, at most: their angles take 8 KiB of LDS
+constexpr int kRotaryThreads = 256;                      // of a workgroup, at most
+constexpr int kRotaryRows = 4;                           // backward: tokens of a thread and tile
+template <int D> constexpr int kRotaryLanes = 2048 / D;  // tokens a workgroup works on side by side, at most: their angles take 8 KiB of LDS
 
 // Pool of pages (fox_paged.hip): pages of 2^shift tokens, (P, H, S, D) keys and values as views with the stride between pages in sb, (P, H, S) log gates.
 struct PagesK {

@@ -11,8 +11,11 @@
 // every pair are in the lane: vectors c and c + R/16 of the rotated part (2c and 2c+1 interleaved, and beyond the rotated
 // part).  Row sums are DPP adds over the D/16 lanes of a head.  The angles are the same for all heads of a token: a workgroup
 // forms them once per token, in 64 bits up to the fraction of a turn (a position of 2^20 would leave 32-bit angles 4 digits),
-// and keeps cosine and sine in LDS.  A thread owns one column (tensor, head, sixteen elements) and walks tokens, so the
-// weights are loaded once and their gradient stays in registers; partial gradients leave once per workgroup and are added in a fixed order.
+// and keeps cosine and sine in LDS.  A thread owns one column (tensor, head, sixteen elements).  Forward it takes one token: four
+// (or two) per thread, with all their rows in flight, keep fewer waves busy and pay only where the weights are long against the
+// rows (us, four / one, rotation B4 T4096 H12 D64 43.9 / 37.3, T50000 H1 D64 31.7 / 16.9, H16 D128 303 / 283, norm and rotation B4 T4096 H16 D128 190 / 181, H12 D64
+// 80.3 / 87.3; 30 shapes geomean 0.94; workgroups of 512 and 1024 threads 1.01 and 1.04 of it).  Backward it walks tokens, so the weights are loaded once and their gradient
+// stays in registers; partial gradients leave once per workgroup and are added in a fixed order.
 //
 // Rows are read through the caches, in which what the projections wrote a moment ago may still be, and written past them.  Norm and rotation, bf16 H16 D128, us by
 // loads / stores, both non-temporal, only the loads, neither, only the stores (as it is): forward B4 T512 10.1, 9.8, 8.6, 7.9, T1024 14.9, 15.2, 13.6, 12.4, T4096 48.8, 45.6, 47.1,
@@ -65,9 +68,9 @@ template <int D>
 __device__ __forceinline__ void place(const RotaryK& a, int& rl, int& col) {
   constexpr int L = D / 16;
   const int tid = threadIdx.x;
-  if (a.cols > 256) {
+  if (a.cols > kRotaryThreads) {
     rl = 0;
-    col = blockIdx.y * 256 + tid;
+    col = blockIdx.y * kRotaryThreads + tid;
   } else if (a.tokens_first) {
     const int unit = tid / L, head = divide(unit, a.by_lanes);
     rl = unit - head * a.lanes;
@@ -123,11 +126,10 @@ __device__ __forceinline__ float rsqrt_ulp(float x) { return __builtin_amdgcn_rs
 
 }  // namespace
 
-template <typename Tr, int D, bool NORM, bool INTERLEAVED, int ROWS>
-__global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
+template <typename Tr, int D, bool NORM, bool INTERLEAVED>
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryK a) {
   constexpr int L = D / 16;
-  __shared__ float2 cs[ROWS * kRotaryLanes<D>][D / 2];
-  const int tid = threadIdx.x;
+  __shared__ float2 cs[kRotaryLanes<D>][D / 2];
   int rl, col;
   place<D>(a, rl, col);
   const bool live = rl < a.lanes && col < a.cols;
@@ -143,49 +145,38 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryK a) {
       w[8 + e] = wp[at.v1 * 8 + e];
     }
   }
-  u32x4 x0[ROWS], x1[ROWS];
-  int64_t to[ROWS];
-#pragma unroll
-  for (int u = 0; u < ROWS; ++u) {   // tokens past the end read the last one and are not stored
-    const int n = (int)min(n0 + rl + (int64_t)u * a.lanes, (int64_t)a.N - 1);
-    const int b = divide(n, a.by_T), t = n - b * a.T;
-    const uint16_t* p = in.ptr + b * in.sb + t * in.st + at.h * in.sh;
-    to[u] = b * out.sb + t * out.st + at.h * out.sh;
-    x0[u] = *reinterpret_cast<const u32x4*>(p + at.v0 * 8);
-    x1[u] = *reinterpret_cast<const u32x4*>(p + at.v1 * 8);
-  }
+  const int n = (int)min(n0 + rl, (int64_t)a.N - 1);   // a token past the end reads the last one and is not stored
+  const int b = divide(n, a.by_T), t = n - b * a.T;
+  const uint16_t* from = in.ptr + b * in.sb + t * in.st + at.h * in.sh;
+  const u32x4 x0 = *reinterpret_cast<const u32x4*>(from + at.v0 * 8), x1 = *reinterpret_cast<const u32x4*>(from + at.v1 * 8);
   make_angles<D>(a, n0, a.tile, cs);
   __syncthreads();
+  float f[16];
+  unpack8r<Tr>(x0, f);
+  unpack8r<Tr>(x1, f + 8);
+  if constexpr (NORM) {
+    float ss = 0.f;
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) {
-    const int tok = rl + u * a.lanes;
-    float f[16];
-    unpack8r<Tr>(x0[u], f);
-    unpack8r<Tr>(x1[u], f + 8);
-    if constexpr (NORM) {
-      float ss = 0.f;
+    for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
+    const float rstd = rsqrt_ulp(head_sum<L>(ss) * (1.0f / D) + a.eps);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
-      const float rstd = rsqrt_ulp(head_sum<L>(ss) * (1.0f / D) + a.eps);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] = f[e] * rstd * w[e];
-    }
-    if (live && n0 + tok < a.N) {
-      turn<INTERLEAVED>(f, cs[tok], at.c * 8, a.R / 2);
-      uint16_t* p = const_cast<uint16_t*>(out.ptr) + to[u];
-      __builtin_nontemporal_store(pack8r<Tr>(f), reinterpret_cast<u32x4*>(p + at.v0 * 8));
-      __builtin_nontemporal_store(pack8r<Tr>(f + 8), reinterpret_cast<u32x4*>(p + at.v1 * 8));
-    }
+    for (int e = 0; e < 16; ++e) f[e] = f[e] * rstd * w[e];
+  }
+  if (live && n0 + rl < a.N) {
+    turn<INTERLEAVED>(f, cs[rl], at.c * 8, a.R / 2);
+    uint16_t* p = const_cast<uint16_t*>(out.ptr) + b * out.sb + t * out.st + at.h * out.sh;
+    __builtin_nontemporal_store(pack8r<Tr>(f), reinterpret_cast<u32x4*>(p + at.v0 * 8));
+    __builtin_nontemporal_store(pack8r<Tr>(f + 8), reinterpret_cast<u32x4*>(p + at.v1 * 8));
   }
 }
 
 // Gradient of the norm and the rotation behind it.  A workgroup walks a strip of `tiles` tiles, kRotaryRows tokens of a thread each: a barrier and new angles
 // per tile, and always the rows of the next token on their way while those of one are used.
 template <typename Tr, int D, bool INTERLEAVED>
-__global__ __launch_bounds__(256, 2) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
+__global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
   constexpr int L = D / 16;
   __shared__ float2 cs[2][kRotaryRows * kRotaryLanes<D>][D / 2];
-  __shared__ __align__(16) float dw_s[256 * 16];
+  __shared__ __align__(16) float dw_s[kRotaryThreads * 16];
   const int tid = threadIdx.x;
   int rl, col;
   place<D>(a, rl, col);
@@ -268,7 +259,8 @@ __global__ __launch_bounds__(256, 2) void qk_norm_rotary_bwd_kernel(const Rotary
   }
 
   // the workgroup's sums in element order: row lanes, and with shared weights heads, one after the other
-  const int cols = a.cols > 256 ? min(256, a.cols - (int)blockIdx.y * 256) : a.cols, col0 = a.cols > 256 ? blockIdx.y * 256 : 0;
+  const bool wide = a.cols > kRotaryThreads;
+  const int cols = wide ? min(kRotaryThreads, a.cols - (int)blockIdx.y * kRotaryThreads) : a.cols, col0 = wide ? blockIdx.y * kRotaryThreads : 0;
   if (live) {
     float* p = dw_s + rl * cols * 16 + (col - col0) / L * D;
 #pragma unroll
@@ -300,22 +292,20 @@ __global__ __launch_bounds__(256, 2) void qk_norm_rotary_bwd_kernel(const Rotary
 }
 
 namespace {
-// How a call over `tokens` tokens is cut: columns, workgroups' worth of them, row lanes of a workgroup, tokens a thread holds, tokens a tile, tiles a workgroup.
+// How a call over `tokens` tokens is cut: columns, workgroups' worth of them, row lanes of a workgroup, tokens a tile, tiles a workgroup.
 struct RotaryPlan {
-  int cols, chunks, lanes, rows, tile, tiles;
+  int cols, chunks, lanes, tile, tiles;
   int64_t strips;
 };
 RotaryPlan rotary_plan(int64_t tokens, int heads, int D, bool bwd) {
   RotaryPlan p;
   p.cols = heads * (D / 16);
-  p.chunks = (p.cols + 255) / 256;
-  p.lanes = p.cols > 256 ? 1 : 256 / p.cols;
+  p.chunks = (p.cols + kRotaryThreads - 1) / kRotaryThreads;
+  p.lanes = p.cols > kRotaryThreads ? 1 : kRotaryThreads / p.cols;
   // as many as LDS holds the angles of: two workgroups a CU in the backward.  A quarter of them, us: few heads leave workgroups of one or two waves (norm and rotation with
   // gradients B8 T4096 H1 D128 43.2 / 28.9, rotation B8 T16000 H1 D64 15.1 / 11.9, B8 T8000 H2 D128 16.3 / 15.0; B33 T9954 H3 D32 29.4 / 31.7, more heads the same)
   if (p.lanes > 2048 / D) p.lanes = 2048 / D;   // kRotaryLanes
-  // forward: four tokens a thread where that still makes four workgroups a CU
-  p.rows = bwd || tokens * p.chunks >= (int64_t)p.lanes * kRotaryRows * 4 * kCus ? kRotaryRows : 1;
-  p.tile = p.lanes * p.rows;
+  p.tile = p.lanes * (bwd ? kRotaryRows : 1);
   // backward: strips for two workgroups a CU, at once; as many partial weight gradients as one launch adds
   const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? (tiles * p.chunks + 2 * kCus - 1) / (2 * kCus) : 1;
   p.tiles = (int)per;
@@ -344,18 +334,13 @@ static hipError_t launch_rotary_d(const RotaryK& args, bool norm, bool interleav
   a.by_cols = divisor(p.cols);
   a.by_lanes = divisor(p.lanes);
   a.tokens_first = a.side[0].in.st < a.side[0].in.sh;
-  const dim3 grid((unsigned)p.strips, (unsigned)p.chunks), block(p.cols > 256 ? 256u : (unsigned)((p.cols * p.lanes + 63) / 64 * 64));
+  const unsigned threads = p.cols > kRotaryThreads ? kRotaryThreads : (p.cols * p.lanes + 63) / 64 * 64;
+  const dim3 grid((unsigned)p.strips, (unsigned)p.chunks), block(threads);
   if (!bwd) {
-    auto launch = [&](auto n, auto i) {
-      if (p.rows == 1) hipLaunchKernelGGL((rotary_kernel<Tr, D, decltype(n)::value, decltype(i)::value, 1>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((rotary_kernel<Tr, D, decltype(n)::value, decltype(i)::value, kRotaryRows>), grid, block, 0, s, a);
-    };
-    const std::true_type yes;
-    const std::false_type no;
-    if (norm && interleaved) launch(yes, yes);
-    else if (norm) launch(yes, no);
-    else if (interleaved) launch(no, yes);
-    else launch(no, no);
+    if (norm && interleaved) hipLaunchKernelGGL((rotary_kernel<Tr, D, true, true>), grid, block, 0, s, a);
+    else if (norm) hipLaunchKernelGGL((rotary_kernel<Tr, D, true, false>), grid, block, 0, s, a);
+    else if (interleaved) hipLaunchKernelGGL((rotary_kernel<Tr, D, false, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((rotary_kernel<Tr, D, false, false>), grid, block, 0, s, a);
     return hipGetLastError();
   }
   if (interleaved) hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<Tr, D, true>), grid, block, 0, s, a);
