@@ -278,6 +278,8 @@ int make_rotary(const fox_rotary_args* a, fox::RotaryK& k, bool bwd) {
     k.side[i].out = to_view(bwd ? s.dx : s.y);
     heads += s.H;
   }
+  // 2^30 threads of sixteen elements and as many again that a workgroup leaves idle: a launch may have 2^32
+  if ((int64_t)a->B * a->T * heads * a->D > (int64_t)1 << 34) return fail(FOX_E_ARG, "the sides together must have at most 2^34 elements");
   if (bwd && norm) {
     if (!a->dweight || !a->workspace) return fail(FOX_E_ARG, "dweight and workspace must not be NULL");
     if ((uintptr_t)a->workspace & 15) return fail(FOX_E_ALIGN, "workspace must be 16-byte aligned");

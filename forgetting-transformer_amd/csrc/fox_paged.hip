@@ -278,7 +278,7 @@ __device__ __forceinline__ PagedShare share_of(const PagedDecodeK& a, int b, int
 // 300 keys 14.6 / 12.0, 1024 of them 25.4 / 19.0, 512 of 700 23.6 / 20.4, D 128, 512 of 150 to 300 18.7 / 16.1, 1024 of 300 39.7 / 32.4.
 template <int D>
 __device__ __forceinline__ int choose_batches(const PagedDecodeK& a, double total, int most) {
-  const int c = max((int)fmin(ceil(total * a.H * a.per_piece), 1 << 24), 1);   // (no row has more batches)
+  const int c = max((int)fmin(ceil(total * a.H * a.per_piece), a.max_keys / paged_batch(D) + 1), 1);   // (no row has more batches)
   if (most <= c || most > 8) return c;
   const float load = (float)total * a.H / 1024.f, rows = (float)a.B * a.H / 1024.f, full = (float)total / ((float)a.B * most);
   const float split = fmaxf(10.f * load, 1.8f * c) + 3.f * fmaxf(load / c, 1.f) + 1.5f;

@@ -429,7 +429,7 @@ int fox_auto_threshold_scan_one_launch(const fox_dims* dims, int32_t* yes);
  * A side is one 16-bit (B, T, H, D) tensor with views like q (stride_t the token's, stride_h the head's) and a head count of its own; two sides
  * (queries and keys) share B, T, D and the positions, one side alone has sides = 1.  The weights are fp32, `weight_stride_h` = D apart for the
  * heads or 0 where one row of D serves them all, on both sides or on neither.  D is one of 16, 32, 64, 128; rotary_dim is positive, at most D, even when interleaved and a
- * multiple of 16 otherwise.  positions: int64 with element strides, or NULL for first_position, first_position + 1, ...
+ * multiple of 16 otherwise.  positions: int64 with element strides, or NULL for first_position, first_position + 1, ...  At most 2^30 tokens and 2^34 elements of the sides together.
  */
 typedef struct fox_rotary_side {
   int32_t H;

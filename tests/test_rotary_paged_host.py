@@ -48,7 +48,8 @@ def test_rotary_c_abi_checks():
     bwd = lambda **k: lib.fox_rotary_bwd(C.byref(args(**k)), None)
     for bad, text in ((dict(D=48), b"head dim"), (dict(R=24), b"rotary_dim"), (dict(R=0), b"rotary_dim"), (dict(R=80), b"rotary_dim"),
                       (dict(R=7, inter=1), b"rotary_dim"), (dict(sides=3), b"sides"), (dict(dtype=2), b"dtype"), (dict(B=0), b"B and T"), (dict(T=-1), b"B and T"),
-                      (dict(B=1 << 20, T=1 << 20), b"2^30"), (dict(H=0), b"heads"), (dict(x=None), b"x is NULL"), (dict(y=None), b"y is NULL"),
+                      (dict(B=1 << 20, T=1 << 20), b"2^30"), (dict(B=1 << 9, T=1 << 20, H=1), b"2^34"),
+                      (dict(B=1 << 9, T=1 << 20, D=16, R=16, st=16, H=3, sides=2), b"2^34"), (dict(H=0), b"heads"), (dict(x=None), b"x is NULL"), (dict(y=None), b"y is NULL"),
                       (dict(freq=None), b"inv_freq"), (dict(w=base, w_sh=5), b"weight_stride_h"), (dict(sides=2, w=base), b"both sides"),
                       (dict(sides=2, w1=base), b"both sides")):
         assert fwd(**bad) == -1 and text in lib.fox_last_error(), (bad, lib.fox_last_error())
