@@ -13,14 +13,14 @@
 // forms them once per token, in 64 bits up to the fraction of a turn (a position of 2^20 would leave 32-bit angles 4 digits),
 // and keeps cosine and sine in LDS.  A thread owns one column (tensor, head, sixteen elements).  Forward it takes one token: four
 // (or two) per thread, with all their rows in flight, keep fewer waves busy and pay only where the weights are long against the
-// rows (us, four / one, rotation B4 T4096 H12 D64 43.9 / 37.3, T50000 H1 D64 31.7 / 16.9, H16 D128 303 / 283, norm and rotation B4 T4096 H16 D128 190 / 181, H12 D64
-// 80.3 / 87.3; 30 shapes geomean 0.94; workgroups of 512 and 1024 threads 1.01 and 1.04 of it).  Backward it walks tokens, so the weights are loaded once and their gradient
+// rows (us, four / one, rotation B4 T16384 H12 D64 43.9 / 37.3, T50000 H1 D64 31.7 / 16.9, H16 D128 303 / 283, norm and rotation B4 T16384 H16 D128 190 / 181, H12 D64
+// 80.3 / 87.3; 30 shapes geomean 0.94; workgroups of 192, 384, 512 and 1024 threads 1.02, 1.00, 1.01 and 1.04 of it).  Backward it walks tokens, so the weights are loaded once and their gradient
 // stays in registers; partial gradients leave once per workgroup and are added in a fixed order.
 //
 // Rows are read through the caches, in which what the projections wrote a moment ago may still be, and written past them.  Norm and rotation, bf16 H16 D128, us by
 // loads / stores, both non-temporal, only the loads, neither, only the stores (as it is): forward B4 T512 10.1, 9.8, 8.6, 7.9, T1024 14.9, 15.2, 13.6, 12.4, T4096 48.8, 45.6, 47.1,
 // 48.8, T16384 179, 202, 178, 183; backward T512 24.7, 22.8, 21.6, 21.3, T4096 81.8, 74.6, 84.2, 68.5, T16384 315, 328, 332, 317.
-// Now 181 and 305 us at T16384 (5.9 and 5.3 TB/s; a copy runs at 5.2).
+// Now 177 and 306 us at T16384 (6.0 and 5.3 TB/s; a copy runs at 5.2).
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
 
