@@ -104,12 +104,13 @@ __device__ __forceinline__ void make_angles(const RotaryK& a, int64_t n0, int to
 // (not turned by zero: an infinite element would make its neighbour NaN).  Halves: all of the lane's pairs or none.
 template <bool INTERLEAVED>
 __device__ __forceinline__ void turn(float (&f)[16], const float2* cs, int first_pair, int half) {
+#pragma clang fp contract(off)
   if (first_pair >= half) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int ia = INTERLEAVED ? 2 * e : e, ib = INTERLEAVED ? 2 * e + 1 : 8 + e;
     const float2 t = cs[first_pair + e];
-    const float x = f[ia], y = f[ib], a = x * t.x - y * t.y, b = x * t.y + y * t.x;
+    const float x = f[ia], y = f[ib], a = fmaf(x, t.x, -(y * t.y)), b = fmaf(x, t.y, y * t.x);
     const bool in = !INTERLEAVED || first_pair + e < half;
     f[ia] = in ? a : x;
     f[ib] = in ? b : y;
@@ -209,7 +210,9 @@ __global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(c
     r.g0 = *reinterpret_cast<const u32x4*>(g + at.v0 * 8);
     r.g1 = *reinterpret_cast<const u32x4*>(g + at.v1 * 8);
   };
+  // Which products are fused into sums is written out: the compiler's choice differed between the copies of this code, so that a token's place in the strip showed in its last bit.
   auto use = [&](const Row& r, int n, const float2* angles) {
+#pragma clang fp contract(off)
     float x[16], g[16];
     unpack8r<Tr>(r.x0, x);
     unpack8r<Tr>(r.x1, x + 8);
@@ -219,17 +222,17 @@ __global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(c
     float ss = 0.f, s1 = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      ss += x[e] * x[e];
-      s1 += g[e] * w[e] * x[e];
+      ss = fmaf(x[e], x[e], ss);
+      s1 = fmaf(g[e] * w[e], x[e], s1);
     }
-    const float rstd = rsqrt_ulp(head_sum<L>(ss) * (1.0f / D) + a.eps);
+    const float rstd = rsqrt_ulp(fmaf(head_sum<L>(ss), 1.0f / D, a.eps));
     const float c1 = head_sum<L>(s1) * rstd * (1.0f / D);
     if (live && n < a.N) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float xhat = x[e] * rstd;
-        dw[e] += g[e] * xhat;
-        g[e] = (g[e] * w[e] - xhat * c1) * rstd;
+        dw[e] = fmaf(g[e], xhat, dw[e]);
+        g[e] = fmaf(g[e], w[e], -(xhat * c1)) * rstd;
       }
       const int b = divide(n, a.by_T), t = n - b * a.T;
       uint16_t* p = const_cast<uint16_t*>(out.ptr) + b * out.sb + t * out.st + at.h * out.sh;

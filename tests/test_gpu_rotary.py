@@ -223,6 +223,44 @@ def test_layouts_types_and_converted_arguments():
     assert torch.equal(qk_norm_rotary(x, k, odd, wk, freq)[0], qk_norm_rotary(x, k, odd.clone(), wk, freq)[0])
 
 
+def test_views_beyond_32_bits():
+    """Tokens whose rows lie further apart than 2^31 elements in all, forward and back, as packed ones."""
+    from forgetting_transformer import qk_norm_rotary, rotary, rotary_frequencies
+    T, H, D, gap = 600, 2, 64, 1 << 22
+    freq = rotary_frequencies(D, device="cuda")
+    mem = torch.empty(T * gap, dtype=torch.bfloat16, device="cuda")
+    far = [mem.as_strided((1, T, H, D), (T * gap, gap, D, 1), i * H * D) for i in range(4)]
+    near = [torch.randn(1, T, H, D, device="cuda").bfloat16() for _ in far]
+    for dst, src in zip(far, near):
+        dst.copy_(src)
+    assert torch.equal(rotary(far[0], freq), rotary(near[0], freq))
+    results = []
+    for q, k, dyq, dyk in (far, near):
+        leaves = [t.detach().requires_grad_() for t in (q, k)] + [torch.linspace(0.5, 1.5, D, device="cuda").requires_grad_() for _ in range(2)]
+        y = qk_norm_rotary(*leaves, freq)
+        results.append([*y, *torch.autograd.grad(y, leaves, [dyq, dyk])])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_many_tokens_as_their_parts():
+    """Rows do not depend on the call they are in: 2^24 and some tokens at once and in parts from their positions on."""
+    from forgetting_transformer import qk_norm_rotary, rotary, rotary_frequencies
+    T, D, cut = (1 << 24) + 77, 16, 1 << 19
+    freq, w = rotary_frequencies(D, device="cuda"), torch.linspace(0.5, 1.5, D, device="cuda")
+    x = torch.randn(1, T, 1, D, device="cuda").bfloat16()
+    k = x.flip(1)
+    y, (yq, yk) = rotary(x, freq), qk_norm_rotary(x, k, w, w, freq)
+    leaf = x.detach().requires_grad_()
+    (dx,) = torch.autograd.grad(qk_norm_rotary(leaf, k, w, w, freq)[0], leaf, k)
+    for at in (0, 5 * cut + 3, T - cut):
+        part = slice(at, at + cut)
+        assert torch.equal(y[:, part], rotary(x[:, part], freq, positions=at))
+        leaf = x[:, part].detach().requires_grad_()
+        pq, pk = qk_norm_rotary(leaf, k[:, part], w, w, freq, positions=at)
+        assert torch.equal(yq[:, part], pq) and torch.equal(yk[:, part], pk)
+        assert torch.equal(dx[:, part], torch.autograd.grad(pq, leaf, k[:, part])[0])
+
+
 def test_unused_outputs_second_derivatives_and_empty_calls():
     from forgetting_transformer import qk_norm_rotary, rotary, rotary_frequencies
     freq = rotary_frequencies(32, device="cuda")
