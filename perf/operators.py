@@ -11,7 +11,6 @@ A case is a dict of plain values.  ``op`` names the operator:
 
 ``draw_seed`` fixes what the amount of work depends on (how long each request is); everything else comes from the seed of ``prepare``.
 """
-import functools
 import math
 import random
 import sys
@@ -25,9 +24,7 @@ _DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 _EPS = 1e-5
 
 
-@functools.lru_cache(maxsize=None)
 def _ft():
-    """This repository's package: looked up once, as a program's import is, not in every pass."""
     pkg = str(Path.cwd() / "forgetting-transformer_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
