@@ -181,6 +181,7 @@ struct RotaryK {
   int64_t w_sh;              // weights of a head and the next: D, or 0 for one row of weights for all
   float* dw;                 // backward: of q's weights, then of k's
   float* dw_partial;
+  int dw_width;              // elements of dw, and of a row of dw_partial; set by the launcher
   int N, T, R;               // N = B * T tokens
   int sign;                  // -1: the other way round
   float eps;

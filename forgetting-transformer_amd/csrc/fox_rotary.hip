@@ -275,16 +275,16 @@ __global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(c
   __syncthreads();
   const int width = cols * 16;
   if (a.w_sh != 0) {
-    float* dst = a.dw_partial + (int64_t)blockIdx.x * a.cols * 16 + col0 * 16;
+    float* dst = a.dw_partial + (int64_t)blockIdx.x * a.dw_width + col0 * 16;
     for (int j = tid; j < width; j += blockDim.x) {
       float sum = dw_s[j];
       for (int r = 1; r < a.lanes; ++r) sum += dw_s[r * width + j];
       dst[j] = sum;
     }
   } else {
-    float* dst = a.dw_partial + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 2 * D;
+    float* dst = a.dw_partial + ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * a.dw_width;
     const int q_elems = min(max(a.side[0].H * D - col0 * 16, 0), width);   // of this workgroup's columns
-    for (int j = tid; j < 2 * D; j += blockDim.x) {
+    for (int j = tid; j < a.dw_width; j += blockDim.x) {   // (2 * D, or D of one side alone)
       const int k0 = j < D ? j : q_elems + j - D, k1 = j < D ? q_elems : width;
       float sum = 0.f;
       for (int r = 0; r < a.lanes; ++r)
@@ -332,6 +332,7 @@ static hipError_t launch_rotary_d(const RotaryK& args, bool norm, bool interleav
   a.lanes = p.lanes;
   a.tile = p.tile;
   a.tiles = p.tiles;
+  a.dw_width = a.w_sh != 0 ? heads * D : a.side[1].H > 0 ? 2 * D : D;   // what the caller's buffer holds: no more is written
   a.by_T = divisor(a.T);
   a.by_half = divisor(a.R / 2);
   a.by_cols = divisor(p.cols);
@@ -350,8 +351,7 @@ static hipError_t launch_rotary_d(const RotaryK& args, bool norm, bool interleav
   else hipLaunchKernelGGL((qk_norm_rotary_bwd_kernel<Tr, D, false>), grid, block, 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const bool shared = a.w_sh == 0;
-  return launch_reduce_rows(a.dw_partial, a.dw, shared ? p.strips * p.chunks : p.strips, shared ? 2 * D : heads * D, s);
+  return launch_reduce_rows(a.dw_partial, a.dw, a.w_sh == 0 ? p.strips * p.chunks : p.strips, a.dw_width, s);
 }
 
 template <typename Tr>

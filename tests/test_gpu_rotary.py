@@ -350,3 +350,46 @@ def test_c_entry():
     _lib.check(lib.fox_rotary_bwd(C.byref(args(none, view(y), view(back))), stream), "fox_rotary_bwd")
     assert torch.equal(back, rotary(y.contiguous(), freq, positions=-torch.arange(11, 41, device="cuda")))
     assert mem.abs().sum() == y.abs().sum()                              # nothing beside the view
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("sides", [1, 2])
+@pytest.mark.parametrize("B,T,H,D", [(2, 30, 5, 64), (1, 1, 1, 16), (1, 700, 40, 128)])
+def test_c_entry_norm_gradients_stay_in_their_buffers(B, T, H, D, sides, shared):
+    """Norm and rotation through the C entry with one side and with two: right gradients, and nothing behind dweight and the workspace."""
+    import ctypes as C
+    from forgetting_transformer import rotary_frequencies
+    from forgetting_transformer.ops import _lib
+    lib = _lib.load()
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x, dy = ([torch.randn(B, T, H, D, generator=gen, device="cuda").bfloat16() for _ in range(sides)] for _ in range(2))
+    w = [torch.rand(1 if shared else H, D, generator=gen, device="cuda") + 0.5 for _ in range(sides)]
+    y, dx = ([torch.empty_like(t) for t in x] for _ in range(2))
+    freq, eps, n = rotary_frequencies(16, device="cuda"), 1e-5, C.c_int64()
+    _lib.check(lib.fox_rotary_workspace_bytes(B * T, sides * H, D, shared, C.byref(n)), "fox_rotary_workspace_bytes")
+    used, guard = sides * w[0].numel(), 4 * D
+    dw = torch.full((used + guard,), 7.0, device="cuda")
+    ws = torch.full((n.value // 4 + guard,), 7.0, device="cuda")
+    view = lambda t: _lib.View(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
+    side = lambda i: _lib.RotarySide(H, view(x[i]), view(y[i] if forward else dy[i]), view(dx[i]), w[i].data_ptr()) if i < sides else _lib.RotarySide()
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for forward in (True, False):
+        args = _lib.RotaryArgs(sides, B, T, D, 0, 16, 0, (_lib.RotarySide * 2)(side(0), side(1)), 0 if shared else D, eps, freq.data_ptr(), None, 0, 0, 11,
+                               dw.data_ptr(), ws.data_ptr())
+        _lib.check((lib.fox_rotary_fwd if forward else lib.fox_rotary_bwd)(C.byref(args), stream), "fox_rotary")
+    assert (dw[used:] == 7.0).all() and (ws[n.value // 4:] == 7.0).all()
+    full = (11 + torch.arange(T, device="cuda")).expand(B, T)
+    for i in range(sides):
+        x64 = x[i].double()
+        rstd = (x64.square().mean(-1, keepdim=True) + eps).rsqrt()
+        xhat, dn = x64 * rstd, turned(dy[i].double(), full, freq, False, back=True)
+        out, gw = xhat * w[i].double(), dn * w[i].double()
+        check("y", y[i], turned(out, full, freq, False), 2.0 ** -18 * out.abs().amax(-1, keepdim=True), torch.bfloat16)
+        largest = rstd * gw.abs().amax(-1, keepdim=True) * (1 + xhat.abs().amax(-1, keepdim=True))
+        check("dx", dx[i], rstd * (gw - xhat * (gw * xhat).mean(-1, keepdim=True)), 2.0 ** -16 * largest, torch.bfloat16)
+        terms = dn * xhat
+        total, size = terms.sum((0, 1)), terms.abs().sum((0, 1))
+        if shared:
+            total, size = total.sum(0), size.sum(0)
+        got = dw[:used].view(sides, -1)[i].double()
+        assert ((got - total.reshape(-1)).abs() <= 2.0 ** -15 * size.reshape(-1) + 1e-30).all()
