@@ -81,6 +81,21 @@ __device__ __forceinline__ void place(const RotaryK& a, int& rl, int& col) {
   }
 }
 
+// Cosine and sine of a number of turns, to 2^-22 of their own magnitude: the hardware's are off by up to 1.25e-7, which is a thousandth of the sine
+// that a low frequency has at its first positions, more than fp16's rounding.  The nearest quarter turn is taken off in 64 bits; Taylor polynomials in
+// the rest r, at most half a quarter, x = r pi / 2: the first terms left out are x^11 / 11! and x^12 / 12!, below 2^-28 of the values.
+// (us, the hardware's / these: rotation B8 T16000 H1 D64 12.0 / 13.5, B8 T8000 H2 D128 15.0 / 16.1; from twelve heads on the same.)
+__device__ __forceinline__ float2 cos_sin_of_turns(double turns) {
+#pragma clang fp contract(off)
+  const double quarters = (turns - rint(turns)) * 4.0, nearest = rint(quarters);
+  const float x = (float)((quarters - nearest) * 1.5707963267948966), z = x * x;
+  const float s = fmaf(x * z, fmaf(z, fmaf(z, fmaf(z, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
+  const float c = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
+  const int q = (int)nearest;   // -2 .. 2
+  const float a = q & 1 ? s : c, b = q & 1 ? c : s;
+  return float2{(q + 1) & 2 ? -a : a, q & 2 ? -b : b};
+}
+
 // cos and sin of the tile's tokens, pair by pair.  Executed by the whole workgroup.
 template <int D>
 __device__ __forceinline__ void make_angles(const RotaryK& a, int64_t n0, int tokens, float2 (*cs)[D / 2]) {
@@ -92,10 +107,8 @@ __device__ __forceinline__ void make_angles(const RotaryK& a, int64_t n0, int to
       const int b = divide((int)n, a.by_T), t = (int)n - b * a.T;
       const int64_t pos = a.positions ? a.positions[b * a.p_sb + t * a.p_st] : a.first + t;
       const double turns = (double)pos * a.inv_freq[pair] * 0.15915494309189535;   // 1 / (2 pi)
-      // the hardware's sine and cosine of a fraction of a turn, off by at most 1.25e-7 over 2^22 of them (the library's, off by 5e-8, are some sixty
-      // instructions, which calls with few heads notice: B8 T16000 H1 D64 17.5 / 15.0 us, B8 T8000 H2 D128 19.0 / 16.5)
-      const float part = (float)(turns - rint(turns)), c = __builtin_amdgcn_cosf(part), s = __builtin_amdgcn_sinf(part);
-      cs[tok][pair] = float2{c, a.sign < 0 ? -s : s};
+      const float2 angle = cos_sin_of_turns(turns);
+      cs[tok][pair] = float2{angle.x, a.sign < 0 ? -angle.y : angle.y};
     }
   }
 }

@@ -393,3 +393,21 @@ def test_c_entry_norm_gradients_stay_in_their_buffers(B, T, H, D, sides, shared)
             total, size = total.sum(0), size.sum(0)
         got = dw[:used].view(sides, -1)[i].double()
         assert ((got - total.reshape(-1)).abs() <= 2.0 ** -15 * size.reshape(-1) + 1e-30).all()
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_small_angles_keep_their_digits(inter):
+    """Unit vectors turn into the cosine and the sine themselves: off by the output's rounding, 2^-22 of their own magnitude (not of the pair's: a low frequency's first
+    positions have sines of 1e-4) and what 64-bit arithmetic leaves of the angle, some 2^-51 of it."""
+    from forgetting_transformer import rotary, rotary_frequencies
+    T, D, dtype = 3000, 128, torch.float16
+    freq = rotary_frequencies(D, device="cuda")
+    x = torch.zeros(1, T, 1, D, device="cuda", dtype=dtype)
+    x[..., slice(0, D, 2) if inter else slice(0, D // 2)] = 1.0
+    for first in (0, -700, 1 << 20):
+        y = rotary(x, freq, positions=first, interleaved=inter)[0, :, 0].double()
+        theta = (first + torch.arange(T, device="cuda")).double()[:, None] * freq
+        for got, ref in zip((y[:, 0::2], y[:, 1::2]) if inter else (y[:, :D // 2], y[:, D // 2:]), (theta.cos(), theta.sin())):
+            bound = half_step(ref, dtype) * (1 + 2.0 ** -10) + 2.0 ** -22 * ref.abs() + 2.0 ** -50 * theta.abs()
+            err = (got - ref).abs()
+            assert (err <= bound).all(), f"{(err / bound).max().item():.3f} of its bound at {first}"
