@@ -135,8 +135,6 @@ __device__ __forceinline__ float head_sum(float x) {
   if constexpr (L > 1) return row_sum<L>(x);
   return x;
 }
-// 1 / sqrt(x) to an ulp, where 1.0f / sqrtf(x) is some thirty instructions (x is a mean square and eps)
-__device__ __forceinline__ float rsqrt_ulp(float x) { return __builtin_amdgcn_rsqf(x); }
 
 }  // namespace
 
@@ -172,7 +170,7 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryK a)
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) ss += f[e] * f[e];
-    const float rstd = rsqrt_ulp(head_sum<L>(ss) * (1.0f / D) + a.eps);
+    const float rstd = 1.0f / sqrtf(head_sum<L>(ss) * (1.0f / D) + a.eps);
 #pragma unroll
     for (int e = 0; e < 16; ++e) f[e] = f[e] * rstd * w[e];
   }
@@ -238,7 +236,7 @@ __global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(c
       ss = fmaf(x[e], x[e], ss);
       s1 = fmaf(g[e] * w[e], x[e], s1);
     }
-    const float rstd = rsqrt_ulp(fmaf(head_sum<L>(ss), 1.0f / D, a.eps));
+    const float rstd = 1.0f / sqrtf(fmaf(head_sum<L>(ss), 1.0f / D, a.eps));
     const float c1 = head_sum<L>(s1) * rstd * (1.0f / D);
     if (live && n < a.N) {
 #pragma unroll

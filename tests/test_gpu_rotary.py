@@ -411,3 +411,19 @@ def test_small_angles_keep_their_digits(inter):
             bound = half_step(ref, dtype) * (1 + 2.0 ** -10) + 2.0 ** -22 * ref.abs() + 2.0 ** -50 * theta.abs()
             err = (got - ref).abs()
             assert (err <= bound).all(), f"{(err / bound).max().item():.3f} of its bound at {first}"
+
+
+def test_norm_of_tiny_rows():
+    """Without eps the norm of a row does not depend on its magnitude, also where the mean square lies below the normal range of fp32 (2^-132 here, exact)."""
+    from forgetting_transformer import qk_norm_rotary, rms_norm, rotary_frequencies
+    D = 64
+    sign = torch.where(torch.rand(1, 9, 2, D, device="cuda") < 0.5, -1.0, 1.0).bfloat16()
+    freq = rotary_frequencies(D, device="cuda") * 0
+    w = torch.rand(2 * D, device="cuda") + 0.5
+    for scale in (1.0, 2.0 ** -60, 2.0 ** -66):
+        leaves = [(sign * scale).requires_grad_(), sign.clone().requires_grad_(), w.clone().requires_grad_(), w.clone().requires_grad_()]
+        yq, yk = qk_norm_rotary(*leaves, freq, eps=0.0)
+        assert torch.equal(yq, (sign * w.view(2, D)).bfloat16()) and torch.equal(yq, yk)
+        g = torch.autograd.grad([yq, yk], leaves, [sign, sign])
+        assert torch.equal(g[2], g[3])
+        assert torch.equal(g[0].double() * scale, g[1].double())
