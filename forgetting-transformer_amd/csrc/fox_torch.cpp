@@ -1121,9 +1121,13 @@ bool overlaps(const Tensor& a, const Tensor& b) {
   return (const char*)a.const_data_ptr() < end(b) && (const char*)b.const_data_ptr() < end(a);
 }
 
+// Pages of S tokens, W of them a request at most: what the kernels take (the Python functions say which limit is passed).
+bool page_size_ok(int64_t S) { return S >= 8 && S <= 4096 && (S & (S - 1)) == 0; }
+bool room_ok(int64_t W, int64_t S) { return W > 0 && page_size_ok(S) && W <= (1 << 30) / S; }
+
 // The integer arguments of page_slots and page_release: lengths (B), block_table (B, W), free_pages (P), free_count (1), none in another's memory,
 // nor `other`, which the calls read, in that of those that they write.
-bool page_state_ok(const Tensor* lengths, const Tensor* table, const Tensor* free_pages, const Tensor* free_count, const Tensor* other, bool in_place) {
+bool page_state_ok(const Tensor* lengths, const Tensor* table, const Tensor* free_pages, const Tensor* free_count, const Tensor* other, int64_t S, bool in_place) {
   if (!lengths || !on_current_gpu(*lengths) || !int32_ok(lengths, *lengths, 1) || !int32_ok(table, *lengths, 2) || !int32_ok(free_pages, *lengths, 1) ||
       !int32_ok(free_count, *lengths, 1) || !other || other->device() != lengths->device() || other->sizes() != lengths->sizes() || !other->is_contiguous())
     return false;
@@ -1133,7 +1137,7 @@ bool page_state_ok(const Tensor* lengths, const Tensor* table, const Tensor* fre
       if (overlaps(*all[i], *all[j])) return false;
   if (overlaps(*other, *table) || overlaps(*other, *free_pages) || (in_place && (overlaps(*other, *lengths) || overlaps(*other, *free_count)))) return false;
   const int64_t B = lengths->size(0), W = table->size(1), P = free_pages->size(0);
-  return B > 0 && B <= 4096 && table->size(0) == B && W > 0 && W <= INT32_MAX && P > 0 && P <= INT32_MAX && free_count->size(0) == 1 &&
+  return B > 0 && B <= 4096 && table->size(0) == B && room_ok(W, S) && P > 0 && P <= INT32_MAX && free_count->size(0) == 1 &&
          (B == 1 || table->stride(0) >= W);
 }
 
@@ -1149,8 +1153,8 @@ PyObject* py_page_slots(PyObject*, PyObject* const* o, Py_ssize_t n) {
     PyErr_Clear();
     return none();
   }
-  if (!page_state_ok(lengths, table, pages, count, fresh, in_place) || fresh->scalar_type() != at::kInt) return none();
-  if (T < 0 || T > INT32_MAX || S < 1 || S > INT32_MAX || !writable(*table) || (in_place && (!writable(*lengths) || !writable(*count)))) return none();
+  if (!page_state_ok(lengths, table, pages, count, fresh, S, in_place) || fresh->scalar_type() != at::kInt) return none();
+  if (T < 0 || T > INT32_MAX || !writable(*table) || (in_place && (!writable(*lengths) || !writable(*count)))) return none();
   Tensor out[7];
   {
     const pybind11::gil_scoped_release no_gil;
@@ -1208,8 +1212,8 @@ PyObject* py_page_release(PyObject*, PyObject* const* o, Py_ssize_t n) {
     PyErr_Clear();
     return none();
   }
-  if (!page_state_ok(lengths, table, pages, count, done, in_place) || done->scalar_type() != at::kBool) return none();
-  if (S < 1 || S > INT32_MAX || !writable(*pages) || (in_place && (!writable(*lengths) || !writable(*count)))) return none();
+  if (!page_state_ok(lengths, table, pages, count, done, S, in_place) || done->scalar_type() != at::kBool) return none();
+  if (!writable(*pages) || (in_place && (!writable(*lengths) || !writable(*count)))) return none();
   Tensor out[2];
   {
     const pybind11::gil_scoped_release no_gil;
@@ -1250,9 +1254,10 @@ PyObject* py_page_release(PyObject*, PyObject* const* o, Py_ssize_t n) {
 bool pages_ok(const Tensor* k, const Tensor* v, const Tensor* g, fox_pages& p) {
   if (!k || !v || !g || k->dim() != 4 || g->dim() != 3 || k->numel() == 0 || !on_current_gpu(*k) || !sixteen_bit(*k) || v->scalar_type() != k->scalar_type() ||
       g->scalar_type() != at::kFloat || v->device() != k->device() || g->device() != k->device() || v->sizes() != k->sizes() ||
-      g->sizes() != k->sizes().slice(0, 3) || !vectors_ok(*k) || !vectors_ok(*v) || !head_dim_ok(k->size(3)))
+      g->sizes() != k->sizes().slice(0, 3) || !vectors_ok(*k) || !vectors_ok(*v) || !head_dim_ok(k->size(3)) ||
+      !page_size_ok(k->size(2)))
     return false;
-  for (int i = 0; i < 3; ++i)
+  for (int i = 0; i < 2; ++i)
     if (k->size(i) > INT32_MAX) return false;
   p = fox_pages{};
   p.P = (int32_t)k->size(0);
@@ -1321,7 +1326,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   fox_paged_decode_args a{};
   if (!pages_ok(kp, vp, gp, a.pages) || !tokens_ok(q, a.pages, *kp) || !int32_ok(table, *kp, 2) || !int32_ok(lengths, *kp, 1)) return none();
   const int64_t B = q->size(0), W = table->size(1), S = a.pages.page_size;
-  if (lengths->size(0) != B || table->size(0) < 1 || W < 1 || table->size(0) > INT32_MAX || W * S > (1 << 30) || B * a.pages.H > (1 << 23)) return none();
+  if (lengths->size(0) != B || table->size(0) < 1 || table->size(0) > INT32_MAX || !room_ok(W, S) || B * a.pages.H > (1 << 23)) return none();
   const Tensor* requests = nullptr;
   if (o[6] != Py_None) {
     requests = tensor_of(o[6]);

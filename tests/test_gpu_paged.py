@@ -498,3 +498,24 @@ def test_c_entries():
     assert state.tolist() == [30, 5, 0] and count.tolist() == [4] and granted.tolist() == [True, True, False]
     assert slots.tolist()[:20] == [10 + i if i < 6 else 5 * 16 + i - 6 for i in range(20)] and set(slots.tolist()[20:]) == {-1}
     assert small.tolist()[0] == [0, 5, 2, 3] and keys.tolist()[:20] == list(range(11, 31)) and req.tolist()[20:] == [-1] * 1480
+
+
+def test_limits_are_assertions():
+    """Page sizes and widths that no kernel takes are refused like any wrong argument, on the GPU as on the CPU, before anything is written."""
+    from forgetting_transformer import page_release, page_slots, paged_append, paged_forgetting_attention
+    lengths, free, count = on_gpu([0, 0]), on_gpu([0, 1, 2, 3]), on_gpu([4])
+    done = torch.tensor([True, False], device="cuda")
+    wide = torch.zeros(1, 1 << 27, dtype=torch.int32, device="cuda")
+    for table, size in ((on_gpu([[0, 1], [2, 3]]), 4), (on_gpu([[0, 1], [2, 3]]), 24), (on_gpu([[0, 1], [2, 3]]), 8192), (wide, 16)):
+        state = (lengths[:len(table)], lengths[:len(table)] + 1, table, free, count)
+        with pytest.raises(AssertionError):
+            page_slots(*state, page_size=size, max_tokens=4)
+        with pytest.raises(AssertionError):
+            page_release(state[0], done[:len(table)], *state[2:], page_size=size)
+    for size in (4, 24, 8192):
+        kp, vp, fp, _ = pool(3, 1, size, 16, torch.bfloat16, 0)
+        x = torch.zeros(2, 1, 16, device="cuda").bfloat16()
+        with pytest.raises(AssertionError):
+            paged_append(x, x, torch.zeros(2, 1, device="cuda"), kp, vp, fp, torch.arange(2, device="cuda"))
+        with pytest.raises(AssertionError):
+            paged_forgetting_attention(x, kp, vp, fp, on_gpu([[0], [1]]), on_gpu([1, 1]))
