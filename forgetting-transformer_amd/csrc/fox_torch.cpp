@@ -1007,6 +1007,8 @@ bool rotary_ok(const Tensor* x) {
   return x && x->dim() == 4 && on_current_gpu(*x) && sixteen_bit(*x) && head_dim_ok(x->size(3)) && vectors_ok(*x);
 }
 
+constexpr int64_t kRotaryElements = (int64_t)1 << 34;   // of a call, at most
+
 // Fills `r` from the arguments both entry points share, for an x that rotary_ok() took; false: not a call for the native path.
 bool parse_rotary(Rotary& r, const Tensor& x, PyObject* inv_freq, PyObject* positions, PyObject* interleaved, PyObject* head_first) {
   if (!flag(interleaved, r.interleaved) || !flag(head_first, r.head_first)) return false;
@@ -1039,7 +1041,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
   TORCH_CHECK(n == 5, "rotary takes 5 arguments");
   const Tensor* x = tensor_of(o[0]);
   Rotary r;
-  if (!rotary_ok(x) || !parse_rotary(r, *x, o[1], o[2], o[3], o[4])) return none();
+  if (!rotary_ok(x) || x->numel() > kRotaryElements || !parse_rotary(r, *x, o[1], o[2], o[3], o[4])) return none();
   Tensor y;
   {
     const pybind11::gil_scoped_release no_gil;
@@ -1060,7 +1062,7 @@ PyObject* py_qk_norm_rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
   TORCH_CHECK(n == 9, "qk_norm_rotary takes 9 arguments");
   const Tensor *q = tensor_of(o[0]), *k = tensor_of(o[1]), *wq = tensor_of(o[2]), *wk = tensor_of(o[3]);
   Rotary r;
-  if (!rotary_ok(q) || !rotary_ok(k) || !wq || !wk || !parse_rotary(r, *q, o[4], o[5], o[6], o[8])) return none();
+  if (!rotary_ok(q) || !rotary_ok(k) || q->numel() + k->numel() > kRotaryElements || !wq || !wk || !parse_rotary(r, *q, o[4], o[5], o[6], o[8])) return none();
   const int ih = r.head_first ? 1 : 2, it = r.head_first ? 2 : 1;
   const int64_t D = q->size(3), Hq = q->size(ih), Hk = k->size(ih);
   if (k->scalar_type() != q->scalar_type() || k->device() != q->device() || k->size(0) != q->size(0) || k->size(it) != q->size(it) || k->size(3) != D ||

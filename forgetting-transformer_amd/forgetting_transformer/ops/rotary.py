@@ -57,6 +57,10 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
+def _check_size(elements: int) -> None:
+    assert elements <= 1 << 34, "at most 2**34 elements in one call"
+
+
 def _check_heads(t: torch.Tensor, name: str) -> torch.Tensor:
     assert t.dim() == 4, f"{name} must be (B, T, H, D), or (B, H, T, D) with head_first"
     assert t.dtype in _DTYPES, f"{name} must be bfloat16 or float16"
@@ -94,11 +98,12 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, *, positions: Positions = No
 
     x: ``(B, T, H, D)`` bfloat16/float16 (``(B, H, T, D)`` with ``head_first``), D one of 16, 32, 64, 128.  The pairs are ``(i, i + R/2)``,
     R a multiple of 16, or ``(2i, 2i+1)`` with ``interleaved``, R even.  positions: integers ``(T,)``, ``(B, T)`` or ``(B, 1)``, the first position
-    as a number, or None (0, 1, ...).  Differentiable with respect to ``x``, any number of times.
+    as a number, or None (0, 1, ...).  At most 2**30 tokens and 2**34 elements.  Differentiable with respect to ``x``, any number of times.
     """
     y = _native.load().rotary(x, inv_freq, positions, interleaved, head_first)   # None: not a call for the native path as it is
     if y is not None:
         return y
+    _check_size(x.numel())
     x = _check_heads(x, "x")
     inv_freq, positions = _check_angles(x, inv_freq, positions, interleaved, head_first)
     with torch.cuda.device(x.device):
@@ -118,6 +123,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     out = _native.load().qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, positions, interleaved, eps, head_first)
     if out is not None:
         return out
+    _check_size(q.numel() + k.numel())
     q, k = _check_heads(q, "q"), _check_heads(k, "k")
     heads = 1 if head_first else 2
     assert q.dtype == k.dtype and q.device == k.device, "q and k must have the same type and device"

@@ -427,3 +427,17 @@ def test_norm_of_tiny_rows():
         g = torch.autograd.grad([yq, yk], leaves, [sign, sign])
         assert torch.equal(g[2], g[3])
         assert torch.equal(g[0].double() * scale, g[1].double())
+
+
+def test_too_many_elements():
+    """Refused as an argument, before anything is allocated for the result."""
+    from forgetting_transformer import qk_norm_rotary, rotary, rotary_frequencies
+    freq, w = rotary_frequencies(128, device="cuda"), torch.ones(128, device="cuda")
+    x = torch.zeros(1, 1, 1, 128, device="cuda").bfloat16()
+    before = torch.cuda.max_memory_allocated()
+    for wide, part in ((x.expand(1 << 14, 1 << 12, 3, 128), x.expand(1 << 14, 1 << 12, 2, 128)), (x.expand(1 << 15, 1 << 12, 2, 128), x.expand(1 << 15, 1 << 12, 1, 128))):
+        with pytest.raises(AssertionError, match="elements"):
+            rotary(wide, freq)
+        with pytest.raises(AssertionError, match="elements"):
+            qk_norm_rotary(part, part if wide.shape[2] == 3 else wide, w, w, freq)
+    assert torch.cuda.max_memory_allocated() == before
