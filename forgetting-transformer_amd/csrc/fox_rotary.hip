@@ -320,7 +320,8 @@ RotaryPlan rotary_plan(int64_t tokens, int heads, int D, bool bwd) {
   // gradients B8 T4096 H1 D128 43.2 / 28.9, rotation B8 T16000 H1 D64 15.1 / 11.9, B8 T8000 H2 D128 16.3 / 15.0; B33 T9954 H3 D32 29.4 / 31.7, more heads the same)
   if (p.lanes > 2048 / D) p.lanes = 2048 / D;   // kRotaryLanes
   p.tile = p.lanes * (bwd ? kRotaryRows : 1);
-  // backward: strips for two workgroups a CU, at once; as many partial weight gradients as one launch adds
+  // backward: strips for two workgroups a CU, at once.  With heads of several workgroups (chunks) that share weights up to 512 + chunks partial
+  // gradients, more than one launch of the reduction adds.
   const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? (tiles * p.chunks + 2 * kCus - 1) / (2 * kCus) : 1;
   p.tiles = (int)per;
   p.strips = (tiles + per - 1) / per;

@@ -441,3 +441,25 @@ def test_too_many_elements():
         with pytest.raises(AssertionError, match="elements"):
             qk_norm_rotary(part, part if wide.shape[2] == 3 else wide, w, w, freq)
     assert torch.cuda.max_memory_allocated() == before
+
+
+def test_weight_gradient_in_two_launches():
+    """Heads of several workgroups that share weights: more partial rows than one launch adds (512 and some), here 513 and the two groups' sums behind them."""
+    import ctypes as C
+    from forgetting_transformer import qk_norm_rotary, rotary_frequencies
+    from forgetting_transformer.ops import _lib
+    B, T, H, D = 1, 15000, 40, 128
+    n = C.c_int64()
+    _lib.check(_lib.load().fox_rotary_workspace_bytes(B * T, 2 * H, D, 1, C.byref(n)), "fox_rotary_workspace_bytes")
+    assert n.value > 512 * 2 * D * 4
+    q, dyq, _, full = inputs(B, T, H, D, torch.bfloat16, 9, False, "none")
+    k, dyk, _, _ = inputs(B, T, H, D, torch.bfloat16, 10, False, "none")
+    freq = rotary_frequencies(D, device="cuda")
+    leaves = [t.requires_grad_() for t in (q, k, *(torch.rand(D, device="cuda") + 0.5 for _ in range(2)))]
+    first = torch.autograd.grad(qk_norm_rotary(*leaves, freq), leaves, [dyq, dyk])
+    again = torch.autograd.grad(qk_norm_rotary(*leaves, freq), leaves, [dyq, dyk])
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    for x, dy, dw in ((q, dyq, first[2]), (k, dyk, first[3])):
+        x64 = x.detach().double()
+        terms = turned(dy.double(), full, freq, False, back=True) * x64 * (x64.square().mean(-1, keepdim=True) + 1e-5).rsqrt()
+        assert ((dw.double() - terms.sum((0, 1, 2))).abs() <= 2.0 ** -15 * terms.abs().sum((0, 1, 2))).all()
