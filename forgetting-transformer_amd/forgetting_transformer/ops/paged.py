@@ -72,7 +72,8 @@ def page_slots(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: tor
 
     The tokens of a step lie one request after the other in ``max_tokens`` places.  New pages come from the top of the stack, in request order, and their numbers go
     into ``block_table`` (in place).  A request gets all its tokens or none (``granted``): none if they end behind ``max_tokens``, if it would need more than W pages or if the
-    stack does not hold its pages and those of the requests in front of it; then its length stays and its tokens have no slot.  Places that hold no token, and tokens without a slot,
+    stack does not hold its pages and those of the requests in front of it; then its length stays and its tokens have no slot.  A request without new tokens ends where the one in
+    front of it ends, so it counts as refused behind ``max_tokens`` too, though nothing of it changes: who preempts by this asks for ``granted | (new_tokens == 0)``.  Places that hold no token, and tokens without a slot,
     have slot and request -1 and see no keys.  ``in_place`` writes the new state into ``lengths`` and ``free_count`` (what a captured step needs), else both are new tensors and the call can be repeated.
     """
     ext = _native.load()

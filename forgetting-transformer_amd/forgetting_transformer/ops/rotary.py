@@ -97,8 +97,10 @@ def rotary(x: torch.Tensor, inv_freq: torch.Tensor, *, positions: Positions = No
     """``x`` with the first ``2 * len(inv_freq)`` elements of every head rotated by ``positions * inv_freq``.
 
     x: ``(B, T, H, D)`` bfloat16/float16 (``(B, H, T, D)`` with ``head_first``), D one of 16, 32, 64, 128.  The pairs are ``(i, i + R/2)``,
-    R a multiple of 16, or ``(2i, 2i+1)`` with ``interleaved``, R even.  positions: integers ``(T,)``, ``(B, T)`` or ``(B, 1)``, the first position
-    as a number, or None (0, 1, ...).  At most 2**30 tokens and 2**34 elements.  Differentiable with respect to ``x``, any number of times.
+    R a multiple of 16, or ``(2i, 2i+1)`` with ``interleaved``, R even.  positions: the first position as a number p (p, p + 1, ...), None (0, 1, ...),
+    or integers ``(T,)``, ``(B, T)`` or ``(B, 1)`` that are the positions themselves, not offsets: ``(B, 1)`` is one position for all tokens of a row, and tokens that follow
+    each other from a start of their own per row are ``start[:, None] + torch.arange(T)``.  At most 2**30 tokens and 2**34 elements.  Differentiable with
+    respect to ``x``, any number of times.
     """
     y = _native.load().rotary(x, inv_freq, positions, interleaved, head_first)   # None: not a call for the native path as it is
     if y is not None:

@@ -10,6 +10,8 @@ and one stack of free pages, since a token has the same slot in each; every laye
         out = cache.attend(q[0], layer)
 
 and ``cache.release(done)`` gives a request's pages back.  Nothing waits for the device, and the state stays in the same tensors, so a step can be captured.
+It keeps no states of a token shift (``FgateDynamicCache`` does), and ``token_shift`` takes whole batches, not a step of several requests' tokens: layers
+with the shift are not served from pages.
 """
 from __future__ import annotations
 

@@ -429,7 +429,7 @@ int fox_auto_threshold_scan_one_launch(const fox_dims* dims, int32_t* yes);
  * A side is one 16-bit (B, T, H, D) tensor with views like q (stride_t the token's, stride_h the head's) and a head count of its own; two sides
  * (queries and keys) share B, T, D and the positions, one side alone has sides = 1.  The weights are fp32, `weight_stride_h` = D apart for the
  * heads or 0 where one row of D serves them all, on both sides or on neither.  D is one of 16, 32, 64, 128; rotary_dim is positive, at most D, even when interleaved and a
- * multiple of 16 otherwise.  positions: int64 with element strides, or NULL for first_position, first_position + 1, ...  At most 2^30 tokens and 2^34 elements of the sides together.
+ * multiple of 16 otherwise.  positions: int64, of token (b, t) at b * position_stride_b + t * position_stride_t, or NULL for first_position, first_position + 1, ...  At most 2^30 tokens and 2^34 elements of the sides together.
  */
 typedef struct fox_rotary_side {
   int32_t H;
@@ -475,7 +475,8 @@ typedef struct fox_pages {
  * Pages and slots of a step's new tokens, max_tokens of them, those of one request after those of the one before it: request b brings new_tokens[b] to the lengths[b]
  * that it has cached.  slots, positions, requests and keys (max_tokens each) get every token's slot, its position in its request, the request and the tokens of it up to this one; new pages come from the top of the stack in
  * request order and go into block_table.  A request is refused, whole, if its tokens end behind max_tokens, if it would need more than W pages, or if the stack
- * does not hold its pages and those of the requests in front of it: its tokens get slot -1, request -1 and 0 keys, its length stays and granted[b] is 0.  Places behind the last token get slot -1,
+ * does not hold its pages and those of the requests in front of it: its tokens get slot -1, request -1 and 0 keys, its length stays and granted[b] is 0.  (A request of no
+ * tokens ends where the one before it does, and is refused behind max_tokens as well.)  Places behind the last token get slot -1,
  * position 0, request -1, 0 keys.  lengths_out and free_count_out may be lengths and free_count (both, or neither).  At most 4096 requests.
  */
 typedef struct fox_page_slots_args {
