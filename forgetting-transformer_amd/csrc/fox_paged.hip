@@ -43,8 +43,9 @@ struct Request {   // of a page_slots, in LDS
 
 }  // namespace
 
-// Every workgroup scans the requests (8 bytes each, from the L2) and serves 1024 tokens; the first one writes the requests' new state.  Bound by
-// latency: the state's round trip, a scan, a binary search in LDS and the round trip of the page; 3.6 us for 4 requests' tokens, 4.1 for 256, where a copy of as much takes 2.2.
+// Every workgroup scans the requests (8 bytes each, from the L2) and serves 1024 tokens; the first one writes the requests'
+// new state.  Bound by latency: the state's round trip, a scan, a binary search in LDS and the round trip of the page; 3.8 us for 256
+// requests' next tokens, 5.2 for 16384 tokens of 64 requests, where a copy of as much takes 2.2.
 __global__ __launch_bounds__(1024) void page_slots_kernel(const PageSlotsK a) {
   __shared__ Request req[kPageRequests];
   __shared__ double waves[2][16];
@@ -65,8 +66,8 @@ __global__ __launch_bounds__(1024) void page_slots_kernel(const PageSlotsK a) {
     }
     const int held = (int)(((int64_t)len + S - 1) >> a.shift);
     const int64_t wanted = ((int64_t)len + fresh + S - 1) >> a.shift, need = wanted - held;
-    // A request that fits no row of the table takes no pages.  One whose tokens end behind the last place takes none either, but all behind it end there as well, so that nobody
-    // who is served counts on it.
+    // A request that fits no row of the table takes no pages.  One whose tokens end behind the last place takes none either,
+    // but all behind it end there as well, so that nobody who is served counts on it.
     const Sums sum = block_scan(fresh, wanted <= a.W ? (double)need : 0.0, waves);
     const double end = tokens + sum.x, taken = pages + sum.y;
     tokens += sum.all_x;
@@ -137,8 +138,8 @@ hipError_t launch_page_slots(const PageSlotsK& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-// The pages of finished requests back on the stack, request by request, a wave each (a page a thread, which looks its request up as page_slots_kernel's tokens do: a quarter of 512
-// requests with 62 pages each 7.9 us, so 6.6).
+// The pages of finished requests back on the stack, request by request, a wave each (a quarter of 512 requests with 62 pages
+// each 6.6 us; a page a thread, which looks its request up as page_slots_kernel's tokens do, 7.9).
 __global__ __launch_bounds__(1024) void page_release_kernel(const PageReleaseK a) {
   __shared__ int32_t place[kPageRequests], held_s[kPageRequests];
   __shared__ double waves[2][16];
@@ -177,9 +178,9 @@ hipError_t launch_page_release(const PageReleaseK& a, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // New tokens' keys, values and log gates into their slots: one 16-byte piece of k and the same piece of v per thread, the thread with a row's
-// first piece also moves its gate.  A plain stream, read through the caches (the projections have just written it) and written past them (the attention reads all of the cache before it
-// comes back to these rows): H16 D128, us, loads non-temporal / stores too / neither / the stores only, as it is: 2048 tokens 9.0 / 8.2 / 7.7 / 7.2, 8192 25.7 / 27.1 / 28.0 / 24.2, 16384
-// 53.2 / 51.4 / 52.6 / 51.0 (5.3 TB/s); 48 tokens 2.5.  Slots outside the pool are left out.
+// first piece also moves its gate.  A plain stream, read through the caches (the projections have just written it) and
+// written past them (the attention reads all of the cache before it comes back to these rows; both past them / as it is,
+// H16 D128, 2048 tokens 8.2 / 7.2 us).  16384 tokens take 49 us (5.5 TB/s), 48 of H12 D64 3.2.  Slots outside the pool are left out.
 template <int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendK a) {
   constexpr int CH = D / 8;
@@ -220,15 +221,18 @@ hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s) {
 // gates behind it (fp64, rounded once per key) relative to the end of the run; where runs are merged their totals shift the maxima of those in front,
 // so every gate is read once.
 //
-// How long the requests are only the device knows.  Every wave works out the same plan from the lengths: batches of four waves' loads, at
-// most kPagedPieces pieces of c batches over all requests and heads together, so that requests of very different lengths still give the
-// workgroups the same share; a workgroup past the last piece ends.  For many rows a launch in front makes the plan once.
+// How long the requests are only the device knows.  Every wave works out the same plan from the lengths: batches of four
+// waves' loads, pieces of c batches, with c chosen so that all rows and heads together fill at most kPagedPieces of them: requests of
+// very different lengths still give the workgroups the same share.  Every (row, head) may add a piece that is not full, so there are up to
+// kPagedPieces + B * H pieces, which is what the grid and the workspace are sized for; a workgroup past the last one ends.
+// For many rows a launch in front makes the plan once.
 //
-// 16 requests of 24576 to 32768 tokens, H16 D128, 580 us: 6.3 TB/s, where a stream that is only read reaches 7.1; 48 requests of up to 8192 tokens, H12 D64, 42.0 us and 4.6 of the
-// merge (5.3 TB/s); one request of 1500 tokens 6.0 us, a chain of four round trips (lengths, table, rows, partials), and 3.7 of the merge.
+// 16 requests of 24576 to 32768 tokens, H16 D128, 572 us: 6.4 TB/s, where a stream that is only read reaches 7.1; 48
+// requests of up to 8192 tokens, H12 D64, 42.1 us and 4.6 of the merge (5.3 TB/s); one request of 1500 tokens, H12 D64, 6.9 us, a
+// chain of four round trips (lengths, table, rows, partials), and 3.7 of the merge.
 //
-// A lane holds the table's entry for one of 64 consecutive pages and takes a row's page from the lane that has it; the entries are read again every 64 pages.
-// Entries outside the pool name no page: their keys are left out and their gates count as 0.
+// A lane holds the table's entry for one of 64 consecutive pages and takes a row's page from the lane that has it; the
+// entries are read again every 64 pages.  Entries outside the pool name no page: their keys are left out and their gates count as 0.
 namespace {
 
 template <typename Tr>
@@ -272,10 +276,11 @@ __device__ __forceinline__ PagedShare share_of(const PagedDecodeK& a, int b, int
   return s;
 }
 
-// Batches a piece.  All rows and heads together make at most about kPagedPieces of them; short rows stay whole where splitting them brings no more than a merge and starts of
-// workgroups.  Both ways in us, from the batches that each of the 1024 workgroups that run at once gets (`load`): 10 for the bytes of one batch each at 6.5 TB/s or 1.8 for each
-// of a run's round trips, 3 for every 1024 workgroups that start, 1.5 for the merge, 3 a batch for the longest rows' tail.  Pages of 16, us, split / as it is now: D 64, 512 requests and heads of
-// 300 keys 14.6 / 12.0, 1024 of them 25.4 / 19.0, 512 of 700 23.6 / 20.4, D 128, 512 of 150 to 300 18.7 / 16.1, 1024 of 300 39.7 / 32.4.
+// Batches a piece.  All rows and heads together fill at most kPagedPieces pieces; short rows stay whole where splitting
+// them brings no more than a merge and starts of workgroups.  Both ways in us, from the batches that each of the 1024
+// workgroups that run at once gets (`load`): 10 for the bytes of one batch each at 6.5 TB/s or 1.8 for each of a run's round
+// trips, 3 for every 1024 workgroups that start, 1.5 for the merge, 3 a batch for the longest rows' tail.  Pages of 16, us,
+// split / as it is: D 64, 1024 requests and heads of 300 keys 25.4 / 19.0, 512 of 700 23.6 / 20.4, D 128, 1024 of 300 39.7 / 32.4.
 template <int D>
 __device__ __forceinline__ int choose_batches(const PagedDecodeK& a, double total, int most) {
   const int c = max((int)fmin(ceil(total * a.H * a.per_piece), a.max_keys / paged_batch(D) + 1), 1);   // (no row has more batches)
@@ -308,7 +313,8 @@ struct PagedPiece {
   int b, piece, first;   // row, its piece, and the row's first piece among all (of one head)
   PagedShare share;
 };
-// The row that piece number p (of one head) belongs to; b < 0: there is none.  The result is the same in all lanes, and in all workgroups, which run this same code.
+// The row that piece number p (of one head) belongs to; b < 0: there is none.  The result is the same in all lanes, and in
+// all workgroups, which run this same code.
 template <int D>
 __device__ __forceinline__ PagedPiece find_piece(const PagedDecodeK& a, int p, int lane) {
   PagedPiece r;
@@ -450,8 +456,9 @@ __global__ __launch_bounds__(256) void paged_decode_kernel(const PagedDecodeK a)
       gx[s] = gp[max(page, 0) * pg.g_sp + (n & in_page) * pg.g_ss];
       if (j >= KPB || end - 1 - j < first || page < 0) gx[s] = 0.f;
     }
-    // The fences keep one row's addresses in registers at a time: 119 to 127 registers, four workgroups a CU (131 to 135 and three at head dims 32 and 64 without them, 36 shapes geomean 1.036 of the time; all rows' pages asked
-    // for first, since a page takes as long as an LDS read).
+    // The fences keep one row's addresses in registers at a time: 119 to 127 registers, four workgroups a CU (without them 131
+    // to 135 and three at head dims 32 and 64, 36 shapes geomean 1.036 of the time; all rows' pages asked for first, since a
+    // page takes as long as an LDS read).
     u32x4 kx[U], vx[U];
     uint32_t ok = 0;
     int pages[U];
@@ -606,7 +613,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedDecodeK a) 
   *reinterpret_cast<u32x2*>(a.o + b * a.o_sb + h * a.o_sh + d) = w;
 }
 
-// Pieces of all rows and heads together, about: eight workgroups a CU.  4, 6, 12 and 16 instead of 8: geomean of 36 shapes 1.014, 1.010, 1.004, 1.011 of the time.
+// Full pieces of all rows and heads together, at most: eight workgroups a CU.  4, 6, 12 and 16 instead of 8: geomean of 36
+// shapes 1.014, 1.010, 1.004, 1.011 of the time.
 constexpr int kPagedPieces = 8 * kCus;
 
 static int64_t most_pieces(int max_keys, int D) {   // of a row
@@ -624,8 +632,8 @@ template <typename Tr, int D>
 static hipError_t launch_paged_decode_d(const PagedDecodeK& args, hipStream_t s) {
   PagedDecodeK a = args;
   a.per_piece = 1.0 / kPagedPieces;
-  // Up to 255 rows every wave works the plan out from the lengths, 64 at a time, which a launch of its own would not make up for (300 keys, H8 D64, us, waves / launch: 256 rows 41.0 / 40.4, 384
-  // 64.5 / 55.6, 1024 216 / 142; 64 rows take 12.2).
+  // Up to 255 rows every wave works the plan out from the lengths, 64 at a time, which a launch of its own would not make
+  // up for (300 keys, H8 D64, us, waves / launch: 256 rows 41.0 / 40.4, 384 64.5 / 55.6, 1024 216 / 142; 64 rows take 12.2).
   a.planned = a.ws_row && a.B >= 256;
   if (a.planned) hipLaunchKernelGGL(paged_plan_kernel<D>, dim3(1), dim3(1024), 0, s, a);
   hipLaunchKernelGGL((paged_decode_kernel<Tr, D>), dim3((unsigned)paged_decode_workgroups(a.B, a.H, a.max_keys, D)), dim3(256), 0, s, a);

@@ -11,16 +11,14 @@
 // every pair are in the lane: vectors c and c + R/16 of the rotated part (2c and 2c+1 interleaved, and beyond the rotated
 // part).  Row sums are DPP adds over the D/16 lanes of a head.  The angles are the same for all heads of a token: a workgroup
 // forms them once per token, in 64 bits up to the fraction of a turn (a position of 2^20 would leave 32-bit angles 4 digits),
-// and keeps cosine and sine in LDS.  A thread owns one column (tensor, head, sixteen elements).  Forward it takes one token: four
-// (or two) per thread, with all their rows in flight, keep fewer waves busy and pay only where the weights are long against the
-// rows (us, four / one, rotation B4 T16384 H12 D64 43.9 / 37.3, T50000 H1 D64 31.7 / 16.9, H16 D128 303 / 283, norm and rotation B4 T16384 H16 D128 190 / 181, H12 D64
-// 80.3 / 87.3; 30 shapes geomean 0.94; workgroups of 192, 384, 512 and 1024 threads 1.02, 1.00, 1.01 and 1.04 of it).  Backward it walks tokens, so the weights are loaded once and their gradient
-// stays in registers; partial gradients leave once per workgroup and are added in a fixed order.
+// and keeps cosine and sine in LDS.  A thread owns one column (tensor, head, sixteen elements).  Forward it takes one token:
+// four, with all their rows in flight, keep fewer waves busy (30 shapes geomean 1.06 of the time).  Backward it walks
+// tokens, so the weights are loaded once and their gradient stays in registers; partial gradients leave once per workgroup
+// and are added in a fixed order.
 //
-// Rows are read through the caches, in which what the projections wrote a moment ago may still be, and written past them.  Norm and rotation, bf16 H16 D128, us by
-// loads / stores, both non-temporal, only the loads, neither, only the stores (as it is): forward B4 T512 10.1, 9.8, 8.6, 7.9, T1024 14.9, 15.2, 13.6, 12.4, T4096 48.8, 45.6, 47.1,
-// 48.8, T16384 179, 202, 178, 183; backward T512 24.7, 22.8, 21.6, 21.3, T4096 81.8, 74.6, 84.2, 68.5, T16384 315, 328, 332, 317.
-// Now 177 and 306 us at T16384 (6.0 and 5.3 TB/s; a copy runs at 5.2).
+// Rows are read through the caches, in which what the projections wrote a moment ago may still be, and written past them
+// (norm and rotation B4 T512 H16 D128, us, both past them / as it is: forward 10.1 / 7.9, backward 24.7 / 21.3; long calls alike).
+// B4 T16384 H16 D128, norm and rotation of q and k: 167 us forward, 296 backward (6.4 and 5.4 TB/s; a copy runs at 5.0 to 5.2).
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
 
@@ -62,8 +60,9 @@ struct Column {
   }
 };
 
-// A thread's row lane and column.  In memory order, so that a wave reads whole lines: the lanes of a head, then the heads of a token or, where a head's tokens lie next to each
-// other, the tokens of a head.  Norm and rotation with gradients of (B, H, T, D) memory, B4 H16, us, heads / tokens first: T8192 D32 163 / 98, D16 63.4 / 46.5, D64 140 / 141 (two tokens a workgroup).
+// A thread's row lane and column.  In memory order, so that a wave reads whole lines: the lanes of a head, then the heads
+// of a token or, where a head's tokens lie next to each other, the tokens of a head (norm and rotation with gradients of
+// (B, H, T, D) memory, B4 T8192 H16 D32, us, heads / tokens first: 163 / 98; D64, two tokens a workgroup, 140 / 141).
 template <int D>
 __device__ __forceinline__ void place(const RotaryK& a, int& rl, int& col) {
   constexpr int L = D / 16;
@@ -82,9 +81,9 @@ __device__ __forceinline__ void place(const RotaryK& a, int& rl, int& col) {
 }
 
 // Cosine and sine of a number of turns, to 2^-22 of their own magnitude: the hardware's are off by up to 1.25e-7, which is a thousandth of the sine
-// that a low frequency has at its first positions, more than fp16's rounding.  The nearest quarter turn is taken off in 64 bits; Taylor polynomials in
-// the rest r, at most half a quarter, x = r pi / 2: the first terms left out are x^11 / 11! and x^12 / 12!, below 2^-28 of the values.
-// (us, the hardware's / these: rotation B8 T16000 H1 D64 12.0 / 13.5, B8 T8000 H2 D128 15.0 / 16.1; from twelve heads on the same.)
+// that a low frequency has at its first positions, more than fp16's rounding.  The nearest quarter turn is taken off in 64
+// bits; Taylor polynomials in the rest, x of at most pi / 4: the first terms left out are x^11 / 11! and x^12 / 12!, below
+// 2^-28 of the values (us, the hardware's / these: rotation B8 T16000 H1 D64 12.0 / 13.5; from twelve heads on the same).
 __device__ __forceinline__ float2 cos_sin_of_turns(double turns) {
 #pragma clang fp contract(off)
   const double quarters = (turns - rint(turns)) * 4.0, nearest = rint(quarters);
@@ -182,8 +181,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(const RotaryK a)
   }
 }
 
-// Gradient of the norm and the rotation behind it.  A workgroup walks a strip of `tiles` tiles, kRotaryRows tokens of a thread each: a barrier and new angles
-// per tile, and always the rows of the next token on their way while those of one are used.
+// Gradient of the norm and the rotation behind it.  A workgroup walks a strip of `tiles` tiles, kRotaryRows tokens of a thread
+// each: a barrier and new angles per tile, and always the rows of the next token on their way while those of one are used.
 template <typename Tr, int D, bool INTERLEAVED>
 __global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(const RotaryK a) {
   constexpr int L = D / 16;
@@ -221,7 +220,8 @@ __global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(c
     r.g0 = *reinterpret_cast<const u32x4*>(g + at.v0 * 8);
     r.g1 = *reinterpret_cast<const u32x4*>(g + at.v1 * 8);
   };
-  // Which products are fused into sums is written out: the compiler's choice differed between the copies of this code, so that a token's place in the strip showed in its last bit.
+  // Which products are fused into sums is written out: the compiler's choice differed between the copies of this code, so
+  // that a token's place in the strip showed in its last bit.
   auto use = [&](const Row& r, int n, const float2* angles) {
 #pragma clang fp contract(off)
     float x[16], g[16];
@@ -306,7 +306,8 @@ __global__ __launch_bounds__(kRotaryThreads, 2) void qk_norm_rotary_bwd_kernel(c
 }
 
 namespace {
-// How a call over `tokens` tokens is cut: columns, workgroups' worth of them, row lanes of a workgroup, tokens a tile, tiles a workgroup.
+// How a call over `tokens` tokens is cut: columns, workgroups' worth of them, row lanes of a workgroup, tokens a tile,
+// tiles a workgroup.
 struct RotaryPlan {
   int cols, chunks, lanes, tile, tiles;
   int64_t strips;
@@ -316,12 +317,12 @@ RotaryPlan rotary_plan(int64_t tokens, int heads, int D, bool bwd) {
   p.cols = heads * (D / 16);
   p.chunks = (p.cols + kRotaryThreads - 1) / kRotaryThreads;
   p.lanes = p.cols > kRotaryThreads ? 1 : kRotaryThreads / p.cols;
-  // as many as LDS holds the angles of: two workgroups a CU in the backward.  A quarter of them, us: few heads leave workgroups of one or two waves (norm and rotation with
-  // gradients B8 T4096 H1 D128 43.2 / 28.9, rotation B8 T16000 H1 D64 15.1 / 11.9, B8 T8000 H2 D128 16.3 / 15.0; B33 T9954 H3 D32 29.4 / 31.7, more heads the same)
+  // as many as LDS holds the angles of: two workgroups a CU in the backward.  With a quarter of them few heads would leave workgroups of one
+  // or two waves (norm and rotation with gradients B8 T4096 H1 D128, us, a quarter / as it is: 43.2 / 28.9; B33 T9954 H3 D32 29.4 / 31.7)
   if (p.lanes > 2048 / D) p.lanes = 2048 / D;   // kRotaryLanes
   p.tile = p.lanes * (bwd ? kRotaryRows : 1);
-  // backward: strips for two workgroups a CU, at once.  With heads of several workgroups (chunks) that share weights up to 512 + chunks partial
-  // gradients, more than one launch of the reduction adds.
+  // backward: strips for two workgroups a CU, at once.  Heads of several workgroups (chunks) that share weights can make
+  // up to 512 + chunks partial gradients, more than one launch of the reduction adds.
   const int64_t tiles = (tokens + p.tile - 1) / p.tile, per = bwd ? (tiles * p.chunks + 2 * kCus - 1) / (2 * kCus) : 1;
   p.tiles = (int)per;
   p.strips = (tiles + per - 1) / per;
