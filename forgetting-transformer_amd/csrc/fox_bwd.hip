@@ -26,6 +26,7 @@
 // recomputed P / dS feed the second MFMA straight from registers.
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
+#include "fox_tiles.hpp"
 
 namespace fox {
 
@@ -61,166 +62,6 @@ __global__ __launch_bounds__(256) void delta_kernel(const BwdK a) {
   }
 }
 
-// ---------------------------------------------------------------------------
-// One step (BMQ query rows) of the dK/dV kernel for one wave (32 key rows).
-// rc_s holds rowc_i / (sm_scale*log2e) and dl_s holds -delta_i.  The wave accumulates the NDB 32-column
-// blocks of dK and dV that start at block db0 (all of them, or one half of the head dim when two waves
-// share a block of keys).
-template <typename Tr, int D, int BMQ = kKvBM, int NDB = (D + 31) / 32>
-__device__ __forceinline__ void dkdv_step(const char* q_tile, const char* do_tile, const float* rc_s, const float* dl_s,
-                                 const u32x4 (&kreg)[D / 16], const u32x4 (&vreg)[D / 16], f32x16 (&dkacc)[NDB],
-                                 f32x16 (&dvacc)[NDB], float& csum, int a_s0, int n, int n_w0, float qk_scale,
-                                 float colc, int lane, int db0 = 0) {
-  constexpr int KK = D / 16, MB = BMQ / 32;
-  const int g = lane >> 5, i = lane & 31;
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int a_b0 = a_s0 + 32 * mb;   // key position of the block's first query row
-    if (a_b0 + 31 < n_w0) continue;    // block entirely above the diagonal for this wave
-    f32x16 s = acc_init(rc_s, 32 * mb, g), dp = acc_init(dl_s, 32 * mb, g);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) s = Tr::mfma32(lds_row_operand<D>(q_tile, 32 * mb + i, 2 * kk + g), kreg[kk], s);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) dp = Tr::mfma32(lds_row_operand<D>(do_tile, 32 * mb + i, 2 * kk + g), vreg[kk], dp);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], qk_scale, -colc));
-    if (a_b0 < n_w0 + 31) {  // causal compare, only on blocks that cross the diagonal
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = (n > a_b0 + c_row(r, g)) ? 0.f : s[r];
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float ds = s[r] * dp[r];
-      dp[r] = ds;
-      csum += ds;
-    }
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const u32x4 pb = pack8<Tr>(s, 8 * hh);
-      const u32x4 dsb = pack8<Tr>(dp, 8 * hh);
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        dvacc[db] = Tr::mfma32(lds_col_operand<D>(do_tile, 32 * mb + 16 * hh, db0 + db, lane), pb, dvacc[db]);
-        dkacc[db] = Tr::mfma32(lds_col_operand<D>(q_tile, 32 * mb + 16 * hh, db0 + db, lane), dsb, dkacc[db]);
-      }
-    }
-  }
-}
-
-// Interior step (every query row of the step sits at or below every key of the
-// tile: no causal compare, nothing to skip): branch-free and software-pipelined by
-// hand, because the kernel holds one wave per SIMD and nobody else can fill the
-// matrix pipe while this wave does its exp/scale arithmetic.  The step is cut
-// into slots; slot b issues, interleaved in chunks of 4 MFMAs + 2 scores,
-//   * the score MFMAs        S, dP   of block b+1,
-//   * the vector arithmetic  P, dS   of block b,
-//   * the accumulation MFMAs dV, dK  of block b-1,
-// which are mutually independent (one MFMA, then a few vector instructions, four times per chunk, in source order
-// between scheduling fences).  The global loads of the next tile are spread over
-// the step as well (dma(k) issues the k-th of NDMA instructions): issued back to back
-// after the barrier by all four waves they would hold every wave's issue slot, and
-// with one wave per SIMD the matrix pipe, for over a thousand cycles per step.
-// The LDS operands of a chunk are requested three
-// chunks (about twelve MFMAs) ahead, across slot boundaries, so their latency hides
-// behind the chunks in between.
-template <typename Tr, int D, int NDMA, typename Dma>
-__device__ __forceinline__ void dkdv_step_interior(const char* q_tile, const char* do_tile, const float* rc_s, const float* dl_s,
-                                          const u32x4 (&kreg)[D / 16], const u32x4 (&vreg)[D / 16],
-                                          f32x16 (&dkacc)[(D + 31) / 32], f32x16 (&dvacc)[(D + 31) / 32], float& csum,
-                                          float qk_scale, float colc, int lane, Dma dma) {
-  constexpr int BMQ = kKvBM, KK = D / 16, DB = (D + 31) / 32, MB = BMQ / 32;
-  // chunks per slot: as many as the larger of the two MFMA groups needs (one k-step of S and dP, one accumulation
-  // pair of dV and dK per chunk), so that every chunk carries matrix work; the 16 scores per lane of a block are
-  // dealt out evenly over them
-  constexpr int NCH = KK > 2 * DB ? KK : 2 * DB, SPC = 16 / NCH;
-  static_assert(16 % NCH == 0 && (SPC == 2 || SPC == 4 || SPC == 8), "whole scores per chunk, whole operands per 8 scores");
-  constexpr int NC = (MB + 2) * NCH;  // chunks of the step: slots -1 .. MB
-  constexpr int PF = 3;               // LDS operands are requested this many chunks before their MFMAs
-  constexpr int kDmaEvery = (NC - NCH) / (NDMA > 0 ? NDMA : 1) > 0 ? (NC - NCH) / (NDMA > 0 ? NDMA : 1) : 1;
-  static_assert(NDMA * kDmaEvery <= NC - NCH, "every load instruction of the next tile finds a chunk");
-  static_assert(KK <= NCH && 2 * DB <= NCH, "one k-step and one accumulation pair per chunk");
-  const int g = lane >> 5, i = lane & 31;
-  f32x16 s[MB], dp[MB];
-  u32x4 pb[MB][2], dsb[MB][2];
-  u32x4 aq[NC + PF], ado[NC + PF], cq[NC + PF], cdo[NC + PF];  // indexed by chunk; only a few are live at a time
-  auto fetch = [&](auto ic) {
-    constexpr int c = decltype(ic)::value;
-    constexpr int slot = c / NCH - 1, u = c % NCH, bs = slot + 1, bc = slot - 1;
-    if constexpr (c < NC && bs < MB && u < KK) {
-      aq[c] = lds_row_operand<D>(q_tile, 32 * bs + i, 2 * u + g);
-      ado[c] = lds_row_operand<D>(do_tile, 32 * bs + i, 2 * u + g);
-    }
-    if constexpr (c < NC && slot >= 1 && u < 2 * DB) {
-      cdo[c] = lds_col_operand<D>(do_tile, 32 * bc + 16 * (u / DB), u % DB, lane);
-      cq[c] = lds_col_operand<D>(q_tile, 32 * bc + 16 * (u / DB), u % DB, lane);
-    }
-  };
-  // the accumulators of block b start from the row terms instead of zero; requested PF chunks early too
-  auto init_block = [&](int b) {  // b is a constant at every call site
-    if (b < MB) {
-      s[b] = acc_init(rc_s, 32 * b, g);
-      dp[b] = acc_init(dl_s, 32 * b, g);
-    }
-  };
-  init_block(0);
-  static_for<0, PF>([&](auto ic) { fetch(ic); });
-  static_for<0, NC>([&](auto ic) {
-    constexpr int c = decltype(ic)::value;
-    constexpr int slot = c / NCH - 1, u = c % NCH;
-    constexpr bool do_s = slot + 1 < MB, do_v = slot >= 0 && slot < MB, do_c = slot >= 1;
-    constexpr int bs = slot + 1, bv = slot, bc = slot - 1;
-    fetch(std::integral_constant<int, c + PF>{});
-    if constexpr (u == (NCH > PF ? NCH - PF : 0)) init_block(bs + 1);
-    // the next tile's load instructions, one every kDmaEvery chunks from the second slot on
-    if constexpr (c >= NCH && (c - NCH) % kDmaEvery == 0 && (c - NCH) / kDmaEvery < NDMA)
-      dma(std::integral_constant<int, (c - NCH) / kDmaEvery>{});
-    // The chunk in issue order, every group fenced so that matrix and vector instructions alternate: S MFMA, exp2 of
-    // SPC scores, dP MFMA, dS and the column sum of those scores, dV MFMA, pack P (when eight scores are complete),
-    // dK MFMA, pack dS.  S and dP accumulate in VGPRs (mfma32_vgpr_acc), so this code keeps the distance between an
-    // MFMA that writes s[b] / dp[b] and the first vector instruction that reads them (12 issued instructions).  Block
-    // b's last S MFMA opens chunk NCH-1 of slot b-1 and its first score is read in chunk 0 of slot b, after that
-    // chunk's S MFMA.  For b >= 1 the instructions in between are the 2*SPC exp2 / fma, the dP MFMA, the 2*SPC multiply
-    // / add and the 8 packs of chunk NCH-1 (it completes eight scores), then the next chunk's operand requests and
-    // S MFMA: >= 20.  dP's last MFMA is followed by 2*SPC + 8 of those, the requests, the S MFMA and 2*SPC exp2 / fma
-    // before dS reads it: >= 18.  Block 0 is computed in a slot without vector work, so its first chunk of vector
-    // work starts with explicit wait states.
-    constexpr bool mf_s = do_s && u < KK, mf_c = do_c && u < 2 * DB;
-    constexpr bool pack_due = do_v && (SPC * (u + 1)) % 8 == 0;   // eight scores complete: one MFMA operand each of P and dS
-    constexpr int hh = pack_due ? SPC * (u + 1) / 8 - 1 : 0;
-    static_assert(SPC >= 2 && NCH * SPC == 16, "the distances above count on at least two scores per chunk, eight per pack");
-    if constexpr (mf_s) Tr::mfma32_vgpr_acc(s[bs], aq[c], kreg[u]);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (do_v && bv == 0 && u == 0) {
-      asm volatile("s_nop 11");
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (do_v) {
-#pragma unroll
-      for (int e = 0; e < SPC; ++e) s[bv][SPC * u + e] = __builtin_amdgcn_exp2f(fmaf(s[bv][SPC * u + e], qk_scale, -colc));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (mf_s) Tr::mfma32_vgpr_acc(dp[bs], ado[c], vreg[u]);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (do_v) {
-#pragma unroll
-      for (int e = 0; e < SPC; ++e) {
-        const float ds = s[bv][SPC * u + e] * dp[bv][SPC * u + e];
-        dp[bv][SPC * u + e] = ds;
-        csum += ds;
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (mf_c) dvacc[u % DB] = Tr::mfma32(cdo[c], pb[bc][u / DB], dvacc[u % DB]);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (pack_due) pb[bv][hh] = pack8<Tr>(s[bv], 8 * hh);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (mf_c) dkacc[u % DB] = Tr::mfma32(cq[c], dsb[bc][u / DB], dkacc[u % DB]);
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (pack_due) dsb[bv][hh] = pack8<Tr>(dp[bv], 8 * hh);
-    __builtin_amdgcn_sched_barrier(0);
-  });
-}
-
 // DSPLIT: the variant for key tiles that pruning leaves a few query steps (class kClassLight).  Such a workgroup
 // is a short chain of loads, a few steps and stores; at one workgroup per CU nothing overlaps with it.  Here two
 // waves share 32 keys, each recomputing S and dP and accumulating one half of the head dim of dK and dV, so that
@@ -232,11 +73,6 @@ __device__ __forceinline__ void dkdv_step_interior(const char* q_tile, const cha
 // them, and the barrier that publishes the step's tiles publishes their delta as well.  The sum is the dQ walk's, bit for bit: the gradient of the
 // gates is the difference of the row sums of dS there and the column sums here, and is only as good as the two see one delta.
 
-// Two elements' part of delta.  (One expression for both walks, with the rounding spelled out.)
-template <typename Tr>
-__device__ __forceinline__ float delta_term(uint32_t o, uint32_t d_o) {
-  return __builtin_fmaf(Tr::lo(o), Tr::lo(d_o), Tr::hi(o) * Tr::hi(d_o));
-}
 template <int D, bool DSPLIT>
 struct DkdvLds {
   static constexpr int BMQ = DSPLIT ? 64 : kKvBM;
@@ -564,52 +400,6 @@ __global__ __launch_bounds__(256, (D <= 64 || DSPLIT) ? 2 : 1) void dkdv_kernel(
   nt = a.n_tiles - 1 - nt;  // the first key tiles see the most query rows: start them first
   dkdv_body<Tr, D, DSPLIT, false>(a, bh, nt, {q_tile0, q_tile1, do_tile0, do_tile1, rc_s0, rc_s1, dl_s0, dl_s1});
 #endif
-}
-
-// ---------------------------------------------------------------------------
-// One 64-key tile of the dQ kernel for one wave (32 query rows).
-// cn_s holds -colc_j / (sm_scale*log2e), the start value of the score accumulators.
-template <typename Tr, int D>
-__device__ __forceinline__ void dq_tile(const char* k_tile, const char* v_tile, const float* cn_s, const u32x4 (&qreg)[D / 16],
-                               const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rsum, int n0, int a_m,
-                               int a_w0, float qk_scale, float rowc, float delta, int lane) {
-  constexpr int BN = kFwdBN, KK = D / 16, DB = (D + 31) / 32, NB = BN / 32;
-  const int g = lane >> 5, i = lane & 31;
-  // dP starts from -delta (constant along a query row, i.e. per lane) instead of zero: the matrix pipe does the
-  // subtraction.  The sixteen equal registers are loop-invariant for the caller.
-  f32x16 neg_delta;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) neg_delta[r] = -delta;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int nb0 = n0 + 32 * nb;
-    if (nb0 > a_w0 + 31) continue;  // block entirely above this wave's rows
-    f32x16 s = acc_init(cn_s, 32 * nb, g);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) s = Tr::mfma32(lds_row_operand<D>(k_tile, 32 * nb + i, 2 * kk + g), qreg[kk], s);
-    f32x16 dp = Tr::mfma32(lds_row_operand<D>(v_tile, 32 * nb + i, g), doreg[0], neg_delta);
-#pragma unroll
-    for (int kk = 1; kk < KK; ++kk) dp = Tr::mfma32(lds_row_operand<D>(v_tile, 32 * nb + i, 2 * kk + g), doreg[kk], dp);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], qk_scale, rowc));
-    if (nb0 + 31 > a_w0) {  // causal compare, only on blocks that cross the diagonal
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = (nb0 + c_row(r, g) > a_m) ? 0.f : s[r];
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float ds = s[r] * dp[r];
-      dp[r] = ds;
-      rsum += ds;
-    }
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const u32x4 dsb = pack8<Tr>(dp, 8 * hh);
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-        dqacc[db] = Tr::mfma32(lds_col_operand<D>(k_tile, 32 * nb + 16 * hh, db, lane), dsb, dqacc[db]);
-    }
-  }
 }
 
 // The kernel's argument block behind a pointer the compiler cannot see through: each kind of workgroup loads its arguments where it needs

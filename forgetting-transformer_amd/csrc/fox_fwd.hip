@@ -31,207 +31,9 @@
 
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
+#include "fox_tiles.hpp"
 
 namespace fox {
-
-constexpr float kLazyMaxLog2 = 8.0f;
-constexpr int kMinPipelinedTiles = 4;   // interior tiles below which the software-pipelined path is not entered
-
-template <typename Tr, int D>
-__device__ __forceinline__ void fwd_tile(const char* k_tile, const char* v_tile, const float* cn_s, const u32x4 (&qreg)[D / 16],
-                                f32x16 (&oacc)[(D + 31) / 32], float& m_i, float& l_i, int n0, int a_m, float qk_scale,
-                                int lane, bool diag) {
-  constexpr int BN = kFwdBN, KK = D / 16, DB = (D + 31) / 32, NB = BN / 32;
-  const int g = lane >> 5, i = lane & 31;
-
-  // S^T = K Q^T + key term
-  f32x16 s[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    u32x4 ka[KK];
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) ka[kk] = lds_row_operand<D>(k_tile, 32 * nb + i, 2 * kk + g);
-    s[nb] = acc_init(cn_s, 32 * nb, g);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) s[nb] = Tr::mfma32(ka[kk], qreg[kk], s[nb]);
-  }
-
-  // scores in the log2 domain and their maximum
-  float mloc = -INFINITY;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[nb][r] *= qk_scale;
-  if (diag) {  // causal compare, only on tiles that cross the diagonal
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = n0 + 32 * nb + c_row(r, g);
-        s[nb][r] = (n > a_m) ? -INFINITY : s[nb][r];
-      }
-  }
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) mloc = fmaxf(mloc, s[nb][r]);
-  mloc = half_max(mloc);
-  const bool raise = mloc > m_i + kLazyMaxLog2;
-  if (__any(raise)) {  // rare: rescale what has been accumulated so far
-    const float m_new = raise ? mloc : m_i;
-    const float alpha = __builtin_amdgcn_exp2f(m_i - m_new);
-    m_i = m_new;
-    l_i *= alpha;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
-  }
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[nb][r] = __builtin_amdgcn_exp2f(s[nb][r] - m_i);
-
-  // O^T += V^T P^T.  The row sum is taken over the probabilities as rounded for the MFMA (the weights that
-  // multiply V then add up to exactly l), two at a time: per-lane partial sum, the two halves are added in the epilogue.
-  float rsum = 0.f;
-#pragma unroll
-  for (int sl = 0; sl < BN / 16; ++sl) {
-    const u32x4 pb = pack8<Tr>(s[sl >> 1], 8 * (sl & 1));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) rsum = Tr::add_pair(pb[e], rsum);
-    u32x4 va[DB];
-#pragma unroll
-    for (int db = 0; db < DB; ++db) va[db] = lds_col_operand<D>(v_tile, 16 * sl, db, lane);
-#pragma unroll
-    for (int db = 0; db < DB; ++db) oacc[db] = Tr::mfma32(va[db], pb, oacc[db]);
-  }
-  l_i += rsum;
-}
-
-// Interior tile (no key of the tile is right of any query row of the workgroup): branch-free and
-// software-pipelined across tiles.  While the vector ALU turns the scores of the current tile into
-// probabilities, the matrix pipe already computes the scores of the next tile (from k_next) and then
-// accumulates the current tile's P V (from v_cur).  s_cur holds the raw scores of the current tile
-// on entry; s_next holds those of the next tile on exit.  Work is issued in small chunks separated
-// by scheduling fences so that MFMA and vector instructions alternate in the instruction stream.
-// dma(u) issues chunk u's share of the global loads of the tiles after next: spread over the tile they
-// do not hold the wave's issue slot back to back right after the barrier.
-template <typename Tr, int D, typename Dma>
-__device__ __forceinline__ void fwd_tile_pipelined(const char* k_next, const char* v_cur, const float* cn_next,
-                                                  const u32x4 (&qreg)[D / 16], f32x16 (&oacc)[(D + 31) / 32], float& m_i,
-                                                  float& l_i, float qk_scale, int lane, f32x16 (&s_cur)[kFwdBN / 32],
-                                                  f32x16 (&s_next)[kFwdBN / 32], Dma dma) {
-  constexpr int BN = kFwdBN, KK = D / 16, DB = (D + 31) / 32, NB = BN / 32, NSL = BN / 16;
-  constexpr int SPC = 16 * NB / KK;  // scores handled per chunk of phase A
-  static_assert(16 * NB % KK == 0 && SPC % 4 == 0, "whole float4 groups of scores per chunk");
-  const int g = lane >> 5, i = lane & 31;
-
-  // Phase A: scores of the next tile  ||  maximum of the current tile's raw scores (sm_scale > 0 here)
-  float mloc = -INFINITY;
-  u32x4 ka[NB][KK + 1];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    ka[nb][0] = lds_row_operand<D>(k_next, 32 * nb + i, g);
-    s_next[nb] = acc_init(cn_next, 32 * nb, g);
-  }
-  static_for<0, KK>([&](auto uc) {
-    constexpr int u = decltype(uc)::value;
-    dma(u);  // this chunk's share of the global loads of the tiles after next
-    if constexpr (u + 1 < KK) {
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) ka[nb][u + 1] = lds_row_operand<D>(k_next, 32 * nb + i, 2 * (u + 1) + g);
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) s_next[nb] = Tr::mfma32(ka[nb][u], qreg[u], s_next[nb]);
-#pragma unroll
-    for (int e = 0; e < SPC; ++e) {
-      const int idx = u * SPC + e;
-      mloc = fmaxf(mloc, s_cur[idx >> 4][idx & 15]);
-    }
-#pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, (SPC / 2 + NB - 1) / NB, 0);  // the chunk's v_max3 dealt out over its MFMAs
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  });
-  mloc = half_max(mloc) * qk_scale;
-  const bool raise = mloc > m_i + kLazyMaxLog2;
-  if (__any(raise)) {  // rare: rescale what has been accumulated so far
-    const float m_new = raise ? mloc : m_i;
-    const float alpha = __builtin_amdgcn_exp2f(m_i - m_new);
-    m_i = m_new;
-    l_i *= alpha;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
-  }
-
-  // Phase B: p = exp2(s*scale - m), row sums, pack  ||  O^T += V^T P^T, one 16-key slice behind
-  const float neg_m = -m_i;
-  float rsum = 0.f;
-  u32x4 pb[NSL];
-  u32x4 va[NSL][DB];
-#pragma unroll
-  for (int c = 0; c <= NSL; ++c) {
-    if (c < NSL) {
-#pragma unroll
-      for (int db = 0; db < DB; ++db) va[c][db] = lds_col_operand<D>(v_cur, 16 * c, db, lane);
-    }
-    if (c >= 1) {
-#pragma unroll
-      for (int db = 0; db < DB; ++db) oacc[db] = Tr::mfma32(va[c - 1][db], pb[c - 1], oacc[db]);
-    }
-    if (c < NSL) {
-      const int nb = c >> 1, r0 = 8 * (c & 1);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s_cur[nb][r0 + e] = __builtin_amdgcn_exp2f(fmaf(s_cur[nb][r0 + e], qk_scale, neg_m));
-      pb[c] = pack8<Tr>(s_cur[nb], r0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) rsum = Tr::add_pair(pb[c][e], rsum);  // row sum of the rounded probabilities
-    }
-    if (c >= 1 && c < NSL) {
-#pragma unroll
-      for (int k = 0; k < DB; ++k) {  // a slice has 16 vector and 8 exp instructions: dealt out over its DB MFMAs
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 16 / DB, 0);
-        __builtin_amdgcn_sched_group_barrier(0x400, 8 / DB, 0);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  l_i += rsum;
-}
-
-// The global loads of a K tile and a V tile, dealt out over the D/16 chunks of a pipelined tile:
-// dma(u) issues chunk u's share.
-template <int D, int AUX>
-struct TileDma {
-  static constexpr int KK = D / 16, PER = DirectTileLoader<D, kFwdBN, 4, AUX>::PER, PER_CHUNK = (2 * PER + KK - 1) / KK;
-  const DirectTileLoader<D, kFwdBN, 4, AUX>& kld;
-  const DirectTileLoader<D, kFwdBN, 4, AUX>& vld;
-  const uint16_t* k_src;
-  const uint16_t* v_src;
-  int k_bytes, v_bytes;
-  char* k_fill;
-  char* v_fill;
-  __device__ __forceinline__ void all() const {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) kld.issue_one(j, k_src, k_bytes, k_fill);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) vld.issue_one(j, v_src, v_bytes, v_fill);
-  }
-  __device__ __forceinline__ void operator()(int u) const {  // u is a constant at every call site
-#pragma unroll
-    for (int r = 0; r < PER_CHUNK; ++r) {
-      const int idx = u * PER_CHUNK + r;
-      if (idx < PER) kld.issue_one(idx, k_src, k_bytes, k_fill);
-      else if (idx < 2 * PER) vld.issue_one(idx - PER, v_src, v_bytes, v_fill);
-    }
-  }
-};
 
 // Cumulative sums c[n] = sum of the gates of keys seq .. n (zero left of seq) for n < hi, into LDS.  As in scan_row: coalesced through LDS,
 // consecutive keys per thread, fp64, rounded once.  Positions from `first` to hi are also stored for the backward, as are the log gates of
