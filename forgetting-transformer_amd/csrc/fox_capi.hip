@@ -324,6 +324,56 @@ int check_room(int W, int page_size) {
   return FOX_OK;
 }
 
+// A (tokens, heads, D) tensor of which the tile loaders read up to 128 rows with 32-bit offsets.
+int check_tokens(const fox_view* v, const char* name) {
+  FOX_TRY(check_view(v, name));
+  if (v->stride_t <= 0 || v->stride_t >= 1 << 23) return fail(FOX_E_ARG, "the token stride of %s must be positive and below 2^23 elements", name);
+  return FOX_OK;
+}
+int check_packed_sizes(int B, int T, int N) {
+  if (B <= 0 || T <= 0 || N <= 0) return fail(FOX_E_ARG, "B, T and N must be positive (got %d, %d, %d)", B, T, N);
+  if (B > 65535) return fail(FOX_E_ARG, "at most 65535 sequences (got %d)", B);
+  if (T > 1 << 30 || N > 1 << 30) return fail(FOX_E_ARG, "at most 2^30 queries and keys (got %d, %d)", T, N);
+  return FOX_OK;
+}
+int make_packed(const fox_packed_args* a, fox::PackedK& k, bool bwd) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  FOX_TRY(check_packed_sizes(a->B, a->T, a->N));
+  FOX_TRY(check_head_dim(a->D));
+  FOX_TRY(check_dtype16(a->dtype));
+  if (a->H <= 0 || a->Hk <= 0 || a->H % a->Hk) return fail(FOX_E_ARG, "the query heads must be a positive multiple of the key heads (got %d, %d)", a->H, a->Hk);
+  if (a->H > 65535) return fail(FOX_E_ARG, "at most 65535 heads (got %d)", a->H);
+  FOX_TRY(check_tokens(&a->q, "q"));
+  FOX_TRY(check_tokens(&a->k, "k"));
+  FOX_TRY(check_tokens(&a->v, "v"));
+  FOX_TRY(check_tokens(&a->o, "o"));
+  if (!a->c || !a->plan) return fail(FOX_E_ARG, "c and plan must not be NULL");
+  if (!bwd && (!a->g || !a->cu_q || !a->cu_k)) return fail(FOX_E_ARG, "g, cu_q and cu_k must not be NULL");
+  if (a->plan_bytes < fox::packed_plan_bytes(a->B, a->T, a->N)) return fail(FOX_E_ARG, "plan too small: %lld bytes", (long long)a->plan_bytes);
+  if ((uintptr_t)a->plan & 15) return fail(FOX_E_ALIGN, "plan must be 16-byte aligned");
+  k = fox::PackedK{};
+  k.q = to_view(a->q); k.k = to_view(a->k); k.v = to_view(a->v); k.o = to_view(a->o);
+  k.g = a->g; k.g_st = a->g_stride_t; k.g_sh = a->g_stride_h;
+  k.cu_q = a->cu_q; k.cu_k = a->cu_k;
+  k.c = a->c; k.lse = a->lse;
+  k.B = a->B; k.T = a->T; k.N = a->N; k.H = a->H; k.Hk = a->Hk; k.group = a->H / a->Hk;
+  k.sm_scale = a->sm_scale;
+  k.plan = fox::packed_plan(a->plan, a->B, a->T, a->N, &k.q_bound, &k.k_bound);
+  const int64_t rows = ((int64_t)a->B + fox::kPackedOuter) * a->H, q_tiles = (int64_t)k.q_bound * a->H, k_tiles = (int64_t)k.k_bound * a->Hk;
+  // (threads of a launch: 1024 a row, 256 a tile)
+  if (rows >= 1 << 22 || q_tiles >= 1 << 24 || k_tiles >= 1 << 24) return fail(FOX_E_ARG, "too many sequences, tiles and heads for one call");
+  if (!bwd) return FOX_OK;
+  FOX_TRY(check_tokens(&a->d_o, "do"));
+  FOX_TRY(check_tokens(&a->dq, "dq"));
+  FOX_TRY(check_tokens(&a->dk, "dk"));
+  FOX_TRY(check_tokens(&a->dv, "dv"));
+  if (!a->lse || !a->dg || !a->delta || !a->dc) return fail(FOX_E_ARG, "lse, dg, delta and dc must not be NULL");
+  k.d_o = to_view(a->d_o); k.dq = to_view(a->dq); k.dk = to_view(a->dk); k.dv = to_view(a->dv);
+  k.dg = a->dg; k.dg_st = a->dg_stride_t; k.dg_sh = a->dg_stride_h;
+  k.delta = a->delta; k.dc = a->dc;
+  return FOX_OK;
+}
+
 // What the forward does with a shape: the key splits its size asks for (only with scratch to hold their partial results), and whether
 // it runs as the paired kernel, which takes the place of the splits.
 struct FwdPlan {
@@ -468,8 +518,9 @@ extern "C" {
 // 0.2.x: fox_bwd_args and the scan entry points differ from 0.1.0; 0.2.1 adds fox_set_stream_min_kv_bytes and fox_probe_mfma, 0.2.2
 // fox_attn_decode, fox_cache_append, fox_qk_norm_threshold and fox_attn_fwd_plan, 0.2.3 fox_attn_fwd_gates, fox_attn_fwd_takes_gates,
 // fox_auto_threshold_scan, fox_attn_decode_counted and fox_attn_bwd_logits, 0.2.4 fox_attn_bwd_one_launch,
-// fox_auto_threshold_scan_one_launch and fox_attn_decode_counters, 0.2.5 the rotation (fox_rotary_*) and the pages (fox_page_*, fox_paged_*)
-int fox_version(void) { return 205; }
+// fox_auto_threshold_scan_one_launch and fox_attn_decode_counters, 0.2.5 the rotation (fox_rotary_*) and the pages (fox_page_*, fox_paged_*),
+// 0.2.6 packed sequences (fox_packed_*)
+int fox_version(void) { return 206; }
 
 const char* fox_last_error(void) { return g_err; }
 
@@ -866,6 +917,25 @@ int fox_cache_append(const fox_cache_append_args* args, void* stream) {
   k.H = args->H; k.T = args->T; k.D = args->D;
   k.total = (uint32_t)total;
   return check_hip(fox::launch_cache_append(k, (hipStream_t)stream), "fox_cache_append");
+}
+
+int fox_packed_plan_bytes(int32_t B, int32_t T, int32_t N, int64_t* bytes) {
+  FOX_TRY(check_packed_sizes(B, T, N));
+  if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
+  *bytes = fox::packed_plan_bytes(B, T, N);
+  return FOX_OK;
+}
+
+int fox_packed_fwd(const fox_packed_args* args, void* stream) {
+  fox::PackedK k;
+  FOX_TRY(make_packed(args, k, false));
+  return check_hip(fox::launch_packed_fwd(k, args->D, args->dtype, (hipStream_t)stream), "fox_packed_fwd");
+}
+
+int fox_packed_bwd(const fox_packed_args* args, void* stream) {
+  fox::PackedK k;
+  FOX_TRY(make_packed(args, k, true));
+  return check_hip(fox::launch_packed_bwd(k, args->D, args->dtype, (hipStream_t)stream), "fox_packed_bwd");
 }
 
 int fox_attn_bwd_delta(const fox_bwd_args* args, void* stream) {

@@ -257,6 +257,34 @@ struct PagedDecodeK {
   double per_piece;                      // 1 / the pieces of all rows and heads together, about; set by the launcher
 };
 
+// Attention over packed sequences (fox_packed.hip).  Sequence b has the queries [q0, q0 + m) and the keys [k0, k0 + n); a tile is 128 rows of either.
+struct PackedItem {
+  int32_t q0, m, k0, n, tile, seq, pad[2];
+};
+struct PackedPlan {                      // in the plan's memory, behind the counts
+  PackedItem *q_items, *k_items;         // tiles of queries and of keys, those of the longest sequences first
+  int4* seqs;                            // {q0, m, k0, n} of the B sequences and of kPackedOuter that hold what belongs to none
+  int32_t* counts;                       // of q_items and k_items
+};
+constexpr int kPackedOuter = 4;          // rows in front of the first and behind the last sequence: queries without keys, keys without queries
+struct PackedK {
+  View q, k, v, o, d_o, dq, dk, dv;      // (T, H, D) and (N, Hk, D): stride of a token in st, of a head in sh
+  const float* g;                        // (N, H) log gates
+  int64_t g_st, g_sh;
+  float* dg;
+  int64_t dg_st, dg_sh;
+  const int32_t *cu_q, *cu_k;            // (B + 1)
+  double* c;                             // (H, N): sums of the gates from the start of each sequence on
+  float* lse;                            // (H, T)
+  float* delta;                          // (H, T), backward
+  float* dc;                             // (H, N), backward
+  PackedPlan plan;
+  int B, T, N, H, Hk, group;             // group = H / Hk query heads on a key head
+  int q_bound, k_bound;                  // tiles, at most
+  float sm_scale;
+  Divisor by_heads, by_xcd_heads;        // of a launch: by the heads, and by those of an XCD
+};
+
 // Tile sizes (see fox_tile_config in the public header)
 constexpr int kXcds = 8, kCus = 256;
 constexpr int kFwdBM = 128;
@@ -394,6 +422,10 @@ hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s);
 hipError_t launch_paged_decode(const PagedDecodeK& a, int D, int dtype, hipStream_t s);
 int64_t paged_decode_rows(int B, int H, int max_keys, int D);   // of workspace; 0: no request is split
 int64_t rotary_workspace_floats(int64_t tokens, int heads, int D, bool shared);
+int64_t packed_plan_bytes(int B, int T, int N);
+PackedPlan packed_plan(void* memory, int B, int T, int N, int* q_bound, int* k_bound);
+hipError_t launch_packed_fwd(const PackedK& a, int D, int dtype, hipStream_t s);
+hipError_t launch_packed_bwd(const PackedK& a, int D, int dtype, hipStream_t s);
 hipError_t launch_shift_fwd(const ShiftK& a, int D, int dtype, hipStream_t s);
 hipError_t launch_shift_bwd(const ShiftK& a, int D, int dtype, hipStream_t s);
 hipError_t launch_cumsum_fwd(const float* g, int64_t sb, int64_t sh, int64_t sn, const int64_t* seq_start, float* c, int B,

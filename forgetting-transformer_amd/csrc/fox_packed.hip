@@ -1,0 +1,953 @@
+// Forgetting Attention over packed sequences for gfx950: forward and backward.
+//
+// The sequences lie one after the other, their ends in cu_q and cu_k on the device.  Query i of a sequence of m queries and n keys sees the keys
+// j <= i + n - m of it; H query heads share Hk key heads, every query head has gates of its own:
+//   s_ij = sm_scale q_i.k_j + c_i - c_j,  c_j = sum of the gates up to j,  o = softmax(s) v;  a row that sees no key is zero
+//   dP = dO V^T,  delta_i = sum_j P_ij dP_ij,  dS = P (dP - delta),  dq = sm_scale dS K,  dk = sm_scale dS^T Q,  dv = P^T dO,
+//   dc_j = -sum_i dS_ij  (a row of dS adds up to zero),  dg_l = sum_{j >= l} dc_j.
+//
+// Who knows how long the sequences are is the device.  One workgroup makes the plan, the list of all tiles of queries and of keys, while the others form the
+// sums of the gates; the attention kernels are launched for as many tiles as there can be (a partial one for every sequence) and those past the
+// list end at once.  A sequence's tiles follow each other, heaviest first, the longest sequences in front.
+//
+// The gates' gradient is a difference of sums over whole rows and columns of dS, so it is formed from 32-bit values throughout, where the rest of the backward can
+// live with the 16 bits of its operands:
+// - c is kept in 64 bits; the kernels subtract a reference near their tile before they round.  Off the diagonal the reference lies between a tile's queries and its
+//   keys, so that a bias is a sum of two terms of one sign and off by its own rounding.  On the diagonal two terms as large as the gates of 128 keys would cancel: there every
+//   bias is the difference of two pairs of 32-bit numbers.  (One reference for all tiles and 32 bits: dg at gates of -2.1 off by 2e-4 of itself, now below 2e-6.)
+// - The row sum of the forward adds the probabilities before they are rounded for the matrix instruction.
+// - o.do is off by the rounding of o and of P; what is missing of delta is sum_j P_ij (dP_ij - o.do), which the dQ kernel has at its end.  It stores
+//   the sum of the two for the dK/dV kernel.
+#include "fox_common.hpp"
+#include "fox_kernels.hpp"
+#include "fox_tiles.hpp"
+
+namespace fox {
+
+namespace {
+
+constexpr int kPackedTile = 128;   // rows of a tile of either kind
+static_assert(kPackedTile == kFwdBM && kPackedTile == kKvBN && kKvBM == kKvBN, "a tile is what a workgroup keeps");
+// Log gates below this close like it: -inf itself would make the difference of two sums behind it undefined.
+constexpr float kLowestGate = -1e6f;
+
+// ---------------------------------------------------------------------------
+// Plan
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int wave_max_scan(int x, int lane) {   // maximum over lanes 0 .. own, of values >= 0
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off);
+    if (lane >= off) x = max(x, y);
+  }
+  return x;
+}
+
+// Place of a length in the order of the plan: shorter sequences come later, in steps of a quarter of a power of two.
+constexpr int kOrderBuckets = 128;
+__device__ __forceinline__ int bucket_of(int rows) {
+  return kOrderBuckets - 1 - min(max((int)(__float_as_uint((float)rows) >> 21) - (127 << 2), 0), kOrderBuckets - 1);
+}
+
+// By one workgroup of NT threads.  Ends that decrease or lie outside the tensors are brought into order, so that no tile leaves them.
+template <int NT>
+__device__ __forceinline__ void make_plan(const PackedK& a) {
+  constexpr int WAVES = NT / 64;
+  __shared__ int wave_q[WAVES], wave_k[WAVES];
+  __shared__ int tiles_q[kOrderBuckets], tiles_k[kOrderBuckets];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.B + kPackedOuter;
+  int4* const seqs = a.plan.seqs;
+  for (int i = tid; i < kOrderBuckets; i += NT) tiles_q[i] = tiles_k[i] = 0;
+  int top_q = 0, top_k = 0;   // largest end so far
+  for (int b0 = 0; b0 < a.B; b0 += NT) {
+    const int b = b0 + tid;
+    const bool in = b < a.B;
+    const int sq = in ? a.cu_q[b] : 0, sk = in ? a.cu_k[b] : 0, last_q = in ? a.cu_q[b + 1] : 0, last_k = in ? a.cu_k[b + 1] : 0;
+    int q = wave_max_scan(max(sq, 0), lane), k = wave_max_scan(max(sk, 0), lane);
+    __syncthreads();
+    if (lane == 63) {
+      wave_q[wave] = q;
+      wave_k[wave] = k;
+    }
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) {
+        q = max(q, wave_q[w]);
+        k = max(k, wave_k[w]);
+      }
+    }
+    q = min(max(q, top_q), a.T);
+    k = min(max(k, top_k), a.N);
+    const int q1 = min(max(q, last_q), a.T), k1 = min(max(k, last_k), a.N);
+    if (in) seqs[b] = make_int4(q, q1 - q, k, k1 - k);
+    for (int w = 0; w < WAVES; ++w) {
+      top_q = max(top_q, wave_q[w]);
+      top_k = max(top_k, wave_k[w]);
+    }
+  }
+  __syncthreads();
+  if (tid < kPackedOuter) {
+    const int4 first = seqs[0], end = seqs[a.B - 1];
+    const int q1 = end.x + end.y, k1 = end.z + end.w;
+    seqs[a.B + tid] = tid == 0 ? make_int4(0, first.x, 0, 0) : tid == 1 ? make_int4(q1, a.T - q1, 0, 0) : tid == 2 ? make_int4(0, 0, 0, first.z)
+                                                                                                   : make_int4(0, 0, k1, a.N - k1);
+  }
+  __syncthreads();
+  // tiles of a bucket, their first places, and each sequence's among them (any order within a bucket)
+  for (int b = tid; b < S; b += NT) {
+    const int4 s = seqs[b];
+    if (s.y > 0) atomicAdd(&tiles_q[bucket_of(s.w)], (s.y + kPackedTile - 1) / kPackedTile);
+    if (s.w > 0) atomicAdd(&tiles_k[bucket_of(s.y)], (s.w + kPackedTile - 1) / kPackedTile);
+  }
+  __syncthreads();
+  if (tid < 2) {
+    int* const tiles = tid ? tiles_k : tiles_q;
+    int sum = 0;
+    for (int i = 0; i < kOrderBuckets; ++i) {
+      const int n = tiles[i];
+      tiles[i] = sum;
+      sum += n;
+    }
+    a.plan.counts[tid] = sum;
+  }
+  __syncthreads();
+  for (int b = wave; b < S; b += WAVES) {   // a wave each
+    const int4 s = seqs[b];
+    const int nq = (s.y + kPackedTile - 1) / kPackedTile, nk = (s.w + kPackedTile - 1) / kPackedTile;
+    int at_q = 0, at_k = 0;
+    if (lane == 0) {
+      if (nq) at_q = atomicAdd(&tiles_q[bucket_of(s.w)], nq);
+      if (nk) at_k = atomicAdd(&tiles_k[bucket_of(s.y)], nk);
+    }
+    at_q = __builtin_amdgcn_readfirstlane(at_q);
+    at_k = __builtin_amdgcn_readfirstlane(at_k);
+    PackedItem it{s.x, s.y, s.z, s.w, 0, b, {0, 0}};
+    for (int t = lane; t < nq; t += 64) {   // the last queries see the most keys
+      it.tile = nq - 1 - t;
+      a.plan.q_items[at_q + t] = it;
+    }
+    for (int t = lane; t < nk; t += 64) {   // the first keys are seen by the most queries
+      it.tile = t;
+      a.plan.k_items[at_k + t] = it;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Sums of the gates
+// ---------------------------------------------------------------------------
+// Running sums of one row of n values by NT threads, from its first element on or from its last.  fp64; load(j) and store(j, sum) take the place in the row.
+template <int NT, bool REVERSE, typename Load, typename Store>
+__device__ __forceinline__ void sum_row(int n, Load load, Store store) {
+  constexpr int PER = 8, WAVES = NT / 64;
+  __shared__ double wave_tot[2][WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  double carry = 0.0;
+  int turn = 0;
+  for (int base = 0; base < n; base += NT * PER, turn ^= 1) {
+    const int at = base + tid * PER;
+    float x[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int i = min(at + e, n - 1), j = REVERSE ? n - 1 - i : i;
+      x[e] = load(j);
+    }
+    double v[PER], run = 0.0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) v[e] = run += at + e < n ? (double)x[e] : 0.0;
+    const double incl = wave_scan(run);
+    double before = carry + lane_before(incl), total = 0.0;
+    if constexpr (WAVES > 1) {
+      if (lane == 63) wave_tot[turn][wave] = incl;
+      __syncthreads();   // (the other buffer of the two was read in front of it)
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const double t = wave_tot[turn][w];
+        if (w < wave) before += t;
+        total += t;
+      }
+    } else {
+      total = of_lane(incl, 63);
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      if (at + e < n) store(REVERSE ? n - 1 - (at + e) : at + e, before + v[e]);
+    }
+    carry += total;
+  }
+}
+
+}  // namespace
+
+// Workgroup 0 makes the plan, the others the sums of a (sequence, head) each.
+template <int NT>
+__global__ __launch_bounds__(NT) void packed_scan_kernel(const PackedK a) {
+  if (blockIdx.x == 0) {
+    make_plan<NT>(a);
+    return;
+  }
+  const int b = divide(blockIdx.x - 1, a.by_heads), h = blockIdx.x - 1 - b * a.H;
+  const int k0 = min(max(a.cu_k[b], 0), a.N), n = min(max(a.cu_k[b + 1], k0), a.N) - k0;
+  const float* g = a.g + (int64_t)k0 * a.g_st + h * a.g_sh;
+  double* c = a.c + (int64_t)h * a.N + k0;
+  sum_row<NT, false>(n, [&](int j) { return fmaxf(g[j * a.g_st], kLowestGate); }, [&](int j, double sum) { c[j] = sum; });
+}
+
+// dg of a (sequence, head) from dc.  The first gate of a sequence moves all its sums alike: an exact zero, as in the rows that belong to none.
+template <int NT>
+__global__ __launch_bounds__(NT) void packed_gate_grad_kernel(const PackedK a) {
+  const int b = divide(blockIdx.x, a.by_heads), h = blockIdx.x - b * a.H;
+  const int4 s = a.plan.seqs[b];
+  const float* dc = a.dc + (int64_t)h * a.N + s.z;
+  float* dg = a.dg + (int64_t)s.z * a.dg_st + h * a.dg_sh;
+  const bool none = b >= a.B;
+  sum_row<NT, true>(s.w, [&](int j) { return dc[j]; }, [&](int j, double sum) { dg[j * a.dg_st] = none || j == 0 ? 0.f : (float)sum; });
+}
+
+namespace {
+
+// Item and head of a workgroup: the heads of an XCD are next to each other where 8 divides them, so that those of a group, which read the same keys, share
+// its L2, and all tiles of a head follow each other there.  `heads` is fixed for a launch, by_heads and by_xcd_heads are its divisors.
+__device__ __forceinline__ void packed_block(const PackedK& a, int heads, int& item, int& head) {
+  const uint32_t id = blockIdx.x;
+  if (heads % kXcds == 0) {
+    const int r = (int)(id / kXcds), per = heads / kXcds;
+    item = divide(r, a.by_xcd_heads);
+    head = (int)(id % kXcds) * per + r - item * per;
+  } else {
+    item = divide((int)id, a.by_heads);
+    head = (int)id - item * heads;
+  }
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Tiles at the diagonal: scores with the biases as differences of pairs, masked (the others: fox_tiles.hpp)
+// ---------------------------------------------------------------------------
+namespace {
+
+// A 64-bit number of log2 units as two of 32 bits.
+struct Pair {
+  float hi, lo;
+};
+__device__ __forceinline__ Pair pair_of(double x) {
+  const float hi = (float)x;
+  return {hi, (float)(x - (double)hi)};
+}
+constexpr double kLog2eD = 1.4426950408889634074;
+
+// x[r] = s[r] scale + (row - column) with the pairs of rows (or columns) c_row(r, g) in LDS; sign -1: LDS holds the columns.
+template <int SIGN>
+__device__ __forceinline__ void add_bias(f32x16& s, const float* hi_s, const float* lo_s, int at, int g, Pair own, float scale) {
+  const f32x16 hi = acc_init(hi_s, at, g), lo = acc_init(lo_s, at, g);
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    s[r] = fmaf(s[r], scale, SIGN > 0 ? (hi[r] - own.hi) + (lo[r] - own.lo) : (own.hi - hi[r]) + (own.lo - lo[r]));
+}
+
+template <typename Tr, int D>
+__device__ __forceinline__ f32x16 dots(const char* tile, int row0, const u32x4 (&reg)[D / 16], f32x16 s, int lane) {
+  const int g = lane >> 5, i = lane & 31;
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) s = Tr::mfma32(lds_row_operand<D>(tile, row0 + i, 2 * kk + g), reg[kk], s);
+  return s;
+}
+__device__ __forceinline__ f32x16 splat(float x) {
+  f32x16 v;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) v[r] = x;
+  return v;
+}
+
+template <typename Tr, int D>
+__device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, const u32x4 (&qreg)[D / 16],
+                                                f32x16 (&oacc)[(D + 31) / 32], float& m_i, float& l_i, int n0, int a_m, Pair row, float qk_scale, int lane) {
+  constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
+  const int g = lane >> 5;
+  f32x16 s[NB];
+  float mloc = -INFINITY;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    s[nb] = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
+    add_bias<-1>(s[nb], hi_s, lo_s, 32 * nb, g, row, qk_scale);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[nb][r] = n0 + 32 * nb + c_row(r, g) > a_m ? -INFINITY : s[nb][r];
+      mloc = fmaxf(mloc, s[nb][r]);
+    }
+  }
+  mloc = half_max(mloc);
+  const bool raise = mloc > m_i + kLazyMaxLog2;
+  if (__any(raise)) {
+    const float m_new = raise ? mloc : m_i, alpha = __builtin_amdgcn_exp2f(m_i - m_new);
+    m_i = m_new;
+    l_i *= alpha;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
+  }
+  float rsum = 0.f;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[nb][r] = __builtin_amdgcn_exp2f(s[nb][r] - m_i);
+      rsum += s[nb][r];
+    }
+  l_i += rsum;
+#pragma unroll
+  for (int sl = 0; sl < BN / 16; ++sl) {
+    const u32x4 pb = pack8<Tr>(s[sl >> 1], 8 * (sl & 1));
+#pragma unroll
+    for (int db = 0; db < DB; ++db) oacc[db] = Tr::mfma32(lds_col_operand<D>(v_tile, 16 * sl, db, lane), pb, oacc[db]);
+  }
+}
+
+// `row`: of the query, its log-normaliser taken off
+template <typename Tr, int D>
+__device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, const u32x4 (&qreg)[D / 16],
+                                               const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rsum, int n0, int a_m, int a_w0, Pair row,
+                                               float qk_scale, float delta, int lane) {
+  constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
+  const int g = lane >> 5;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const int nb0 = n0 + 32 * nb;
+    if (nb0 > a_w0 + 31) continue;   // entirely above this wave's rows
+    f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
+    f32x16 dp = dots<Tr, D>(v_tile, 32 * nb, doreg, splat(-delta), lane);
+    add_bias<-1>(s, hi_s, lo_s, 32 * nb, g, row, qk_scale);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = nb0 + c_row(r, g) > a_m ? 0.f : __builtin_amdgcn_exp2f(s[r]);
+      dp[r] *= p;
+      rsum += dp[r];
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const u32x4 dsb = pack8<Tr>(dp, 8 * hh);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) dqacc[db] = Tr::mfma32(lds_col_operand<D>(k_tile, 32 * nb + 16 * hh, db, lane), dsb, dqacc[db]);
+    }
+  }
+}
+
+// hi_s, lo_s: of the rows, their log-normalisers taken off; dl_s: -delta
+template <typename Tr, int D>
+__device__ __forceinline__ void packed_dkdv_step(const char* q_tile, const char* do_tile, const float* hi_s, const float* lo_s, const float* dl_s, const u32x4 (&kreg)[D / 16],
+                                                 const u32x4 (&vreg)[D / 16], f32x16 (&dkacc)[(D + 31) / 32], f32x16 (&dvacc)[(D + 31) / 32], float& csum, int a_s0, int n,
+                                                 int n_w0, Pair col, float qk_scale, int lane) {
+  constexpr int DB = (D + 31) / 32, MB = kKvBM / 32;
+  const int g = lane >> 5;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int a_b0 = a_s0 + 32 * mb;
+    if (a_b0 + 31 < n_w0) continue;   // entirely above the diagonal for this wave
+    f32x16 s = dots<Tr, D>(q_tile, 32 * mb, kreg, splat(0.f), lane);
+    f32x16 dp = dots<Tr, D>(do_tile, 32 * mb, vreg, acc_init(dl_s, 32 * mb, g), lane);
+    add_bias<1>(s, hi_s, lo_s, 32 * mb, g, col, qk_scale);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = n > a_b0 + c_row(r, g) ? 0.f : __builtin_amdgcn_exp2f(s[r]);
+      dp[r] *= s[r];
+      csum += dp[r];
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const u32x4 pb = pack8<Tr>(s, 8 * hh), dsb = pack8<Tr>(dp, 8 * hh);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        dvacc[db] = Tr::mfma32(lds_col_operand<D>(do_tile, 32 * mb + 16 * hh, db, lane), pb, dvacc[db]);
+        dkacc[db] = Tr::mfma32(lds_col_operand<D>(q_tile, 32 * mb + 16 * hh, db, lane), dsb, dkacc[db]);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Forward: four waves, 32 query rows each, K and V tiles of 64 keys in two alternating LDS buffers, the tiles at the diagonal one by one and
+// the others software-pipelined (the tile code and its reasons: fox_tiles.hpp, fox_fwd.hip).
+// ---------------------------------------------------------------------------
+template <typename Tr, int D>
+__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const PackedK a) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int BM = kFwdBM, BN = kFwdBN, KK = D / 16, DB = (D + 31) / 32, NB = BN / 32;
+  __shared__ __align__(16) char k_tile0[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) char k_tile1[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) char v_tile0[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) char v_tile1[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) float cn_s0[BN];
+  __shared__ __align__(16) float cn_s1[BN];
+  __shared__ __align__(16) float lo_s0[BN];
+  __shared__ __align__(16) float lo_s1[BN];
+  int item, h;
+  packed_block(a, a.H, item, h);
+  if (item >= a.plan.counts[0]) return;
+  const PackedItem it = a.plan.q_items[item];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, i = lane & 31;
+  const int M = it.m, N = it.n, p_seq = N - M, m0 = it.tile * BM;
+  const int hk = h / a.group;
+  const double* c_row = a.c + (int64_t)h * a.N + it.k0;
+  const uint16_t* qp = a.q.ptr + (int64_t)it.q0 * a.q.st + h * a.q.sh;
+  const uint16_t* kp = a.k.ptr + (int64_t)it.k0 * a.k.st + hk * a.k.sh;
+  const uint16_t* vp = a.v.ptr + (int64_t)it.k0 * a.v.st + hk * a.v.sh;
+  uint16_t* op = const_cast<uint16_t*>(a.o.ptr) + (int64_t)it.q0 * a.o.st + h * a.o.sh;
+  const int a0 = p_seq + m0, hi = min(N, a0 + BM);   // key position of the first row, one past the last key that a row sees
+  const int m = m0 + 32 * wave + i, a_m = p_seq + m, a_w0 = a0 + 32 * wave;
+  const float qk_scale = nonzero_scale(a.sm_scale * kLog2e), inv_scale = 1.0f / qk_scale;
+  const bool wave_has_rows = m0 + 32 * wave < M;
+
+  const DirectTileLoader<D, BN, 4, 0> kld(a.k.st, wave, lane), vld(a.v.st, wave, lane);
+  const int n_tiles = hi > 0 ? (hi + BN - 1) / BN : 0;   // walked from the last down
+  f32x16 oacc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) oacc[db][r] = 0.f;
+  float m_i = -3.0e38f, l_i = 0.f;   // (finite: a row that has seen no key yet yields exp2(-inf) = 0)
+  if (n_tiles > 0) {
+    kld.issue(kp, a.k.st, (n_tiles - 1) * BN, N, k_tile0);
+    vld.issue(vp, a.v.st, (n_tiles - 1) * BN, N, v_tile0);
+    u32x4 qreg[KK];
+    load_row_operand_regs<D>(qreg, qp, a.q.st, m, M, g);
+    const double c_ref = c_row[min(max(a0, 0), N - 1)];
+    // the key terms of a tile: requested here, worked out where they go to LDS, a tile later
+    double cn_raw = 0.0;
+    bool cn_ok = false;
+    auto issue_cn = [&](int n0) {
+      if (tid < BN) {
+        cn_ok = n0 + tid < N;
+        cn_raw = c_row[min(n0 + tid, N - 1)];
+      }
+    };
+    // at the diagonal a pair, elsewhere the start value of the score accumulators; keys past the last one get a probability of zero
+    auto store_pair = [&](float* hi, float* lo) {
+      const Pair c = pair_of((cn_raw - c_ref) * kLog2eD);
+      hi[tid] = cn_ok ? c.hi : INFINITY;
+      lo[tid] = cn_ok ? c.lo : 0.f;
+    };
+    auto cn_term = [&]() { return cn_ok ? (float)(c_ref - cn_raw) * kLog2e * inv_scale : -INFINITY; };   // (the scale is positive where it is used)
+    auto issue = [&](int n0, char* kt, char* vt) {
+      issue_cn(n0);   // small load first: the counter of loads retires in order
+      kld.issue(kp, a.k.st, n0, N, kt);
+      vld.issue(vp, a.v.st, n0, N, vt);
+    };
+    issue_cn((n_tiles - 1) * BN);
+    const Pair row = pair_of((c_row[min(max(a_m, 0), N - 1)] - c_ref) * kLog2eD);
+    auto compute = [&](int n0, const char* kt, const char* vt, const float* hi, const float* lo) {
+      if (n0 > a_w0 + 31 || !wave_has_rows) return;   // tile entirely above this wave's rows
+      packed_fwd_tile<Tr, D>(kt, vt, hi, lo, qreg, oacc, m_i, l_i, n0, a_m, row, qk_scale, lane);
+    };
+    // tiles at the diagonal; all of them where the pipelined code, which needs a positive scale and a few tiles, is not entered
+    int n_diag = 0;
+    while (n_diag < n_tiles && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
+    if (!(qk_scale > 0.f) || n_tiles - n_diag < kMinPipelinedTiles) n_diag = n_tiles;
+    const int t_stop = n_tiles - n_diag;
+    if (n_diag > 0 && tid < BN) store_pair(cn_s0, lo_s0);
+    for (int t = n_tiles - 1; t >= t_stop; t -= 2) {
+      wait_vmem_all();
+      __syncthreads();
+      if (t - 1 >= t_stop) issue((t - 1) * BN, k_tile1, v_tile1);
+      compute(t * BN, k_tile0, v_tile0, cn_s0, lo_s0);
+      if (t - 1 < t_stop) break;
+      if (tid < BN) store_pair(cn_s1, lo_s1);
+      wait_vmem_all();
+      __syncthreads();
+      if (t - 2 >= t_stop) issue((t - 2) * BN, k_tile0, v_tile0);
+      compute((t - 1) * BN, k_tile1, v_tile1, cn_s1, lo_s1);
+      if (t - 2 >= t_stop && tid < BN) store_pair(cn_s0, lo_s0);
+    }
+    if (t_stop > 0) {   // K runs one tile ahead of V: iteration j computes S(j + 1) and P(j) V(j)
+      auto int_n0 = [&](int j) { return (t_stop - 1 - j) * BN; };
+      auto issue_k = [&](int j, char* kt) {
+        issue_cn(int_n0(j));
+        kld.issue(kp, a.k.st, int_n0(j), N, kt);
+      };
+      if (n_diag > 0) {
+        __syncthreads();   // every wave is done with every buffer
+        issue_k(0, k_tile0);
+      }
+      if (tid < BN) cn_s0[tid] = cn_term();
+      wait_vmem_all();
+      __syncthreads();
+      if (t_stop > 1) issue_k(1, k_tile1);
+      vld.issue(vp, a.v.st, int_n0(0), N, v_tile0);
+      f32x16 s_a[NB], s_b[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        if (!wave_has_rows) break;
+        s_a[nb] = acc_init(cn_s0, 32 * nb, g);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) s_a[nb] = Tr::mfma32(lds_row_operand<D>(k_tile0, 32 * nb + i, 2 * kk + g), qreg[kk], s_a[nb]);
+      }
+      auto pipelined_tile = [&](int j, const char* k_nx, const char* v_cur, const float* cn_nx, char* k_fill, char* v_fill, f32x16 (&s_cur)[NB],
+                                f32x16 (&s_nx)[NB]) {
+        const bool more_k = j + 2 < t_stop, more_v = j + 1 < t_stop;
+        const int nk = more_k ? int_n0(j + 2) : 0, nv = more_v ? int_n0(j + 1) : 0;
+        if (more_k) issue_cn(nk);
+        const uint16_t *k_src = kp + (int64_t)nk * a.k.st, *v_src = vp + (int64_t)nv * a.v.st;
+        const int k_bytes = kld.extent(a.k.st, nk, more_k ? N : nk), v_bytes = vld.extent(a.v.st, nv, more_v ? N : nv);
+        const TileDma<D, 0> dma{kld, vld, k_src, v_src, k_bytes, v_bytes, k_fill, v_fill};
+        if (wave_has_rows) fwd_tile_pipelined<Tr, D, true>(k_nx, v_cur, cn_nx, qreg, oacc, m_i, l_i, qk_scale, lane, s_cur, s_nx, dma, row.hi);
+        else dma.all();
+      };
+      for (int j = 0; j < t_stop; j += 2) {
+        wait_vmem_all();
+        if (j + 1 < t_stop && tid < BN) cn_s1[tid] = cn_term();
+        __syncthreads();
+        pipelined_tile(j, k_tile1, v_tile0, cn_s1, k_tile0, v_tile1, s_a, s_b);
+        if (j + 1 >= t_stop) break;
+        wait_vmem_all();
+        if (j + 2 < t_stop && tid < BN) cn_s0[tid] = cn_term();
+        __syncthreads();
+        pipelined_tile(j + 1, k_tile0, v_tile1, cn_s0, k_tile1, v_tile0, s_b, s_a);
+      }
+    }
+  }
+  const float l_tot = half_sum(l_i);
+  const bool empty = a_m < 0 || n_tiles <= 0;
+  const float inv = empty ? 0.f : 1.0f / l_tot;
+  if (a.lse && m < M && g == 0) a.lse[(int64_t)h * a.T + it.q0 + m] = empty ? -INFINITY : m_i * kLn2 + __logf(l_tot);
+  // o leaves through LDS, a tile buffer per wave, so that the global stores are whole rows
+  static_assert(kStoreStageBytes<D> <= Tile<D>::bytes(BN), "one wave stages in one tile buffer");
+  wait_vmem_all();
+  __syncthreads();
+  char* stage = wave == 0 ? k_tile0 : wave == 1 ? k_tile1 : wave == 2 ? v_tile0 : v_tile1;
+  store_rows_via_lds<Tr, D>(stage, oacc, inv, op, a.o.st, m0 + 32 * wave, M, lane);
+#endif
+}
+
+// ---------------------------------------------------------------------------
+// dQ: the same walk with Q and dO in registers.  It leaves delta in full for the dK/dV kernel, which runs behind it.
+// ---------------------------------------------------------------------------
+template <typename Tr, int D>
+__global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int BM = kFwdBM, BN = kFwdBN, KK = D / 16, DB = (D + 31) / 32;
+  __shared__ __align__(16) char k_tile0[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) char k_tile1[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) char v_tile0[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) char v_tile1[Tile<D>::bytes(BN)];
+  __shared__ __align__(16) float cn_s0[BN];
+  __shared__ __align__(16) float cn_s1[BN];
+  __shared__ __align__(16) float lo_s0[BN];
+  __shared__ __align__(16) float lo_s1[BN];
+  int item, h;
+  packed_block(a, a.H, item, h);
+  if (item >= a.plan.counts[0]) return;
+  const PackedItem it = a.plan.q_items[item];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, i = lane & 31;
+  const int M = it.m, N = it.n, p_seq = N - M, m0 = it.tile * BM;
+  const int hk = h / a.group;
+  const double* c_row = a.c + (int64_t)h * a.N + it.k0;
+  const int64_t row0 = (int64_t)h * a.T + it.q0;
+  const uint16_t* qp = a.q.ptr + (int64_t)it.q0 * a.q.st + h * a.q.sh;
+  const uint16_t* dop = a.d_o.ptr + (int64_t)it.q0 * a.d_o.st + h * a.d_o.sh;
+  const uint16_t* op = a.o.ptr + (int64_t)it.q0 * a.o.st + h * a.o.sh;
+  const uint16_t* kp = a.k.ptr + (int64_t)it.k0 * a.k.st + hk * a.k.sh;
+  const uint16_t* vp = a.v.ptr + (int64_t)it.k0 * a.v.st + hk * a.v.sh;
+  uint16_t* dqp = const_cast<uint16_t*>(a.dq.ptr) + (int64_t)it.q0 * a.dq.st + h * a.dq.sh;
+  const int a0 = p_seq + m0, hi = min(N, a0 + BM);
+  const int m = m0 + 32 * wave + i, a_m = p_seq + m, a_w0 = a0 + 32 * wave;
+  const float qk_scale = nonzero_scale(a.sm_scale * kLog2e), inv_scale = 1.0f / qk_scale;
+  const bool wave_has_rows = m0 + 32 * wave < M;
+  const int n_tiles = hi > 0 ? (hi + BN - 1) / BN : 0;
+
+  f32x16 dqacc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dqacc[db][r] = 0.f;
+  float delta = 0.f, rsum = 0.f;
+  if (n_tiles > 0) {
+    const DirectTileLoader<D, BN> kld(a.k.st, wave, lane), vld(a.v.st, wave, lane);
+    kld.issue(kp, a.k.st, (n_tiles - 1) * BN, N, k_tile0);
+    vld.issue(vp, a.v.st, (n_tiles - 1) * BN, N, v_tile0);
+    u32x4 qreg[KK], doreg[KK], oreg[KK];
+    load_row_operand_regs<D>(qreg, qp, a.q.st, m, M, g);
+    load_row_operand_regs<D>(doreg, dop, a.d_o.st, m, M, g);
+    load_row_operand_regs<D>(oreg, op, a.o.st, m, M, g);
+    const double c_ref = c_row[min(max(a0, 0), N - 1)], c_m = c_row[min(max(a_m, 0), N - 1)];
+    const float l = a.lse[row0 + min(m, M - 1)];
+    double cn_raw = 0.0;
+    bool cn_ok = false;
+    auto issue_cn = [&](int n0) {
+      if (tid < BN) {
+        cn_ok = n0 + tid < N;
+        cn_raw = c_row[min(n0 + tid, N - 1)];
+      }
+    };
+    auto store_pair = [&](float* hi, float* lo) {
+      const Pair c = pair_of((cn_raw - c_ref) * kLog2eD);
+      hi[tid] = cn_ok ? c.hi : INFINITY;
+      lo[tid] = cn_ok ? c.lo : 0.f;
+    };
+    auto cn_term = [&]() { return (float)(c_ref - cn_raw) * kLog2e * inv_scale; };   // (off the diagonal every key is one)
+    auto issue = [&](int n0, char* kt, char* vt) {
+      issue_cn(n0);
+      kld.issue(kp, a.k.st, n0, N, kt);
+      vld.issue(vp, a.v.st, n0, N, vt);
+    };
+    issue_cn((n_tiles - 1) * BN);
+    // rows past M and rows that see no key (lse = -inf) get -inf
+    const bool row_ok = m < M && l > -INFINITY;
+    Pair row = pair_of((c_m - c_ref) * kLog2eD);
+    const float rowc = row_ok ? row.hi - l * kLog2e : -INFINITY;
+    row = row_ok ? Pair{row.hi, row.lo - l * kLog2e} : Pair{-INFINITY, 0.f};
+    {
+      float part = 0.f;   // each half of the wave holds half of the row
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part += delta_term<Tr>(oreg[kk][e], doreg[kk][e]);
+      delta = half_sum(part);
+    }
+    // the tiles at the diagonal, an even number of them so that the others find the same buffers free (or all tiles)
+    int n_diag = 0;
+    while (n_diag < n_tiles && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
+    n_diag = min(n_diag + (n_diag & 1), n_tiles);
+    const int t_stop = n_tiles - n_diag;
+    if (tid < BN) {
+      if (n_diag > 0) store_pair(cn_s0, lo_s0);
+      else cn_s0[tid] = cn_term();
+    }
+    auto next_terms = [&](int t, float* cn, float* lo) {   // of tile t, which has been requested
+      if (tid < BN) {
+        if (t >= t_stop) store_pair(cn, lo);
+        else cn[tid] = cn_term();
+      }
+    };
+    for (int t = n_tiles - 1; t >= t_stop; t -= 2) {
+      wait_vmem_all();
+      __syncthreads();
+      if (t >= 1) issue((t - 1) * BN, k_tile1, v_tile1);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, lane);
+      if (t < 1) break;
+      next_terms(t - 1, cn_s1, lo_s1);
+      wait_vmem_all();
+      __syncthreads();
+      if (t >= 2) issue((t - 2) * BN, k_tile0, v_tile0);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, lane);
+      if (t >= 2) next_terms(t - 2, cn_s0, lo_s0);
+    }
+    for (int t = t_stop - 1; t >= 0; t -= 2) {
+      wait_vmem_all();
+      __syncthreads();
+      if (t >= 1) issue((t - 1) * BN, k_tile1, v_tile1);
+      if (wave_has_rows) dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, qk_scale, rowc, delta, lane);
+      if (t < 1) break;
+      if (tid < BN) cn_s1[tid] = cn_term();
+      wait_vmem_all();
+      __syncthreads();
+      if (t >= 2) issue((t - 2) * BN, k_tile0, v_tile0);
+      if (wave_has_rows) dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, qk_scale, rowc, delta, lane);
+      if (t >= 2 && tid < BN) cn_s0[tid] = cn_term();
+    }
+  }
+  const float rtot = half_sum(rsum);
+  if (m < M && g == 0) a.delta[row0 + m] = delta + rtot;
+  __syncthreads();
+  char* stage = wave == 0 ? k_tile0 : wave == 1 ? k_tile1 : wave == 2 ? v_tile0 : v_tile1;
+  store_rows_via_lds<Tr, D>(stage, dqacc, a.sm_scale, dqp, a.dq.st, m0 + 32 * wave, M, lane);
+#endif
+}
+
+// ---------------------------------------------------------------------------
+// dK/dV: one workgroup keeps 128 keys of a key head (K, V and the accumulators in registers) and walks the query rows that see them in steps of 128, for
+// one query head of the group after the other: the sums over the group never leave the registers.
+// ---------------------------------------------------------------------------
+template <typename Tr, int D>
+__global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const PackedK a) {
+#ifdef __HIP_DEVICE_COMPILE__
+  constexpr int BN = kKvBN, BMQ = kKvBM, KK = D / 16, DB = (D + 31) / 32;
+  __shared__ __align__(16) char q_tile0[Tile<D>::bytes(BMQ)];
+  __shared__ __align__(16) char q_tile1[Tile<D>::bytes(BMQ)];
+  __shared__ __align__(16) char do_tile0[Tile<D>::bytes(BMQ)];
+  __shared__ __align__(16) char do_tile1[Tile<D>::bytes(BMQ)];
+  __shared__ __align__(16) float rc_s0[BMQ];
+  __shared__ __align__(16) float rc_s1[BMQ];
+  __shared__ __align__(16) float lo_s0[BMQ];
+  __shared__ __align__(16) float lo_s1[BMQ];
+  __shared__ __align__(16) float dl_s0[BMQ];
+  __shared__ __align__(16) float dl_s1[BMQ];
+  int item, hk;
+  packed_block(a, a.Hk, item, hk);
+  if (item >= a.plan.counts[1]) return;
+  const PackedItem it = a.plan.k_items[item];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, i = lane & 31;
+  const int M = it.m, N = it.n, p_seq = N - M, n0 = it.tile * BN;
+  const uint16_t* kp = a.k.ptr + (int64_t)it.k0 * a.k.st + hk * a.k.sh;
+  const uint16_t* vp = a.v.ptr + (int64_t)it.k0 * a.v.st + hk * a.v.sh;
+  uint16_t* dkp = const_cast<uint16_t*>(a.dk.ptr) + (int64_t)it.k0 * a.dk.st + hk * a.dk.sh;
+  uint16_t* dvp = const_cast<uint16_t*>(a.dv.ptr) + (int64_t)it.k0 * a.dv.st + hk * a.dv.sh;
+  // rows whose key position reaches this tile; a step may begin above them, and all that lies left of key 0 or above a key is masked
+  const int m_lo = max(n0 - p_seq, 0) / BMQ * BMQ;
+  const int n_steps = M > m_lo ? (M - m_lo + BMQ - 1) / BMQ : 0;
+  int n_diag = 0;
+  while (n_diag < n_steps && p_seq + m_lo + n_diag * BMQ < n0 + BN - 1) ++n_diag;
+  const int n_int = n_steps - n_diag, m_top = m_lo + (n_steps - 1) * BMQ;
+  const int n_w0 = n0 + 32 * wave, n = n_w0 + i;
+  const float qk_scale = nonzero_scale(a.sm_scale * kLog2e), inv_scale = 1.0f / qk_scale;
+  const DirectTileLoader<D, BMQ> qld(a.q.st, wave, lane), dold(a.d_o.st, wave, lane);
+
+  f32x16 dkacc[DB], dvacc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { dkacc[db][r] = 0.f; dvacc[db][r] = 0.f; }
+  u32x4 kreg[KK], vreg[KK];
+  if (n_steps > 0) {
+    load_row_operand_regs<D>(kreg, kp, a.k.st, n, N, g);
+    load_row_operand_regs<D>(vreg, vp, a.v.st, n, N, g);
+  }
+
+  // A step is a (query head, first row).  Its tiles and its rows' terms are requested while the step before it is computed, across the heads as well; the terms
+  // are worked out where they go to LDS, a quarter of the rows a wave, and so is the key's own term of a new head.
+  struct Step {
+    int j, ms;   // head within the group, first row
+  };
+  const bool row_lane = lane < BMQ / 4;
+  const int row_slot = wave * (BMQ / 4) + lane;
+  float l_raw = 0.f, d_raw = 0.f;
+  double c_raw = 0.0, c_ref = 0.0, c_key = 0.0;   // of the step requested last
+  bool row_ok = false;
+  auto head_of = [&](int j) { return hk * a.group + j; };
+  auto issue_rows = [&](Step s) {
+    const int h = head_of(s.j);
+    const double* c_row = a.c + (int64_t)h * a.N + it.k0;
+    const int64_t rows = (int64_t)h * a.T + it.q0;
+    c_ref = c_row[min(n0 + BN, N) - 1];   // the tile's last key: between its keys and the rows below the diagonal
+    c_key = c_row[min(n, N - 1)];
+    if (row_lane) {
+      const int mm = s.ms + row_slot, mc = min(mm, M - 1);
+      row_ok = mm < M;
+      l_raw = a.lse[rows + mc];
+      c_raw = c_row[min(max(p_seq + mc, 0), N - 1)];
+      d_raw = a.delta[rows + mc];
+    }
+  };
+  // at the diagonal a pair, else the start value of the score accumulators; rows past M and those that see no key get a probability of zero
+  auto on_diagonal = [&](Step s) { return p_seq + s.ms < n0 + BN - 1; };
+  auto store_rows = [&](Step s, float* rc, float* lo, float* dl) {
+    if (row_lane) {
+      const bool ok = row_ok && l_raw > -INFINITY;
+      if (on_diagonal(s)) {
+        const Pair c = pair_of((c_raw - c_ref) * kLog2eD);
+        rc[row_slot] = ok ? c.hi : -INFINITY;
+        lo[row_slot] = ok ? c.lo - l_raw * kLog2e : 0.f;
+      } else {
+        rc[row_slot] = ok ? ((float)(c_raw - c_ref) - l_raw) * kLog2e * inv_scale : copysignf(INFINITY, -inv_scale);
+      }
+      dl[row_slot] = ok ? -d_raw : 0.f;
+    }
+  };
+  auto q_at = [&](Step s) { return a.q.ptr + head_of(s.j) * a.q.sh + (int64_t)(it.q0 + s.ms) * a.q.st; };
+  auto do_at = [&](Step s) { return a.d_o.ptr + head_of(s.j) * a.d_o.sh + (int64_t)(it.q0 + s.ms) * a.d_o.st; };
+  constexpr int PER = DirectTileLoader<D, BMQ>::PER;
+  auto issue = [&](Step s, char* qt, char* dot) {
+    issue_rows(s);   // small loads first: the counter of loads retires in order
+    const uint16_t *qs = q_at(s), *ds = do_at(s);
+    const int q_bytes = qld.extent(a.q.st, s.ms, M), do_bytes = dold.extent(a.d_o.st, s.ms, M);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) qld.issue_one(e, qs, q_bytes, qt);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) dold.issue_one(e, ds, do_bytes, dot);
+  };
+  Pair col{0.f, 0.f};   // of the lane's key, for the head that is being computed
+  auto new_key_term = [&]() {
+    col = pair_of((c_key - c_ref) * kLog2eD);
+    if (n >= N) col = {INFINITY, 0.f};
+  };
+  float csum = 0.f;
+  // dc of a head's keys; `more`: its other steps have left their part there
+  auto store_dc = [&](int j, bool more) {
+    const float ctot = half_sum(csum);
+    float* dc = a.dc + (int64_t)head_of(j) * a.N + it.k0 + n;
+    if (n < N && g == 0) *dc = (more ? *dc : 0.f) - ctot;
+    csum = 0.f;
+  };
+
+  if (n_steps == 0) {
+    for (int j = 0; j < a.group; ++j) store_dc(j, false);
+  } else if constexpr (D <= 64) {
+    // every head's steps, those at the diagonal first, in turn from two sets of buffers
+    auto next = [&](Step s) {
+      const int idx = s.ms < m_lo + n_diag * BMQ ? (s.ms - m_lo) / BMQ : n_diag + (m_top - s.ms) / BMQ, up = idx + 1;
+      if (up == n_steps) return Step{s.j + 1, n_diag > 0 ? m_lo : m_top};
+      return Step{s.j, up < n_diag ? m_lo + up * BMQ : m_top - (up - n_diag) * BMQ};
+    };
+    Step cur{0, n_diag > 0 ? m_lo : m_top};
+    issue(cur, q_tile1, do_tile1);
+    store_rows(cur, rc_s1, lo_s1, dl_s1);
+    new_key_term();
+    wait_vmem_all();
+    for (int t = 0;; ++t) {
+      const bool odd = t & 1;
+      const Step nx = next(cur);
+      const bool more = nx.j < a.group;
+      __syncthreads();
+      if (more) issue(nx, odd ? q_tile1 : q_tile0, odd ? do_tile1 : do_tile0);
+      const char *qt = odd ? q_tile0 : q_tile1, *dot = odd ? do_tile0 : do_tile1;
+      const float *rc = odd ? rc_s0 : rc_s1, *dl = odd ? dl_s0 : dl_s1;
+      if (on_diagonal(cur)) packed_dkdv_step<Tr, D>(qt, dot, rc, odd ? lo_s0 : lo_s1, dl, kreg, vreg, dkacc, dvacc, csum, p_seq + cur.ms, n, n_w0, col, qk_scale, lane);
+      else dkdv_step<Tr, D>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, csum, p_seq + cur.ms, n, n_w0, qk_scale, col.hi, lane);
+      if (nx.j != cur.j) store_dc(cur.j, false);
+      if (!more) break;
+      store_rows(nx, odd ? rc_s1 : rc_s0, odd ? lo_s1 : lo_s0, odd ? dl_s1 : dl_s0);
+      if (nx.j != cur.j) new_key_term();
+      wait_vmem_all();
+      cur = nx;
+    }
+  } else {
+    // First the steps at the diagonal of all heads, then the others, pipelined: one wave per SIMD, whose registers hold one kind of step at a time.
+    const int diag_steps = n_diag * a.group, int_steps = n_int * a.group;
+    for (int j = 0, d = 0, t = 0; t < diag_steps; ++t) {
+      const Step s{j, m_lo + d * BMQ};
+      if (t > 0) __syncthreads();   // buffers 1 are free again
+      issue(s, q_tile1, do_tile1);
+      store_rows(s, rc_s1, lo_s1, dl_s1);
+      new_key_term();
+      wait_vmem_all();
+      __syncthreads();
+      if (t == diag_steps - 1 && n_int > 0) issue(Step{0, m_top}, q_tile0, do_tile0);
+      packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rc_s1, lo_s1, dl_s1, kreg, vreg, dkacc, dvacc, csum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
+      if (++d == n_diag) {
+        store_dc(j++, false);
+        d = 0;
+      }
+    }
+    if (n_int > 0) {
+      if (n_diag == 0) issue(Step{0, m_top}, q_tile0, do_tile0);
+      store_rows(Step{0, m_top}, rc_s0, lo_s0, dl_s0);
+      new_key_term();
+    }
+    Step cur{0, m_top};
+    const int m_int = m_lo + n_diag * BMQ;   // first row of the interior steps
+    // a step from one set of buffers, the next one's tiles into the other; an empty extent where there is none (zeros into the free buffers)
+    auto interior = [&](const char* qt, const char* dot, const float* rc, const float* dl, char* qf, char* dof, float* rcf, float* dlf, bool more) {
+      const bool last = cur.ms == m_int;   // of its head
+      const Step nx = last ? Step{cur.j + 1, m_top} : Step{cur.j, cur.ms - BMQ};
+      if (more) issue_rows(nx);
+      const uint16_t *qs = q_at(more ? nx : cur), *ds = do_at(more ? nx : cur);
+      const int q_bytes = more ? qld.extent(a.q.st, nx.ms, M) : 0, do_bytes = more ? dold.extent(a.d_o.st, nx.ms, M) : 0;
+      dkdv_step_interior<Tr, D, 2 * PER>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, csum, qk_scale, col.hi, lane, [&](auto k) {
+        constexpr int K = decltype(k)::value;
+        if constexpr (K < PER) qld.issue_one(K, qs, q_bytes, qf);
+        else dold.issue_one(K - PER, ds, do_bytes, dof);
+      });
+      if (last) store_dc(cur.j, n_diag > 0);
+      if (more) {
+        store_rows(nx, rcf, nullptr, dlf);   // (off the diagonal)
+        if (last) new_key_term();
+      }
+      cur = nx;
+    };
+    for (int t = 0; t < int_steps; t += 2) {
+      wait_vmem_all();
+      __syncthreads();
+      interior(q_tile0, do_tile0, rc_s0, dl_s0, q_tile1, do_tile1, rc_s1, dl_s1, t + 1 < int_steps);
+      if (t + 1 >= int_steps) break;
+      wait_vmem_all();
+      __syncthreads();
+      interior(q_tile1, do_tile1, rc_s1, dl_s1, q_tile0, do_tile0, rc_s0, dl_s0, t + 2 < int_steps);
+    }
+    wait_vmem_all();   // (the last interior step requested empty tiles)
+  }
+  static_assert(2 * kStoreStageBytes<D> <= Tile<D>::bytes(BMQ), "two waves stage in one tile buffer");
+  __syncthreads();
+  char* stage = (wave < 2 ? q_tile0 : do_tile0) + (wave & 1) * kStoreStageBytes<D>;
+  store_rows_via_lds<Tr, D>(stage, dkacc, a.sm_scale, dkp, a.dk.st, n_w0, N, lane);
+  store_rows_via_lds<Tr, D>(stage, dvacc, 1.0f, dvp, a.dv.st, n_w0, N, lane);
+#endif
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+namespace {
+
+// Tiles of `rows` rows in B sequences and the two ends outside them, at most: each of the sequences that are not empty may have a partial one.
+int tile_bound(int B, int rows) {
+  const int64_t partial = (int64_t)B + 2 < rows ? (int64_t)B + 2 : rows;
+  return (int)(rows / kPackedTile + partial);
+}
+int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+}  // namespace
+
+int64_t packed_plan_bytes(int B, int T, int N) {
+  return 256 + up((int64_t)(B + kPackedOuter) * sizeof(int4)) + ((int64_t)tile_bound(B, T) + tile_bound(B, N)) * (int64_t)sizeof(PackedItem);
+}
+PackedPlan packed_plan(void* memory, int B, int T, int N, int* q_bound, int* k_bound) {
+  PackedPlan p;
+  char* at = (char*)memory;
+  p.counts = (int32_t*)at;
+  p.seqs = (int4*)(at += 256);
+  p.q_items = (PackedItem*)(at += up((int64_t)(B + kPackedOuter) * sizeof(int4)));
+  *q_bound = tile_bound(B, T);
+  *k_bound = tile_bound(B, N);
+  p.k_items = p.q_items + *q_bound;
+  return p;
+}
+
+// Threads for rows of which the average has so many elements: a row is one workgroup's, and few elements keep few threads busy.
+static int row_threads(int64_t elements, int rows) {
+  const int64_t mean = elements / (rows < 1 ? 1 : rows);
+  return mean <= 256 ? 64 : mean <= 1024 ? 256 : 1024;
+}
+
+template <typename Tr, int D>
+static hipError_t packed_fwd_d(const PackedK& args, hipStream_t s) {
+  PackedK a = args;
+  a.by_heads = divisor(a.H);
+  a.by_xcd_heads = divisor(a.H % kXcds ? 1 : a.H / kXcds);
+  const dim3 rows((unsigned)(1 + (int64_t)a.B * a.H));
+  switch (row_threads(a.N, a.B)) {
+    case 64: hipLaunchKernelGGL(packed_scan_kernel<64>, rows, dim3(64), 0, s, a); break;
+    case 256: hipLaunchKernelGGL(packed_scan_kernel<256>, rows, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(packed_scan_kernel<1024>, rows, dim3(1024), 0, s, a);
+  }
+  hipLaunchKernelGGL((packed_fwd_kernel<Tr, D>), dim3((unsigned)((int64_t)a.q_bound * a.H)), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+template <typename Tr, int D>
+static hipError_t packed_bwd_d(const PackedK& args, hipStream_t s) {
+  PackedK a = args;
+  a.by_heads = divisor(a.H);
+  a.by_xcd_heads = divisor(a.H % kXcds ? 1 : a.H / kXcds);
+  hipLaunchKernelGGL((packed_dq_kernel<Tr, D>), dim3((unsigned)((int64_t)a.q_bound * a.H)), dim3(256), 0, s, a);
+  PackedK k = a;
+  k.by_heads = divisor(a.Hk);
+  k.by_xcd_heads = divisor(a.Hk % kXcds ? 1 : a.Hk / kXcds);
+  hipLaunchKernelGGL((packed_dkdv_kernel<Tr, D>), dim3((unsigned)((int64_t)a.k_bound * a.Hk)), dim3(256), 0, s, k);
+  const dim3 rows((unsigned)((int64_t)(a.B + kPackedOuter) * a.H));
+  switch (row_threads(a.N, a.B)) {
+    case 64: hipLaunchKernelGGL(packed_gate_grad_kernel<64>, rows, dim3(64), 0, s, a); break;
+    case 256: hipLaunchKernelGGL(packed_gate_grad_kernel<256>, rows, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(packed_gate_grad_kernel<1024>, rows, dim3(1024), 0, s, a);
+  }
+  return hipGetLastError();
+}
+
+template <typename Tr>
+static hipError_t packed_t(const PackedK& a, int D, bool bwd, hipStream_t s) {
+  switch (D) {
+    case 16: return bwd ? packed_bwd_d<Tr, 16>(a, s) : packed_fwd_d<Tr, 16>(a, s);
+    case 32: return bwd ? packed_bwd_d<Tr, 32>(a, s) : packed_fwd_d<Tr, 32>(a, s);
+    case 64: return bwd ? packed_bwd_d<Tr, 64>(a, s) : packed_fwd_d<Tr, 64>(a, s);
+    case 128: return bwd ? packed_bwd_d<Tr, 128>(a, s) : packed_fwd_d<Tr, 128>(a, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+hipError_t launch_packed_fwd(const PackedK& a, int D, int dtype, hipStream_t s) {
+  return dtype == 0 ? packed_t<Bf16>(a, D, false, s) : packed_t<Fp16>(a, D, false, s);
+}
+hipError_t launch_packed_bwd(const PackedK& a, int D, int dtype, hipStream_t s) {
+  return dtype == 0 ? packed_t<Bf16>(a, D, true, s) : packed_t<Fp16>(a, D, true, s);
+}
+
+}  // namespace fox

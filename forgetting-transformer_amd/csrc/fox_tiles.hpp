@@ -92,11 +92,13 @@ __device__ __forceinline__ void fwd_tile(const char* k_tile, const char* v_tile,
 // by scheduling fences so that MFMA and vector instructions alternate in the instruction stream.
 // dma(u) issues chunk u's share of the global loads of the tiles after next: spread over the tile they
 // do not hold the wave's issue slot back to back right after the barrier.
-template <typename Tr, int D, typename Dma>
+// ROW_TERM: m_i counts the term of the row, and the row sum is taken over the probabilities in 32 bits, for a backward whose probabilities are to add up to one
+// better than their 16-bit rounding does (fox_packed.hip).
+template <typename Tr, int D, bool ROW_TERM = false, typename Dma>
 __device__ __forceinline__ void fwd_tile_pipelined(const char* k_next, const char* v_cur, const float* cn_next,
                                                   const u32x4 (&qreg)[D / 16], f32x16 (&oacc)[(D + 31) / 32], float& m_i,
                                                   float& l_i, float qk_scale, int lane, f32x16 (&s_cur)[kFwdBN / 32],
-                                                  f32x16 (&s_next)[kFwdBN / 32], Dma dma) {
+                                                  f32x16 (&s_next)[kFwdBN / 32], Dma dma, float row_term = 0.f) {
   constexpr int BN = kFwdBN, KK = D / 16, DB = (D + 31) / 32, NB = BN / 32, NSL = BN / 16;
   constexpr int SPC = 16 * NB / KK;  // scores handled per chunk of phase A
   static_assert(16 * NB % KK == 0 && SPC % 4 == 0, "whole float4 groups of scores per chunk");
@@ -132,6 +134,7 @@ __device__ __forceinline__ void fwd_tile_pipelined(const char* k_next, const cha
     __builtin_amdgcn_sched_barrier(0);
   });
   mloc = half_max(mloc) * qk_scale;
+  if constexpr (ROW_TERM) mloc += row_term;
   const bool raise = mloc > m_i + kLazyMaxLog2;
   if (__any(raise)) {  // rare: rescale what has been accumulated so far
     const float m_new = raise ? mloc : m_i;
@@ -145,7 +148,7 @@ __device__ __forceinline__ void fwd_tile_pipelined(const char* k_next, const cha
   }
 
   // Phase B: p = exp2(s*scale - m), row sums, pack  ||  O^T += V^T P^T, one 16-key slice behind
-  const float neg_m = -m_i;
+  const float neg_m = ROW_TERM ? row_term - m_i : -m_i;
   float rsum = 0.f;
   u32x4 pb[NSL];
   u32x4 va[NSL][DB];
@@ -164,14 +167,19 @@ __device__ __forceinline__ void fwd_tile_pipelined(const char* k_next, const cha
 #pragma unroll
       for (int e = 0; e < 8; ++e) s_cur[nb][r0 + e] = __builtin_amdgcn_exp2f(fmaf(s_cur[nb][r0 + e], qk_scale, neg_m));
       pb[c] = pack8<Tr>(s_cur[nb], r0);
+      if constexpr (ROW_TERM) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) rsum = Tr::add_pair(pb[c][e], rsum);  // row sum of the rounded probabilities
+        for (int e = 0; e < 8; ++e) rsum += s_cur[nb][r0 + e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) rsum = Tr::add_pair(pb[c][e], rsum);  // row sum of the rounded probabilities
+      }
     }
     if (c >= 1 && c < NSL) {
 #pragma unroll
-      for (int k = 0; k < DB; ++k) {  // a slice has 16 vector and 8 exp instructions: dealt out over its DB MFMAs
+      for (int k = 0; k < DB; ++k) {  // a slice has 16 vector (20 with ROW_TERM) and 8 exp instructions: dealt out over its DB MFMAs
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, 16 / DB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (ROW_TERM ? 20 : 16) / DB, 0);
         __builtin_amdgcn_sched_group_barrier(0x400, 8 / DB, 0);
       }
     }

@@ -689,6 +689,98 @@ struct QkNormRotaryNode : public torch::autograd::Function<QkNormRotaryNode> {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
+// packed sequences
+// ---------------------------------------------------------------------------------------------------------------
+// A (T, H, D) tensor of tokens; only token and head strides count.
+fox_view token_view(const Tensor& t) { return fox_view{t.data_ptr(), t.stride(0), t.stride(1), t.stride(0)}; }
+// What the tile loaders take: tokens behind each other, not too far apart for 32-bit offsets within a tile.
+bool packed_ok(const Tensor& t) { return vectors_ok(t) && t.stride(0) > 0 && t.stride(0) < (1 << 23); }
+Tensor packed_rows(const Tensor& t) { return packed_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+struct PackedForward {   // what a forward leaves behind
+  Tensor o, c, lse, plan;
+};
+fox_packed_args packed_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& c, const Tensor& lse, const Tensor& plan, int64_t B, double scale) {
+  fox_packed_args a{};
+  a.B = (int32_t)B;
+  a.T = (int32_t)q.size(0);
+  a.N = (int32_t)k.size(0);
+  a.H = (int32_t)q.size(1);
+  a.Hk = (int32_t)k.size(1);
+  a.D = (int32_t)q.size(2);
+  a.dtype = dtype_code(q);
+  a.q = token_view(q);
+  a.k = token_view(k);
+  a.v = token_view(v);
+  a.o = token_view(o);
+  a.c = const_cast<double*>(c.const_data_ptr<double>());
+  a.lse = lse.defined() ? const_cast<float*>(lse.const_data_ptr<float>()) : nullptr;
+  a.plan = const_cast<void*>(plan.const_data_ptr());
+  a.plan_bytes = plan.numel();
+  a.sm_scale = (float)scale;
+  return a;
+}
+PackedForward run_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& cu_q, const Tensor& cu_k, double scale, bool keep) {
+  PackedForward f;
+  const int64_t B = cu_q.size(0) - 1, T = q.size(0), N = k.size(0), H = q.size(1);
+  if (T == 0 || N == 0) {   // nobody sees anything
+    f.o = at::zeros(q.sizes(), q.options());
+    return f;
+  }
+  int64_t plan_bytes = 0;
+  check(fox_packed_plan_bytes((int32_t)B, (int32_t)T, (int32_t)N, &plan_bytes), "fox_packed_plan_bytes");
+  f.o = at::empty(q.sizes(), q.options());
+  f.c = at::empty({H, N}, q.options().dtype(at::kDouble));
+  if (keep) f.lse = at::empty({H, T}, q.options().dtype(at::kFloat));
+  f.plan = empty_bytes_like(q, plan_bytes);
+  fox_packed_args a = packed_args(q, k, v, f.o, f.c, f.lse, f.plan, B, scale);
+  a.g = g.const_data_ptr<float>();
+  a.g_stride_t = g.stride(0);
+  a.g_stride_h = g.stride(1);
+  a.cu_q = cu_q.const_data_ptr<int32_t>();
+  a.cu_k = cu_k.const_data_ptr<int32_t>();
+  check(fox_packed_fwd(&a, stream_of(q)), "fox_packed_fwd");
+  return f;
+}
+
+struct PackedNode : public torch::autograd::Function<PackedNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& cu_q, const Tensor& cu_k, double scale) {
+    PackedForward f = run_packed(q, k, v, g, cu_q, cu_k, scale, true);
+    // (the plan stands for the ends of the sequences, which may be changed before the backward; the gates are not read again)
+    ctx->save_for_backward({q, k, v, f.o, f.c, f.lse, f.plan});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["B"] = cu_q.size(0) - 1;
+    return f.o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined()) return variable_list(7);
+    TORCH_CHECK(!at::GradMode::is_enabled(), "forgetting_attention_packed has no second derivative (create_graph)");
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor q = packed_rows(s[0]), k = packed_rows(s[1]), v = packed_rows(s[2]);
+    const c10::DeviceGuard guard(q.device());
+    const int64_t T = q.size(0), N = k.size(0), H = q.size(1);
+    const auto floats = q.options().dtype(at::kFloat);
+    if (T == 0 || N == 0)
+      return {at::zeros(q.sizes(), q.options()), at::zeros(k.sizes(), k.options()), at::zeros(v.sizes(), v.options()), at::zeros({N, H}, floats), Tensor(), Tensor(), Tensor()};
+    const Tensor o = packed_rows(s[3]), c = packed(s[4]), lse = packed(s[5]), plan = packed(s[6]), d_o = packed_rows(grads[0]);
+    Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options()), dg = at::empty({N, H}, floats);
+    Tensor scratch = at::empty({H * (T + N)}, floats);
+    fox_packed_args a = packed_args(q, k, v, o, c, lse, plan, ctx->saved_data["B"].toInt(), ctx->saved_data["scale"].toDouble());
+    a.d_o = token_view(d_o);
+    a.dq = token_view(dq);
+    a.dk = token_view(dk);
+    a.dv = token_view(dv);
+    a.dg = dg.mutable_data_ptr<float>();
+    a.dg_stride_t = H;
+    a.dg_stride_h = 1;
+    a.delta = scratch.mutable_data_ptr<float>();
+    a.dc = a.delta + H * T;
+    check(fox_packed_bwd(&a, stream_of(q)), "fox_packed_bwd");
+    return {dq, dk, dv, dg, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------------------
 // Python entry points (METH_FASTCALL: the arguments come as a plain array).  Each returns None when the call is not one it
 // handles.  The interpreter lock is free while they allocate, launch and build the graph: a launch may wait for room in a
 // queue, and threads that drive other streams or devices must not wait with it (the argument array keeps its objects alive).
@@ -1275,8 +1367,6 @@ bool pages_ok(const Tensor* k, const Tensor* v, const Tensor* g, fox_pages& p) {
   p.g_stride_t = g->stride(2);
   return true;
 }
-// A (T, H, D) tensor of tokens; only token and head strides count.
-fox_view token_view(const Tensor& t) { return fox_view{t.data_ptr(), t.stride(0), t.stride(1), t.stride(0)}; }
 bool tokens_ok(const Tensor* t, const fox_pages& p, const Tensor& pages) {
   return t && t->dim() == 3 && t->scalar_type() == pages.scalar_type() && t->device() == pages.device() && t->size(1) == p.H && t->size(2) == p.D &&
          t->size(0) <= INT32_MAX && vectors_ok(*t);
@@ -1375,6 +1465,46 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// packed_attention(q, k, v, log_fgate, cu_seqlens, cu_seqlens_k, sm_scale)
+PyObject* py_packed_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 7, "packed_attention takes 7 arguments");
+  const Tensor *q = tensor_of(o[0]), *k = tensor_of(o[1]), *v = tensor_of(o[2]), *g = tensor_of(o[3]), *cu_q = tensor_of(o[4]);
+  if (!q || !k || !v || !g || !cu_q || q->dim() != 3 || k->dim() != 3 || g->dim() != 2 || !on_current_gpu(*q) || !sixteen_bit(*q)) return none();
+  for (const Tensor* t : {k, v, g})
+    if (t->device() != q->device()) return none();
+  const int64_t T = q->size(0), N = k->size(0), H = q->size(1), Hk = k->size(1), D = q->size(2);
+  if (k->scalar_type() != q->scalar_type() || v->scalar_type() != q->scalar_type() || g->scalar_type() != at::kFloat || v->sizes() != k->sizes() || k->size(2) != D ||
+      !head_dim_ok(D) || Hk < 1 || H < 1 || H % Hk || g->size(0) != N || g->size(1) != H || T > (1 << 30) || N > (1 << 30))
+    return none();
+  if (!packed_ok(*q) || !packed_ok(*k) || !packed_ok(*v) || !int32_ok(cu_q, *q, 1) || cu_q->size(0) < 2 || cu_q->size(0) > 65536) return none();
+  const Tensor* cu_k = cu_q;
+  if (o[5] != Py_None) {
+    cu_k = tensor_of(o[5]);
+    if (!int32_ok(cu_k, *q, 1) || cu_k->size(0) != cu_q->size(0)) return none();
+  } else if (N != T) {
+    return none();
+  }
+  double scale = 1.0 / std::sqrt((double)D);
+  if (o[6] != Py_None) scale = PyFloat_AsDouble(o[6]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  Tensor out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    if (needs_graph({q, k, v, g})) {
+      out = PackedNode::apply(*q, *k, *v, *g, *cu_q, *cu_k, scale);
+    } else {
+      const at::NoGradGuard no_grad;
+      out = run_packed(*q, *k, *v, *g, *cu_q, *cu_k, scale, false).o;
+    }
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // record_bounds(list or None)
 PyObject* py_record_bounds(PyObject*, PyObject* list) {
   if (list != Py_None && !PyList_Check(list)) {
@@ -1402,6 +1532,7 @@ PyMethodDef methods[] = {
     {"page_release", (PyCFunction)(void (*)(void))py_page_release, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
+    {"packed_attention", (PyCFunction)(void (*)(void))py_packed_attention, METH_FASTCALL, nullptr},
     {"token_shift", (PyCFunction)(void (*)(void))py_token_shift, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_fox_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -172,6 +172,13 @@ class PagedDecodeArgs(C.Structure):
                 ("requests", C.c_void_p), ("sm_scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+class PackedArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "T", "N", "H", "Hk", "D", "dtype")] + [(n, View) for n in ("q", "k", "v", "o")] + [
+        ("g", C.c_void_p), ("g_stride_t", C.c_int64), ("g_stride_h", C.c_int64), ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("sm_scale", C.c_float),
+        ("c", C.c_void_p), ("lse", C.c_void_p), ("plan", C.c_void_p), ("plan_bytes", C.c_int64)] + [(n, View) for n in ("d_o", "dq", "dk", "dv")] + [
+        ("dg", C.c_void_p), ("dg_stride_t", C.c_int64), ("dg_stride_h", C.c_int64), ("delta", C.c_void_p), ("dc", C.c_void_p)]
+
+
 # every symbol include/fox_attn.h declares: name -> (restype, argtypes)
 SIGNATURES = {
     "fox_version": (C.c_int, []),
@@ -224,6 +231,9 @@ SIGNATURES = {
     "fox_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
     "fox_paged_decode": (C.c_int, [C.POINTER(PagedDecodeArgs), C.c_void_p]),
     "fox_paged_decode_workspace_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.POINTER(C.c_int64)]),
+    "fox_packed_fwd": (C.c_int, [C.POINTER(PackedArgs), C.c_void_p]),
+    "fox_packed_bwd": (C.c_int, [C.POINTER(PackedArgs), C.c_void_p]),
+    "fox_packed_plan_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
     "fox_token_shift_fwd": (C.c_int, [C.POINTER(ShiftArgs), C.c_void_p]),
     "fox_token_shift_bwd": (C.c_int, [C.POINTER(ShiftArgs), C.c_void_p]),
 }

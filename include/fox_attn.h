@@ -544,6 +544,38 @@ typedef struct fox_paged_decode_args {
 int fox_paged_decode(const fox_paged_decode_args* args, void* stream);
 int fox_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int64_t max_keys, int64_t* bytes);
 
+/*
+ * Forgetting Attention over packed sequences.  B sequences lie one after the other: queries cu_q[b] .. cu_q[b+1] - 1 and keys cu_k[b] .. cu_k[b+1] - 1 belong to sequence b (int32
+ * ends on the device, not decreasing).  Query i of m sees the keys j <= i + n - m of the n of its sequence; one that sees none gives zeros, and so do rows that belong to
+ * no sequence, in gradients as well.  Query head h reads key head h / (H / Hk) and has log gates of its own:
+ *   s_ij = sm_scale q_i.k_j + c_i - c_j,  c_j = sum of the sequence's gates up to key j,  o = softmax(s) v.
+ * q, o, d_o, dq: (T, H, D); k, v, dk, dv: (N, Hk, D), 16-bit; stride_t is a token's, stride_h a head's, stride_b is not used; token strides are positive and below 2^23.
+ * c (H, N) fp64, lse (H, T) and the plan are written by the forward and read by the backward, which takes them in place of g, cu_q and cu_k; lse may be NULL for a forward alone.  The plan holds
+ * fox_packed_plan_bytes() bytes, 16-byte aligned.  Log gates below -1e6 count as that.
+ */
+typedef struct fox_packed_args {
+  int32_t B, T, N, H, Hk, D, dtype;
+  fox_view q, k, v, o;
+  const float* g;             /* (N, H) */
+  int64_t g_stride_t, g_stride_h;
+  const int32_t* cu_q;        /* B + 1 */
+  const int32_t* cu_k;
+  float sm_scale;
+  double* c;
+  float* lse;
+  void* plan;
+  int64_t plan_bytes;
+  /* backward; o as the forward left it */
+  fox_view d_o, dq, dk, dv;
+  float* dg;                  /* (N, H), written */
+  int64_t dg_stride_t, dg_stride_h;
+  float* delta;               /* (H, T), scratch */
+  float* dc;                  /* (H, N), scratch */
+} fox_packed_args;
+int fox_packed_fwd(const fox_packed_args* args, void* stream);
+int fox_packed_bwd(const fox_packed_args* args, void* stream);
+int fox_packed_plan_bytes(int32_t B, int32_t T, int32_t N, int64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
