@@ -240,10 +240,14 @@ constexpr double kLog2eD = 1.4426950408889634074;
 // x[r] = s[r] scale + (row - column) with the pairs of rows (or columns) c_row(r, g) in LDS; sign -1: LDS holds the columns.
 template <int SIGN>
 __device__ __forceinline__ void add_bias(f32x16& s, const float* hi_s, const float* lo_s, int at, int g, Pair own, float scale) {
-  const f32x16 hi = acc_init(hi_s, at, g), lo = acc_init(lo_s, at, g);
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-    s[r] = fmaf(s[r], scale, SIGN > 0 ? (hi[r] - own.hi) + (lo[r] - own.lo) : (own.hi - hi[r]) + (own.lo - lo[r]));
+  for (int q4 = 0; q4 < 4; ++q4) {   // (four at a time: all of them at once do not fit the registers of dQ at head dim 128)
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(&hi_s[at + 8 * q4 + 4 * g]), lo = *reinterpret_cast<const f32x4*>(&lo_s[at + 8 * q4 + 4 * g]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      s[4 * q4 + e] = fmaf(s[4 * q4 + e], scale, SIGN > 0 ? (hi[e] - own.hi) + (lo[e] - own.lo) : (own.hi - hi[e]) + (own.lo - lo[e]));
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 template <typename Tr, int D>
@@ -305,6 +309,31 @@ __device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* 
   }
 }
 
+// Off the diagonal of a tile that every row of the wave sees: cn_s holds the start values of the score accumulators, rowc the row's term.  (dq_tile without its causal
+// part, whose row positions the registers of head dim 128 have no room for.)
+template <typename Tr, int D>
+__device__ __forceinline__ void packed_dq_interior(const char* k_tile, const char* v_tile, const float* cn_s, const u32x4 (&qreg)[D / 16], const u32x4 (&doreg)[D / 16],
+                                                   f32x16 (&dqacc)[(D + 31) / 32], float& rsum, float qk_scale, float rowc, float delta, int lane) {
+  constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
+  const int g = lane >> 5;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, acc_init(cn_s, 32 * nb, g), lane);
+    f32x16 dp = dots<Tr, D>(v_tile, 32 * nb, doreg, splat(-delta), lane);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      dp[r] *= __builtin_amdgcn_exp2f(fmaf(s[r], qk_scale, rowc));
+      rsum += dp[r];
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const u32x4 dsb = pack8<Tr>(dp, 8 * hh);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) dqacc[db] = Tr::mfma32(lds_col_operand<D>(k_tile, 32 * nb + 16 * hh, db, lane), dsb, dqacc[db]);
+    }
+  }
+}
+
 // `row`: of the query, its log-normaliser taken off
 template <typename Tr, int D>
 __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, const u32x4 (&qreg)[D / 16],
@@ -317,12 +346,13 @@ __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v
     const int nb0 = n0 + 32 * nb;
     if (nb0 > a_w0 + 31) continue;   // entirely above this wave's rows
     f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
-    f32x16 dp = dots<Tr, D>(v_tile, 32 * nb, doreg, splat(-delta), lane);
     add_bias<-1>(s, hi_s, lo_s, 32 * nb, g, row, qk_scale);
 #pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = nb0 + c_row(r, g) > a_m ? 0.f : __builtin_amdgcn_exp2f(s[r]);
+    f32x16 dp = dots<Tr, D>(v_tile, 32 * nb, doreg, splat(-delta), lane);
+#pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float p = nb0 + c_row(r, g) > a_m ? 0.f : __builtin_amdgcn_exp2f(s[r]);
-      dp[r] *= p;
+      dp[r] *= s[r];
       rsum += dp[r];
     }
 #pragma unroll
@@ -638,13 +668,13 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
       wait_vmem_all();
       __syncthreads();
       if (t >= 1) issue((t - 1) * BN, k_tile1, v_tile1);
-      if (wave_has_rows) dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, qk_scale, rowc, delta, lane);
+      if (wave_has_rows) packed_dq_interior<Tr, D>(k_tile0, v_tile0, cn_s0, qreg, doreg, dqacc, rsum, qk_scale, rowc, delta, lane);
       if (t < 1) break;
       if (tid < BN) cn_s1[tid] = cn_term();
       wait_vmem_all();
       __syncthreads();
       if (t >= 2) issue((t - 2) * BN, k_tile0, v_tile0);
-      if (wave_has_rows) dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, qk_scale, rowc, delta, lane);
+      if (wave_has_rows) packed_dq_interior<Tr, D>(k_tile1, v_tile1, cn_s1, qreg, doreg, dqacc, rsum, qk_scale, rowc, delta, lane);
       if (t >= 2 && tid < BN) cn_s0[tid] = cn_term();
     }
   }
