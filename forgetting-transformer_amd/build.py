@@ -23,7 +23,7 @@ CSRC = ROOT / "csrc"
 OBJ_DIR = ROOT / "build"
 LIB_PATH = ROOT / "forgetting_transformer" / "_lib" / "libfox_attn.so"
 USAGE_PATH = LIB_PATH.with_name("kernel_resources.json")   # registers, spills, LDS of every kernel, from the compiler
-SOURCES = ["fox_fwd.hip", "fox_decode.hip", "fox_bwd.hip", "fox_scan.hip", "fox_shift.hip", "fox_norm_gate.hip", "fox_rotary.hip", "fox_paged.hip", "fox_packed.hip", "fox_probe.hip", "fox_capi.hip"]
+SOURCES = ["fox_fwd.hip", "fox_decode.hip", "fox_bwd.hip", "fox_scan.hip", "fox_shift.hip", "fox_norm_gate.hip", "fox_rotary.hip", "fox_paged.hip", "fox_paged8.hip", "fox_packed.hip", "fox_probe.hip", "fox_capi.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
 TORCH_EXT = "fox_torch.cpp"                                # the operators' host side, a Python extension over the C ABI

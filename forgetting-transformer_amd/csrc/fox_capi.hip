@@ -314,6 +314,33 @@ int make_pages(const fox_pages& p, fox::PagesK& k) {
   k.P = p.P;
   return FOX_OK;
 }
+// 8-bit pages: 16-byte vectors of codes
+int check_codes(const fox_view* v, const char* name) {
+  FOX_TRY(check_view(v, name));
+  if ((v->stride_b & 15) || (v->stride_h & 15) || (v->stride_t & 15)) return fail(FOX_E_ALIGN, "strides of %s must be multiples of 16 elements", name);
+  return FOX_OK;
+}
+int make_pages8(const fox_pages8& p, fox::Pages8K& k, bool plain) {   // plain: 16-bit pages are taken as well
+  FOX_TRY(check_head_dim(p.D));
+  if (p.codes != FOX_CODES_E4M3 && p.codes != FOX_CODES_INT8 && !(plain && p.codes == FOX_CODES_NONE)) return fail(FOX_E_ARG, "codes must be FOX_CODES_E4M3 or FOX_CODES_INT8 (got %d)", p.codes);
+  if (p.P <= 0 || p.H <= 0 || p.Hk <= 0 || p.H % p.Hk) return fail(FOX_E_ARG, "pages and heads must be positive, the query heads a multiple of the key heads (got %d, %d, %d)", p.P, p.H, p.Hk);
+  FOX_TRY(page_shift(p.page_size, &k.shift));
+  k.block_shift = k.shift < 4 ? k.shift : 4;
+  if (p.codes == FOX_CODES_NONE) {
+    FOX_TRY(check_view(&p.k, "k pages"));
+    FOX_TRY(check_view(&p.v, "v pages"));
+  } else {
+    FOX_TRY(check_codes(&p.k, "k pages"));
+    FOX_TRY(check_codes(&p.v, "v pages"));
+    if (!p.k_scales || !p.v_scales) return fail(FOX_E_ARG, "the scales must not be NULL");
+  }
+  if (!p.g) return fail(FOX_E_ARG, "the pages of the log gates must not be NULL");
+  k.k = {(uint8_t*)p.k.ptr, p.k.stride_b, p.k.stride_h, p.k.stride_t, p.k_scales, p.k_scales_stride_p, p.k_scales_stride_h, p.k_scales_stride_t};
+  k.v = {(uint8_t*)p.v.ptr, p.v.stride_b, p.v.stride_h, p.v.stride_t, p.v_scales, p.v_scales_stride_p, p.v_scales_stride_h, p.v_scales_stride_t};
+  k.g = p.g; k.g_sp = p.g_stride_p; k.g_sh = p.g_stride_h; k.g_ss = p.g_stride_t;
+  k.P = p.P;
+  return FOX_OK;
+}
 int check_table(int B, int W, int P) {
   if (B <= 0 || W <= 0 || P <= 0) return fail(FOX_E_ARG, "requests, pages of a request and pages of the pool must be positive (got %d, %d, %d)", B, W, P);
   if (B > fox::kPageRequests) return fail(FOX_E_ARG, "at most %d requests (got %d)", fox::kPageRequests, B);
@@ -519,7 +546,7 @@ extern "C" {
 // fox_attn_decode, fox_cache_append, fox_qk_norm_threshold and fox_attn_fwd_plan, 0.2.3 fox_attn_fwd_gates, fox_attn_fwd_takes_gates,
 // fox_auto_threshold_scan, fox_attn_decode_counted and fox_attn_bwd_logits, 0.2.4 fox_attn_bwd_one_launch,
 // fox_auto_threshold_scan_one_launch and fox_attn_decode_counters, 0.2.5 the rotation (fox_rotary_*) and the pages (fox_page_*, fox_paged_*),
-// 0.2.6 packed sequences (fox_packed_*)
+// 0.2.6 packed sequences (fox_packed_*) and 8-bit pages (fox_paged8_*, fox_paged_gather)
 int fox_version(void) { return 206; }
 
 const char* fox_last_error(void) { return g_err; }
@@ -917,6 +944,103 @@ int fox_cache_append(const fox_cache_append_args* args, void* stream) {
   k.H = args->H; k.T = args->T; k.D = args->D;
   k.total = (uint32_t)total;
   return check_hip(fox::launch_cache_append(k, (hipStream_t)stream), "fox_cache_append");
+}
+
+int fox_paged8_append(const fox_paged8_append_args* a, void* stream) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  fox::Paged8AppendK k{};
+  FOX_TRY(make_pages8(a->pages, k.pages, false));
+  FOX_TRY(check_dtype16(a->dtype));
+  if (a->T <= 0) return fail(FOX_E_ARG, "T must be positive (got %d)", a->T);
+  FOX_TRY(check_view(&a->k, "k"));
+  FOX_TRY(check_view(&a->v, "v"));
+  if (!a->g || !a->slots) return fail(FOX_E_ARG, "g and slots must not be NULL");
+  if ((int64_t)a->T * a->pages.Hk > 1 << 28) return fail(FOX_E_ARG, "too many tokens for one call");   // (a wave each)
+  k.k = (const uint16_t*)a->k.ptr; k.k_st = a->k.stride_t; k.k_sh = a->k.stride_h;
+  k.v = (const uint16_t*)a->v.ptr; k.v_st = a->v.stride_t; k.v_sh = a->v.stride_h;
+  k.g = a->g; k.g_st = a->g_stride_t; k.g_sh = a->g_stride_h;
+  k.slots = a->slots;
+  k.T = a->T; k.H = a->pages.H; k.Hk = a->pages.Hk; k.group = k.H / k.Hk;
+  k.by_heads = fox::divisor(k.Hk);
+  return check_hip(fox::launch_paged8_append(k, a->pages.D, a->dtype, a->pages.codes, (hipStream_t)stream), "fox_paged8_append");
+}
+
+int fox_paged_gather(const fox_paged_gather_args* a, void* stream) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  fox::PagedGatherK k{};
+  FOX_TRY(make_pages8(a->pages, k.pages, true));
+  FOX_TRY(check_dtype16(a->dtype));
+  FOX_TRY(check_table(a->B, a->W, a->pages.P));
+  FOX_TRY(check_room(a->W, a->pages.page_size));
+  if (a->requests_in_table <= 0 || a->T <= 0) return fail(FOX_E_ARG, "requests and T must be positive (got %d, %d)", a->requests_in_table, a->T);
+  if (!a->requests && a->B > a->requests_in_table) return fail(FOX_E_ARG, "%d rows but %d requests in the table", a->B, a->requests_in_table);
+  if (!a->block_table || !a->ends || !a->k || !a->v || !a->g) return fail(FOX_E_ARG, "block_table, ends, k, v and g must not be NULL");
+  if (((uintptr_t)a->k | (uintptr_t)a->v) & 15) return fail(FOX_E_ALIGN, "k and v must be 16-byte aligned");
+  if (a->T > 1 << 30 || a->pages.H > 1 << 20) return fail(FOX_E_ARG, "too many tokens or heads for one call");   // (32 tokens of all heads are counted in 32 bits)
+  k.table = a->block_table; k.table_sb = a->block_table_stride;
+  k.requests = a->requests; k.ends = a->ends;
+  k.k = (uint16_t*)a->k; k.v = (uint16_t*)a->v; k.g = a->g;
+  k.B = a->B; k.R = a->requests_in_table; k.W = a->W; k.T = a->T;
+  k.H = a->pages.H; k.Hk = a->pages.Hk; k.group = k.H / k.Hk;
+  return check_hip(fox::launch_paged_gather(k, a->pages.D, a->dtype, a->pages.codes, (hipStream_t)stream), "fox_paged_gather");
+}
+
+// Workgroups of a piece, and rows of the workspace: a piece has one for each of the query heads.
+static int paged8_parts(int H, int Hk) { return Hk * ((H / Hk + fox::kPaged8Heads - 1) / fox::kPaged8Heads); }
+static int64_t paged8_rows(int B, int H, int Hk, int max_keys, int D) {
+  const int wide = paged8_parts(H, Hk);
+  return (fox::paged_decode_rows(B, wide, max_keys, D) + wide - 1) / wide * H;
+}
+int fox_paged8_decode_workspace_bytes(int32_t B, int32_t H, int32_t Hk, int32_t D, int64_t max_keys, int64_t* bytes) {
+  if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
+  FOX_TRY(check_head_dim(D));
+  if (H <= 0 || Hk <= 0 || H % Hk) return fail(FOX_E_ARG, "the query heads must be a positive multiple of the key heads (got %d, %d)", H, Hk);
+  if (B <= 0 || (int64_t)B * H > (1 << 23) || max_keys <= 0 || max_keys > (1 << 30)) return fail(FOX_E_ARG, "B and max_keys must be positive, B * H at most 2^23, max_keys at most 2^30");
+  const int64_t rows = paged8_rows(B, H, Hk, (int)max_keys, D);
+  *bytes = rows ? rows * (int64_t)(D * sizeof(float) + sizeof(fox::DecodePartial)) + (B + 1) * (int64_t)sizeof(fox::PagedRow) : 0;
+  return FOX_OK;
+}
+
+int fox_paged8_decode(const fox_paged8_decode_args* a, void* stream) {
+  if (!a) return fail(FOX_E_ARG, "args is NULL");
+  fox::Paged8DecodeK k{};
+  FOX_TRY(make_pages8(a->pages, k.pages, false));
+  FOX_TRY(check_dtype16(a->dtype));
+  const int H = a->pages.H, Hk = a->pages.Hk, D = a->pages.D;
+  if (a->B <= 0 || a->requests_in_table <= 0 || a->W <= 0) return fail(FOX_E_ARG, "rows, requests and pages of a request must be positive (got %d, %d, %d)", a->B, a->requests_in_table, a->W);
+  if (!a->requests && a->B > a->requests_in_table) return fail(FOX_E_ARG, "%d rows but %d requests in the table", a->B, a->requests_in_table);
+  FOX_TRY(check_room(a->W, a->pages.page_size));
+  if (a->max_length < 0) return fail(FOX_E_ARG, "max_length must not be negative");
+  if (!a->block_table || !a->lengths) return fail(FOX_E_ARG, "block_table and lengths must not be NULL");
+  FOX_TRY(check_view(&a->q, "q"));
+  FOX_TRY(check_view(&a->o, "o"));
+  fox::PagedDecodeK& r = k.row;
+  const int room = a->W * a->pages.page_size;
+  r.max_keys = a->max_length > 0 && a->max_length < room ? a->max_length : room;
+  int64_t bytes = 0;
+  FOX_TRY(fox_paged8_decode_workspace_bytes(a->B, H, Hk, D, r.max_keys, &bytes));
+  if (bytes > 0 && (!a->workspace || a->workspace_bytes < bytes)) return fail(FOX_E_ARG, "workspace holds %lld bytes, %lld are needed", a->workspace ? (long long)a->workspace_bytes : 0ll, (long long)bytes);
+  if ((uintptr_t)a->workspace & 15) return fail(FOX_E_ALIGN, "workspace must be 16-byte aligned");
+  r.pages.P = k.pages.P; r.pages.shift = k.pages.shift;
+  r.q = (const uint16_t*)a->q.ptr; r.q_sb = a->q.stride_b; r.q_sh = a->q.stride_h;
+  r.o = (uint16_t*)a->o.ptr; r.o_sb = a->o.stride_b; r.o_sh = a->o.stride_h;
+  r.table = a->block_table; r.table_sb = a->block_table_stride;
+  r.lengths = a->lengths; r.requests = a->requests;
+  r.B = a->B; r.R = a->requests_in_table; r.W = a->W;
+  r.sm_scale = a->sm_scale;
+  k.heads = H; k.Hk = Hk; k.group = H / Hk;
+  r.H = paged8_parts(H, Hk);
+  k.parts = r.H / Hk;
+  r.by_heads = fox::divisor(r.H);
+  k.by_parts = fox::divisor(k.parts);
+  const fox::Pages8K& p = k.pages;
+  k.gates_in_vectors = p.g_ss == 1 && !(p.g_sp & 3) && !(p.g_sh & 3) && !((uintptr_t)p.g & 15);
+  if (const int64_t rows = paged8_rows(a->B, H, Hk, r.max_keys, D)) {
+    r.ws_o = (float*)a->workspace;
+    r.ws_p = (fox::DecodePartial*)(r.ws_o + rows * D);
+    r.ws_row = (fox::PagedRow*)(r.ws_p + rows);
+  }
+  return check_hip(fox::launch_paged8_decode(k, D, a->dtype, a->pages.codes, (hipStream_t)stream), "fox_paged8_decode");
 }
 
 int fox_packed_plan_bytes(int32_t B, int32_t T, int32_t N, int64_t* bytes) {

@@ -255,7 +255,51 @@ struct PagedDecodeK {
   PagedRow* ws_row;                      // (B + 1); null where no row can be more than one piece
   bool planned;                          // ws_row is filled by a launch in front, set by the launcher
   double per_piece;                      // 1 / the pieces of all rows and heads together, about; set by the launcher
+  float batch_us;                        // what a batch of keys for each of the workgroups that run at once takes; set by the launcher
 };
+
+// Pages of 8-bit keys and values (fox_paged8.hip): codes (P, Hk, S, D), a scale for every block of 2^block_shift tokens and head, (P, Hk, S >> block_shift), log gates of
+// the query heads as above.  Strides in elements; a page's in sp, a head's in sh, a token's or a block's in st.
+enum : int { kCodesE4m3 = 0, kCodesInt8 = 1, kCodesNone = 2 };   // the last: 16-bit pages (paged_gather_kernel)
+struct Pages8K {
+  struct Codes {
+    uint8_t* ptr;
+    int64_t sp, sh, st;
+    float* scale;
+    int64_t s_sp, s_sh, s_st;
+  };
+  Codes k, v;
+  float* g;
+  int64_t g_sp, g_sh, g_ss;
+  int P, shift, block_shift;
+};
+struct Paged8AppendK {
+  Pages8K pages;
+  const uint16_t *k, *v;
+  int64_t k_st, k_sh, v_st, v_sh;
+  const float* g;
+  int64_t g_st, g_sh;
+  const int64_t* slots;
+  int T, H, Hk, group;
+  Divisor by_heads;                      // key heads
+};
+struct PagedGatherK {
+  Pages8K pages;                         // 16-bit pages: strides of those, no scales
+  const int32_t* table;
+  int64_t table_sb;
+  const int32_t *requests, *ends;        // (B) or null, (B + 1)
+  uint16_t *k, *v;                       // (T, Hk, D) contiguous
+  float* g;                              // (T, H) contiguous
+  int B, R, W, T, H, Hk, group;
+};
+struct Paged8DecodeK {
+  PagedDecodeK row;                      // pages unused but for P and shift; H counts the workgroups of a piece: key heads times parts of their groups
+  Pages8K pages;
+  int heads, Hk, group, parts;           // query heads, key heads, query heads of one, and in how many parts of up to 16 a group is taken
+  Divisor by_parts;
+  bool gates_in_vectors;                 // four gates of consecutive tokens can be read at once
+};
+constexpr int kPaged8Heads = 16;         // query heads of a workgroup: the columns of a matrix instruction
 
 // Attention over packed sequences (fox_packed.hip).  Sequence b has the queries [q0, q0 + m) and the keys [k0, k0 + n); a tile is 128 rows of either.
 struct PackedItem {
@@ -421,6 +465,11 @@ hipError_t launch_page_release(const PageReleaseK& a, hipStream_t s);
 hipError_t launch_paged_append(const PagedAppendK& a, int D, hipStream_t s);
 hipError_t launch_paged_decode(const PagedDecodeK& a, int D, int dtype, hipStream_t s);
 int64_t paged_decode_rows(int B, int H, int max_keys, int D);   // of workspace; 0: no request is split
+hipError_t launch_paged_plan(const PagedDecodeK& a, int D, hipStream_t s);
+hipError_t launch_paged_merge(const PagedDecodeK& a, int D, int dtype, hipStream_t s);
+hipError_t launch_paged8_append(const Paged8AppendK& a, int D, int dtype, int codes, hipStream_t s);
+hipError_t launch_paged_gather(const PagedGatherK& a, int D, int dtype, int codes, hipStream_t s);
+hipError_t launch_paged8_decode(const Paged8DecodeK& a, int D, int dtype, int codes, hipStream_t s);
 int64_t rotary_workspace_floats(int64_t tokens, int heads, int D, bool shared);
 int64_t packed_plan_bytes(int B, int T, int N);
 PackedPlan packed_plan(void* memory, int B, int T, int N, int* q_bound, int* k_bound);

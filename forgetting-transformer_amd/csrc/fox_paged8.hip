@@ -1,0 +1,610 @@
+// Pages of 8-bit keys and values for gfx950: the append that quantises, the gather that reads back, and Forgetting Attention of one new token per request.
+//
+// A page of S tokens holds the codes of every key head's keys and values (P, Hk, S, D) and one fp32 scale for each block of G = min(S, 16) tokens and head; an
+// element stands for code * scale.  The log gates, one for every query head, stay in 32 bits.  Codes are e4m3 (largest 448) or whole numbers (largest 127).
+//
+// The scales that the append gives are powers of two.  x / scale is exact then, so a code is one rounding of its element (to the nearest, ties to the even one) and a block
+// whose scale has to grow is rounded again from its codes without another error; e4m3 has as many bits at any scale, whole numbers lose half a bit
+// on average against the scale that just fits.  The readers take any scales.
+#include "fox_common.hpp"
+#include "fox_kernels.hpp"
+#include "fox_paged_plan.hpp"
+
+namespace fox {
+
+namespace {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+struct E4m3 {
+  static constexpr float kLargest = 448.f;
+  // exponent field of the smallest power of two by which a magnitude fits: 448 is 1.75 * 2^8
+  static __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) { return (int)((amax_bits + 0x1fffffu) >> 23) - 8; }
+  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {   // of values within the largest, or NaN
+    uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+  }
+  static __device__ __forceinline__ void decode4(uint32_t w, float (&f)[4]) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    f[0] = lo[0]; f[1] = lo[1]; f[2] = hi[0]; f[3] = hi[1];
+  }
+  static __device__ __forceinline__ float clamped(float x) { return x == x ? fminf(fmaxf(x, -kLargest), kLargest) : x; }   // NaN stays one
+  // four codes as bf16, which holds every one of them
+  static __device__ __forceinline__ u32x2 bf16x4(uint32_t w) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
+  }
+};
+struct Int8 {
+  static constexpr float kLargest = 127.f;
+  static __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) { return (int)((amax_bits + 0x1ffffu) >> 23) - 6; }   // 127 is 1.984375 * 2^6
+  static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    auto one = [](float x) { return (uint32_t)(int)__builtin_rintf(x) & 0xffu; };
+    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+  }
+  static __device__ __forceinline__ void decode4(uint32_t w, float (&f)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(w >> (8 * e));
+  }
+  static __device__ __forceinline__ float clamped(float x) { return x == x ? fminf(fmaxf(x, -kLargest), kLargest) : 0.f; }   // NaN becomes zero
+  static __device__ __forceinline__ u32x2 bf16x4(uint32_t w) {
+    float f[4];
+    decode4(w, f);
+    return u32x2{Bf16::pack2(f[0], f[1]), Bf16::pack2(f[2], f[3])};
+  }
+};
+
+template <typename Tr>
+__device__ __forceinline__ void unpack8(const u32x4& v, float (&f)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[2 * e] = Tr::lo(v[e]);
+    f[2 * e + 1] = Tr::hi(v[e]);
+  }
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Append
+// ---------------------------------------------------------------------------
+namespace {
+
+// One tensor's rows of a run: `len` consecutive tokens into rows row0 .. of a block, whose rows in front of row0 stay.  Executed by a whole wave; lane / LPR is the row of a
+// load, LPR lanes of eight elements each.
+template <typename Tr, typename C, int D>
+__device__ __forceinline__ void append_rows(const u32x4 (&x)[(16 * (D / 8) + 63) / 64], uint8_t* block, int64_t st, float* scale_at, int row0, int len, int lane) {
+  constexpr int LPR = D / 8, R = 64 / LPR, NIT = (16 + R - 1) / R;
+  const int r = lane / LPR, ch = lane % LPR;
+  uint32_t amax = 0;   // bits of the largest finite magnitude
+#pragma unroll
+  for (int it = 0; it < NIT; ++it) {
+    float f[8];
+    unpack8<Tr>(x[it], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t m = __float_as_uint(f[e]) & 0x7fffffffu;
+      if (it * R + r < len && m < 0x7f800000u) amax = max(amax, m);
+    }
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, off));
+  float scale = __uint_as_float((uint32_t)max(C::scale_exponent(amax), 1) << 23);
+  const float old = row0 > 0 ? *scale_at : 0.f;
+  scale = fmaxf(scale, old);
+  if (row0 > 0 && scale != old) {   // the rows in front, rounded again to the larger scale
+    const float ratio = old / scale;
+    u32x2 w[NIT];
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) w[it] = *reinterpret_cast<const u32x2*>(block + min(it * R + r, row0 - 1) * st + 8 * ch);
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      u32x2 y;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float f[4];
+        C::decode4(w[it][i], f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = C::clamped(f[e] * ratio);
+        y[i] = C::encode4(f[0], f[1], f[2], f[3]);
+      }
+      if (it * R + r < row0) *reinterpret_cast<u32x2*>(block + (it * R + r) * st + 8 * ch) = y;
+    }
+  }
+  const float inv = 1.0f / scale;
+#pragma unroll
+  for (int it = 0; it < NIT; ++it) {
+    float f[8];
+    unpack8<Tr>(x[it], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = C::clamped(f[e] * inv);
+    const u32x2 y = {C::encode4(f[0], f[1], f[2], f[3]), C::encode4(f[4], f[5], f[6], f[7])};
+    if (it * R + r < len) *reinterpret_cast<u32x2*>(block + (row0 + it * R + r) * st + 8 * ch) = y;
+  }
+  if (lane == 0 && scale != old) *scale_at = scale;
+}
+
+}  // namespace
+
+// A run is what lies in one block of consecutive slots of consecutive tokens; its first token's wave of a key head takes it whole, so that the block's scale is known before
+// a code is written and nobody waits for anybody.  A wave looks at CHUNK tokens of a head for the beginnings of runs: one token each where there are few (the next tokens
+// of a step are runs of their own), sixteen where prompts fill whole blocks.
+template <typename Tr, typename C, int D, int CHUNK>
+__global__ __launch_bounds__(256) void paged8_append_kernel(const Paged8AppendK a) {
+  constexpr int LPR = D / 8, R = 64 / LPR, NIT = (16 + R - 1) / R;
+  const int lane = threadIdx.x & 63, unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunk = divide(unit, a.by_heads), hk = unit - chunk * a.Hk, t0 = chunk * CHUNK;
+  if (t0 >= a.T) return;
+  const Pages8K& pg = a.pages;
+  const int64_t slots = (int64_t)pg.P << pg.shift;
+  const int block_rows = 1 << pg.block_shift;
+  // lane i has the slot of token t0 - 1 + i
+  int64_t slot = -2;
+  if (lane <= CHUNK + 15) {
+    const int t = t0 - 1 + lane;
+    if (t >= 0 && t < a.T) slot = a.slots[t];
+  }
+  if (slot < 0 || slot >= slots) slot = -2;
+  const int64_t before = __shfl_up(slot, 1);
+  const bool follows = lane > 0 && slot >= 0 && before == slot - 1 && (slot & (block_rows - 1)) != 0;
+  uint64_t starts = __ballot(lane > 0 && lane <= CHUNK && slot >= 0 && !follows);
+  const uint64_t rest = __ballot(follows);
+  const int r = lane / LPR, ch = lane % LPR;
+  while (starts) {
+    const int i = __ffsll((unsigned long long)starts) - 1;
+    starts &= starts - 1;
+    const int len = 1 + (__ffsll((unsigned long long)~(rest >> (i + 1))) - 1);   // (the run ends within the lanes that have a slot)
+    const int64_t first = ((int64_t)__builtin_amdgcn_readlane((int)(slot >> 32), i) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)slot, i);
+    const int t = t0 - 1 + i;
+    u32x4 kx[NIT], vx[NIT];
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int64_t row = t + min(it * R + r, len - 1);
+      kx[it] = *reinterpret_cast<const u32x4*>(a.k + row * a.k_st + hk * a.k_sh + 8 * ch);
+      vx[it] = *reinterpret_cast<const u32x4*>(a.v + row * a.v_st + hk * a.v_sh + 8 * ch);
+    }
+    const int64_t page = first >> pg.shift;
+    const int at = (int)(first & ((1 << pg.shift) - 1)), block = at >> pg.block_shift, row0 = at & (block_rows - 1);
+    // the gates of the group's query heads: a token each of sixteen lanes
+    const int tok = lane & 15;
+    if (tok < len) {
+      for (int j = lane >> 4; j < a.group; j += 4) {
+        const int h = hk * a.group + j;
+        pg.g[page * pg.g_sp + h * pg.g_sh + (at + tok) * pg.g_ss] = a.g[(int64_t)(t + tok) * a.g_st + h * a.g_sh];
+      }
+    }
+    append_rows<Tr, C, D>(kx, pg.k.ptr + page * pg.k.sp + hk * pg.k.sh + (at - row0) * pg.k.st, pg.k.st, pg.k.scale + page * pg.k.s_sp + hk * pg.k.s_sh + block * pg.k.s_st, row0, len, lane);
+    append_rows<Tr, C, D>(vx, pg.v.ptr + page * pg.v.sp + hk * pg.v.sh + (at - row0) * pg.v.st, pg.v.st, pg.v.scale + page * pg.v.s_sp + hk * pg.v.s_sh + block * pg.v.s_st, row0, len, lane);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Gather: the first tokens of requests out of their pages, one request after the other, in 16 bits.  A workgroup takes kGatherTokens places: their requests from a search
+// in the ends, their pages from the table, then rows of eight elements a lane, head by head, so that the codes of neighbouring tokens are read as they lie.
+// ---------------------------------------------------------------------------
+constexpr int kGatherTokens = 32;
+
+template <typename Tr, int CODES, int D>
+__global__ __launch_bounds__(256) void paged_gather_kernel(const PagedGatherK a, const Divisor by_heads) {
+  constexpr int LPR = D / 8, TOK = kGatherTokens, PER_HEAD = TOK * LPR;
+  __shared__ int32_t ends[kPageRequests + 1];
+  __shared__ int64_t slot_s[TOK];   // -1: zeros
+  const int tid = threadIdx.x;
+  const Pages8K& pg = a.pages;
+  for (int i = tid; i <= a.B; i += 256) ends[i] = a.ends[i];
+  __syncthreads();
+  const int64_t t0 = (int64_t)blockIdx.x * TOK;
+  if (tid < TOK) {
+    const int64_t t = t0 + tid;
+    int lo = 0, hi = a.B;   // the first request whose tokens end behind t
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (ends[mid + 1] > t) hi = mid;
+      else lo = mid + 1;
+    }
+    int64_t slot = -1;
+    if (lo < a.B && t >= ends[lo]) {
+      const int64_t pos = t - ends[lo], idx = pos >> pg.shift;
+      const int who = a.requests ? a.requests[lo] : lo;
+      if ((uint32_t)who < (uint32_t)a.R && idx < a.W) {
+        const int page = a.table[who * a.table_sb + idx];
+        if ((uint32_t)page < (uint32_t)pg.P) slot = ((int64_t)page << pg.shift) + (pos & ((1 << pg.shift) - 1));
+      }
+    }
+    slot_s[tid] = slot;
+  }
+  __syncthreads();
+  const int count = (int)min((int64_t)TOK, a.T - t0);
+  for (int idx = tid; idx < PER_HEAD * a.Hk; idx += 256) {
+    const int hk = idx / PER_HEAD, in = idx % PER_HEAD, tok = in / LPR, ch = in % LPR;
+    if (tok >= count) continue;
+    const int64_t slot = slot_s[tok], from = slot < 0 ? 0 : slot;
+    const int64_t page = from >> pg.shift;
+    const int at = (int)(from & ((1 << pg.shift) - 1));
+    u32x4 out[2];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const Pages8K::Codes& c = side ? pg.v : pg.k;
+      if constexpr (CODES == kCodesNone) {
+        out[side] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(c.ptr) + page * c.sp + hk * c.sh + at * c.st + 8 * ch);
+      } else {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(c.ptr + page * c.sp + hk * c.sh + at * c.st + 8 * ch);
+        const float scale = c.scale[page * c.s_sp + hk * c.s_sh + (at >> pg.block_shift) * c.s_st];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float f[4];
+          if constexpr (CODES == kCodesE4m3) E4m3::decode4(w[i], f);
+          else Int8::decode4(w[i], f);
+          out[side][2 * i] = Tr::pack2(f[0] * scale, f[1] * scale);
+          out[side][2 * i + 1] = Tr::pack2(f[2] * scale, f[3] * scale);
+        }
+      }
+      if (slot < 0) out[side] = u32x4{0u, 0u, 0u, 0u};
+    }
+    const int64_t to = ((t0 + tok) * a.Hk + hk) * D + 8 * ch;
+    *reinterpret_cast<u32x4*>(a.k + to) = out[0];
+    *reinterpret_cast<u32x4*>(a.v + to) = out[1];
+  }
+  for (int idx = tid; idx < count * a.H; idx += 256) {
+    const int tok = divide(idx, by_heads), h = idx - tok * a.H;
+    const int64_t slot = slot_s[tok], from = slot < 0 ? 0 : slot;
+    const float g = pg.g[(from >> pg.shift) * pg.g_sp + h * pg.g_sh + (from & ((1 << pg.shift) - 1)) * pg.g_ss];
+    a.g[t0 * a.H + idx] = slot < 0 ? 0.f : g;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention of one token per row over the 8-bit pages of its request, the query heads of a group together:
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(q.k_j sm_scale + sum of the log gates behind j up to the row's last key),  k = code * scale.
+//
+// 2*D bytes of codes a key and key head, 4*D flops for each of its query heads, so the group's heads share what is read: they are the sixteen columns of the matrix
+// instructions (a group of one wastes fifteen, which costs nothing here: a CU's matrix units could take twelve times what memory brings).  Codes become bf16 on their way,
+// exactly, and what they are multiplied by is held in two bf16 parts, q where it has eleven bits and p always: the products are as good as 32 bits.
+//
+//   S (16 keys x heads) = K Q^T: a lane holds 16 consecutive codes of a key, the contraction runs over the lanes' own order of the elements.
+//   O^T (16 elements x heads) += V^T P^T: S leaves a lane four keys of one head, which are its part of P^T as they are; V goes through LDS and comes back transposed.
+//
+// A wave walks whole batches of keys from the last one on, its sum of the gates behind it in 64 bits; runs, pieces, plan and merge are those of the 16-bit pages
+// (fox_paged.hip).  Runs begin at multiples of a batch, so that sixteen keys lie in one block and four gates behind each other.
+// ---------------------------------------------------------------------------
+namespace {
+
+__device__ __forceinline__ f32x4 mfma16(const u32x4& x, const u32x4& y, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+// Two bf16 whose sum is x to 16 bits
+struct Split {
+  uint32_t hi, lo;   // of two numbers
+};
+__device__ __forceinline__ Split split2(float x, float y) {
+  Split s;
+  s.hi = Bf16::pack2(x, y);
+  s.lo = Bf16::pack2(x - Bf16::lo(s.hi), y - Bf16::hi(s.hi));
+  return s;
+}
+
+}  // namespace
+
+template <typename Tr, typename C, int D>
+__global__ __launch_bounds__(256) void paged8_decode_kernel(const Paged8DecodeK a8) {
+  constexpr int KPB = paged_batch(D) / 4;      // keys of a wave's batch
+  constexpr int NT = KPB / 16;                 // tiles of sixteen keys
+  constexpr int LB = D >= 64 ? 16 : 8;         // codes a lane loads of a key at once
+  constexpr int NL = D >= 64 ? D / 64 : 1;     // such loads
+  constexpr int KS = D >= 32 ? D / 32 : 1;     // k-steps of a score
+  constexpr int RS = 2 * D + (D >= 64 ? 32 : 16);   // bytes from one key to the next in LDS
+  constexpr bool kSplitQ = std::is_same_v<Tr, Fp16>;
+  constexpr int AS = D + 4;                    // floats of a head's accumulator at the merge, where it takes the place of V
+  static_assert(16 * AS * 4 <= 32 * RS, "a wave's accumulators fit where its V was");
+  __shared__ __align__(16) char v_s[4][32 * RS];
+  __shared__ float part_m[4][16], part_l[4][16];
+  __shared__ double part_g[4][16];
+
+  const PagedDecodeK& a = a8.row;
+  const Pages8K& pg = a8.pages;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i16 = lane & 15, g = lane >> 4;
+  const int number = divide(blockIdx.x, a.by_heads), hp = blockIdx.x - number * a.H;
+  const PagedPiece at = find_piece<D>(a, number, lane);
+  if (at.b < 0) return;   // (the same in all waves)
+  if (a.ws_row && !a.planned && at.piece == 0 && hp == 0 && tid == 0) a.ws_row[at.b] = PagedRow{at.first, at.share.pieces};   // for the merge
+  const int b = at.b, hk = divide(hp, a8.by_parts), part = hp - hk * a8.parts;
+  const int heads = min(a8.group - part * kPaged8Heads, kPaged8Heads), h0 = hk * a8.group + part * kPaged8Heads;   // of this workgroup
+  const int32_t* table = a.table + (a.requests ? a.requests[b] : b) * a.table_sb;
+  const uint8_t *kp = pg.k.ptr + hk * pg.k.sh, *vp = pg.v.ptr + hk * pg.v.sh;
+  const float *ks = pg.k.scale + hk * pg.k.s_sh, *vs = pg.v.scale + hk * pg.v.s_sh;
+  const float* gp = pg.g + (h0 + min(i16, heads - 1)) * pg.g_sh;   // (columns without a head repeat the last one's)
+  const int in_page = (1 << pg.shift) - 1;
+
+  // run of this wave in batches, from the last
+  const int keys = at.share.keys, all = (keys + KPB - 1) / KPB;
+  const int b1 = max(all - (at.piece * 4 + wave) * at.share.batches, 0), b0 = max(b1 - at.share.batches, 0);
+
+  // element e of k-step s of a lane is number elem0(s) + e of its row
+  auto elem0 = [&](int s) { return D >= 64 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 8 * g; };
+  u32x4 qh[KS], ql[KS];
+  {
+    const uint16_t* qp = a.q + b * a.q_sb + (h0 + min(i16, heads - 1)) * a.q_sh;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const bool there = i16 < heads && (D >= 32 || g < 2);
+      u32x4 x = *reinterpret_cast<const u32x4*>(qp + (D >= 32 || g < 2 ? elem0(s) : 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!there) x[e] = 0u;
+        if constexpr (kSplitQ) {
+          const Split p = split2(Tr::lo(x[e]), Tr::hi(x[e]));
+          qh[s][e] = p.hi;
+          ql[s][e] = p.lo;
+        } else {
+          qh[s][e] = x[e];
+        }
+      }
+    }
+  }
+  const float qk_scale = a.sm_scale * kLog2e;
+  float m = -3.0e38f, l = 0.f;   // of this lane's head; finite floor: what has seen no key yet yields exp2(-inf) = 0
+  f32x4 acc[D / 16];
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  double behind = 0.0;           // sum of the run's gates behind the batch, of this lane's head
+  int page0 = INT32_MAX, entry = -1;   // this lane has the table's entry for page page0 + lane
+  char* const v_tile = v_s[wave];
+
+  for (int batch = b1 - 1; batch >= b0; --batch) {
+    const int n0 = batch * KPB;
+    if ((n0 >> pg.shift) < page0) {
+      page0 = max(((min(n0 + KPB, keys) - 1) >> pg.shift) - 63, 0);
+      entry = table[min(page0 + lane, a.W - 1)];
+      if ((uint32_t)entry >= (uint32_t)pg.P) entry = -1;
+    }
+    // of keys past the last one: that of the last
+    auto page_of = [&](int n) { return __builtin_amdgcn_ds_bpermute(((min(n, keys - 1) >> pg.shift) - page0) << 2, entry); };
+    // codes of this lane's key of every tile
+    u32x4 kx[NT][NL], vx[NT][NL];
+    bool key_ok[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = n0 + 16 * t + i16, page = page_of(n), row = min(n, keys - 1) & in_page;
+      key_ok[t] = n < keys && page >= 0;
+      const int64_t from = max(page, 0);
+      const uint8_t *k = kp + from * pg.k.sp + row * pg.k.st, *v = vp + from * pg.v.sp + row * pg.v.st;
+#pragma unroll
+      for (int c = 0; c < NL; ++c) {
+        if constexpr (LB == 16) {
+          kx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k + 64 * c + 16 * g));
+          vx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v + 64 * c + 16 * g));
+        } else {
+          const int o = D == 32 ? 8 * g : 8 * (g & 1);
+          const u32x2 kw = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(k + o)), vw = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(v + o));
+          kx[t][c] = u32x4{kw[0], kw[1], 0u, 0u};
+          vx[t][c] = u32x4{vw[0], vw[1], 0u, 0u};
+        }
+      }
+    }
+    // gates and scales of the four keys of every tile whose scores this lane will have
+    f32x4 gx[NT];
+    float sk[NT], sv[NT];
+    bool page_ok[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = n0 + 16 * t + 4 * g, page = page_of(n), row = min(n, (keys - 1) & ~3) & in_page;   // (a multiple of four)
+      page_ok[t] = page >= 0;
+      const int64_t from = max(page, 0);
+      const float* p = gp + from * pg.g_sp;
+      if (a8.gates_in_vectors) {
+        gx[t] = *reinterpret_cast<const f32x4*>(p + row);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) gx[t][r] = p[(row + r) * pg.g_ss];
+      }
+      sk[t] = ks[from * pg.k.s_sp + (row >> pg.block_shift) * pg.k.s_st];
+      sv[t] = vs[from * pg.v.s_sp + (row >> pg.block_shift) * pg.v.s_st];
+    }
+    // scores
+    f32x4 s[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int step = 0; step < KS; ++step) {
+        const u32x4& w = kx[t][LB == 16 ? step >> 1 : 0];
+        const int o = LB == 16 ? 2 * (step & 1) : 0;
+        const u32x2 x0 = C::bf16x4(w[o]), x1 = C::bf16x4(w[o + 1]);
+        const u32x4 ka = {x0[0], x0[1], x1[0], x1[1]};
+        s[t] = mfma16(ka, qh[step], s[t]);
+        if constexpr (kSplitQ) s[t] = mfma16(ka, ql[step], s[t]);
+      }
+    }
+    // biases, from the last tile on, and the maximum
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = NT - 1; t >= 0; --t) {
+      float own[4], sum = 0.f;   // own[r]: gates of the lane's keys behind key r
+#pragma unroll
+      for (int r = 3; r >= 0; --r) {
+        own[r] = sum;
+        sum += page_ok[t] && n0 + 16 * t + 4 * g + r < keys ? gx[t][r] : 0.f;
+      }
+      const float next = __shfl_xor(sum, 16), pair = sum + next, other = __shfl_xor(pair, 32);
+      const float after = (g & 1 ? 0.f : next) + (g & 2 ? 0.f : other);   // of the lanes whose keys lie behind
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float bias = (float)(behind + (double)(own[r] + after)) * kLog2e;
+        const float x = fmaf(s[t][r], sk[t] * qk_scale, bias);
+        s[t][r] = page_ok[t] && n0 + 16 * t + 4 * g + r < keys ? x : -INFINITY;
+        top = fmaxf(top, s[t][r]);
+      }
+      behind += (double)(pair + other);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float m_new = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - m_new);
+    m = m_new;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[d] *= alpha;
+    // O^T += V^T P^T, 32 keys at a time
+#pragma unroll
+    for (int u = 0; u < NT / 2; ++u) {
+      u32x4 ph, pl;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(s[2 * u + t][r] - m);
+          l += p[r];
+          p[r] = p[r] > 0.f ? p[r] * sv[2 * u + t] : 0.f;   // (a block that holds no key may have any scale)
+        }
+        const Split x = split2(p[0], p[1]), y = split2(p[2], p[3]);
+        ph[2 * t] = x.hi; ph[2 * t + 1] = y.hi;
+        pl[2 * t] = x.lo; pl[2 * t + 1] = y.lo;
+      }
+      __builtin_amdgcn_wave_barrier();   // (the reads of the 32 keys before come first)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        char* row = v_tile + (16 * t + i16) * RS;
+#pragma unroll
+        for (int c = 0; c < NL; ++c) {
+          u32x4 w = vx[2 * u + t][c];
+          if (!key_ok[2 * u + t]) w = u32x4{0u, 0u, 0u, 0u};   // what is masked may hold anything, NaN among it
+#pragma unroll
+          for (int half = 0; half < LB / 8; ++half) {
+            const u32x2 x0 = C::bf16x4(w[2 * half]), x1 = C::bf16x4(w[2 * half + 1]);
+            const int d = LB == 16 ? 64 * c + 16 * g + 8 * half : 8 * g;
+            if (D >= 32 || g < 2) *reinterpret_cast<u32x4*>(row + 2 * d) = u32x4{x0[0], x0[1], x1[0], x1[1]};
+          }
+        }
+      }
+      staged_rows_visible();
+      const char* src = v_tile + (4 * g + (i16 >> 2)) * RS + 8 * (i16 & 3);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const u32x2 lo = lds_tr_read(src + 32 * d), hi = lds_tr_read(src + 16 * RS + 32 * d);
+        const u32x4 va = {lo[0], lo[1], hi[0], hi[1]};
+        acc[d] = mfma16(va, ph, acc[d]);
+        acc[d] = mfma16(va, pl, acc[d]);
+      }
+    }
+  }
+
+  // merge the waves, each shifted by the gates of the runs behind its own
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (g == 0) {
+    part_m[wave][i16] = m;
+    part_l[wave][i16] = l;
+    part_g[wave][i16] = behind;
+  }
+  __builtin_amdgcn_wave_barrier();   // (the last reads of V come first)
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(v_tile + (i16 * AS + 16 * d + 4 * g) * 4) = acc[d];
+  __syncthreads();
+  constexpr int CPH = D / 4;   // threads of a head, four elements each
+  for (int idx = tid; idx < heads * CPH; idx += 256) {
+    const int j = idx / CPH, d = idx % CPH * 4, h = h0 + j;
+    float mw[4], top = part_m[0][j];
+    double shift = 0.0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      mw[w] = part_m[w][j] + (float)shift * kLog2e;
+      shift += part_g[w][j];
+      top = fmaxf(top, mw[w]);
+    }
+    float lt = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float weight = __builtin_amdgcn_exp2f(mw[w] - top);
+      lt += part_l[w][j] * weight;
+      o += *reinterpret_cast<const f32x4*>(v_s[w] + (j * AS + d) * 4) * weight;
+    }
+    if (at.share.pieces > 1) {   // accumulator, maximum and sum relative to the piece's last key, sum of its gates
+      const int64_t row = (int64_t)number * a8.heads + h;
+      *reinterpret_cast<f32x4*>(a.ws_o + row * D + d) = o;
+      if (d == 0) a.ws_p[row] = DecodePartial{shift, top, lt};
+    } else {
+      const float inv = lt > 0.f ? 1.0f / lt : 0.f;   // no key at all: o = 0
+      *reinterpret_cast<u32x2*>(a.o + b * a.o_sb + h * a.o_sh + d) = u32x2{Tr::pack2(o[0] * inv, o[1] * inv), Tr::pack2(o[2] * inv, o[3] * inv)};
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+template <typename Tr, typename C, int D>
+static hipError_t append_d(const Paged8AppendK& a, hipStream_t s) {
+  const auto grid = [&](int chunk) { return dim3((unsigned)(((int64_t)((a.T + chunk - 1) / chunk) * a.Hk + 3) / 4)); };
+  if ((int64_t)a.T * a.Hk <= 16 * kCus) hipLaunchKernelGGL((paged8_append_kernel<Tr, C, D, 1>), grid(1), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((paged8_append_kernel<Tr, C, D, 16>), grid(16), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+template <typename Tr, typename C, int D>
+static hipError_t decode8_d(const Paged8DecodeK& args, hipStream_t s) {
+  Paged8DecodeK a = args;
+  a.row.per_piece = 1.0 / kPagedPieces;
+  a.row.batch_us = 5.f;
+  a.row.planned = plan_ahead(a.row);
+  if (a.row.planned) {
+    const hipError_t e = launch_paged_plan(a.row, D, s);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D>), dim3((unsigned)paged_decode_workgroups(a.row.B, a.row.H, a.row.max_keys, D)), dim3(256), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || most_pieces(a.row.max_keys, D) <= 1) return e;
+  PagedDecodeK m = a.row;   // the merge goes by query heads
+  m.H = a.heads;
+  m.by_heads = divisor(a.heads);
+  return launch_paged_merge(m, D, std::is_same_v<Tr, Bf16> ? 0 : 1, s);
+}
+
+#define FOX_BY_HEAD_DIM(D, CALL)         \
+  switch (D) {                           \
+    case 16: return CALL(16);            \
+    case 32: return CALL(32);            \
+    case 64: return CALL(64);            \
+    case 128: return CALL(128);          \
+    default: return hipErrorInvalidValue; \
+  }
+
+template <typename Tr, typename C>
+static hipError_t append_t(const Paged8AppendK& a, int D, hipStream_t s) {
+#define FOX_CALL(N) append_d<Tr, C, N>(a, s)
+  FOX_BY_HEAD_DIM(D, FOX_CALL)
+#undef FOX_CALL
+}
+template <typename Tr, typename C>
+static hipError_t decode8_t(const Paged8DecodeK& a, int D, hipStream_t s) {
+#define FOX_CALL(N) decode8_d<Tr, C, N>(a, s)
+  FOX_BY_HEAD_DIM(D, FOX_CALL)
+#undef FOX_CALL
+}
+template <typename Tr, int CODES, int D>
+static hipError_t gather_d(const PagedGatherK& a, hipStream_t s) {
+  hipLaunchKernelGGL((paged_gather_kernel<Tr, CODES, D>), dim3((unsigned)(((int64_t)a.T + kGatherTokens - 1) / kGatherTokens)), dim3(256), 0, s, a, divisor(a.H));
+  return hipGetLastError();
+}
+template <typename Tr, int CODES>
+static hipError_t gather_t(const PagedGatherK& a, int D, hipStream_t s) {
+#define FOX_CALL(N) gather_d<Tr, CODES, N>(a, s)
+  FOX_BY_HEAD_DIM(D, FOX_CALL)
+#undef FOX_CALL
+}
+
+hipError_t launch_paged8_append(const Paged8AppendK& a, int D, int dtype, int codes, hipStream_t s) {
+  if (codes == kCodesE4m3) return dtype == 0 ? append_t<Bf16, E4m3>(a, D, s) : append_t<Fp16, E4m3>(a, D, s);
+  return dtype == 0 ? append_t<Bf16, Int8>(a, D, s) : append_t<Fp16, Int8>(a, D, s);
+}
+hipError_t launch_paged_gather(const PagedGatherK& a, int D, int dtype, int codes, hipStream_t s) {
+  if (codes == kCodesNone) return gather_t<Bf16, kCodesNone>(a, D, s);   // (copied: the type does not matter)
+  if (codes == kCodesE4m3) return dtype == 0 ? gather_t<Bf16, kCodesE4m3>(a, D, s) : gather_t<Fp16, kCodesE4m3>(a, D, s);
+  return dtype == 0 ? gather_t<Bf16, kCodesInt8>(a, D, s) : gather_t<Fp16, kCodesInt8>(a, D, s);
+}
+hipError_t launch_paged8_decode(const Paged8DecodeK& a, int D, int dtype, int codes, hipStream_t s) {
+  if (codes == kCodesE4m3) return dtype == 0 ? decode8_t<Bf16, E4m3>(a, D, s) : decode8_t<Fp16, E4m3>(a, D, s);
+  return dtype == 0 ? decode8_t<Bf16, Int8>(a, D, s) : decode8_t<Fp16, Int8>(a, D, s);
+}
+
+}  // namespace fox

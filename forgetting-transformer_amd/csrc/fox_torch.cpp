@@ -1465,6 +1465,204 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Pages of 8-bit codes (P, Hk, S, D), their scales (P, Hk, S / G) and the log gates of the query heads (P, H, S); `plain`: 16-bit pages without scales are taken as well.
+bool pages8_ok(const Tensor* k, const Tensor* v, const Tensor* ks, const Tensor* vs, const Tensor* g, bool plain, fox_pages8& p) {
+  if (!k || !v || !g || k->dim() != 4 || g->dim() != 3 || k->numel() == 0 || !on_current_gpu(*k) || v->scalar_type() != k->scalar_type() || g->scalar_type() != at::kFloat ||
+      v->device() != k->device() || g->device() != k->device() || v->sizes() != k->sizes() || !head_dim_ok(k->size(3)) || !page_size_ok(k->size(2)))
+    return false;
+  const int64_t P = k->size(0), Hk = k->size(1), S = k->size(2), H = g->size(1);
+  if (P > INT32_MAX || Hk > INT32_MAX || H > INT32_MAX || H < 1 || H % Hk || g->size(0) != P || g->size(2) != S) return false;
+  p = fox_pages8{};
+  const auto type = k->scalar_type();
+  if (type == at::kFloat8_e4m3fn || type == at::kChar) {
+    p.codes = type == at::kChar ? FOX_CODES_INT8 : FOX_CODES_E4M3;
+    for (const Tensor* t : {k, v}) {
+      if (t->stride(3) != 1 || (reinterpret_cast<uintptr_t>(t->const_data_ptr()) & 15)) return false;
+      for (int i = 0; i < 3; ++i)
+        if (t->stride(i) & 15) return false;
+    }
+    if (!ks || !vs) return false;
+    for (const Tensor* t : {ks, vs})
+      if (t->dim() != 3 || t->scalar_type() != at::kFloat || t->device() != k->device() || t->size(0) != P || t->size(1) != Hk || t->size(2) != S / std::min<int64_t>(S, 16)) return false;
+    p.k_scales = const_cast<float*>(ks->const_data_ptr<float>());
+    p.k_scales_stride_p = ks->stride(0); p.k_scales_stride_h = ks->stride(1); p.k_scales_stride_t = ks->stride(2);
+    p.v_scales = const_cast<float*>(vs->const_data_ptr<float>());
+    p.v_scales_stride_p = vs->stride(0); p.v_scales_stride_h = vs->stride(1); p.v_scales_stride_t = vs->stride(2);
+  } else {
+    if (!plain || !sixteen_bit(*k) || ks || vs || !vectors_ok(*k) || !vectors_ok(*v)) return false;
+    p.codes = FOX_CODES_NONE;
+  }
+  p.P = (int32_t)P;
+  p.H = (int32_t)H;
+  p.Hk = (int32_t)Hk;
+  p.page_size = (int32_t)S;
+  p.D = (int32_t)k->size(3);
+  p.k = view_of(*k, true);
+  p.v = view_of(*v, true);
+  p.g = const_cast<float*>(g->const_data_ptr<float>());
+  p.g_stride_p = g->stride(0); p.g_stride_h = g->stride(1); p.g_stride_t = g->stride(2);
+  return true;
+}
+// A 16-bit (T, heads, D) tensor of tokens.
+bool tokens16_ok(const Tensor* t, int64_t heads, int64_t D, const Tensor& pages) {
+  return t && t->dim() == 3 && sixteen_bit(*t) && t->device() == pages.device() && t->size(1) == heads && t->size(2) == D && t->size(0) <= INT32_MAX && vectors_ok(*t);
+}
+
+// paged8_append(k, v, log_fgate, k_pages, v_pages, k_scales, v_scales, log_fgate_pages, slots) -> True
+PyObject* py_paged8_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 9, "paged8_append takes 9 arguments");
+  const Tensor *k = tensor_of(o[0]), *v = tensor_of(o[1]), *g = tensor_of(o[2]), *slots = tensor_of(o[8]);
+  const Tensor* to[5];   // pages of keys and values, their scales, pages of gates
+  for (int i = 0; i < 5; ++i) to[i] = tensor_of(o[3 + i]);
+  fox_paged8_append_args a{};
+  if (!pages8_ok(to[0], to[1], to[2], to[3], to[4], false, a.pages) || !tokens16_ok(k, a.pages.Hk, a.pages.D, *to[0]) || !tokens16_ok(v, a.pages.Hk, a.pages.D, *to[0]) ||
+      v->size(0) != k->size(0) || v->scalar_type() != k->scalar_type())
+    return none();
+  const int64_t T = k->size(0);
+  if (T * a.pages.Hk > (1 << 28)) return none();
+  if (!g || g->dim() != 2 || g->scalar_type() != at::kFloat || g->device() != k->device() || g->size(0) != T || g->size(1) != a.pages.H) return none();
+  if (!slots || slots->dim() != 1 || slots->size(0) != T || slots->scalar_type() != at::kLong || slots->device() != k->device() || !slots->is_contiguous()) return none();
+  if (needs_graph({k, v, g})) return none();
+  const Tensor* from[4] = {k, v, g, slots};
+  for (int i = 0; i < 5; ++i) {
+    if (!writable(*to[i])) return none();
+    for (const Tensor* f : from)
+      if (overlaps(*to[i], *f)) return none();
+    for (int j = 0; j < i; ++j) {   // (pages of keys and values, and their scales, may lie between each other, but are not the same)
+      const bool pair = (i == 1 && j == 0) || (i == 3 && j == 2);
+      if (pair ? to[i]->const_data_ptr() == to[j]->const_data_ptr() : overlaps(*to[i], *to[j])) return none();
+    }
+  }
+  if (T > 0) {
+    const pybind11::gil_scoped_release no_gil;
+    a.T = (int32_t)T;
+    a.dtype = dtype_code(*k);
+    a.k = token_view(*k);
+    a.v = token_view(*v);
+    a.g = g->const_data_ptr<float>();
+    a.g_stride_t = g->stride(0);
+    a.g_stride_h = g->stride(1);
+    a.slots = slots->const_data_ptr<int64_t>();
+    check(fox_paged8_append(&a, stream_of(*k)), "fox_paged8_append");
+  }
+  for (const Tensor* t : to) wrote(*t);
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_gather(k_pages, v_pages, log_fgate_pages, block_table, ends, requests, max_tokens, k_scales, v_scales, fp16) -> (k, v, log_fgate)
+PyObject* py_paged_gather(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 10, "paged_gather takes 10 arguments");
+  const Tensor *kp = tensor_of(o[0]), *vp = tensor_of(o[1]), *gp = tensor_of(o[2]), *table = tensor_of(o[3]), *ends = tensor_of(o[4]);
+  const Tensor *ks = nullptr, *vs = nullptr, *requests = nullptr;
+  if (o[7] != Py_None && !(ks = tensor_of(o[7]))) return none();
+  if (o[8] != Py_None && !(vs = tensor_of(o[8]))) return none();
+  fox_paged_gather_args a{};
+  if (!pages8_ok(kp, vp, ks, vs, gp, true, a.pages) || !int32_ok(table, *kp, 2) || !int32_ok(ends, *kp, 1)) return none();
+  const int64_t B = ends->size(0) - 1, W = table->size(1), S = a.pages.page_size;
+  if (B < 1 || B > 4096 || table->size(0) < 1 || table->size(0) > INT32_MAX || !room_ok(W, S)) return none();
+  if (o[5] != Py_None) {
+    requests = tensor_of(o[5]);
+    if (!int32_ok(requests, *kp, 1) || requests->size(0) != B) return none();
+  } else if (table->size(0) != B) {
+    return none();
+  }
+  const int64_t T = PyLong_AsLongLong(o[6]);
+  bool fp16 = false;
+  if (PyErr_Occurred() || !flag(o[9], fp16)) {
+    PyErr_Clear();
+    return none();
+  }
+  if (T < 0 || T > (1 << 30) || a.pages.H > (1 << 20) || needs_graph({kp, vp, gp, ks, vs})) return none();
+  Tensor out[3];
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const at::NoGradGuard no_grad;
+    const auto type = kp->options().dtype(a.pages.codes == FOX_CODES_NONE ? kp->scalar_type() : fp16 ? at::kHalf : at::kBFloat16);
+    for (int i = 0; i < 2; ++i) out[i] = at::empty({T, a.pages.Hk, a.pages.D}, type);
+    out[2] = at::empty({T, a.pages.H}, gp->options());
+    if (T > 0) {
+      a.B = (int32_t)B;
+      a.requests_in_table = (int32_t)table->size(0);
+      a.W = (int32_t)W;
+      a.T = (int32_t)T;
+      a.dtype = dtype_code(out[0]);
+      a.block_table = table->const_data_ptr<int32_t>();
+      a.block_table_stride = table->stride(0);
+      a.requests = requests ? requests->const_data_ptr<int32_t>() : nullptr;
+      a.ends = ends->const_data_ptr<int32_t>();
+      a.k = out[0].mutable_data_ptr();
+      a.v = out[1].mutable_data_ptr();
+      a.g = out[2].mutable_data_ptr<float>();
+      check(fox_paged_gather(&a, stream_of(*kp)), "fox_paged_gather");
+    }
+  }
+  PyObject* result = PyTuple_New(3);
+  if (!result) return nullptr;
+  for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(out[i]));
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged8_attention(q, k_pages, v_pages, k_scales, v_scales, log_fgate_pages, block_table, lengths, requests, sm_scale, max_length)
+PyObject* py_paged8_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 11, "paged8_attention takes 11 arguments");
+  const Tensor *q = tensor_of(o[0]), *kp = tensor_of(o[1]), *vp = tensor_of(o[2]), *ks = tensor_of(o[3]), *vs = tensor_of(o[4]), *gp = tensor_of(o[5]), *table = tensor_of(o[6]),
+               *lengths = tensor_of(o[7]);
+  fox_paged8_decode_args a{};
+  if (!pages8_ok(kp, vp, ks, vs, gp, false, a.pages) || !tokens16_ok(q, a.pages.H, a.pages.D, *kp) || !int32_ok(table, *kp, 2) || !int32_ok(lengths, *kp, 1)) return none();
+  const int64_t B = q->size(0), W = table->size(1), S = a.pages.page_size;
+  if (lengths->size(0) != B || table->size(0) < 1 || table->size(0) > INT32_MAX || !room_ok(W, S) || B * a.pages.H > (1 << 23)) return none();
+  const Tensor* requests = nullptr;
+  if (o[8] != Py_None) {
+    requests = tensor_of(o[8]);
+    if (!int32_ok(requests, *kp, 1) || requests->size(0) != B) return none();
+  } else if (table->size(0) != B) {
+    return none();
+  }
+  double scale = 1.0 / std::sqrt((double)a.pages.D);
+  if (o[9] != Py_None) scale = PyFloat_AsDouble(o[9]);
+  int64_t most = 0;
+  if (o[10] != Py_None) most = PyLong_AsLongLong(o[10]);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return none();
+  }
+  if ((o[10] != Py_None && most < 1) || needs_graph({q, kp, vp, ks, vs, gp})) return none();
+  Tensor out;
+  {
+    const pybind11::gil_scoped_release no_gil;
+    const at::NoGradGuard no_grad;
+    out = at::empty(q->sizes(), q->options());
+    if (B > 0) {
+      a.B = (int32_t)B;
+      a.requests_in_table = (int32_t)table->size(0);
+      a.W = (int32_t)W;
+      a.max_length = (int32_t)(most > W * S ? 0 : most);
+      a.dtype = dtype_code(*q);
+      a.q = token_view(*q);
+      a.o = token_view(out);
+      a.block_table = table->const_data_ptr<int32_t>();
+      a.block_table_stride = table->stride(0);
+      a.lengths = lengths->const_data_ptr<int32_t>();
+      a.requests = requests ? requests->const_data_ptr<int32_t>() : nullptr;
+      a.sm_scale = (float)scale;
+      check(fox_paged8_decode_workspace_bytes(a.B, a.pages.H, a.pages.Hk, a.pages.D, a.max_length ? a.max_length : W * S, &a.workspace_bytes), "fox_paged8_decode_workspace_bytes");
+      Tensor ws;
+      if (a.workspace_bytes > 0) {
+        ws = empty_bytes_like(*q, a.workspace_bytes);
+        a.workspace = ws.mutable_data_ptr();
+      }
+      check(fox_paged8_decode(&a, stream_of(*q)), "fox_paged8_decode");
+    }
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
 // packed_attention(q, k, v, log_fgate, cu_seqlens, cu_seqlens_k, sm_scale)
 PyObject* py_packed_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1532,6 +1730,9 @@ PyMethodDef methods[] = {
     {"page_release", (PyCFunction)(void (*)(void))py_page_release, METH_FASTCALL, nullptr},
     {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL, nullptr},
     {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
+    {"paged8_append", (PyCFunction)(void (*)(void))py_paged8_append, METH_FASTCALL, nullptr},
+    {"paged_gather", (PyCFunction)(void (*)(void))py_paged_gather, METH_FASTCALL, nullptr},
+    {"paged8_attention", (PyCFunction)(void (*)(void))py_paged8_attention, METH_FASTCALL, nullptr},
     {"packed_attention", (PyCFunction)(void (*)(void))py_packed_attention, METH_FASTCALL, nullptr},
     {"token_shift", (PyCFunction)(void (*)(void))py_token_shift, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -172,6 +172,32 @@ class PagedDecodeArgs(C.Structure):
                 ("requests", C.c_void_p), ("sm_scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
+CODES_E4M3 = 0
+CODES_INT8 = 1
+CODES_NONE = 2   # 16-bit pages: fox_paged_gather only
+
+
+class Pages8(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("P", "H", "Hk", "page_size", "D", "codes")] + [("k", View), ("v", View)] + [
+        (n + s, t) for n in ("k_scales", "v_scales", "g") for s, t in (("", C.c_void_p), ("_stride_p", C.c_int64), ("_stride_h", C.c_int64), ("_stride_t", C.c_int64))]
+
+
+class Paged8AppendArgs(C.Structure):
+    _fields_ = [("pages", Pages8), ("T", C.c_int32), ("dtype", C.c_int32), ("k", View), ("v", View), ("g", C.c_void_p), ("g_stride_t", C.c_int64),
+                ("g_stride_h", C.c_int64), ("slots", C.c_void_p)]
+
+
+class PagedGatherArgs(C.Structure):
+    _fields_ = [("pages", Pages8)] + [(n, C.c_int32) for n in ("B", "requests_in_table", "W", "T", "dtype")] + [
+        ("block_table", C.c_void_p), ("block_table_stride", C.c_int64)] + [(n, C.c_void_p) for n in ("requests", "ends", "k", "v", "g")]
+
+
+class Paged8DecodeArgs(C.Structure):
+    _fields_ = [("pages", Pages8)] + [(n, C.c_int32) for n in ("B", "requests_in_table", "W", "max_length", "dtype")] + [
+        ("q", View), ("o", View), ("block_table", C.c_void_p), ("block_table_stride", C.c_int64), ("lengths", C.c_void_p),
+        ("requests", C.c_void_p), ("sm_scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
 class PackedArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("B", "T", "N", "H", "Hk", "D", "dtype")] + [(n, View) for n in ("q", "k", "v", "o")] + [
         ("g", C.c_void_p), ("g_stride_t", C.c_int64), ("g_stride_h", C.c_int64), ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("sm_scale", C.c_float),
@@ -231,6 +257,10 @@ SIGNATURES = {
     "fox_paged_append": (C.c_int, [C.POINTER(PagedAppendArgs), C.c_void_p]),
     "fox_paged_decode": (C.c_int, [C.POINTER(PagedDecodeArgs), C.c_void_p]),
     "fox_paged_decode_workspace_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.POINTER(C.c_int64)]),
+    "fox_paged8_append": (C.c_int, [C.POINTER(Paged8AppendArgs), C.c_void_p]),
+    "fox_paged_gather": (C.c_int, [C.POINTER(PagedGatherArgs), C.c_void_p]),
+    "fox_paged8_decode": (C.c_int, [C.POINTER(Paged8DecodeArgs), C.c_void_p]),
+    "fox_paged8_decode_workspace_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.POINTER(C.c_int64)]),
     "fox_packed_fwd": (C.c_int, [C.POINTER(PackedArgs), C.c_void_p]),
     "fox_packed_bwd": (C.c_int, [C.POINTER(PackedArgs), C.c_void_p]),
     "fox_packed_plan_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),

@@ -545,6 +545,74 @@ int fox_paged_decode(const fox_paged_decode_args* args, void* stream);
 int fox_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t D, int64_t max_keys, int64_t* bytes);
 
 /*
+ * Pages of 8-bit keys and values: codes (P, Hk, page_size, D), e4m3 or whole numbers, and a fp32 scale for every block of G = min(page_size, 16) tokens and key head,
+ * (P, Hk, page_size / G); an element stands for code * scale.  Log gates are fp32, of the H query heads (H a multiple of Hk), (P, H, page_size).
+ * Codes are 16-byte aligned and their strides multiples of 16.  FOX_CODES_NONE, for fox_paged_gather alone: 16-bit keys and values (strides multiples of 8), no scales.
+ */
+enum { FOX_CODES_E4M3 = 0, FOX_CODES_INT8 = 1, FOX_CODES_NONE = 2 };
+typedef struct fox_pages8 {
+  int32_t P, H, Hk, page_size, D, codes;
+  fox_view k, v;              /* stride_b: from page to page, stride_t: from token to token inside one */
+  float* k_scales;
+  int64_t k_scales_stride_p, k_scales_stride_h, k_scales_stride_t;
+  float* v_scales;
+  int64_t v_scales_stride_p, v_scales_stride_h, v_scales_stride_t;
+  float* g;
+  int64_t g_stride_p, g_stride_h, g_stride_t;
+} fox_pages8;
+
+/*
+ * Keys and values (T, Hk, D), 16-bit, and log gates (T, H) of T tokens into their slots.  A token whose slot is not in the pool is left out.  Slots are distinct, and those in one
+ * block belong to consecutive tokens and follow each other (as fox_page_slots gives them).  A block whose first slot is among them starts anew, with the smallest power of two as
+ * its scale by which the largest finite magnitude of its new rows fits the codes (448, 127; at least 2^-126).  Another keeps the rows in front of the new ones and takes the larger of
+ * that and its scale; if it grows the rows in front are rounded again, code * (old / new).  A code is the nearest to x / scale, ties to the even one; infinities
+ * become the largest code, NaN stays one in e4m3 and becomes 0 in whole numbers.  Rows behind the new ones are left as they were.
+ */
+typedef struct fox_paged8_append_args {
+  fox_pages8 pages;
+  int32_t T, dtype;
+  fox_view k, v;
+  const float* g;
+  int64_t g_stride_t, g_stride_h;
+  const int64_t* slots;
+} fox_paged8_append_args;
+int fox_paged8_append(const fox_paged8_append_args* args, void* stream);
+
+/*
+ * The cached tokens of B requests out of their pages, one request after the other: places ends[b] .. ends[b + 1] - 1 get the first tokens of the request in row requests[b] of the
+ * table (or b), code * scale rounded to 16 bits.  Places of no request, and tokens whose page or request the table does not name, are zeros.  k, v (T, Hk, D) and g (T, H)
+ * are contiguous and 16-byte aligned.  At most 4096 requests.
+ */
+typedef struct fox_paged_gather_args {
+  fox_pages8 pages;
+  int32_t B, requests_in_table, W, T, dtype;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* requests;    /* or NULL */
+  const int32_t* ends;        /* B + 1 */
+  void* k;
+  void* v;
+  float* g;
+} fox_paged_gather_args;
+int fox_paged_gather(const fox_paged_gather_args* args, void* stream);
+
+/* fox_paged_decode over 8-bit pages: one token of H query heads per row, query head h reads key head h / (H / Hk). */
+typedef struct fox_paged8_decode_args {
+  fox_pages8 pages;
+  int32_t B, requests_in_table, W, max_length, dtype;
+  fox_view q, o;              /* (B, H, D): stride_t is not used */
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  const int32_t* lengths;
+  const int32_t* requests;    /* or NULL */
+  float sm_scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} fox_paged8_decode_args;
+int fox_paged8_decode(const fox_paged8_decode_args* args, void* stream);
+int fox_paged8_decode_workspace_bytes(int32_t B, int32_t H, int32_t Hk, int32_t D, int64_t max_keys, int64_t* bytes);
+
+/*
  * Forgetting Attention over packed sequences.  B sequences lie one after the other: queries cu_q[b] .. cu_q[b+1] - 1 and keys cu_k[b] .. cu_k[b+1] - 1 belong to sequence b (int32
  * ends on the device, not decreasing).  Query i of m sees the keys j <= i + n - m of the n of its sequence; one that sees none gives zeros, and so do rows that belong to
  * no sequence, in gradients as well.  Query head h reads key head h / (H / Hk) and has log gates of its own:
