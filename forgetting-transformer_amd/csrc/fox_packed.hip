@@ -313,18 +313,20 @@ __device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* 
 // part, whose row positions the registers of head dim 128 have no room for.)
 template <typename Tr, int D>
 __device__ __forceinline__ void packed_dq_interior(const char* k_tile, const char* v_tile, const float* cn_s, const u32x4 (&qreg)[D / 16], const u32x4 (&doreg)[D / 16],
-                                                   f32x16 (&dqacc)[(D + 31) / 32], float& rsum, float qk_scale, float rowc, float delta, int lane) {
+                                                   f32x16 (&dqacc)[(D + 31) / 32], float& rows, float qk_scale, float rowc, float delta, int lane) {
   constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
   const int g = lane >> 5;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, acc_init(cn_s, 32 * nb, g), lane);
     f32x16 dp = dots<Tr, D>(v_tile, 32 * nb, doreg, splat(-delta), lane);
+    float rsum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       dp[r] *= __builtin_amdgcn_exp2f(fmaf(s[r], qk_scale, rowc));
       rsum += dp[r];
     }
+    rows += rsum;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const u32x4 dsb = pack8<Tr>(dp, 8 * hh);
@@ -337,7 +339,7 @@ __device__ __forceinline__ void packed_dq_interior(const char* k_tile, const cha
 // `row`: of the query, its log-normaliser taken off
 template <typename Tr, int D>
 __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, const u32x4 (&qreg)[D / 16],
-                                               const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rsum, int n0, int a_m, int a_w0, Pair row,
+                                               const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rows, int n0, int a_m, int a_w0, Pair row,
                                                float qk_scale, float delta, int lane) {
   constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
   const int g = lane >> 5;
@@ -350,11 +352,13 @@ __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = nb0 + c_row(r, g) > a_m ? 0.f : __builtin_amdgcn_exp2f(s[r]);
     f32x16 dp = dots<Tr, D>(v_tile, 32 * nb, doreg, splat(-delta), lane);
+    float rsum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       dp[r] *= s[r];
       rsum += dp[r];
     }
+    rows += rsum;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const u32x4 dsb = pack8<Tr>(dp, 8 * hh);
@@ -592,7 +596,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dqacc[db][r] = 0.f;
-  float delta = 0.f, rsum = 0.f;
+  float delta = 0.f;
+  float rsum = 0.f;   // (of sums of tiles: thousands of terms of either sign one by one are only good to 1e-6 of them)
   if (n_tiles > 0) {
     const DirectTileLoader<D, BN> kld(a.k.st, wave, lane), vld(a.v.st, wave, lane);
     kld.issue(kp, a.k.st, (n_tiles - 1) * BN, N, k_tile0);
@@ -792,13 +797,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     col = pair_of((c_key - c_ref) * kLog2eD);
     if (n >= N) col = {INFINITY, 0.f};
   };
-  float csum = 0.f;
+  double csum = 0.0;   // (steps in 32 bits, their sum in 64, as in dQ)
   // dc of a head's keys; `more`: its other steps have left their part there
   auto store_dc = [&](int j, bool more) {
-    const float ctot = half_sum(csum);
+    const float ctot = half_sum((float)csum);
     float* dc = a.dc + (int64_t)head_of(j) * a.N + it.k0 + n;
     if (n < N && g == 0) *dc = (more ? *dc : 0.f) - ctot;
-    csum = 0.f;
+    csum = 0.0;
   };
 
   if (n_steps == 0) {
@@ -823,8 +828,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       if (more) issue(nx, odd ? q_tile1 : q_tile0, odd ? do_tile1 : do_tile0);
       const char *qt = odd ? q_tile0 : q_tile1, *dot = odd ? do_tile0 : do_tile1;
       const float *rc = odd ? rc_s0 : rc_s1, *dl = odd ? dl_s0 : dl_s1;
-      if (on_diagonal(cur)) packed_dkdv_step<Tr, D>(qt, dot, rc, odd ? lo_s0 : lo_s1, dl, kreg, vreg, dkacc, dvacc, csum, p_seq + cur.ms, n, n_w0, col, qk_scale, lane);
-      else dkdv_step<Tr, D>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, csum, p_seq + cur.ms, n, n_w0, qk_scale, col.hi, lane);
+      float sum = 0.f;
+      if (on_diagonal(cur)) packed_dkdv_step<Tr, D>(qt, dot, rc, odd ? lo_s0 : lo_s1, dl, kreg, vreg, dkacc, dvacc, sum, p_seq + cur.ms, n, n_w0, col, qk_scale, lane);
+      else dkdv_step<Tr, D>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, sum, p_seq + cur.ms, n, n_w0, qk_scale, col.hi, lane);
+      csum += (double)sum;
       if (nx.j != cur.j) store_dc(cur.j, false);
       if (!more) break;
       store_rows(nx, odd ? rc_s1 : rc_s0, odd ? lo_s1 : lo_s0, odd ? dl_s1 : dl_s0);
@@ -844,7 +851,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       wait_vmem_all();
       __syncthreads();
       if (t == diag_steps - 1 && n_int > 0) issue(Step{0, m_top}, q_tile0, do_tile0);
-      packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rc_s1, lo_s1, dl_s1, kreg, vreg, dkacc, dvacc, csum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
+      float sum = 0.f;
+      packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rc_s1, lo_s1, dl_s1, kreg, vreg, dkacc, dvacc, sum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
+      csum += (double)sum;
       if (++d == n_diag) {
         store_dc(j++, false);
         d = 0;
@@ -864,11 +873,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       if (more) issue_rows(nx);
       const uint16_t *qs = q_at(more ? nx : cur), *ds = do_at(more ? nx : cur);
       const int q_bytes = more ? qld.extent(a.q.st, nx.ms, M) : 0, do_bytes = more ? dold.extent(a.d_o.st, nx.ms, M) : 0;
-      dkdv_step_interior<Tr, D, 2 * PER>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, csum, qk_scale, col.hi, lane, [&](auto k) {
+      float sum = 0.f;
+      dkdv_step_interior<Tr, D, 2 * PER>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, sum, qk_scale, col.hi, lane, [&](auto k) {
         constexpr int K = decltype(k)::value;
         if constexpr (K < PER) qld.issue_one(K, qs, q_bytes, qf);
         else dold.issue_one(K - PER, ds, do_bytes, dof);
       });
+      csum += (double)sum;
       if (last) store_dc(cur.j, n_diag > 0);
       if (more) {
         store_rows(nx, rcf, nullptr, dlf);   // (off the diagonal)
