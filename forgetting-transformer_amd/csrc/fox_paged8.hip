@@ -34,6 +34,10 @@ struct E4m3 {
     return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
   }
+  static __device__ __forceinline__ u32x2 f16x4(uint32_t w) {   // as fp16, which does as well
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))};
+  }
 };
 struct Int8 {
   static constexpr float kLargest = 127.f;
@@ -51,6 +55,11 @@ struct Int8 {
     float f[4];
     decode4(w, f);
     return u32x2{Bf16::pack2(f[0], f[1]), Bf16::pack2(f[2], f[3])};
+  }
+  static __device__ __forceinline__ u32x2 f16x4(uint32_t w) {
+    float f[4];
+    decode4(w, f);
+    return u32x2{Fp16::pack2(f[0], f[1]), Fp16::pack2(f[2], f[3])};
   }
 };
 
@@ -258,8 +267,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const PagedGatherK a,
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(q.k_j sm_scale + sum of the log gates behind j up to the row's last key),  k = code * scale.
 //
 // 2*D bytes of codes a key and key head, 4*D flops for each of its query heads, so the group's heads share what is read: they are the sixteen columns of the matrix
-// instructions (a group of one wastes fifteen, which costs nothing here: a CU's matrix units could take twelve times what memory brings).  Codes become bf16 on their way,
-// exactly, and what they are multiplied by is held in two bf16 parts, q where it has eleven bits and p always: the products are as good as 32 bits.
+// instructions (a group of one wastes fifteen, which costs nothing here: a CU's matrix units could take twelve times what memory brings).  Codes become 16-bit numbers on their
+// way, exactly: those of K in the type of q, those of V in bf16, whose range has room for p times any scale, with p in two bf16 parts.  The products are as good as 32 bits.
 //
 //   S (16 keys x heads) = K Q^T: a lane holds 16 consecutive codes of a key, the contraction runs over the lanes' own order of the elements.
 //   O^T (16 elements x heads) += V^T P^T: S leaves a lane four keys of one head, which are its part of P^T as they are; V goes through LDS and comes back transposed.
@@ -271,6 +280,18 @@ namespace {
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& x, const u32x4& y, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+// of codes of K (8 of each lane) and q
+template <typename Tr, typename C>
+__device__ __forceinline__ f32x4 score16(uint32_t w0, uint32_t w1, const u32x4& q, const f32x4& c) {
+  if constexpr (std::is_same_v<Tr, Fp16>) {
+    const u32x2 x0 = C::f16x4(w0), x1 = C::f16x4(w1);
+    const u32x4 k = {x0[0], x0[1], x1[0], x1[1]};
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+  } else {
+    const u32x2 x0 = C::bf16x4(w0), x1 = C::bf16x4(w1);
+    return mfma16(u32x4{x0[0], x0[1], x1[0], x1[1]}, q, c);
+  }
 }
 // Two bf16 whose sum is x to 16 bits
 struct Split {
@@ -285,15 +306,19 @@ __device__ __forceinline__ Split split2(float x, float y) {
 
 }  // namespace
 
-template <typename Tr, typename C, int D>
-__global__ __launch_bounds__(256) void paged8_decode_kernel(const Paged8DecodeK a8) {
-  constexpr int KPB = paged_batch(D) / 4;      // keys of a wave's batch
-  constexpr int NT = KPB / 16;                 // tiles of sixteen keys
+// Keys that a wave has in registers at once.
+template <int D> constexpr int kPaged8Keys = D >= 128 ? 32 : 64;
+
+// VECTORS: four gates of consecutive tokens are read at once.  (Where the kernel chooses at run time nobody knows how many loads are on their way, and every step waits for all.)
+template <typename Tr, typename C, int D, bool VECTORS>
+__global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8DecodeK a8) {
+  constexpr int KEYS = kPaged8Keys<D>, NT = KEYS / 16;   // tiles of sixteen keys
+  constexpr int STEPS = paged_batch(D) / 4 / KEYS;       // of a wave's batch
   constexpr int LB = D >= 64 ? 16 : 8;         // codes a lane loads of a key at once
   constexpr int NL = D >= 64 ? D / 64 : 1;     // such loads
   constexpr int KS = D >= 32 ? D / 32 : 1;     // k-steps of a score
   constexpr int RS = 2 * D + (D >= 64 ? 32 : 16);   // bytes from one key to the next in LDS
-  constexpr bool kSplitQ = std::is_same_v<Tr, Fp16>;
+  typedef std::conditional_t<LB == 16, u32x4, u32x2> Load;
   constexpr int AS = D + 4;                    // floats of a head's accumulator at the merge, where it takes the place of V
   static_assert(16 * AS * 4 <= 32 * RS, "a wave's accumulators fit where its V was");
   __shared__ __align__(16) char v_s[4][32 * RS];
@@ -314,106 +339,95 @@ __global__ __launch_bounds__(256) void paged8_decode_kernel(const Paged8DecodeK 
   const uint8_t *kp = pg.k.ptr + hk * pg.k.sh, *vp = pg.v.ptr + hk * pg.v.sh;
   const float *ks = pg.k.scale + hk * pg.k.s_sh, *vs = pg.v.scale + hk * pg.v.s_sh;
   const float* gp = pg.g + (h0 + min(i16, heads - 1)) * pg.g_sh;   // (columns without a head repeat the last one's)
-  const int in_page = (1 << pg.shift) - 1;
+  const int in_page = (1 << pg.shift) - 1, lane_off = LB == 16 ? 16 * g : D == 32 ? 8 * g : 8 * (g & 1);   // (of a lane's codes in a row)
 
-  // run of this wave in batches, from the last
-  const int keys = at.share.keys, all = (keys + KPB - 1) / KPB;
-  const int b1 = max(all - (at.piece * 4 + wave) * at.share.batches, 0), b0 = max(b1 - at.share.batches, 0);
+  // run of this wave in steps, from the last
+  const int keys = at.share.keys, all = (keys + KEYS * STEPS - 1) / (KEYS * STEPS), per = at.share.batches;
+  const int b1 = max(all - (at.piece * 4 + wave) * per, 0), s0 = max(b1 - per, 0) * STEPS, s1 = min(b1 * STEPS, (keys + KEYS - 1) / KEYS);
 
   // element e of k-step s of a lane is number elem0(s) + e of its row
   auto elem0 = [&](int s) { return D >= 64 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 8 * g; };
-  u32x4 qh[KS], ql[KS];
-  {
-    const uint16_t* qp = a.q + b * a.q_sb + (h0 + min(i16, heads - 1)) * a.q_sh;
+  u32x4 q[KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const bool there = i16 < heads && (D >= 32 || g < 2);
-      u32x4 x = *reinterpret_cast<const u32x4*>(qp + (D >= 32 || g < 2 ? elem0(s) : 0));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (!there) x[e] = 0u;
-        if constexpr (kSplitQ) {
-          const Split p = split2(Tr::lo(x[e]), Tr::hi(x[e]));
-          qh[s][e] = p.hi;
-          ql[s][e] = p.lo;
-        } else {
-          qh[s][e] = x[e];
-        }
-      }
-    }
+  for (int s = 0; s < KS; ++s) {
+    const bool there = D >= 32 || g < 2;
+    q[s] = *reinterpret_cast<const u32x4*>(a.q + b * a.q_sb + (h0 + min(i16, heads - 1)) * a.q_sh + (there ? elem0(s) : 0));
+    if (!there || i16 >= heads) q[s] = u32x4{0u, 0u, 0u, 0u};
   }
   const float qk_scale = a.sm_scale * kLog2e;
   float m = -3.0e38f, l = 0.f;   // of this lane's head; finite floor: what has seen no key yet yields exp2(-inf) = 0
   f32x4 acc[D / 16];
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  double behind = 0.0;           // sum of the run's gates behind the batch, of this lane's head
+  double behind = 0.0;           // sum of the run's gates behind the step, of this lane's head
   int page0 = INT32_MAX, entry = -1;   // this lane has the table's entry for page page0 + lane
   char* const v_tile = v_s[wave];
 
-  for (int batch = b1 - 1; batch >= b0; --batch) {
-    const int n0 = batch * KPB;
+  // What a step needs, each part requested for the next step as soon as this one has used it: the codes and gates of K before the weights are worked out, those of V when they
+  // are in LDS.  A step's loads are in flight during most of the one before, without a second set of registers: four waves a SIMD.
+  Load kx[NT][NL], vx[NT][NL];   // codes of this lane's key of every tile
+  f32x4 gate[NT];                // of the four keys of every tile whose scores this lane will have,
+  float ksc[NT], vsc[NT];        // their scales
+  int page[NT], page4[NT];
+  uint32_t ok = 0, ok_v = 0;     // bit t: this lane's key of tile t may be read (ok_v: of the codes of V); bit 8 + 4 t + r: its r-th score counts
+  auto fetch_k = [&](int step) {
+    const int n0 = step * KEYS;
     if ((n0 >> pg.shift) < page0) {
-      page0 = max(((min(n0 + KPB, keys) - 1) >> pg.shift) - 63, 0);
+      page0 = max(((min(n0 + KEYS, keys) - 1) >> pg.shift) - 63, 0);
       entry = table[min(page0 + lane, a.W - 1)];
       if ((uint32_t)entry >= (uint32_t)pg.P) entry = -1;
+      asm volatile("" : "+v"(entry));   // (waited for here: behind the branch every step would wait for all that is on its way)
     }
     // of keys past the last one: that of the last
     auto page_of = [&](int n) { return __builtin_amdgcn_ds_bpermute(((min(n, keys - 1) >> pg.shift) - page0) << 2, entry); };
-    // codes of this lane's key of every tile
-    u32x4 kx[NT][NL], vx[NT][NL];
-    bool key_ok[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int n = n0 + 16 * t + i16, page = page_of(n), row = min(n, keys - 1) & in_page;
-      key_ok[t] = n < keys && page >= 0;
-      const int64_t from = max(page, 0);
-      const uint8_t *k = kp + from * pg.k.sp + row * pg.k.st, *v = vp + from * pg.v.sp + row * pg.v.st;
-#pragma unroll
-      for (int c = 0; c < NL; ++c) {
-        if constexpr (LB == 16) {
-          kx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k + 64 * c + 16 * g));
-          vx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v + 64 * c + 16 * g));
-        } else {
-          const int o = D == 32 ? 8 * g : 8 * (g & 1);
-          const u32x2 kw = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(k + o)), vw = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(v + o));
-          kx[t][c] = u32x4{kw[0], kw[1], 0u, 0u};
-          vx[t][c] = u32x4{vw[0], vw[1], 0u, 0u};
-        }
-      }
+      page[t] = page_of(n0 + 16 * t + i16);
+      page4[t] = page_of(n0 + 16 * t + 4 * g);
     }
-    // gates and scales of the four keys of every tile whose scores this lane will have
-    f32x4 gx[NT];
-    float sk[NT], sv[NT];
-    bool page_ok[NT];
+    ok = 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int n = n0 + 16 * t + 4 * g, page = page_of(n), row = min(n, (keys - 1) & ~3) & in_page;   // (a multiple of four)
-      page_ok[t] = page >= 0;
-      const int64_t from = max(page, 0);
+      const int n = n0 + 16 * t + i16, row = min(n, keys - 1) & in_page;
+      ok |= (uint32_t)(n < keys && page[t] >= 0) << t;
+      const uint8_t* k = kp + (int64_t)max(page[t], 0) * pg.k.sp + row * pg.k.st + lane_off;
+#pragma unroll
+      for (int c = 0; c < NL; ++c) kx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(k + 64 * c));
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int n = n0 + 16 * t + 4 * g, row = min(n, (keys - 1) & ~3) & in_page;   // (a multiple of four)
+      const int64_t from = max(page4[t], 0);
       const float* p = gp + from * pg.g_sp;
-      if (a8.gates_in_vectors) {
-        gx[t] = *reinterpret_cast<const f32x4*>(p + row);
+      if constexpr (VECTORS) {
+        gate[t] = *reinterpret_cast<const f32x4*>(p + row);
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) gx[t][r] = p[(row + r) * pg.g_ss];
+        for (int r = 0; r < 4; ++r) gate[t][r] = p[(row + r) * pg.g_ss];
       }
-      sk[t] = ks[from * pg.k.s_sp + (row >> pg.block_shift) * pg.k.s_st];
-      sv[t] = vs[from * pg.v.s_sp + (row >> pg.block_shift) * pg.v.s_st];
+      ksc[t] = ks[from * pg.k.s_sp + (row >> pg.block_shift) * pg.k.s_st];
+      if (page4[t] >= 0) ok |= ((1u << min(max(keys - n, 0), 4)) - 1) << (8 + 4 * t);
     }
-    // scores
+  };
+  auto fetch_v = [&](int step, int t) {   // behind fetch_k of the same step
+    const int n = step * KEYS + 16 * t + i16, row = min(n, keys - 1) & in_page;
+    const uint8_t* v = vp + (int64_t)max(page[t], 0) * pg.v.sp + row * pg.v.st + lane_off;
+#pragma unroll
+    for (int c = 0; c < NL; ++c) vx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(v + 64 * c));
+    const int row4 = min(step * KEYS + 16 * t + 4 * g, (keys - 1) & ~3) & in_page;
+    vsc[t] = vs[(int64_t)max(page4[t], 0) * pg.v.s_sp + (row4 >> pg.block_shift) * pg.v.s_st];
+  };
+  auto work = [&](int step, auto more) {   // more: there is a step in front of this one
+    constexpr bool kMore = decltype(more)::value;
     f32x4 s[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int step = 0; step < KS; ++step) {
-        const u32x4& w = kx[t][LB == 16 ? step >> 1 : 0];
-        const int o = LB == 16 ? 2 * (step & 1) : 0;
-        const u32x2 x0 = C::bf16x4(w[o]), x1 = C::bf16x4(w[o + 1]);
-        const u32x4 ka = {x0[0], x0[1], x1[0], x1[1]};
-        s[t] = mfma16(ka, qh[step], s[t]);
-        if constexpr (kSplitQ) s[t] = mfma16(ka, ql[step], s[t]);
+      for (int i = 0; i < KS; ++i) {
+        const Load& w = kx[t][LB == 16 ? i >> 1 : 0];
+        const int o = LB == 16 ? 2 * (i & 1) : 0;
+        s[t] = score16<Tr, C>(w[o], w[o + 1], q[i], s[t]);
       }
     }
     // biases, from the last tile on, and the maximum
@@ -424,19 +438,20 @@ __global__ __launch_bounds__(256) void paged8_decode_kernel(const Paged8DecodeK 
 #pragma unroll
       for (int r = 3; r >= 0; --r) {
         own[r] = sum;
-        sum += page_ok[t] && n0 + 16 * t + 4 * g + r < keys ? gx[t][r] : 0.f;
+        sum += ok >> (8 + 4 * t + r) & 1 ? gate[t][r] : 0.f;
       }
       const float next = __shfl_xor(sum, 16), pair = sum + next, other = __shfl_xor(pair, 32);
-      const float after = (g & 1 ? 0.f : next) + (g & 2 ? 0.f : other);   // of the lanes whose keys lie behind
+      const float after = (float)behind + ((g & 1 ? 0.f : next) + (g & 2 ? 0.f : other));   // with those of the lanes whose keys lie behind
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float bias = (float)(behind + (double)(own[r] + after)) * kLog2e;
-        const float x = fmaf(s[t][r], sk[t] * qk_scale, bias);
-        s[t][r] = page_ok[t] && n0 + 16 * t + 4 * g + r < keys ? x : -INFINITY;
+        const float y = fmaf(s[t][r], ksc[t] * qk_scale, (own[r] + after) * kLog2e);
+        s[t][r] = ok >> (8 + 4 * t + r) & 1 ? y : -INFINITY;
         top = fmaxf(top, s[t][r]);
       }
       behind += (double)(pair + other);
     }
+    ok_v = ok;
+    if constexpr (kMore) fetch_k(step - 1);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const float m_new = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - m_new);
@@ -455,27 +470,32 @@ __global__ __launch_bounds__(256) void paged8_decode_kernel(const Paged8DecodeK 
         for (int r = 0; r < 4; ++r) {
           p[r] = __builtin_amdgcn_exp2f(s[2 * u + t][r] - m);
           l += p[r];
-          p[r] = p[r] > 0.f ? p[r] * sv[2 * u + t] : 0.f;   // (a block that holds no key may have any scale)
+          p[r] = p[r] > 0.f ? p[r] * vsc[2 * u + t] : 0.f;   // (a block that holds no key may have any scale)
         }
-        const Split x = split2(p[0], p[1]), y = split2(p[2], p[3]);
-        ph[2 * t] = x.hi; ph[2 * t + 1] = y.hi;
-        pl[2 * t] = x.lo; pl[2 * t + 1] = y.lo;
+        const Split y0 = split2(p[0], p[1]), y1 = split2(p[2], p[3]);
+        ph[2 * t] = y0.hi; ph[2 * t + 1] = y1.hi;
+        pl[2 * t] = y0.lo; pl[2 * t + 1] = y1.lo;
       }
       __builtin_amdgcn_wave_barrier();   // (the reads of the 32 keys before come first)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         char* row = v_tile + (16 * t + i16) * RS;
+        const bool there = ok_v >> (2 * u + t) & 1;
 #pragma unroll
         for (int c = 0; c < NL; ++c) {
-          u32x4 w = vx[2 * u + t][c];
-          if (!key_ok[2 * u + t]) w = u32x4{0u, 0u, 0u, 0u};   // what is masked may hold anything, NaN among it
+          const Load w = vx[2 * u + t][c];
 #pragma unroll
           for (int half = 0; half < LB / 8; ++half) {
-            const u32x2 x0 = C::bf16x4(w[2 * half]), x1 = C::bf16x4(w[2 * half + 1]);
+            // what is masked may hold anything, NaN among it
+            const u32x2 x0 = C::bf16x4(there ? w[2 * half] : 0u), x1 = C::bf16x4(there ? w[2 * half + 1] : 0u);
             const int d = LB == 16 ? 64 * c + 16 * g + 8 * half : 8 * g;
             if (D >= 32 || g < 2) *reinterpret_cast<u32x4*>(row + 2 * d) = u32x4{x0[0], x0[1], x1[0], x1[1]};
           }
         }
+      }
+      if constexpr (kMore) {
+        fetch_v(step - 1, 2 * u);
+        fetch_v(step - 1, 2 * u + 1);
       }
       staged_rows_visible();
       const char* src = v_tile + (4 * g + (i16 >> 2)) * RS + 8 * (i16 & 3);
@@ -487,6 +507,13 @@ __global__ __launch_bounds__(256) void paged8_decode_kernel(const Paged8DecodeK 
         acc[d] = mfma16(va, pl, acc[d]);
       }
     }
+  };
+  if (s1 > s0) {
+    fetch_k(s1 - 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) fetch_v(s1 - 1, t);
+    for (int step = s1 - 1; step > s0; --step) work(step, std::true_type{});
+    work(s0, std::false_type{});
   }
 
   // merge the waves, each shifted by the gates of the runs behind its own
@@ -551,7 +578,9 @@ static hipError_t decode8_d(const Paged8DecodeK& args, hipStream_t s) {
     const hipError_t e = launch_paged_plan(a.row, D, s);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D>), dim3((unsigned)paged_decode_workgroups(a.row.B, a.row.H, a.row.max_keys, D)), dim3(256), 0, s, a);
+  const dim3 grid((unsigned)paged_decode_workgroups(a.row.B, a.row.H, a.row.max_keys, D));
+  if (a.gates_in_vectors) hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, false>), grid, dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || most_pieces(a.row.max_keys, D) <= 1) return e;
   PagedDecodeK m = a.row;   // the merge goes by query heads
