@@ -1034,6 +1034,12 @@ int fox_paged8_decode(const fox_paged8_decode_args* a, void* stream) {
   r.by_heads = fox::divisor(r.H);
   k.by_parts = fox::divisor(k.parts);
   const fox::Pages8K& p = k.pages;
+  // (the kernel multiplies pages, rows and blocks by 32-bit strides)
+  const int64_t page_strides[5] = {p.k.sp, p.v.sp, p.g_sp, p.k.s_sp, p.v.s_sp}, row_strides[5] = {p.k.st, p.v.st, p.g_ss, p.k.s_st, p.v.s_st};
+  for (int i = 0; i < 5; ++i) {
+    if (page_strides[i] < 0 || page_strides[i] > 0xffffffffLL || row_strides[i] < 0 || row_strides[i] * a->pages.page_size > 0xffffffffLL)
+      return fail(FOX_E_ARG, "pages of the pool, and tokens and blocks of a page, must lie behind each other within 2^32 elements");
+  }
   k.gates_in_vectors = p.g_ss == 1 && !(p.g_sp & 3) && !(p.g_sh & 3) && !((uintptr_t)p.g & 15);
   if (const int64_t rows = paged8_rows(a->B, H, Hk, r.max_keys, D)) {
     r.ws_o = (float*)a->workspace;

@@ -340,6 +340,9 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
   const float *ks = pg.k.scale + hk * pg.k.s_sh, *vs = pg.v.scale + hk * pg.v.s_sh;
   const float* gp = pg.g + (h0 + min(i16, heads - 1)) * pg.g_sh;   // (columns without a head repeat the last one's)
   const int in_page = (1 << pg.shift) - 1, lane_off = LB == 16 ? 16 * g : D == 32 ? 8 * g : 8 * (g & 1);   // (of a lane's codes in a row)
+  // (strides in 32 bits: an address is one multiplication of 32 bits by 32)
+  const uint32_t k_sp = (uint32_t)pg.k.sp, k_st = (uint32_t)pg.k.st, v_sp = (uint32_t)pg.v.sp, v_st = (uint32_t)pg.v.st, g_sp = (uint32_t)pg.g_sp, g_ss = (uint32_t)pg.g_ss;
+  const uint32_t ks_sp = (uint32_t)pg.k.s_sp, ks_st = (uint32_t)pg.k.s_st, vs_sp = (uint32_t)pg.v.s_sp, vs_st = (uint32_t)pg.v.s_st;
 
   // run of this wave in steps, from the last
   const int keys = at.share.keys, all = (keys + KEYS * STEPS - 1) / (KEYS * STEPS), per = at.share.batches;
@@ -369,7 +372,11 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
   f32x4 gate[NT];                // of the four keys of every tile whose scores this lane will have,
   float ksc[NT], vsc[NT];        // their scales
   int page[NT], page4[NT];
-  uint32_t ok = 0, ok_v = 0;     // bit t: this lane's key of tile t may be read (ok_v: of the codes of V); bit 8 + 4 t + r: its r-th score counts
+  bool whole = true;             // every key of the step counts; else
+  uint32_t ok = 0;               // bit t: this lane's key of tile t does, bit 8 + 4 t + r: its r-th score
+  const uint32_t lane_row = i16 & in_page, k_lane = lane_row * k_st + lane_off, v_lane = lane_row * v_st + lane_off, g_lane = (4 * g & in_page) * g_ss;
+  // A tile begins at a multiple of sixteen tokens: a lane's row in its page is the tile's and its own, both fixed, and the blocks of its keys are the tile's.  Rows past the
+  // last key lie on the last key's page.
   auto fetch_k = [&](int step) {
     const int n0 = step * KEYS;
     if ((n0 >> pg.shift) < page0) {
@@ -378,44 +385,53 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
       if ((uint32_t)entry >= (uint32_t)pg.P) entry = -1;
       asm volatile("" : "+v"(entry));   // (waited for here: behind the branch every step would wait for all that is on its way)
     }
-    // of keys past the last one: that of the last
     auto page_of = [&](int n) { return __builtin_amdgcn_ds_bpermute(((min(n, keys - 1) >> pg.shift) - page0) << 2, entry); };
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       page[t] = page_of(n0 + 16 * t + i16);
       page4[t] = page_of(n0 + 16 * t + 4 * g);
     }
-    ok = 0;
+    bool all = n0 + KEYS <= keys;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) all &= page[t] >= 0;
+    whole = __all(all);
+    ok = ~0u;
+    if (!whole) {
+      ok = 0;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        ok |= (uint32_t)(n0 + 16 * t + i16 < keys && page[t] >= 0) << t;
+        if (page4[t] >= 0) ok |= ((1u << min(max(keys - (n0 + 16 * t + 4 * g), 0), 4)) - 1) << (8 + 4 * t);
+        page[t] = max(page[t], 0);
+        page4[t] = max(page4[t], 0);
+      }
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int n = n0 + 16 * t + i16, row = min(n, keys - 1) & in_page;
-      ok |= (uint32_t)(n < keys && page[t] >= 0) << t;
-      const uint8_t* k = kp + (int64_t)max(page[t], 0) * pg.k.sp + row * pg.k.st + lane_off;
+      const uint32_t row = (n0 + 16 * t) & in_page;
+      const uint8_t* k = kp + (uint64_t)(uint32_t)page[t] * k_sp + (row * k_st + k_lane);
 #pragma unroll
       for (int c = 0; c < NL; ++c) kx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(k + 64 * c));
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int n = n0 + 16 * t + 4 * g, row = min(n, (keys - 1) & ~3) & in_page;   // (a multiple of four)
-      const int64_t from = max(page4[t], 0);
-      const float* p = gp + from * pg.g_sp;
+      const uint32_t row = (n0 + 16 * t) & in_page;
+      const float* p = gp + ((uint64_t)(uint32_t)page4[t] * g_sp + (row * g_ss + g_lane));
       if constexpr (VECTORS) {
-        gate[t] = *reinterpret_cast<const f32x4*>(p + row);
+        gate[t] = *reinterpret_cast<const f32x4*>(p);
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) gate[t][r] = p[(row + r) * pg.g_ss];
+        for (int r = 0; r < 4; ++r) gate[t][r] = p[r * g_ss];
       }
-      ksc[t] = ks[from * pg.k.s_sp + (row >> pg.block_shift) * pg.k.s_st];
-      if (page4[t] >= 0) ok |= ((1u << min(max(keys - n, 0), 4)) - 1) << (8 + 4 * t);
+      ksc[t] = ks[(uint64_t)(uint32_t)page4[t] * ks_sp + (row >> pg.block_shift) * ks_st];
     }
   };
   auto fetch_v = [&](int step, int t) {   // behind fetch_k of the same step
-    const int n = step * KEYS + 16 * t + i16, row = min(n, keys - 1) & in_page;
-    const uint8_t* v = vp + (int64_t)max(page[t], 0) * pg.v.sp + row * pg.v.st + lane_off;
+    const uint32_t row = (step * KEYS + 16 * t) & in_page;
+    const uint8_t* v = vp + (uint64_t)(uint32_t)page[t] * v_sp + (row * v_st + v_lane);
 #pragma unroll
     for (int c = 0; c < NL; ++c) vx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(v + 64 * c));
-    const int row4 = min(step * KEYS + 16 * t + 4 * g, (keys - 1) & ~3) & in_page;
-    vsc[t] = vs[(int64_t)max(page4[t], 0) * pg.v.s_sp + (row4 >> pg.block_shift) * pg.v.s_st];
+    vsc[t] = vs[(uint64_t)(uint32_t)page4[t] * vs_sp + (row >> pg.block_shift) * vs_st];
   };
   auto work = [&](int step, auto more) {   // more: there is a step in front of this one
     constexpr bool kMore = decltype(more)::value;
@@ -430,6 +446,15 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
         s[t] = score16<Tr, C>(w[o], w[o + 1], q[i], s[t]);
       }
     }
+    // What is masked may hold anything, NaN among it; in most steps nothing is.
+    const bool whole_now = whole;
+    const uint32_t ok_now = ok;
+    if (!whole_now) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) gate[t][r] = ok >> (8 + 4 * t + r) & 1 ? gate[t][r] : 0.f;
+    }
     // biases, from the last tile on, and the maximum
     float top = -INFINITY;
 #pragma unroll
@@ -438,30 +463,49 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
 #pragma unroll
       for (int r = 3; r >= 0; --r) {
         own[r] = sum;
-        sum += ok >> (8 + 4 * t + r) & 1 ? gate[t][r] : 0.f;
+        sum += gate[t][r];
       }
       const float next = __shfl_xor(sum, 16), pair = sum + next, other = __shfl_xor(pair, 32);
       const float after = (float)behind + ((g & 1 ? 0.f : next) + (g & 2 ? 0.f : other));   // with those of the lanes whose keys lie behind
+      const float scale = ksc[t] * qk_scale;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float y = fmaf(s[t][r], ksc[t] * qk_scale, (own[r] + after) * kLog2e);
-        s[t][r] = ok >> (8 + 4 * t + r) & 1 ? y : -INFINITY;
-        top = fmaxf(top, s[t][r]);
-      }
+      for (int r = 0; r < 4; ++r) s[t][r] = fmaf(s[t][r], scale, (own[r] + after) * kLog2e);
       behind += (double)(pair + other);
     }
-    ok_v = ok;
+    if (!whole_now) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[t][r] = ok_now >> (8 + 4 * t + r) & 1 ? s[t][r] : -INFINITY;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) top = fmaxf(top, s[t][r]);
     if constexpr (kMore) fetch_k(step - 1);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float m_new = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - m_new);
-    m = m_new;
-    l *= alpha;
+    // The maximum is raised when a step exceeds it by more than 2^8, which is rare behind the first ones.
+    const bool raise = top > m + 8.f;
+    if (__any(raise)) {
+      const float m_new = raise ? top : m, alpha = __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= alpha;
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) acc[d] *= alpha;
+      for (int d = 0; d < D / 16; ++d) acc[d] *= alpha;
+    }
     // O^T += V^T P^T, 32 keys at a time
 #pragma unroll
     for (int u = 0; u < NT / 2; ++u) {
+      if (!whole_now) {
+#pragma unroll
+        for (int t = 2 * u; t < 2 * u + 2; ++t) {
+          if ((ok_now >> (8 + 4 * t) & 15) == 0) vsc[t] = 0.f;   // (a block that holds no key may have any scale)
+#pragma unroll
+          for (int c = 0; c < NL; ++c)
+            if (!(ok_now >> t & 1)) vx[t][c] = Load{};
+        }
+      }
       u32x4 ph, pl;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -470,7 +514,7 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
         for (int r = 0; r < 4; ++r) {
           p[r] = __builtin_amdgcn_exp2f(s[2 * u + t][r] - m);
           l += p[r];
-          p[r] = p[r] > 0.f ? p[r] * vsc[2 * u + t] : 0.f;   // (a block that holds no key may have any scale)
+          p[r] *= vsc[2 * u + t];
         }
         const Split y0 = split2(p[0], p[1]), y1 = split2(p[2], p[3]);
         ph[2 * t] = y0.hi; ph[2 * t + 1] = y1.hi;
@@ -480,14 +524,12 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         char* row = v_tile + (16 * t + i16) * RS;
-        const bool there = ok_v >> (2 * u + t) & 1;
 #pragma unroll
         for (int c = 0; c < NL; ++c) {
           const Load w = vx[2 * u + t][c];
 #pragma unroll
           for (int half = 0; half < LB / 8; ++half) {
-            // what is masked may hold anything, NaN among it
-            const u32x2 x0 = C::bf16x4(there ? w[2 * half] : 0u), x1 = C::bf16x4(there ? w[2 * half + 1] : 0u);
+            const u32x2 x0 = C::bf16x4(w[2 * half]), x1 = C::bf16x4(w[2 * half + 1]);
             const int d = LB == 16 ? 64 * c + 16 * g + 8 * half : 8 * g;
             if (D >= 32 || g < 2) *reinterpret_cast<u32x4*>(row + 2 * d) = u32x4{x0[0], x0[1], x1[0], x1[1]};
           }
