@@ -270,7 +270,8 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const PagedGatherK a,
 // instructions (a group of one wastes fifteen, which costs nothing here: a CU's matrix units could take twelve times what memory brings).  Codes become 16-bit numbers on their
 // way, exactly: those of K in the type of q, those of V in bf16, whose range has room for p times any scale, with p in two bf16 parts.  The products are as good as 32 bits.
 //
-//   S (16 keys x heads) = K Q^T: a lane holds 16 consecutive codes of a key, the contraction runs over the lanes' own order of the elements.
+//   S (16 keys x heads) = K Q^T: a lane holds 16 consecutive codes of a key, the contraction runs over the lanes' own order of the elements.  Rows of 128 codes are loaded as whole
+//     lines and come to their lanes through LDS: in the operand's own order a load touches half of every line, and memory gives 5.0 TB/s in place of 6.4.
 //   O^T (16 elements x heads) += V^T P^T: S leaves a lane four keys of one head, which are its part of P^T as they are; V goes through LDS and comes back transposed.
 //
 // A wave walks whole batches of keys from the last one on, its sum of the gates behind it in 64 bits; runs, pieces, plan and merge are those of the 16-bit pages
@@ -314,14 +315,17 @@ template <typename Tr, typename C, int D, bool VECTORS>
 __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8DecodeK a8) {
   constexpr int KEYS = kPaged8Keys<D>, NT = KEYS / 16;   // tiles of sixteen keys
   constexpr int STEPS = paged_batch(D) / 4 / KEYS;       // of a wave's batch
-  constexpr int LB = D >= 64 ? 16 : 8;         // codes a lane loads of a key at once
-  constexpr int NL = D >= 64 ? D / 64 : 1;     // such loads
+  constexpr int LB = D >= 64 ? 16 : 8;         // codes a lane loads at once
+  constexpr int NL = D >= 64 ? D / 64 : 1;     // loads of a tile
+  constexpr bool LINES = D == 128;             // a load takes eight whole rows of 128 bytes, else all sixteen rows
   constexpr int KS = D >= 32 ? D / 32 : 1;     // k-steps of a score
   constexpr int RS = 2 * D + (D >= 64 ? 32 : 16);   // bytes from one key to the next in LDS
   typedef std::conditional_t<LB == 16, u32x4, u32x2> Load;
   constexpr int AS = D + 4;                    // floats of a head's accumulator at the merge, where it takes the place of V
   static_assert(16 * AS * 4 <= 32 * RS, "a wave's accumulators fit where its V was");
+  constexpr int KRS = D + 16;                  // bytes from one key to the next where K goes through LDS
   __shared__ __align__(16) char v_s[4][32 * RS];
+  static_assert(!LINES || KEYS * KRS <= 32 * RS, "K passes through the place of V, before V");
   __shared__ float part_m[4][16], part_l[4][16];
   __shared__ double part_g[4][16];
 
@@ -339,7 +343,7 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
   const uint8_t *kp = pg.k.ptr + hk * pg.k.sh, *vp = pg.v.ptr + hk * pg.v.sh;
   const float *ks = pg.k.scale + hk * pg.k.s_sh, *vs = pg.v.scale + hk * pg.v.s_sh;
   const float* gp = pg.g + (h0 + min(i16, heads - 1)) * pg.g_sh;   // (columns without a head repeat the last one's)
-  const int in_page = (1 << pg.shift) - 1, lane_off = LB == 16 ? 16 * g : D == 32 ? 8 * g : 8 * (g & 1);   // (of a lane's codes in a row)
+  const int in_page = (1 << pg.shift) - 1;
   // (strides in 32 bits: an address is one multiplication of 32 bits by 32)
   const uint32_t k_sp = (uint32_t)pg.k.sp, k_st = (uint32_t)pg.k.st, v_sp = (uint32_t)pg.v.sp, v_st = (uint32_t)pg.v.st, g_sp = (uint32_t)pg.g_sp, g_ss = (uint32_t)pg.g_ss;
   const uint32_t ks_sp = (uint32_t)pg.k.s_sp, ks_st = (uint32_t)pg.k.s_st, vs_sp = (uint32_t)pg.v.s_sp, vs_st = (uint32_t)pg.v.s_st;
@@ -367,16 +371,24 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
   char* const v_tile = v_s[wave];
 
   // What a step needs, each part requested for the next step as soon as this one has used it: the codes and gates of K before the weights are worked out, those of V when they
-  // are in LDS.  A step's loads are in flight during most of the one before, without a second set of registers: four waves a SIMD.
-  Load kx[NT][NL], vx[NT][NL];   // codes of this lane's key of every tile
+  // are in LDS.  A step's loads are in flight during most of the one before, without a second set of registers.
+  Load kx[NT][NL], vx[NT][NL];   // codes of this lane's keys of every tile
   f32x4 gate[NT];                // of the four keys of every tile whose scores this lane will have,
   float ksc[NT], vsc[NT];        // their scales
-  int page[NT], page4[NT];
+  int page[2 * NT];              // of every eight keys
   bool whole = true;             // every key of the step counts; else
-  uint32_t ok = 0;               // bit t: this lane's key of tile t does, bit 8 + 4 t + r: its r-th score
-  const uint32_t lane_row = i16 & in_page, k_lane = lane_row * k_st + lane_off, v_lane = lane_row * v_st + lane_off, g_lane = (4 * g & in_page) * g_ss;
+  uint32_t ok = 0;               // bit NL t + c: this lane's key of load c of tile t does, bit 8 + 4 t + r: its r-th score
   // A tile begins at a multiple of sixteen tokens: a lane's row in its page is the tile's and its own, both fixed, and the blocks of its keys are the tile's.  Rows past the
   // last key lie on the last key's page.
+  const uint32_t lane_row = LINES ? lane >> 3 : i16 & in_page, lane_off = LINES ? 16 * (lane & 7) : LB == 16 ? 16 * g : D == 32 ? 8 * g : 8 * (g & 1);
+  const uint32_t k_lane = lane_row * k_st + lane_off, v_lane = lane_row * v_st + lane_off, g_lane = (4 * g & in_page) * g_ss;
+  // address of load c of tile t, in codes from the beginning of the head's
+  auto code_at = [&](int n0, int t, int c, uint32_t sp, uint32_t st, uint32_t own) {
+    const int first = n0 + 16 * t + (LINES ? 8 * c : 0);
+    const uint32_t p = LINES ? page[2 * t + c] : i16 < 8 ? page[2 * t] : page[2 * t + 1];
+    return (uint64_t)p * sp + ((first & in_page) * st + own + (LINES ? 0 : 64 * c));
+  };
+  auto page_of_scores = [&](int t) { return (uint32_t)(g < 2 ? page[2 * t] : page[2 * t + 1]); };
   auto fetch_k = [&](int step) {
     const int n0 = step * KEYS;
     if ((n0 >> pg.shift) < page0) {
@@ -385,57 +397,64 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
       if ((uint32_t)entry >= (uint32_t)pg.P) entry = -1;
       asm volatile("" : "+v"(entry));   // (waited for here: behind the branch every step would wait for all that is on its way)
     }
-    auto page_of = [&](int n) { return __builtin_amdgcn_ds_bpermute(((min(n, keys - 1) >> pg.shift) - page0) << 2, entry); };
+    whole = n0 + KEYS <= keys;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      page[t] = page_of(n0 + 16 * t + i16);
-      page4[t] = page_of(n0 + 16 * t + 4 * g);
+    for (int e = 0; e < 2 * NT; ++e) {
+      page[e] = __builtin_amdgcn_readlane(entry, (min(n0 + 8 * e, keys - 1) >> pg.shift) - page0);
+      whole &= page[e] >= 0;
     }
-    bool all = n0 + KEYS <= keys;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) all &= page[t] >= 0;
-    whole = __all(all);
-    ok = ~0u;
     if (!whole) {
       ok = 0;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        ok |= (uint32_t)(n0 + 16 * t + i16 < keys && page[t] >= 0) << t;
-        if (page4[t] >= 0) ok |= ((1u << min(max(keys - (n0 + 16 * t + 4 * g), 0), 4)) - 1) << (8 + 4 * t);
-        page[t] = max(page[t], 0);
-        page4[t] = max(page4[t], 0);
+#pragma unroll
+        for (int c = 0; c < NL; ++c) {
+          const int n = n0 + 16 * t + (LINES ? 8 * c + (lane >> 3) : i16), p = LINES ? page[2 * t + c] : i16 < 8 ? page[2 * t] : page[2 * t + 1];
+          ok |= (uint32_t)(n < keys && p >= 0) << (NL * t + c);
+        }
+        if ((int)page_of_scores(t) >= 0) ok |= ((1u << min(max(keys - (n0 + 16 * t + 4 * g), 0), 4)) - 1) << (8 + 4 * t);
       }
+#pragma unroll
+      for (int e = 0; e < 2 * NT; ++e) page[e] = max(page[e], 0);
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const uint32_t row = (n0 + 16 * t) & in_page;
-      const uint8_t* k = kp + (uint64_t)(uint32_t)page[t] * k_sp + (row * k_st + k_lane);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int c = 0; c < NL; ++c) kx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(k + 64 * c));
-    }
+      for (int c = 0; c < NL; ++c) kx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(kp + code_at(n0, t, c, k_sp, k_st, k_lane)));
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const uint32_t row = (n0 + 16 * t) & in_page;
-      const float* p = gp + ((uint64_t)(uint32_t)page4[t] * g_sp + (row * g_ss + g_lane));
+      const uint32_t row = (n0 + 16 * t) & in_page, p = page_of_scores(t);
+      const float* at = gp + ((uint64_t)p * g_sp + (row * g_ss + g_lane));
       if constexpr (VECTORS) {
-        gate[t] = *reinterpret_cast<const f32x4*>(p);
+        gate[t] = *reinterpret_cast<const f32x4*>(at);
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) gate[t][r] = p[r * g_ss];
+        for (int r = 0; r < 4; ++r) gate[t][r] = at[r * g_ss];
       }
-      ksc[t] = ks[(uint64_t)(uint32_t)page4[t] * ks_sp + (row >> pg.block_shift) * ks_st];
+      ksc[t] = ks[(uint64_t)p * ks_sp + (row >> pg.block_shift) * ks_st];
     }
   };
   auto fetch_v = [&](int step, int t) {   // behind fetch_k of the same step
-    const uint32_t row = (step * KEYS + 16 * t) & in_page;
-    const uint8_t* v = vp + (uint64_t)(uint32_t)page[t] * v_sp + (row * v_st + v_lane);
+    const int n0 = step * KEYS;
 #pragma unroll
-    for (int c = 0; c < NL; ++c) vx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(v + 64 * c));
-    vsc[t] = vs[(uint64_t)(uint32_t)page4[t] * vs_sp + (row >> pg.block_shift) * vs_st];
+    for (int c = 0; c < NL; ++c) vx[t][c] = __builtin_nontemporal_load(reinterpret_cast<const Load*>(vp + code_at(n0, t, c, v_sp, v_st, v_lane)));
+    vsc[t] = vs[(uint64_t)page_of_scores(t) * vs_sp + (((n0 + 16 * t) & in_page) >> pg.block_shift) * vs_st];
   };
   auto work = [&](int step, auto more) {   // more: there is a step in front of this one
     constexpr bool kMore = decltype(more)::value;
     f32x4 s[NT];
+    if constexpr (LINES) {   // whole rows: a lane's part of the operand lies with other lanes
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < NL; ++c) *reinterpret_cast<Load*>(v_tile + (16 * t + 8 * c + (lane >> 3)) * KRS + 16 * (lane & 7)) = kx[t][c];
+      staged_rows_visible();
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < NL; ++c) kx[t][c] = *reinterpret_cast<const Load*>(v_tile + (16 * t + i16) * KRS + 64 * c + 16 * g);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -503,7 +522,7 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
           if ((ok_now >> (8 + 4 * t) & 15) == 0) vsc[t] = 0.f;   // (a block that holds no key may have any scale)
 #pragma unroll
           for (int c = 0; c < NL; ++c)
-            if (!(ok_now >> t & 1)) vx[t][c] = Load{};
+            if (!(ok_now >> (NL * t + c) & 1)) vx[t][c] = Load{};
         }
       }
       u32x4 ph, pl;
@@ -523,14 +542,14 @@ __global__ __launch_bounds__(256, 3) void paged8_decode_kernel(const Paged8Decod
       __builtin_amdgcn_wave_barrier();   // (the reads of the 32 keys before come first)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        char* row = v_tile + (16 * t + i16) * RS;
 #pragma unroll
         for (int c = 0; c < NL; ++c) {
           const Load w = vx[2 * u + t][c];
+          char* row = v_tile + (LINES ? 16 * t + 8 * c + (lane >> 3) : 16 * t + i16) * RS;
 #pragma unroll
           for (int half = 0; half < LB / 8; ++half) {
             const u32x2 x0 = C::bf16x4(w[2 * half]), x1 = C::bf16x4(w[2 * half + 1]);
-            const int d = LB == 16 ? 64 * c + 16 * g + 8 * half : 8 * g;
+            const int d = LINES ? 16 * (lane & 7) + 8 * half : LB == 16 ? 64 * c + 16 * g + 8 * half : 8 * g;
             if (D >= 32 || g < 2) *reinterpret_cast<u32x4*>(row + 2 * d) = u32x4{x0[0], x0[1], x1[0], x1[1]};
           }
         }
