@@ -460,3 +460,75 @@ def test_what_the_kernels_do_not_take_is_copied():
     table, n = on_gpu([[0, 1, 2], [3, 4, 5]]), on_gpu([40, 17])
     a = paged_forgetting_attention_8bit(q, *pages, table.t().contiguous().t(), torch.stack([n, n], 1)[:, 0])
     assert torch.equal(a, paged_forgetting_attention_8bit(q.contiguous(), *pages, table, n))
+
+
+@pytest.mark.parametrize("codes,dtype,H,Hk", [("e4m3", torch.bfloat16, 6, 2), ("int8", torch.float16, 4, 4), (None, torch.bfloat16, 3, 3)])
+def test_cache_of_a_model(codes, dtype, H, Hk):
+    """PagedFgateCache over two layers: prompts in pieces, refused and idle requests, tokens, a release; against attention over everything that each request has brought."""
+    from forgetting_transformer import PagedFgateCache
+    D, B, S, layers = 64, 4, 16, 2
+    cache_ = PagedFgateCache(layers, H, D, num_pages=24, max_requests=B, max_length=200, page_size=S, dtype=dtype, cache_dtype=CODES[codes][0] if codes else None, num_kv_heads=Hk)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    u = torch.finfo(dtype).eps / 2
+
+    def held(layer):
+        ks, vs = (x[layer] if x is not None else torch.ones(24, Hk, 1, device="cuda") for x in (cache_.key_scales, cache_.value_scales))
+        return cache_.key_pages[layer], cache_.value_pages[layer], ks, vs, cache_.log_fgate_pages[layer]
+
+    def step(new, room, prompts, max_keys=None):
+        s = cache_.schedule(on_gpu(new), room, prompts=prompts)
+        for layer in range(layers):
+            q, k, v = (torch.randn(room, h, D, generator=g, device="cuda").to(dtype) for h in (H, Hk, Hk))
+            cache_.update(k, v, torch.nn.functional.logsigmoid(torch.randn(room, H, generator=g, device="cuda") + 2.0), layer)
+            out = cache_.attend_prompts(q, layer, max_keys=max_keys) if prompts else cache_.attend(q, layer)
+            kp, vp, ks, vs, fp = held(layer)
+            if codes is None:      # the reference takes a block of sixteen tokens
+                ks, vs = (x.expand(24, Hk, S // 16).contiguous() for x in (ks, vs))
+            want, top = attention_reference(q, kp, vp, ks, vs, fp, cache_.block_table.tolist(), s.keys.tolist(), s.requests.tolist(), D ** -0.5)
+            assert ((out.double() - want).abs() <= u * want.abs() + ((u if prompts else 0.0) + 2.0 ** -12) * top).all()
+            assert not out[s.requests < 0].any()
+        return s
+
+    step([50, 0, 90, 17], 200, True)
+    s = step([30, 5, 0, 300], 400, True)          # the last one has no room
+    assert s.granted.tolist()[3] is False
+    step([1, 1, 1, 1], B, False)
+    step([1, 0, 1, 0], B, True, max_keys=400)
+    cache_.release(on_gpu([True, False, False, False], torch.bool))
+    step([40, 3, 3, 3], 60, True)
+    step([1, 1, 1, 1], B, False)
+
+
+def test_a_captured_step_of_prompts():
+    """The cache's step of prompts in a graph, replayed for pieces of other lengths with eager work between."""
+    from forgetting_transformer import PagedFgateCache
+    H, D, B, room = 4, 32, 3, 64
+    make = lambda: PagedFgateCache(1, H, D, num_pages=30, max_requests=B, max_length=160, page_size=16, cache_dtype=torch.float8_e4m3fn)
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    xs = [[torch.randn(room, H, D, generator=gen, device="cuda").bfloat16() for _ in range(3)] + [-torch.rand(room, H, generator=gen, device="cuda"), on_gpu(n)]
+          for n in ([20, 1, 0], [5, 30, 29], [0, 0, 3], [40, 2, 2], [1, 1, 1])]
+
+    def step(cache_, x):
+        cache_.schedule(x[4], room, prompts=True)
+        cache_.update(x[1], x[2], x[3], 0)
+        return cache_.attend_prompts(x[0], 0)
+
+    eager = make()
+    want = [step(eager, x) for x in xs]
+    cache_, buf = make(), [t.clone() for t in xs[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(make(), buf)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cache_, buf)
+    for i, x in enumerate(xs):
+        for b, t in zip(buf, x):
+            b.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]), i
+        step(eager, [*x[:4], torch.zeros_like(x[4])])
+        torch.cuda.synchronize()
