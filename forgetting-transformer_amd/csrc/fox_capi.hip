@@ -363,21 +363,28 @@ int check_packed_sizes(int B, int T, int N) {
   if (T > 1 << 30 || N > 1 << 30) return fail(FOX_E_ARG, "at most 2^30 queries and keys (got %d, %d)", T, N);
   return FOX_OK;
 }
+int check_packed_heads(int H, int Hk) {
+  if (H <= 0 || Hk <= 0 || H % Hk) return fail(FOX_E_ARG, "the query heads must be a positive multiple of the key heads (got %d, %d)", H, Hk);
+  if (H > 65535) return fail(FOX_E_ARG, "at most 65535 heads (got %d)", H);
+  return FOX_OK;
+}
 int make_packed(const fox_packed_args* a, fox::PackedK& k, bool bwd) {
   if (!a) return fail(FOX_E_ARG, "args is NULL");
   FOX_TRY(check_packed_sizes(a->B, a->T, a->N));
   FOX_TRY(check_head_dim(a->D));
   FOX_TRY(check_dtype16(a->dtype));
-  if (a->H <= 0 || a->Hk <= 0 || a->H % a->Hk) return fail(FOX_E_ARG, "the query heads must be a positive multiple of the key heads (got %d, %d)", a->H, a->Hk);
-  if (a->H > 65535) return fail(FOX_E_ARG, "at most 65535 heads (got %d)", a->H);
+  FOX_TRY(check_packed_heads(a->H, a->Hk));
   FOX_TRY(check_tokens(&a->q, "q"));
   FOX_TRY(check_tokens(&a->k, "k"));
   FOX_TRY(check_tokens(&a->v, "v"));
   FOX_TRY(check_tokens(&a->o, "o"));
   if (!a->c || !a->plan) return fail(FOX_E_ARG, "c and plan must not be NULL");
   if (!bwd && (!a->g || !a->cu_q || !a->cu_k)) return fail(FOX_E_ARG, "g, cu_q and cu_k must not be NULL");
-  if (a->plan_bytes < fox::packed_plan_bytes(a->B, a->T, a->N)) return fail(FOX_E_ARG, "plan too small: %lld bytes", (long long)a->plan_bytes);
-  if ((uintptr_t)a->plan & 15) return fail(FOX_E_ALIGN, "plan must be 16-byte aligned");
+  const fox::PackedShape shape = fox::packed_shape(a->B, a->T, a->N, a->H, a->Hk, a->D);
+  const int64_t workspace = bwd ? shape.bwd_bytes : shape.fwd_bytes;
+  if (a->plan_bytes < shape.plan_bytes) return fail(FOX_E_ARG, "plan too small: %lld bytes", (long long)a->plan_bytes);
+  if (workspace > 0 && (!a->workspace || a->workspace_bytes < workspace)) return fail(FOX_E_ARG, "workspace too small: %lld bytes", (long long)a->workspace_bytes);
+  if (((uintptr_t)a->plan | (uintptr_t)a->workspace) & 15) return fail(FOX_E_ALIGN, "plan and workspace must be 16-byte aligned");
   k = fox::PackedK{};
   k.q = to_view(a->q); k.k = to_view(a->k); k.v = to_view(a->v); k.o = to_view(a->o);
   k.g = a->g; k.g_st = a->g_stride_t; k.g_sh = a->g_stride_h;
@@ -385,8 +392,8 @@ int make_packed(const fox_packed_args* a, fox::PackedK& k, bool bwd) {
   k.c = a->c; k.lse = a->lse;
   k.B = a->B; k.T = a->T; k.N = a->N; k.H = a->H; k.Hk = a->Hk; k.group = a->H / a->Hk;
   k.sm_scale = a->sm_scale;
-  k.plan = fox::packed_plan(a->plan, a->B, a->T, a->N, &k.q_bound, &k.k_bound);
-  const int64_t rows = ((int64_t)a->B + fox::kPackedOuter) * a->H, q_tiles = (int64_t)k.q_bound * a->H, k_tiles = (int64_t)k.k_bound * a->Hk;
+  fox::packed_memory(k, shape, a->plan, a->workspace);
+  const int64_t rows = ((int64_t)a->B + fox::kPackedOuter) * a->H, q_tiles = ((int64_t)k.q_bound + k.q_extra) * a->H, k_tiles = ((int64_t)k.k_bound + k.k_extra) * a->Hk;
   // (threads of a launch: 1024 a row, 256 a tile)
   if (rows >= 1 << 22 || q_tiles >= 1 << 24 || k_tiles >= 1 << 24) return fail(FOX_E_ARG, "too many sequences, tiles and heads for one call");
   if (!bwd) return FOX_OK;
@@ -1049,10 +1056,15 @@ int fox_paged8_decode(const fox_paged8_decode_args* a, void* stream) {
   return check_hip(fox::launch_paged8_decode(k, D, a->dtype, a->pages.codes, (hipStream_t)stream), "fox_paged8_decode");
 }
 
-int fox_packed_plan_bytes(int32_t B, int32_t T, int32_t N, int64_t* bytes) {
+int fox_packed_bytes(int32_t B, int32_t T, int32_t N, int32_t H, int32_t Hk, int32_t D, int64_t* plan, int64_t* fwd_workspace, int64_t* bwd_workspace) {
   FOX_TRY(check_packed_sizes(B, T, N));
-  if (!bytes) return fail(FOX_E_ARG, "bytes is NULL");
-  *bytes = fox::packed_plan_bytes(B, T, N);
+  FOX_TRY(check_head_dim(D));
+  FOX_TRY(check_packed_heads(H, Hk));
+  if (!plan || !fwd_workspace || !bwd_workspace) return fail(FOX_E_ARG, "plan, fwd_workspace and bwd_workspace must not be NULL");
+  const fox::PackedShape s = fox::packed_shape(B, T, N, H, Hk, D);
+  *plan = s.plan_bytes;
+  *fwd_workspace = s.fwd_bytes;
+  *bwd_workspace = s.bwd_bytes;
   return FOX_OK;
 }
 

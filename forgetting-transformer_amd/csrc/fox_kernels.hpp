@@ -303,10 +303,12 @@ constexpr int kPaged8Heads = 16;         // query heads of a workgroup: the colu
 
 // Attention over packed sequences (fox_packed.hip).  Sequence b has the queries [q0, q0 + m) and the keys [k0, k0 + n); a tile is 128 rows of either.
 struct PackedItem {
-  int32_t q0, m, k0, n, tile, seq, pad[2];
+  int32_t q0, m, k0, n, tile;
+  int32_t part, parts, slot;             // of a tile whose walk is cut; its first place among those of all parts
 };
 struct PackedPlan {                      // in the plan's memory, behind the counts
   PackedItem *q_items, *k_items;         // tiles of queries and of keys, those of the longest sequences first
+  int32_t* seq_parts;                    // parts of the tiles of a sequence (where there are too many sequences for LDS)
   int4* seqs;                            // {q0, m, k0, n} of the B sequences and of kPackedOuter that hold what belongs to none
   int32_t* counts;                       // of q_items and k_items
 };
@@ -325,6 +327,9 @@ struct PackedK {
   PackedPlan plan;
   int B, T, N, H, Hk, group;             // group = H / Hk query heads on a key head
   int q_bound, k_bound;                  // tiles, at most
+  int q_extra, k_extra;                  // parts of those that are cut, at most; 0: none is
+  float *q_parts, *k_parts;              // what the parts leave
+  uint32_t *q_arrived, *k_arrived;       // parts that have
   float sm_scale;
   Divisor by_heads, by_xcd_heads;        // of a launch: by the heads, and by those of an XCD
 };
@@ -471,8 +476,13 @@ hipError_t launch_paged8_append(const Paged8AppendK& a, int D, int dtype, int co
 hipError_t launch_paged_gather(const PagedGatherK& a, int D, int dtype, int codes, hipStream_t s);
 hipError_t launch_paged8_decode(const Paged8DecodeK& a, int D, int dtype, int codes, hipStream_t s);
 int64_t rotary_workspace_floats(int64_t tokens, int heads, int D, bool shared);
-int64_t packed_plan_bytes(int B, int T, int N);
-PackedPlan packed_plan(void* memory, int B, int T, int N, int* q_bound, int* k_bound);
+struct PackedShape {
+  int q_bound, k_bound, q_extra, k_extra;
+  int64_t seqs_at, seq_parts_at, items_at, plan_bytes;                                              // in the plan
+  int64_t q_arrived_at, k_parts_at, k_arrived_at, fwd_bytes, bwd_bytes;      // in a workspace
+};
+PackedShape packed_shape(int B, int T, int N, int H, int Hk, int D);
+void packed_memory(PackedK& a, const PackedShape& s, void* plan, void* workspace);
 hipError_t launch_packed_fwd(const PackedK& a, int D, int dtype, hipStream_t s);
 hipError_t launch_packed_bwd(const PackedK& a, int D, int dtype, hipStream_t s);
 hipError_t launch_shift_fwd(const ShiftK& a, int D, int dtype, hipStream_t s);

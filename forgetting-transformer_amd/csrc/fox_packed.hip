@@ -6,9 +6,12 @@
 //   dP = dO V^T,  delta_i = sum_j P_ij dP_ij,  dS = P (dP - delta),  dq = sm_scale dS K,  dk = sm_scale dS^T Q,  dv = P^T dO,
 //   dc_j = -sum_i dS_ij  (a row of dS adds up to zero),  dg_l = sum_{j >= l} dc_j.
 //
-// Who knows how long the sequences are is the device.  One workgroup makes the plan, the list of all tiles of queries and of keys, while the others form the
+// Who knows how long the sequences are is the device.  Two workgroups make the plan, the lists of all tiles of queries and of keys, while the others form the
 // sums of the gates; the attention kernels are launched for as many tiles as there can be (a partial one for every sequence) and those past the
 // list end at once.  A sequence's tiles follow each other, heaviest first, the longest sequences in front.
+//
+// A tile whose walk is longer than a workgroup's share of all of them is cut into parts, each a workgroup's: long documents or pieces of long prompts next to short
+// ones would otherwise be walked by a few workgroups at the end.  The part that arrives last adds them up, in their order.
 //
 // The gates' gradient is a difference of sums over whole rows and columns of dS, so it is formed from 32-bit values throughout, where the rest of the backward can
 // live with the 16 bits of its operands:
@@ -18,6 +21,8 @@
 // - The row sum of the forward adds the probabilities before they are rounded for the matrix instruction.
 // - o.do is off by the rounding of o and of P; what is missing of delta is sum_j P_ij (dP_ij - o.do), which the dQ kernel has at its end.  It stores
 //   the sum of the two for the dK/dV kernel.
+#include <algorithm>
+
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
 #include "fox_tiles.hpp"
@@ -30,6 +35,8 @@ constexpr int kPackedTile = 128;   // rows of a tile of either kind
 static_assert(kPackedTile == kFwdBM && kPackedTile == kKvBN && kKvBM == kKvBN, "a tile is what a workgroup keeps");
 // Log gates below this close like it: -inf itself would make the difference of two sums behind it undefined.
 constexpr float kLowestGate = -1e6f;
+// Shares below which no walk is cut, in 64 keys and 128 rows of a head.
+constexpr int kQueryShare = 4, kKeyShare = 4, kNoShare = 0x7fffffff;
 
 // ---------------------------------------------------------------------------
 // Plan
@@ -43,22 +50,99 @@ __device__ __forceinline__ int wave_max_scan(int x, int lane) {   // maximum ove
   return x;
 }
 
+__device__ __forceinline__ int wave_sum_scan(int x, int lane) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  return x;
+}
+
 // Place of a length in the order of the plan: shorter sequences come later, in steps of a quarter of a power of two.
 constexpr int kOrderBuckets = 128;
 __device__ __forceinline__ int bucket_of(int rows) {
   return kOrderBuckets - 1 - min(max((int)(__float_as_uint((float)rows) >> 21) - (127 << 2), 0), kOrderBuckets - 1);
 }
 
-// By one workgroup of NT threads.  Ends that decrease or lie outside the tensors are brought into order, so that no tile leaves them.
-template <int NT>
-__device__ __forceinline__ void make_plan(const PackedK& a) {
+// How a walk of `units` is cut: parts of at most `share`, but no more than the root of the units, since one workgroup reads all parts again.  Where
+// rows are the parts, part * ceil(units / parts) is below the units for every part: none is empty.
+struct Share {
+  int units;
+  float inverse;
+};
+__device__ __forceinline__ int parts_of(int units, Share share) {
+  return units <= share.units ? 1 : min((int)((float)units * share.inverse) + 1, (int)__builtin_amdgcn_sqrtf((float)units));
+}
+// x / y of integers below 2^24
+__device__ __forceinline__ int quotient(int x, int y) {
+  const int q = (int)((float)x * __builtin_amdgcn_rcpf((float)y)), r = x - q * y;
+  return r < 0 ? q - 1 : r >= y ? q + 1 : q;
+}
+// Tiles of keys that a tile of queries walks
+__device__ __forceinline__ int key_tiles(int m, int n, int tile) {
+  const int hi = min(n, n - m + (tile + 1) * kPackedTile);
+  return hi > 0 ? (hi + kFwdBN - 1) / kFwdBN : 0;
+}
+// First row, in steps, that a tile of keys walks, and the steps
+__device__ __forceinline__ int first_row(int m, int n, int tile) { return max(tile * kKvBN - (n - m), 0) / kKvBM * kKvBM; }
+__device__ __forceinline__ int row_steps(int m, int n, int tile) {
+  const int lo = first_row(m, n, tile);
+  return m > lo ? (m - lo + kKvBM - 1) / kKvBM : 0;
+}
+// The parts of a tile of keys: by the group's heads first (dc is a head's then), each head's rows only where there are more parts than heads.
+struct KeyParts {
+  int heads, rows, head_span, row_span;   // parts either way; heads and steps of a part
+};
+__device__ __forceinline__ KeyParts key_parts(int steps, int group, int parts) {
+  KeyParts p;
+  const int heads = min(parts, group), rows = max(min(quotient(parts, group), steps), 1);
+  p.head_span = quotient(group + heads - 1, heads);
+  p.heads = quotient(group + p.head_span - 1, p.head_span);
+  p.row_span = max(quotient(steps + rows - 1, rows), 1);
+  p.rows = max(quotient(steps + p.row_span - 1, p.row_span), 1);
+  return p;
+}
+
+// At least the units of a sequence's tiles of queries (keys), in 64 keys (128 rows of a head).
+__device__ __forceinline__ int64_t query_units(int m, int n) {
+  const int64_t p = (int64_t)n - m, tiles = (m + kPackedTile - 1) / kPackedTile, t0 = p < 0 ? min(-p / kPackedTile, tiles) : 0, c = tiles - t0;
+  return (c * p + c * (t0 + tiles + 1) * (kPackedTile / 2) + kFwdBN - 1) / kFwdBN + c;
+}
+__device__ __forceinline__ int64_t key_units(int m, int n, int group) {
+  const int64_t p = (int64_t)n - m, tiles = (n + kPackedTile - 1) / kPackedTile, a = p < 0 ? 0 : min(p / kPackedTile + 1, tiles), c = tiles - a;
+  return ((a * m + c * n - c * (a + tiles - 1) * (kPackedTile / 2)) / kKvBM + 2 * tiles) * group;
+}
+
+constexpr int kNearSequences = 128;   // so many and their parts lie in LDS
+struct PlanMemory {
+  int4 seqs[kNearSequences];
+  int parts[kNearSequences];
+  int buckets[kOrderBuckets];
+  unsigned long long units;
+  int slots, top[2][16];
+};
+
+// The list of the tiles of queries, or of those of keys, by one workgroup of NT threads.  Ends that decrease or lie outside the tensors are brought into order, so
+// that no tile leaves them.
+template <int NT, bool KEYS>
+__device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
   constexpr int WAVES = NT / 64;
-  __shared__ int wave_q[WAVES], wave_k[WAVES];
-  __shared__ int tiles_q[kOrderBuckets], tiles_k[kOrderBuckets];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, S = a.B + kPackedOuter;
-  int4* const seqs = a.plan.seqs;
-  for (int i = tid; i < kOrderBuckets; i += NT) tiles_q[i] = tiles_k[i] = 0;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), S = a.B + kPackedOuter;
+  const int extra = KEYS ? a.k_extra : a.q_extra;
+  const bool near = S <= kNearSequences;
+  int4* const seqs = near ? mem.seqs : a.plan.seqs + (KEYS ? S : 0);
+  int* const seq_parts = near ? mem.parts : a.plan.seq_parts + (KEYS ? S : 0);
+  for (int i = tid; i < kOrderBuckets; i += NT) mem.buckets[i] = 0;
+  if (tid == 0) {
+    mem.units = 0;
+    mem.slots = 0;
+  }
+  if (!KEYS) {
+    for (int i = tid; i < a.q_extra * a.H; i += NT) a.q_arrived[i] = 0;
+  }
   int top_q = 0, top_k = 0;   // largest end so far
+  int64_t units = 0;
   for (int b0 = 0; b0 < a.B; b0 += NT) {
     const int b = b0 + tid;
     const bool in = b < a.B;
@@ -66,69 +150,93 @@ __device__ __forceinline__ void make_plan(const PackedK& a) {
     int q = wave_max_scan(max(sq, 0), lane), k = wave_max_scan(max(sk, 0), lane);
     __syncthreads();
     if (lane == 63) {
-      wave_q[wave] = q;
-      wave_k[wave] = k;
+      mem.top[0][wave] = q;
+      mem.top[1][wave] = k;
     }
     __syncthreads();
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) {
-        q = max(q, wave_q[w]);
-        k = max(k, wave_k[w]);
-      }
+    for (int w = 0; w < wave; ++w) {
+      q = max(q, mem.top[0][w]);
+      k = max(k, mem.top[1][w]);
     }
     q = min(max(q, top_q), a.T);
     k = min(max(k, top_k), a.N);
     const int q1 = min(max(q, last_q), a.T), k1 = min(max(k, last_k), a.N);
-    if (in) seqs[b] = make_int4(q, q1 - q, k, k1 - k);
+    if (in) {
+      const int4 s = make_int4(q, q1 - q, k, k1 - k);
+      seqs[b] = s;
+      if (near && !KEYS) a.plan.seqs[b] = s;
+      units += KEYS ? key_units(s.y, s.w, a.group) : query_units(s.y, s.w);
+      // what belongs to none of them
+      if (b == 0) {
+        seqs[a.B] = make_int4(0, q, 0, 0);
+        seqs[a.B + 2] = make_int4(0, 0, 0, k);
+      }
+      if (b == a.B - 1) {
+        seqs[a.B + 1] = make_int4(q1, a.T - q1, 0, 0);
+        seqs[a.B + 3] = make_int4(0, 0, k1, a.N - k1);
+      }
+    }
     for (int w = 0; w < WAVES; ++w) {
-      top_q = max(top_q, wave_q[w]);
-      top_k = max(top_k, wave_k[w]);
+      top_q = max(top_q, mem.top[0][w]);
+      top_k = max(top_k, mem.top[1][w]);
     }
   }
+  if (units > 0) atomicAdd(&mem.units, (unsigned long long)units);
   __syncthreads();
-  if (tid < kPackedOuter) {
-    const int4 first = seqs[0], end = seqs[a.B - 1];
-    const int q1 = end.x + end.y, k1 = end.z + end.w;
-    seqs[a.B + tid] = tid == 0 ? make_int4(0, first.x, 0, 0) : tid == 1 ? make_int4(q1, a.T - q1, 0, 0) : tid == 2 ? make_int4(0, 0, 0, first.z)
-                                                                                                   : make_int4(0, 0, k1, a.N - k1);
+  if (near && !KEYS && tid < kPackedOuter) a.plan.seqs[a.B + tid] = seqs[a.B + tid];
+  Share share{kNoShare, 0.f};   // a workgroup's: so many that no more parts than `extra` come of it
+  if (extra > 0) {
+    const unsigned long long u = max((2 * mem.units + extra - 1) / extra, (unsigned long long)(KEYS ? kKeyShare : kQueryShare));
+    share.units = (int)min(u, (unsigned long long)kNoShare);
+    share.inverse = 1.0f / (float)share.units;
   }
-  __syncthreads();
-  // tiles of a bucket, their first places, and each sequence's among them (any order within a bucket)
-  for (int b = tid; b < S; b += NT) {
+  auto tiles_of = [&](int4 s) { return ((KEYS ? s.w : s.y) + kPackedTile - 1) / kPackedTile; };
+  auto bucket = [&](int4 s) { return bucket_of(KEYS ? s.y : s.w); };
+  auto tile_parts = [&](int4 s, int t) {
+    if (!KEYS) return parts_of(key_tiles(s.y, s.w, t), share);
+    const int steps = row_steps(s.y, s.w, t), parts = parts_of(steps * a.group, share);
+    if (parts == 1) return 1;
+    const KeyParts p = key_parts(steps, a.group, parts);
+    return p.heads * p.rows;
+  };
+  // parts of a bucket, their first places, and each sequence's among them (any order within a bucket); a wave a sequence
+  for (int b = wave; b < S; b += WAVES) {
     const int4 s = seqs[b];
-    if (s.y > 0) atomicAdd(&tiles_q[bucket_of(s.w)], (s.y + kPackedTile - 1) / kPackedTile);
-    if (s.w > 0) atomicAdd(&tiles_k[bucket_of(s.y)], (s.w + kPackedTile - 1) / kPackedTile);
-  }
-  __syncthreads();
-  if (tid < 2) {
-    int* const tiles = tid ? tiles_k : tiles_q;
-    int sum = 0;
-    for (int i = 0; i < kOrderBuckets; ++i) {
-      const int n = tiles[i];
-      tiles[i] = sum;
-      sum += n;
-    }
-    a.plan.counts[tid] = sum;
-  }
-  __syncthreads();
-  for (int b = wave; b < S; b += WAVES) {   // a wave each
-    const int4 s = seqs[b];
-    const int nq = (s.y + kPackedTile - 1) / kPackedTile, nk = (s.w + kPackedTile - 1) / kPackedTile;
-    int at_q = 0, at_k = 0;
+    const int tiles = tiles_of(s);
+    int parts = 0;
+    for (int t = lane; t < tiles; t += 64) parts += tile_parts(s, t);
+    parts = __shfl(wave_sum_scan(parts, lane), 63);
     if (lane == 0) {
-      if (nq) at_q = atomicAdd(&tiles_q[bucket_of(s.w)], nq);
-      if (nk) at_k = atomicAdd(&tiles_k[bucket_of(s.y)], nk);
+      seq_parts[b] = parts;
+      if (parts > 0) atomicAdd(&mem.buckets[bucket(s)], parts);
     }
-    at_q = __builtin_amdgcn_readfirstlane(at_q);
-    at_k = __builtin_amdgcn_readfirstlane(at_k);
-    PackedItem it{s.x, s.y, s.z, s.w, 0, b, {0, 0}};
-    for (int t = lane; t < nq; t += 64) {   // the last queries see the most keys
-      it.tile = nq - 1 - t;
-      a.plan.q_items[at_q + t] = it;
-    }
-    for (int t = lane; t < nk; t += 64) {   // the first keys are seen by the most queries
-      it.tile = t;
-      a.plan.k_items[at_k + t] = it;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    static_assert(kOrderBuckets == 128, "two a lane");
+    const int x = mem.buckets[2 * lane], y = mem.buckets[2 * lane + 1], end = wave_sum_scan(x + y, lane);
+    mem.buckets[2 * lane] = end - x - y;
+    mem.buckets[2 * lane + 1] = end - y;
+    if (lane == 63) a.plan.counts[KEYS] = end;
+  }
+  __syncthreads();
+  PackedItem* const items = KEYS ? a.plan.k_items : a.plan.q_items;
+  for (int b = wave; b < S; b += WAVES) {
+    const int4 s = seqs[b];
+    const int tiles = tiles_of(s);
+    int at = 0;
+    if (tiles == 0) continue;
+    if (lane == 0) at = atomicAdd(&mem.buckets[bucket(s)], seq_parts[b]);
+    at = __builtin_amdgcn_readfirstlane(at);
+    PackedItem it{s.x, s.y, s.z, s.w, 0, 0, 0, 0};
+    for (int t0 = 0; t0 < tiles; t0 += 64) {   // the last queries see the most keys, the first keys are seen by the most queries
+      const int t = t0 + lane;
+      it.tile = KEYS ? t : tiles - 1 - t;
+      it.parts = t < tiles ? tile_parts(s, it.tile) : 0;
+      const int end = wave_sum_scan(it.parts, lane);
+      it.slot = it.parts > 1 ? atomicAdd(&mem.slots, it.parts) : 0;
+      for (it.part = 0; it.part < it.parts; ++it.part) items[at + end - it.parts + it.part] = it;
+      at += __shfl(end, 63);
     }
   }
 }
@@ -141,37 +249,39 @@ template <int NT, bool REVERSE, typename Load, typename Store>
 __device__ __forceinline__ void sum_row(int n, Load load, Store store) {
   constexpr int PER = 8, WAVES = NT / 64;
   __shared__ double wave_tot[2][WAVES];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x % NT, lane = tid & 63, wave = tid >> 6;
   double carry = 0.0;
   int turn = 0;
   for (int base = 0; base < n; base += NT * PER, turn ^= 1) {
-    const int at = base + tid * PER;
+    const int at = base + wave * 64 * PER + lane;   // a wave's places follow each other, and so do those of a load
     float x[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const int i = min(at + e, n - 1), j = REVERSE ? n - 1 - i : i;
+      const int i = min(at + 64 * e, n - 1), j = REVERSE ? n - 1 - i : i;
       x[e] = load(j);
     }
     double v[PER], run = 0.0;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) v[e] = run += at + e < n ? (double)x[e] : 0.0;
-    const double incl = wave_scan(run);
-    double before = carry + lane_before(incl), total = 0.0;
+    for (int e = 0; e < PER; ++e) {
+      const double incl = wave_scan(at + 64 * e < n ? (double)x[e] : 0.0);
+      v[e] = run + incl;
+      run += of_lane(incl, 63);
+    }
+    double before = carry, total = run;
     if constexpr (WAVES > 1) {
-      if (lane == 63) wave_tot[turn][wave] = incl;
+      if (lane == 63) wave_tot[turn][wave] = run;
       __syncthreads();   // (the other buffer of the two was read in front of it)
+      total = 0.0;
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
         const double t = wave_tot[turn][w];
         if (w < wave) before += t;
         total += t;
       }
-    } else {
-      total = of_lane(incl, 63);
     }
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      if (at + e < n) store(REVERSE ? n - 1 - (at + e) : at + e, before + v[e]);
+      if (at + 64 * e < n) store(REVERSE ? n - 1 - (at + 64 * e) : at + 64 * e, before + v[e]);
     }
     carry += total;
   }
@@ -179,24 +289,37 @@ __device__ __forceinline__ void sum_row(int n, Load load, Store store) {
 
 }  // namespace
 
-// Workgroup 0 makes the plan, the others the sums of a (sequence, head) each.
+// The first workgroups make the plan (that of the keys only where a backward may follow), the others the sums of a (sequence, head) each; with NT = 64 of sixteen.
 template <int NT>
-__global__ __launch_bounds__(NT) void packed_scan_kernel(const PackedK a) {
-  if (blockIdx.x == 0) {
-    make_plan<NT>(a);
-    return;
-  }
-  const int b = divide(blockIdx.x - 1, a.by_heads), h = blockIdx.x - 1 - b * a.H;
+__global__ __launch_bounds__(1024) void packed_scan_kernel(const PackedK a) {
+  constexpr int THREADS = 1024;
+  __shared__ PlanMemory mem;
+  const int plans = a.lse ? 2 : 1;
+  if (blockIdx.x == 0) return make_plan<THREADS, false>(a, mem);
+  if (blockIdx.x < plans) return make_plan<THREADS, true>(a, mem);
+  const int row = (blockIdx.x - plans) * (THREADS / NT) + threadIdx.x / NT;
+  if (row >= a.B * a.H) return;
+  const int b = divide(row, a.by_heads), h = row - b * a.H;
   const int k0 = min(max(a.cu_k[b], 0), a.N), n = min(max(a.cu_k[b + 1], k0), a.N) - k0;
   const float* g = a.g + (int64_t)k0 * a.g_st + h * a.g_sh;
   double* c = a.c + (int64_t)h * a.N + k0;
   sum_row<NT, false>(n, [&](int j) { return fmaxf(g[j * a.g_st], kLowestGate); }, [&](int j, double sum) { c[j] = sum; });
 }
 
+// The backward's counters of arrived parts: its own, since two of one forward may run at once.  (Those of the forward are cleared next to its plan.)
+__global__ __launch_bounds__(256) void packed_clear_kernel(const PackedK a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < a.q_extra * a.H) a.q_arrived[i] = 0;
+  if (i < a.k_extra * a.Hk) a.k_arrived[i] = 0;
+}
+
 // dg of a (sequence, head) from dc.  The first gate of a sequence moves all its sums alike: an exact zero, as in the rows that belong to none.
 template <int NT>
-__global__ __launch_bounds__(NT) void packed_gate_grad_kernel(const PackedK a) {
-  const int b = divide(blockIdx.x, a.by_heads), h = blockIdx.x - b * a.H;
+__global__ __launch_bounds__(1024) void packed_gate_grad_kernel(const PackedK a) {
+  constexpr int THREADS = 1024;
+  const int row = blockIdx.x * (THREADS / NT) + threadIdx.x / NT;
+  if (row >= (a.B + kPackedOuter) * a.H) return;
+  const int b = divide(row, a.by_heads), h = row - b * a.H;
   const int4 s = a.plan.seqs[b];
   const float* dc = a.dc + (int64_t)h * a.N + s.z;
   float* dg = a.dg + (int64_t)s.z * a.dg_st + h * a.dg_sh;
@@ -403,6 +526,67 @@ __device__ __forceinline__ void packed_dkdv_step(const char* q_tile, const char*
 }  // namespace
 
 // ---------------------------------------------------------------------------
+// Parts of a walk: accumulators of 128 rows as the waves hold them, then two numbers a row; read and written past the L2 of an XCD (fox_common.hpp)
+// ---------------------------------------------------------------------------
+namespace {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <int D> constexpr int kAccFloats = (D + 31) / 32 * 32 * kPackedTile;
+template <int D> constexpr int kQueryPartFloats = kAccFloats<D> + 2 * kPackedTile;       // forward: maximum and sum; dQ: row sum of dS
+template <int D> constexpr int kKeyPartFloats = 2 * kAccFloats<D> + kPackedTile;         // dK, dV; dc
+
+template <int DB>
+__device__ __forceinline__ void store_part(float* part, const f32x16 (&acc)[DB], int wave, int lane) {
+  double* at = reinterpret_cast<double*>(part) + wave * DB * 512 + lane;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) store_agent(at + db * 512 + r * 32, __builtin_bit_cast(double, f32x2{acc[db][r], acc[db][r + 1]}));
+}
+template <int DB>
+__device__ __forceinline__ void add_part(const float* part, f32x16 (&acc)[DB], float weight, int wave, int lane) {
+  const double* at = reinterpret_cast<const double*>(part) + wave * DB * 512 + lane;
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    double x[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) x[r] = load_agent(at + db * 512 + r * 64);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const f32x2 y = __builtin_bit_cast(f32x2, x[r]);
+      acc[db][2 * r] = fmaf(y[0], weight, acc[db][2 * r]);
+      acc[db][2 * r + 1] = fmaf(y[1], weight, acc[db][2 * r + 1]);
+    }
+  }
+}
+template <int DB>
+__device__ __forceinline__ void clear(f32x16 (&acc)[DB]) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db) acc[db] = splat(0.f);
+}
+// Whether this workgroup is the last of a tile's parts to arrive.  Every thread calls it, behind its stores.
+__device__ __forceinline__ bool last_part(uint32_t* arrived, int parts) {
+  __shared__ bool last;
+  stores_complete();
+  __syncthreads();
+  if (threadIdx.x == 0) last = arrive(arrived) == (uint32_t)parts - 1u;
+  __syncthreads();
+  return last;
+}
+// The tiles of keys [begin, end) of a part, those of the last keys in part 0.
+struct Walk {
+  int begin, end;
+};
+__device__ __forceinline__ Walk walk_of(const PackedItem& it) {
+  const int tiles = key_tiles(it.m, it.n, it.tile);
+  if (it.parts == 1) return {0, tiles};
+  const int span = (tiles + it.parts - 1) / it.parts, end = tiles - it.part * span;
+  return {max(end - span, 0), end};
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
 // Forward: four waves, 32 query rows each, K and V tiles of 64 keys in two alternating LDS buffers, the tiles at the diagonal one by one and
 // the others software-pipelined (the tile code and its reasons: fox_tiles.hpp, fox_fwd.hip).
 // ---------------------------------------------------------------------------
@@ -430,13 +614,14 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
   const uint16_t* kp = a.k.ptr + (int64_t)it.k0 * a.k.st + hk * a.k.sh;
   const uint16_t* vp = a.v.ptr + (int64_t)it.k0 * a.v.st + hk * a.v.sh;
   uint16_t* op = const_cast<uint16_t*>(a.o.ptr) + (int64_t)it.q0 * a.o.st + h * a.o.sh;
-  const int a0 = p_seq + m0, hi = min(N, a0 + BM);   // key position of the first row, one past the last key that a row sees
+  const int a0 = p_seq + m0;   // key position of the first row
   const int m = m0 + 32 * wave + i, a_m = p_seq + m, a_w0 = a0 + 32 * wave;
   const float qk_scale = nonzero_scale(a.sm_scale * kLog2e), inv_scale = 1.0f / qk_scale;
   const bool wave_has_rows = m0 + 32 * wave < M;
 
   const DirectTileLoader<D, BN, 4, 0> kld(a.k.st, wave, lane), vld(a.v.st, wave, lane);
-  const int n_tiles = hi > 0 ? (hi + BN - 1) / BN : 0;   // walked from the last down
+  const Walk walk = walk_of(it);   // from the last tile down
+  const int n_tiles = walk.end, t_begin = walk.begin;
   f32x16 oacc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -478,9 +663,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
     };
     // tiles at the diagonal; all of them where the pipelined code, which needs a positive scale and a few tiles, is not entered
     int n_diag = 0;
-    while (n_diag < n_tiles && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
-    if (!(qk_scale > 0.f) || n_tiles - n_diag < kMinPipelinedTiles) n_diag = n_tiles;
-    const int t_stop = n_tiles - n_diag;
+    while (n_diag < n_tiles - t_begin && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
+    if (!(qk_scale > 0.f) || n_tiles - t_begin - n_diag < kMinPipelinedTiles) n_diag = n_tiles - t_begin;
+    const int t_stop = n_tiles - n_diag, n_int = t_stop - t_begin;
     if (n_diag > 0 && tid < BN) store_pair(cn_s0, lo_s0);
     for (int t = n_tiles - 1; t >= t_stop; t -= 2) {
       wait_vmem_all();
@@ -495,7 +680,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
       compute((t - 1) * BN, k_tile1, v_tile1, cn_s1, lo_s1);
       if (t - 2 >= t_stop && tid < BN) store_pair(cn_s0, lo_s0);
     }
-    if (t_stop > 0) {   // K runs one tile ahead of V: iteration j computes S(j + 1) and P(j) V(j)
+    if (n_int > 0) {   // K runs one tile ahead of V: iteration j computes S(j + 1) and P(j) V(j)
       auto int_n0 = [&](int j) { return (t_stop - 1 - j) * BN; };
       auto issue_k = [&](int j, char* kt) {
         issue_cn(int_n0(j));
@@ -508,7 +693,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
       if (tid < BN) cn_s0[tid] = cn_term();
       wait_vmem_all();
       __syncthreads();
-      if (t_stop > 1) issue_k(1, k_tile1);
+      if (n_int > 1) issue_k(1, k_tile1);
       vld.issue(vp, a.v.st, int_n0(0), N, v_tile0);
       f32x16 s_a[NB], s_b[NB];
 #pragma unroll
@@ -520,7 +705,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
       }
       auto pipelined_tile = [&](int j, const char* k_nx, const char* v_cur, const float* cn_nx, char* k_fill, char* v_fill, f32x16 (&s_cur)[NB],
                                 f32x16 (&s_nx)[NB]) {
-        const bool more_k = j + 2 < t_stop, more_v = j + 1 < t_stop;
+        const bool more_k = j + 2 < n_int, more_v = j + 1 < n_int;
         const int nk = more_k ? int_n0(j + 2) : 0, nv = more_v ? int_n0(j + 1) : 0;
         if (more_k) issue_cn(nk);
         const uint16_t *k_src = kp + (int64_t)nk * a.k.st, *v_src = vp + (int64_t)nv * a.v.st;
@@ -529,20 +714,43 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
         if (wave_has_rows) fwd_tile_pipelined<Tr, D, true>(k_nx, v_cur, cn_nx, qreg, oacc, m_i, l_i, qk_scale, lane, s_cur, s_nx, dma, row.hi);
         else dma.all();
       };
-      for (int j = 0; j < t_stop; j += 2) {
+      for (int j = 0; j < n_int; j += 2) {
         wait_vmem_all();
-        if (j + 1 < t_stop && tid < BN) cn_s1[tid] = cn_term();
+        if (j + 1 < n_int && tid < BN) cn_s1[tid] = cn_term();
         __syncthreads();
         pipelined_tile(j, k_tile1, v_tile0, cn_s1, k_tile0, v_tile1, s_a, s_b);
-        if (j + 1 >= t_stop) break;
+        if (j + 1 >= n_int) break;
         wait_vmem_all();
-        if (j + 2 < t_stop && tid < BN) cn_s0[tid] = cn_term();
+        if (j + 2 < n_int && tid < BN) cn_s0[tid] = cn_term();
         __syncthreads();
         pipelined_tile(j + 1, k_tile0, v_tile1, cn_s0, k_tile1, v_tile0, s_b, s_a);
       }
     }
   }
-  const float l_tot = half_sum(l_i);
+  float l_tot = half_sum(l_i);
+  if (it.parts > 1) {
+    constexpr int ACC = kAccFloats<D>;
+    const int row = wave * 32 + i;
+    float* parts = a.q_parts + ((int64_t)it.slot * a.H + h) * kQueryPartFloats<D>;   // the tile's, H apart
+    const int64_t step = (int64_t)a.H * kQueryPartFloats<D>;
+    if (wave_has_rows) {
+      float* own = parts + it.part * step;
+      store_part<DB>(own, oacc, wave, lane);
+      store_agent(own + ACC + g * BM + row, g ? l_tot : m_i);
+    }
+    if (!last_part(a.q_arrived + (int64_t)it.slot * a.H + h, it.parts)) return;
+    if (wave_has_rows) {
+      for (int p = 0; p < it.parts; ++p) m_i = fmaxf(m_i, load_agent(parts + p * step + ACC + row));
+      clear(oacc);
+      l_tot = 0.f;
+      for (int p = 0; p < it.parts; ++p) {
+        const float* part = parts + p * step;
+        const float weight = __builtin_amdgcn_exp2f(load_agent(part + ACC + row) - m_i);
+        l_tot = fmaf(load_agent(part + ACC + BM + row), weight, l_tot);
+        add_part<DB>(part, oacc, weight, wave, lane);
+      }
+    }
+  }
   const bool empty = a_m < 0 || n_tiles <= 0;
   const float inv = empty ? 0.f : 1.0f / l_tot;
   if (a.lse && m < M && g == 0) a.lse[(int64_t)h * a.T + it.q0 + m] = empty ? -INFINITY : m_i * kLn2 + __logf(l_tot);
@@ -585,11 +793,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
   const uint16_t* kp = a.k.ptr + (int64_t)it.k0 * a.k.st + hk * a.k.sh;
   const uint16_t* vp = a.v.ptr + (int64_t)it.k0 * a.v.st + hk * a.v.sh;
   uint16_t* dqp = const_cast<uint16_t*>(a.dq.ptr) + (int64_t)it.q0 * a.dq.st + h * a.dq.sh;
-  const int a0 = p_seq + m0, hi = min(N, a0 + BM);
+  const int a0 = p_seq + m0;
   const int m = m0 + 32 * wave + i, a_m = p_seq + m, a_w0 = a0 + 32 * wave;
   const float qk_scale = nonzero_scale(a.sm_scale * kLog2e), inv_scale = 1.0f / qk_scale;
   const bool wave_has_rows = m0 + 32 * wave < M;
-  const int n_tiles = hi > 0 ? (hi + BN - 1) / BN : 0;
+  const Walk walk = walk_of(it);
+  const int n_tiles = walk.end, t_begin = walk.begin;
 
   f32x16 dqacc[DB];
 #pragma unroll
@@ -643,8 +852,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
     }
     // the tiles at the diagonal, an even number of them so that the others find the same buffers free (or all tiles)
     int n_diag = 0;
-    while (n_diag < n_tiles && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
-    n_diag = min(n_diag + (n_diag & 1), n_tiles);
+    while (n_diag < n_tiles - t_begin && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
+    n_diag = min(n_diag + (n_diag & 1), n_tiles - t_begin);
     const int t_stop = n_tiles - n_diag;
     if (tid < BN) {
       if (n_diag > 0) store_pair(cn_s0, lo_s0);
@@ -659,31 +868,52 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
     for (int t = n_tiles - 1; t >= t_stop; t -= 2) {
       wait_vmem_all();
       __syncthreads();
-      if (t >= 1) issue((t - 1) * BN, k_tile1, v_tile1);
+      if (t > t_begin) issue((t - 1) * BN, k_tile1, v_tile1);
       if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, lane);
-      if (t < 1) break;
+      if (t <= t_begin) break;
       next_terms(t - 1, cn_s1, lo_s1);
       wait_vmem_all();
       __syncthreads();
-      if (t >= 2) issue((t - 2) * BN, k_tile0, v_tile0);
+      if (t - 1 > t_begin) issue((t - 2) * BN, k_tile0, v_tile0);
       if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, lane);
-      if (t >= 2) next_terms(t - 2, cn_s0, lo_s0);
+      if (t - 1 > t_begin) next_terms(t - 2, cn_s0, lo_s0);
     }
-    for (int t = t_stop - 1; t >= 0; t -= 2) {
+    for (int t = t_stop - 1; t >= t_begin; t -= 2) {
       wait_vmem_all();
       __syncthreads();
-      if (t >= 1) issue((t - 1) * BN, k_tile1, v_tile1);
+      if (t > t_begin) issue((t - 1) * BN, k_tile1, v_tile1);
       if (wave_has_rows) packed_dq_interior<Tr, D>(k_tile0, v_tile0, cn_s0, qreg, doreg, dqacc, rsum, qk_scale, rowc, delta, lane);
-      if (t < 1) break;
+      if (t <= t_begin) break;
       if (tid < BN) cn_s1[tid] = cn_term();
       wait_vmem_all();
       __syncthreads();
-      if (t >= 2) issue((t - 2) * BN, k_tile0, v_tile0);
+      if (t - 1 > t_begin) issue((t - 2) * BN, k_tile0, v_tile0);
       if (wave_has_rows) packed_dq_interior<Tr, D>(k_tile1, v_tile1, cn_s1, qreg, doreg, dqacc, rsum, qk_scale, rowc, delta, lane);
-      if (t >= 2 && tid < BN) cn_s0[tid] = cn_term();
+      if (t - 1 > t_begin && tid < BN) cn_s0[tid] = cn_term();
     }
   }
-  const float rtot = half_sum(rsum);
+  float rtot = half_sum(rsum);
+  if (it.parts > 1) {
+    constexpr int ACC = kAccFloats<D>;
+    const int row = wave * 32 + i;
+    float* parts = a.q_parts + ((int64_t)it.slot * a.H + h) * kQueryPartFloats<D>;
+    const int64_t step = (int64_t)a.H * kQueryPartFloats<D>;
+    if (wave_has_rows) {
+      float* own = parts + it.part * step;
+      store_part<DB>(own, dqacc, wave, lane);
+      if (g == 0) store_agent(own + ACC + row, rtot);
+    }
+    if (!last_part(a.q_arrived + (int64_t)it.slot * a.H + h, it.parts)) return;
+    if (wave_has_rows) {
+      clear(dqacc);
+      rtot = 0.f;
+      for (int p = 0; p < it.parts; ++p) {
+        const float* part = parts + p * step;
+        rtot += load_agent(part + ACC + row);
+        add_part<DB>(part, dqacc, 1.f, wave, lane);
+      }
+    }
+  }
   if (m < M && g == 0) a.delta[row0 + m] = delta + rtot;
   __syncthreads();
   char* stage = wave == 0 ? k_tile0 : wave == 1 ? k_tile1 : wave == 2 ? v_tile0 : v_tile1;
@@ -720,8 +950,16 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
   uint16_t* dkp = const_cast<uint16_t*>(a.dk.ptr) + (int64_t)it.k0 * a.dk.st + hk * a.dk.sh;
   uint16_t* dvp = const_cast<uint16_t*>(a.dv.ptr) + (int64_t)it.k0 * a.dv.st + hk * a.dv.sh;
   // rows whose key position reaches this tile; a step may begin above them, and all that lies left of key 0 or above a key is masked
-  const int m_lo = max(n0 - p_seq, 0) / BMQ * BMQ;
-  const int n_steps = M > m_lo ? (M - m_lo + BMQ - 1) / BMQ : 0;
+  int m_lo = first_row(M, N, it.tile), n_steps = row_steps(M, N, it.tile), j0 = 0, j1 = a.group;
+  KeyParts cut{1, 1, 0, 0};
+  if (it.parts > 1) {
+    cut = key_parts(n_steps, a.group, it.parts);
+    const int hp = it.part / cut.rows, first = (it.part - hp * cut.rows) * cut.row_span;
+    j0 = hp * cut.head_span;
+    j1 = min(j0 + cut.head_span, a.group);
+    m_lo += first * BMQ;
+    n_steps = min(n_steps - first, cut.row_span);
+  }
   int n_diag = 0;
   while (n_diag < n_steps && p_seq + m_lo + n_diag * BMQ < n0 + BN - 1) ++n_diag;
   const int n_int = n_steps - n_diag, m_top = m_lo + (n_steps - 1) * BMQ;
@@ -799,8 +1037,14 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
   };
   double csum = 0.0;   // (steps in 32 bits, their sum in 64, as in dQ)
   // dc of a head's keys; `more`: its other steps have left their part there
+  float dc_part = 0.f;   // where the rows are cut the part has one head
   auto store_dc = [&](int j, bool more) {
     const float ctot = half_sum((float)csum);
+    if (cut.rows > 1) {
+      dc_part -= ctot;
+      csum = 0.0;
+      return;
+    }
     float* dc = a.dc + (int64_t)head_of(j) * a.N + it.k0 + n;
     if (n < N && g == 0) *dc = (more ? *dc : 0.f) - ctot;
     csum = 0.0;
@@ -815,7 +1059,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       if (up == n_steps) return Step{s.j + 1, n_diag > 0 ? m_lo : m_top};
       return Step{s.j, up < n_diag ? m_lo + up * BMQ : m_top - (up - n_diag) * BMQ};
     };
-    Step cur{0, n_diag > 0 ? m_lo : m_top};
+    Step cur{j0, n_diag > 0 ? m_lo : m_top};
     issue(cur, q_tile1, do_tile1);
     store_rows(cur, rc_s1, lo_s1, dl_s1);
     new_key_term();
@@ -823,7 +1067,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     for (int t = 0;; ++t) {
       const bool odd = t & 1;
       const Step nx = next(cur);
-      const bool more = nx.j < a.group;
+      const bool more = nx.j < j1;
       __syncthreads();
       if (more) issue(nx, odd ? q_tile1 : q_tile0, odd ? do_tile1 : do_tile0);
       const char *qt = odd ? q_tile0 : q_tile1, *dot = odd ? do_tile0 : do_tile1;
@@ -841,8 +1085,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     }
   } else {
     // First the steps at the diagonal of all heads, then the others, pipelined: one wave per SIMD, whose registers hold one kind of step at a time.
-    const int diag_steps = n_diag * a.group, int_steps = n_int * a.group;
-    for (int j = 0, d = 0, t = 0; t < diag_steps; ++t) {
+    const int diag_steps = n_diag * (j1 - j0), int_steps = n_int * (j1 - j0);
+    for (int j = j0, d = 0, t = 0; t < diag_steps; ++t) {
       const Step s{j, m_lo + d * BMQ};
       if (t > 0) __syncthreads();   // buffers 1 are free again
       issue(s, q_tile1, do_tile1);
@@ -850,7 +1094,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       new_key_term();
       wait_vmem_all();
       __syncthreads();
-      if (t == diag_steps - 1 && n_int > 0) issue(Step{0, m_top}, q_tile0, do_tile0);
+      if (t == diag_steps - 1 && n_int > 0) issue(Step{j0, m_top}, q_tile0, do_tile0);
       float sum = 0.f;
       packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rc_s1, lo_s1, dl_s1, kreg, vreg, dkacc, dvacc, sum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
       csum += (double)sum;
@@ -860,11 +1104,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       }
     }
     if (n_int > 0) {
-      if (n_diag == 0) issue(Step{0, m_top}, q_tile0, do_tile0);
-      store_rows(Step{0, m_top}, rc_s0, lo_s0, dl_s0);
+      if (n_diag == 0) issue(Step{j0, m_top}, q_tile0, do_tile0);
+      store_rows(Step{j0, m_top}, rc_s0, lo_s0, dl_s0);
       new_key_term();
     }
-    Step cur{0, m_top};
+    Step cur{j0, m_top};
     const int m_int = m_lo + n_diag * BMQ;   // first row of the interior steps
     // a step from one set of buffers, the next one's tiles into the other; an empty extent where there is none (zeros into the free buffers)
     auto interior = [&](const char* qt, const char* dot, const float* rc, const float* dl, char* qf, char* dof, float* rcf, float* dlf, bool more) {
@@ -898,6 +1142,32 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     }
     wait_vmem_all();   // (the last interior step requested empty tiles)
   }
+  if (it.parts > 1) {
+    constexpr int ACC = kAccFloats<D>;
+    const int key = wave * 32 + i;
+    float* parts = a.k_parts + ((int64_t)it.slot * a.Hk + hk) * kKeyPartFloats<D>;
+    const int64_t step = (int64_t)a.Hk * kKeyPartFloats<D>;
+    if (n_w0 < N) {
+      float* own = parts + it.part * step;
+      store_part<DB>(own, dkacc, wave, lane);
+      store_part<DB>(own + ACC, dvacc, wave, lane);
+      if (g == 0) store_agent(own + 2 * ACC + key, dc_part);
+    }
+    if (!last_part(a.k_arrived + (int64_t)it.slot * a.Hk + hk, it.parts)) return;
+    if (n_w0 < N) {
+      clear(dkacc);
+      clear(dvacc);
+      for (int p = 0; p < it.parts; ++p) {
+        add_part<DB>(parts + p * step, dkacc, 1.f, wave, lane);
+        add_part<DB>(parts + p * step + ACC, dvacc, 1.f, wave, lane);
+      }
+      for (int hp = 0; cut.rows > 1 && hp < cut.heads; ++hp) {
+        float sum = 0.f;
+        for (int r = 0; r < cut.rows; ++r) sum += load_agent(parts + (hp * cut.rows + r) * step + 2 * ACC + key);
+        if (n < N && g == 0) a.dc[(int64_t)head_of(hp) * a.N + it.k0 + n] = sum;
+      }
+    }
+  }
   static_assert(2 * kStoreStageBytes<D> <= Tile<D>::bytes(BMQ), "two waves stage in one tile buffer");
   __syncthreads();
   char* stage = (wave < 2 ? q_tile0 : do_tile0) + (wave & 1) * kStoreStageBytes<D>;
@@ -917,42 +1187,61 @@ int tile_bound(int B, int rows) {
   return (int)(rows / kPackedTile + partial);
 }
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+// More parts than tiles, at most: twice as many as workgroups run at once for a head, none where the longest walk there can be stays whole.
+int extra_parts(int at_once, int heads, int tiles, int64_t longest, int least) {
+  const int64_t target = at_once / heads, most = tiles * longest / least * 2;
+  return target < 2 || longest <= least ? 0 : (int)(2 * target < most ? 2 * target : most);
+}
 
 }  // namespace
 
-int64_t packed_plan_bytes(int B, int T, int N) {
-  return 256 + up((int64_t)(B + kPackedOuter) * sizeof(int4)) + ((int64_t)tile_bound(B, T) + tile_bound(B, N)) * (int64_t)sizeof(PackedItem);
+PackedShape packed_shape(int B, int T, int N, int H, int Hk, int D) {
+  PackedShape s;
+  s.q_bound = tile_bound(B, T);
+  s.k_bound = tile_bound(B, N);
+  s.q_extra = extra_parts((D <= 64 ? 3 : 2) * kCus, H, s.q_bound, ((int64_t)N + kFwdBN - 1) / kFwdBN, kQueryShare);
+  s.k_extra = extra_parts((D <= 64 ? 2 : 1) * kCus, Hk, s.k_bound, ((int64_t)T + kKvBM - 1) / kKvBM * (H / Hk), kKeyShare);
+  s.seqs_at = 256;
+  const int64_t seqs = (int64_t)B + kPackedOuter;   // once for the queries, once for the keys
+  s.seq_parts_at = s.seqs_at + up(2 * seqs * sizeof(int4));
+  s.items_at = s.seq_parts_at + up(2 * seqs * sizeof(int32_t));
+  s.plan_bytes = s.items_at + ((int64_t)s.q_bound + s.q_extra + s.k_bound + s.k_extra) * (int64_t)sizeof(PackedItem);
+  const int64_t acc = (int64_t)(D + 31) / 32 * 32 * kPackedTile, q_rows = (int64_t)s.q_extra * H, k_rows = (int64_t)s.k_extra * Hk;
+  s.q_arrived_at = up(q_rows * (acc + 2 * kPackedTile) * 4);
+  s.fwd_bytes = s.k_parts_at = s.q_arrived_at + up(q_rows * 4);
+  s.k_arrived_at = s.k_parts_at + up(k_rows * (2 * acc + kPackedTile) * 4);
+  s.bwd_bytes = s.k_arrived_at + up(k_rows * 4);
+  return s;
 }
-PackedPlan packed_plan(void* memory, int B, int T, int N, int* q_bound, int* k_bound) {
-  PackedPlan p;
-  char* at = (char*)memory;
-  p.counts = (int32_t*)at;
-  p.seqs = (int4*)(at += 256);
-  p.q_items = (PackedItem*)(at += up((int64_t)(B + kPackedOuter) * sizeof(int4)));
-  *q_bound = tile_bound(B, T);
-  *k_bound = tile_bound(B, N);
-  p.k_items = p.q_items + *q_bound;
-  return p;
+void packed_memory(PackedK& a, const PackedShape& s, void* plan, void* workspace) {
+  char *at = (char*)plan, *ws = (char*)workspace;
+  a.q_bound = s.q_bound;
+  a.k_bound = s.k_bound;
+  a.q_extra = s.q_extra;
+  a.k_extra = s.k_extra;
+  a.plan.counts = (int32_t*)at;
+  a.plan.seqs = (int4*)(at + s.seqs_at);
+  a.plan.seq_parts = (int32_t*)(at + s.seq_parts_at);
+  a.plan.q_items = (PackedItem*)(at + s.items_at);
+  a.plan.k_items = a.plan.q_items + s.q_bound + s.q_extra;
+  a.q_parts = (float*)ws;
+  a.q_arrived = (uint32_t*)(ws + s.q_arrived_at);
+  a.k_parts = (float*)(ws + s.k_parts_at);
+  a.k_arrived = (uint32_t*)(ws + s.k_arrived_at);
 }
 
-// Threads for rows of which the average has so many elements: a row is one workgroup's, and few elements keep few threads busy.
-static int row_threads(int64_t elements, int rows) {
-  const int64_t mean = elements / (rows < 1 ? 1 : rows);
-  return mean <= 256 ? 64 : mean <= 1024 ? 256 : 1024;
-}
+// Whether a row of the scans is a wave's rather than a workgroup's: where there are more rows than workgroups of 1024 at once, and the average row has little for 1024 threads.
+static bool short_rows(int64_t elements, int rows, int heads) { return (int64_t)rows * heads > 2 * kCus && elements <= (int64_t)512 * rows; }
 
 template <typename Tr, int D>
 static hipError_t packed_fwd_d(const PackedK& args, hipStream_t s) {
   PackedK a = args;
   a.by_heads = divisor(a.H);
   a.by_xcd_heads = divisor(a.H % kXcds ? 1 : a.H / kXcds);
-  const dim3 rows((unsigned)(1 + (int64_t)a.B * a.H));
-  switch (row_threads(a.N, a.B)) {
-    case 64: hipLaunchKernelGGL(packed_scan_kernel<64>, rows, dim3(64), 0, s, a); break;
-    case 256: hipLaunchKernelGGL(packed_scan_kernel<256>, rows, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL(packed_scan_kernel<1024>, rows, dim3(1024), 0, s, a);
-  }
-  hipLaunchKernelGGL((packed_fwd_kernel<Tr, D>), dim3((unsigned)((int64_t)a.q_bound * a.H)), dim3(256), 0, s, a);
+  const int rows = a.B * a.H, plans = a.lse ? 2 : 1;
+  if (short_rows(a.N, a.B, a.H)) hipLaunchKernelGGL(packed_scan_kernel<64>, dim3((unsigned)(plans + (rows + 15) / 16)), dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL(packed_scan_kernel<1024>, dim3((unsigned)(plans + rows)), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL((packed_fwd_kernel<Tr, D>), dim3((unsigned)(((int64_t)a.q_bound + a.q_extra) * a.H)), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 template <typename Tr, int D>
@@ -960,17 +1249,16 @@ static hipError_t packed_bwd_d(const PackedK& args, hipStream_t s) {
   PackedK a = args;
   a.by_heads = divisor(a.H);
   a.by_xcd_heads = divisor(a.H % kXcds ? 1 : a.H / kXcds);
-  hipLaunchKernelGGL((packed_dq_kernel<Tr, D>), dim3((unsigned)((int64_t)a.q_bound * a.H)), dim3(256), 0, s, a);
+  const int counters = std::max(a.q_extra * a.H, a.k_extra * a.Hk);
+  if (counters > 0) hipLaunchKernelGGL(packed_clear_kernel, dim3((unsigned)((counters + 255) / 256)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((packed_dq_kernel<Tr, D>), dim3((unsigned)(((int64_t)a.q_bound + a.q_extra) * a.H)), dim3(256), 0, s, a);
   PackedK k = a;
   k.by_heads = divisor(a.Hk);
   k.by_xcd_heads = divisor(a.Hk % kXcds ? 1 : a.Hk / kXcds);
-  hipLaunchKernelGGL((packed_dkdv_kernel<Tr, D>), dim3((unsigned)((int64_t)a.k_bound * a.Hk)), dim3(256), 0, s, k);
-  const dim3 rows((unsigned)((int64_t)(a.B + kPackedOuter) * a.H));
-  switch (row_threads(a.N, a.B)) {
-    case 64: hipLaunchKernelGGL(packed_gate_grad_kernel<64>, rows, dim3(64), 0, s, a); break;
-    case 256: hipLaunchKernelGGL(packed_gate_grad_kernel<256>, rows, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL(packed_gate_grad_kernel<1024>, rows, dim3(1024), 0, s, a);
-  }
+  hipLaunchKernelGGL((packed_dkdv_kernel<Tr, D>), dim3((unsigned)(((int64_t)a.k_bound + a.k_extra) * a.Hk)), dim3(256), 0, s, k);
+  const int rows = (a.B + kPackedOuter) * a.H;
+  if (short_rows(a.N, a.B, a.H)) hipLaunchKernelGGL(packed_gate_grad_kernel<64>, dim3((unsigned)((rows + 15) / 16)), dim3(1024), 0, s, a);
+  else hipLaunchKernelGGL(packed_gate_grad_kernel<1024>, dim3((unsigned)rows), dim3(1024), 0, s, a);
   return hipGetLastError();
 }
 

@@ -697,6 +697,12 @@ fox_view token_view(const Tensor& t) { return fox_view{t.data_ptr(), t.stride(0)
 bool packed_ok(const Tensor& t) { return vectors_ok(t) && t.stride(0) > 0 && t.stride(0) < (1 << 23); }
 Tensor packed_rows(const Tensor& t) { return packed_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+struct PackedBytes {
+  int64_t plan = 0, fwd = 0, bwd = 0;
+  PackedBytes(const Tensor& q, const Tensor& k, int64_t B) {
+    check(fox_packed_bytes((int32_t)B, (int32_t)q.size(0), (int32_t)k.size(0), (int32_t)q.size(1), (int32_t)k.size(1), (int32_t)q.size(2), &plan, &fwd, &bwd), "fox_packed_bytes");
+  }
+};
 struct PackedForward {   // what a forward leaves behind
   Tensor o, c, lse, plan;
 };
@@ -727,18 +733,20 @@ PackedForward run_packed(const Tensor& q, const Tensor& k, const Tensor& v, cons
     f.o = at::zeros(q.sizes(), q.options());
     return f;
   }
-  int64_t plan_bytes = 0;
-  check(fox_packed_plan_bytes((int32_t)B, (int32_t)T, (int32_t)N, &plan_bytes), "fox_packed_plan_bytes");
+  const PackedBytes bytes(q, k, B);
   f.o = at::empty(q.sizes(), q.options());
   f.c = at::empty({H, N}, q.options().dtype(at::kDouble));
   if (keep) f.lse = at::empty({H, T}, q.options().dtype(at::kFloat));
-  f.plan = empty_bytes_like(q, plan_bytes);
+  f.plan = empty_bytes_like(q, bytes.plan);
+  const Tensor workspace = empty_bytes_like(q, bytes.fwd);
   fox_packed_args a = packed_args(q, k, v, f.o, f.c, f.lse, f.plan, B, scale);
   a.g = g.const_data_ptr<float>();
   a.g_stride_t = g.stride(0);
   a.g_stride_h = g.stride(1);
   a.cu_q = cu_q.const_data_ptr<int32_t>();
   a.cu_k = cu_k.const_data_ptr<int32_t>();
+  a.workspace = workspace.mutable_data_ptr();
+  a.workspace_bytes = bytes.fwd;
   check(fox_packed_fwd(&a, stream_of(q)), "fox_packed_fwd");
   return f;
 }
@@ -775,6 +783,10 @@ struct PackedNode : public torch::autograd::Function<PackedNode> {
     a.dg_stride_h = 1;
     a.delta = scratch.mutable_data_ptr<float>();
     a.dc = a.delta + H * T;
+    const PackedBytes bytes(q, k, a.B);
+    const Tensor workspace = empty_bytes_like(q, bytes.bwd);
+    a.workspace = workspace.mutable_data_ptr();
+    a.workspace_bytes = bytes.bwd;
     check(fox_packed_bwd(&a, stream_of(q)), "fox_packed_bwd");
     return {dq, dk, dv, dg, Tensor(), Tensor(), Tensor()};
   }

@@ -202,7 +202,7 @@ class PackedArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("B", "T", "N", "H", "Hk", "D", "dtype")] + [(n, View) for n in ("q", "k", "v", "o")] + [
         ("g", C.c_void_p), ("g_stride_t", C.c_int64), ("g_stride_h", C.c_int64), ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("sm_scale", C.c_float),
         ("c", C.c_void_p), ("lse", C.c_void_p), ("plan", C.c_void_p), ("plan_bytes", C.c_int64)] + [(n, View) for n in ("d_o", "dq", "dk", "dv")] + [
-        ("dg", C.c_void_p), ("dg_stride_t", C.c_int64), ("dg_stride_h", C.c_int64), ("delta", C.c_void_p), ("dc", C.c_void_p)]
+        ("dg", C.c_void_p), ("dg_stride_t", C.c_int64), ("dg_stride_h", C.c_int64), ("delta", C.c_void_p), ("dc", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
 
 # every symbol include/fox_attn.h declares: name -> (restype, argtypes)
@@ -263,7 +263,7 @@ SIGNATURES = {
     "fox_paged8_decode_workspace_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.POINTER(C.c_int64)]),
     "fox_packed_fwd": (C.c_int, [C.POINTER(PackedArgs), C.c_void_p]),
     "fox_packed_bwd": (C.c_int, [C.POINTER(PackedArgs), C.c_void_p]),
-    "fox_packed_plan_bytes": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
+    "fox_packed_bytes": (C.c_int, [C.c_int32] * 6 + [C.POINTER(C.c_int64)] * 3),
     "fox_token_shift_fwd": (C.c_int, [C.POINTER(ShiftArgs), C.c_void_p]),
     "fox_token_shift_bwd": (C.c_int, [C.POINTER(ShiftArgs), C.c_void_p]),
 }

@@ -618,8 +618,8 @@ int fox_paged8_decode_workspace_bytes(int32_t B, int32_t H, int32_t Hk, int32_t 
  * no sequence, in gradients as well.  Query head h reads key head h / (H / Hk) and has log gates of its own:
  *   s_ij = sm_scale q_i.k_j + c_i - c_j,  c_j = sum of the sequence's gates up to key j,  o = softmax(s) v.
  * q, o, d_o, dq: (T, H, D); k, v, dk, dv: (N, Hk, D), 16-bit; stride_t is a token's, stride_h a head's, stride_b is not used; token strides are positive and below 2^23.
- * c (H, N) fp64, lse (H, T) and the plan are written by the forward and read by the backward, which takes them in place of g, cu_q and cu_k; lse may be NULL for a forward alone.  The plan holds
- * fox_packed_plan_bytes() bytes, 16-byte aligned.  Log gates below -1e6 count as that.
+ * c (H, N) fp64, lse (H, T) and the plan are written by the forward and read by the backward, which takes them in place of g, cu_q and cu_k; lse may be NULL for a forward alone.  The plan and each
+ * call's workspace hold the bytes that fox_packed_bytes() gives, 16-byte aligned; calls that may run at once need workspaces of their own.  Log gates below -1e6 count as that.
  */
 typedef struct fox_packed_args {
   int32_t B, T, N, H, Hk, D, dtype;
@@ -639,10 +639,12 @@ typedef struct fox_packed_args {
   int64_t dg_stride_t, dg_stride_h;
   float* delta;               /* (H, T), scratch */
   float* dc;                  /* (H, N), scratch */
+  void* workspace;            /* NULL where none is needed */
+  int64_t workspace_bytes;
 } fox_packed_args;
 int fox_packed_fwd(const fox_packed_args* args, void* stream);
 int fox_packed_bwd(const fox_packed_args* args, void* stream);
-int fox_packed_plan_bytes(int32_t B, int32_t T, int32_t N, int64_t* bytes);
+int fox_packed_bytes(int32_t B, int32_t T, int32_t N, int32_t H, int32_t Hk, int32_t D, int64_t* plan, int64_t* fwd_workspace, int64_t* bwd_workspace);
 
 #ifdef __cplusplus
 }

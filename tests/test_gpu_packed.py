@@ -127,6 +127,13 @@ CASES = [  # new tokens, tokens in front, H, Hk, D, dtype, more
     ([3] * 150, [0] * 150, 5, 5, 64, torch.bfloat16, dict(pad=7)),
     ([60, 200], [-20, -200], 4, 2, 64, torch.bfloat16, {}),           # more queries than keys: the first see none; none at all
     ([100, 0, 300], [-100, 50, -299], 3, 3, 128, torch.float16, {}),
+    # walks that are cut: rows of the one head, heads of a group, both; a few queries far into their keys; queries without keys at the top
+    ([1800, 40, 3], [0, 0, 0], 1, 1, 64, torch.bfloat16, dict(lead=5)),
+    ([900, 12], [0, 0], 8, 1, 64, torch.float16, dict(pad=3)),
+    ([1300, 5], [0, 50], 2, 1, 128, torch.bfloat16, {}),
+    ([2, 130], [6000, 10], 2, 2, 32, torch.bfloat16, {}),
+    ([1], [9000], 16, 4, 16, torch.float16, {}),
+    ([1500, 20], [-700, 0], 1, 1, 128, torch.bfloat16, {}),
 ]
 
 

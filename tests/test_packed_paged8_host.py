@@ -17,27 +17,32 @@ def _buffer(n=8192):
 def test_packed_c_abi_checks():
     lib = _lib.load()
     _keep, base = _buffer(1 << 16)
-    n = C.c_int64(-1)
-    assert lib.fox_packed_plan_bytes(3, 500, 700, C.byref(n)) == 0 and n.value > 0
-    room = n.value
-    for B, T, N in ((0, 5, 5), (1, 0, 5), (1, 5, 0), (65536, 5, 5), (1, (1 << 30) + 1, 5)):
-        assert lib.fox_packed_plan_bytes(B, T, N, C.byref(n)) == -1
-    assert lib.fox_packed_plan_bytes(1, 5, 5, None) == -1
+    n = [C.c_int64(-1) for _ in range(3)]
+    size = lambda *a: lib.fox_packed_bytes(*a, *(C.byref(x) for x in n))
+    assert size(3, 500, 700, 4, 2, 64) == 0 and all(x.value > 0 for x in n)
+    room, ws = n[0].value, {"fwd": n[1].value, "bwd": n[2].value}
+    assert size(3, 500, 256, 4, 2, 64) == 0 and n[1].value == 0 < n[2].value      # walks of few keys stay whole
+    assert size(3, 500, 700, 512, 512, 64) == 0 and n[1].value == n[2].value == 0   # as do those of many heads
+    for bad in ((0, 5, 5, 4, 2, 64), (1, 0, 5, 4, 2, 64), (1, 5, 0, 4, 2, 64), (65536, 5, 5, 4, 2, 64), (1, (1 << 30) + 1, 5, 4, 2, 64), (1, 5, 5, 3, 2, 64), (1, 5, 5, 4, 2, 48)):
+        assert size(*bad) == -1
+    assert lib.fox_packed_bytes(1, 5, 5, 4, 2, 64, None, C.byref(n[0]), C.byref(n[1])) == -1
+    big = 1 << 40
 
-    def args(B=3, T=500, N=700, H=4, Hk=2, D=64, dtype=0, q=base, k=base, v=base, o=base, st=256, g=base, cu=base, c=base, lse=base, plan=base, bytes=room, d_o=base, dq=base, dk=base,
+    def args(B=3, T=500, N=700, H=4, Hk=2, D=64, dtype=0, q=base, k=base, v=base, o=base, st=256, g=base, cu=base, c=base, lse=base, plan=base, bytes=room, work=base, space=big, d_o=base, dq=base, dk=base,
              dv=base, dg=base, delta=base, dc=base):
         view = lambda p: _lib.View(p, 0, 64, st)
         return _lib.PackedArgs(B, T, N, H, Hk, D, dtype, view(q), view(k), view(v), view(o), g, 4, 1, cu, cu, 1.0, c, lse, plan, bytes, view(d_o), view(dq), view(dk), view(dv), dg, 4, 1,
-                               delta, dc)
+                               delta, dc, work, space)
 
     fwd = lambda **k: lib.fox_packed_fwd(C.byref(args(**k)), None)
     bwd = lambda **k: lib.fox_packed_bwd(C.byref(args(**k)), None)
     for call in (fwd, bwd):
         for bad, text in ((dict(B=0), b"positive"), (dict(T=0), b"positive"), (dict(B=70000), b"65535"), (dict(D=48), b"head dim"), (dict(dtype=2), b"dtype"), (dict(H=3), b"multiple"),
                           (dict(Hk=0), b"multiple"), (dict(H=70000, Hk=1), b"65535"), (dict(st=1 << 23), b"2^23"), (dict(st=0), b"2^23"), (dict(c=None), b"c and plan"),
-                          (dict(plan=None), b"c and plan"), (dict(bytes=room - 1), b"plan too small"), (dict(B=60000, H=100, Hk=100, bytes=1 << 40), b"too many")):
+                          (dict(plan=None), b"c and plan"), (dict(bytes=room - 1), b"plan too small"), (dict(space=ws["fwd"] - 1), b"workspace too small"), (dict(work=None), b"workspace too small"), (dict(B=60000, H=100, Hk=100, bytes=1 << 40), b"too many")):
             assert call(**bad) == -1 and text in lib.fox_last_error(), (bad, lib.fox_last_error())
-        assert call(q=base + 2) == -2 and call(k=base + 4) == -2 and call(o=base + 8) == -2 and call(plan=base + 4) == -2 and call(st=60) == -2 and call(v=None) == -1
+        assert call(q=base + 2) == -2 and call(k=base + 4) == -2 and call(o=base + 8) == -2 and call(plan=base + 4) == -2 and call(work=base + 8) == -2 and call(st=60) == -2 and call(v=None) == -1
+    assert bwd(space=ws["bwd"] - 1) == -1
     assert fwd(g=None) == -1 and fwd(cu=None) == -1
     for bad in ("lse", "dg", "delta", "dc", "d_o", "dq", "dk", "dv"):
         assert bwd(**{bad: None}) == -1
