@@ -307,8 +307,7 @@ struct PackedItem {
   int32_t part, parts, slot;             // of a tile whose walk is cut; its first place among those of all parts
 };
 struct PackedPlan {                      // in the plan's memory, behind the counts
-  PackedItem *q_items, *k_items;         // tiles of queries and of keys, those of the longest sequences first
-  int32_t* seq_parts;                    // parts of the tiles of a sequence (where there are too many sequences for LDS)
+  PackedItem *q_items, *k_items;         // tiles of queries and of keys, the longest walks first
   int4* seqs;                            // {q0, m, k0, n} of the B sequences and of kPackedOuter that hold what belongs to none
   int32_t* counts;                       // of q_items and k_items
 };
@@ -328,6 +327,7 @@ struct PackedK {
   int B, T, N, H, Hk, group;             // group = H / Hk query heads on a key head
   int q_bound, k_bound;                  // tiles, at most
   int q_extra, k_extra;                  // parts of those that are cut, at most; 0: none is
+  int q_groups, k_groups;                // of sequences, in the order of the lists
   float *q_parts, *k_parts;              // what the parts leave
   uint32_t *q_arrived, *k_arrived;       // parts that have
   float sm_scale;
@@ -477,8 +477,8 @@ hipError_t launch_paged_gather(const PagedGatherK& a, int D, int dtype, int code
 hipError_t launch_paged8_decode(const Paged8DecodeK& a, int D, int dtype, int codes, hipStream_t s);
 int64_t rotary_workspace_floats(int64_t tokens, int heads, int D, bool shared);
 struct PackedShape {
-  int q_bound, k_bound, q_extra, k_extra;
-  int64_t seqs_at, seq_parts_at, items_at, plan_bytes;                                              // in the plan
+  int q_bound, k_bound, q_extra, k_extra, q_groups, k_groups;
+  int64_t seqs_at, items_at, plan_bytes;                            // in the plan
   int64_t q_arrived_at, k_parts_at, k_arrived_at, fwd_bytes, bwd_bytes;      // in a workspace
 };
 PackedShape packed_shape(int B, int T, int N, int H, int Hk, int D);

@@ -8,7 +8,7 @@
 //
 // Who knows how long the sequences are is the device.  Two workgroups make the plan, the lists of all tiles of queries and of keys, while the others form the
 // sums of the gates; the attention kernels are launched for as many tiles as there can be (a partial one for every sequence) and those past the
-// list end at once.  A sequence's tiles follow each other, heaviest first, the longest sequences in front.
+// list end at once.  The longest walks come first.
 //
 // A tile whose walk is longer than a workgroup's share of all of them is cut into parts, each a workgroup's: long documents or pieces of long prompts next to short
 // ones would otherwise be walked by a few workgroups at the end.  The part that arrives last adds them up, in their order.
@@ -59,20 +59,20 @@ __device__ __forceinline__ int wave_sum_scan(int x, int lane) {
   return x;
 }
 
-// Place of a length in the order of the plan: shorter sequences come later, in steps of a quarter of a power of two.
-constexpr int kOrderBuckets = 128;
-__device__ __forceinline__ int bucket_of(int rows) {
-  return kOrderBuckets - 1 - min(max((int)(__float_as_uint((float)rows) >> 21) - (127 << 2), 0), kOrderBuckets - 1);
+// Place of a walk in the order of its group: shorter ones come later, in steps of a quarter of a power of two.
+constexpr int kOrderLengths = 64, kOrderGroups = 16;
+__device__ __forceinline__ int order_of(int units) {
+  return kOrderLengths - 1 - min(max((int)(__float_as_uint((float)units) >> 21) - (127 << 2), 0), kOrderLengths - 1);
 }
 
 // How a walk of `units` is cut: parts of at most `share`, but no more than the root of the units, since one workgroup reads all parts again.  Where
 // rows are the parts, part * ceil(units / parts) is below the units for every part: none is empty.
 struct Share {
-  int units;
-  float inverse;
+  int whole;       // walks up to this stay whole
+  float inverse;   // of the share
 };
 __device__ __forceinline__ int parts_of(int units, Share share) {
-  return units <= share.units ? 1 : min((int)((float)units * share.inverse) + 1, (int)__builtin_amdgcn_sqrtf((float)units));
+  return units <= share.whole ? 1 : min((int)((float)units * share.inverse) + 1, (int)__builtin_amdgcn_sqrtf((float)units));
 }
 // x / y of integers below 2^24
 __device__ __forceinline__ int quotient(int x, int y) {
@@ -114,13 +114,12 @@ __device__ __forceinline__ int64_t key_units(int m, int n, int group) {
   return ((a * m + c * n - c * (a + tiles - 1) * (kPackedTile / 2)) / kKvBM + 2 * tiles) * group;
 }
 
-constexpr int kNearSequences = 128;   // so many and their parts lie in LDS
+constexpr int kNearSequences = 128;   // so many lie in LDS
 struct PlanMemory {
   int4 seqs[kNearSequences];
-  int parts[kNearSequences];
-  int buckets[kOrderBuckets];
+  int buckets[kOrderGroups * kOrderLengths];
   unsigned long long units;
-  int slots, top[2][16];
+  int slots, top[2][16], waves[16];
 };
 
 // The list of the tiles of queries, or of those of keys, by one workgroup of NT threads.  Ends that decrease or lie outside the tensors are brought into order, so
@@ -132,8 +131,8 @@ __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
   const int extra = KEYS ? a.k_extra : a.q_extra;
   const bool near = S <= kNearSequences;
   int4* const seqs = near ? mem.seqs : a.plan.seqs + (KEYS ? S : 0);
-  int* const seq_parts = near ? mem.parts : a.plan.seq_parts + (KEYS ? S : 0);
-  for (int i = tid; i < kOrderBuckets; i += NT) mem.buckets[i] = 0;
+  static_assert(NT == kOrderGroups * kOrderLengths, "a bucket a thread");
+  mem.buckets[tid] = 0;
   if (tid == 0) {
     mem.units = 0;
     mem.slots = 0;
@@ -184,59 +183,64 @@ __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
   if (units > 0) atomicAdd(&mem.units, (unsigned long long)units);
   __syncthreads();
   if (near && !KEYS && tid < kPackedOuter) a.plan.seqs[a.B + tid] = seqs[a.B + tid];
-  Share share{kNoShare, 0.f};   // a workgroup's: so many that no more parts than `extra` come of it
+  // A workgroup's share: so many that no more parts than `extra` come of it.  Walks of queries stay whole up to two shares: the longest start first, and
+  // a part costs a start and a merge.  (Two / one, us: 8 x 768 tokens, 12 heads, D 64: forward 22.3 / 29.0, dQ 28.6 / 37.2; pieces of prompts of up to 12800 keys 155 / 170; documents of
+  // 150 to 2048 tokens 34.8 / 36.0 and 44.1 / 45.9.  dK/dV of those, whose workgroups are fewer and walk in longer steps: 63.6 / 49.0.)
+  Share share{kNoShare, 0.f};
   if (extra > 0) {
     const unsigned long long u = max((2 * mem.units + extra - 1) / extra, (unsigned long long)(KEYS ? kKeyShare : kQueryShare));
-    share.units = (int)min(u, (unsigned long long)kNoShare);
-    share.inverse = 1.0f / (float)share.units;
+    share.whole = (int)min(KEYS ? u : 2 * u, (unsigned long long)kNoShare);
+    share.inverse = 1.0f / (float)u;
   }
   auto tiles_of = [&](int4 s) { return ((KEYS ? s.w : s.y) + kPackedTile - 1) / kPackedTile; };
-  auto bucket = [&](int4 s) { return bucket_of(KEYS ? s.y : s.w); };
-  auto tile_parts = [&](int4 s, int t) {
-    if (!KEYS) return parts_of(key_tiles(s.y, s.w, t), share);
-    const int steps = row_steps(s.y, s.w, t), parts = parts_of(steps * a.group, share);
-    if (parts == 1) return 1;
-    const KeyParts p = key_parts(steps, a.group, parts);
-    return p.heads * p.rows;
+  // sequences whose keys (queries) an XCD's cache holds together are a group; within it the longest walks come first
+  const int groups = KEYS ? a.k_groups : a.q_groups;
+  const float per_token = (float)groups / (float)(KEYS ? a.T : a.N);
+  struct Tile {
+    int parts, bucket;
   };
-  // parts of a bucket, their first places, and each sequence's among them (any order within a bucket); a wave a sequence
+  auto tile_of = [&](int4 s, int t) {
+    const int steps = KEYS ? row_steps(s.y, s.w, t) : 0, units = KEYS ? steps * a.group : key_tiles(s.y, s.w, t);
+    Tile r;
+    r.parts = parts_of(units, share);
+    const int first = min((int)((float)(KEYS ? s.x : s.z) * per_token), groups - 1) * kOrderLengths;
+    r.bucket = first + order_of(r.parts > 1 ? quotient(min(units, 1 << 23), r.parts) : units);
+    if (KEYS && r.parts > 1) {
+      const KeyParts p = key_parts(steps, a.group, r.parts);
+      r.parts = p.heads * p.rows;
+    }
+    return r;
+  };
+  // parts of a bucket, their first places, and each tile's among them (any order within a bucket); a wave a sequence
   for (int b = wave; b < S; b += WAVES) {
     const int4 s = seqs[b];
     const int tiles = tiles_of(s);
-    int parts = 0;
-    for (int t = lane; t < tiles; t += 64) parts += tile_parts(s, t);
-    parts = __shfl(wave_sum_scan(parts, lane), 63);
-    if (lane == 0) {
-      seq_parts[b] = parts;
-      if (parts > 0) atomicAdd(&mem.buckets[bucket(s)], parts);
+    for (int t = lane; t < tiles; t += 64) {
+      const Tile x = tile_of(s, t);
+      atomicAdd(&mem.buckets[x.bucket], x.parts);
     }
   }
   __syncthreads();
-  if (wave == 0) {
-    static_assert(kOrderBuckets == 128, "two a lane");
-    const int x = mem.buckets[2 * lane], y = mem.buckets[2 * lane + 1], end = wave_sum_scan(x + y, lane);
-    mem.buckets[2 * lane] = end - x - y;
-    mem.buckets[2 * lane + 1] = end - y;
-    if (lane == 63) a.plan.counts[KEYS] = end;
-  }
+  const int own = mem.buckets[tid];
+  int end = wave_sum_scan(own, lane);
+  if (lane == 63) mem.waves[wave] = end;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) end += mem.waves[w];
+  mem.buckets[tid] = end - own;
+  if (tid == NT - 1) a.plan.counts[KEYS] = end;
   __syncthreads();
   PackedItem* const items = KEYS ? a.plan.k_items : a.plan.q_items;
   for (int b = wave; b < S; b += WAVES) {
     const int4 s = seqs[b];
     const int tiles = tiles_of(s);
-    int at = 0;
-    if (tiles == 0) continue;
-    if (lane == 0) at = atomicAdd(&mem.buckets[bucket(s)], seq_parts[b]);
-    at = __builtin_amdgcn_readfirstlane(at);
     PackedItem it{s.x, s.y, s.z, s.w, 0, 0, 0, 0};
-    for (int t0 = 0; t0 < tiles; t0 += 64) {   // the last queries see the most keys, the first keys are seen by the most queries
-      const int t = t0 + lane;
-      it.tile = KEYS ? t : tiles - 1 - t;
-      it.parts = t < tiles ? tile_parts(s, it.tile) : 0;
-      const int end = wave_sum_scan(it.parts, lane);
-      it.slot = it.parts > 1 ? atomicAdd(&mem.slots, it.parts) : 0;
-      for (it.part = 0; it.part < it.parts; ++it.part) items[at + end - it.parts + it.part] = it;
-      at += __shfl(end, 63);
+    for (int t = lane; t < tiles; t += 64) {
+      const Tile x = tile_of(s, t);
+      PackedItem* const at = items + atomicAdd(&mem.buckets[x.bucket], x.parts);
+      it.tile = t;
+      it.parts = x.parts;
+      it.slot = x.parts > 1 ? atomicAdd(&mem.slots, x.parts) : 0;
+      for (it.part = 0; it.part < x.parts; ++it.part) at[it.part] = it;
     }
   }
 }
@@ -360,15 +364,35 @@ __device__ __forceinline__ Pair pair_of(double x) {
 }
 constexpr double kLog2eD = 1.4426950408889634074;
 
+// x - y, y a number of 32 bits: the upper half's rounding goes to the lower one.
+__device__ __forceinline__ Pair less(Pair x, float y) {
+  const float hi = x.hi - y, b = hi - x.hi;
+  return {hi, x.lo + ((x.hi - (hi - b)) - (y + b))};
+}
+// Sums of gates, in log2 units from the tile's reference on, up to which their upper halves alone are good enough: a bias is off by 2^-19 then.  (A training step of eight documents
+// of 768 tokens, D 64: 124 us with pairs everywhere.)
+constexpr float kStrongGates = 32.f;
+
 // x[r] = s[r] scale + (row - column) with the pairs of rows (or columns) c_row(r, g) in LDS; sign -1: LDS holds the columns.
 template <int SIGN>
-__device__ __forceinline__ void add_bias(f32x16& s, const float* hi_s, const float* lo_s, int at, int g, Pair own, float scale) {
+__device__ __forceinline__ void add_pairs(f32x16& s, const float* hi_s, const float* lo_s, int at, int g, Pair own, float scale) {
 #pragma unroll
   for (int q4 = 0; q4 < 4; ++q4) {   // (four at a time: all of them at once do not fit the registers of dQ at head dim 128)
     const f32x4 hi = *reinterpret_cast<const f32x4*>(&hi_s[at + 8 * q4 + 4 * g]), lo = *reinterpret_cast<const f32x4*>(&lo_s[at + 8 * q4 + 4 * g]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       s[4 * q4 + e] = fmaf(s[4 * q4 + e], scale, SIGN > 0 ? (hi[e] - own.hi) + (lo[e] - own.lo) : (own.hi - hi[e]) + (own.lo - lo[e]));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+// The same; the columns' upper halves alone where no gate is strong.
+__device__ __forceinline__ void add_bias(f32x16& s, const float* hi_s, const float* lo_s, int at, int g, Pair own, float scale, bool strong) {
+  if (strong) return add_pairs<-1>(s, hi_s, lo_s, at, g, own, scale);
+#pragma unroll
+  for (int q4 = 0; q4 < 4; ++q4) {
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(&hi_s[at + 8 * q4 + 4 * g]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[4 * q4 + e] = fmaf(s[4 * q4 + e], scale, own.hi - hi[e]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -387,48 +411,49 @@ __device__ __forceinline__ f32x16 splat(float x) {
   return v;
 }
 
+// A running maximum and sum for every 32 keys: those above the rows of the wave cost nothing, and only those at the diagonal are masked.
 template <typename Tr, int D>
-__device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, const u32x4 (&qreg)[D / 16],
-                                                f32x16 (&oacc)[(D + 31) / 32], float& m_i, float& l_i, int n0, int a_m, Pair row, float qk_scale, int lane) {
+__device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, bool strong, const u32x4 (&qreg)[D / 16],
+                                                f32x16 (&oacc)[(D + 31) / 32], float& m_i, float& l_i, int n0, int a_m, int a_w0, Pair row, float qk_scale, int lane) {
   constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
   const int g = lane >> 5;
-  f32x16 s[NB];
-  float mloc = -INFINITY;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
-    s[nb] = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
-    add_bias<-1>(s[nb], hi_s, lo_s, 32 * nb, g, row, qk_scale);
+    const int nb0 = n0 + 32 * nb;
+    if (nb0 > a_w0 + 31) continue;
+    f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
+    add_bias(s, hi_s, lo_s, 32 * nb, g, row, qk_scale, strong);
+    if (nb0 + 31 > a_w0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = nb0 + c_row(r, g) > a_m ? -INFINITY : s[r];
+    }
+    float mloc = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mloc = fmaxf(mloc, s[r]);
+    mloc = half_max(mloc);
+    const bool raise = mloc > m_i + kLazyMaxLog2;
+    if (__any(raise)) {
+      const float m_new = raise ? mloc : m_i, alpha = __builtin_amdgcn_exp2f(m_i - m_new);
+      m_i = m_new;
+      l_i *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
+    }
+    float rsum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[nb][r] = n0 + 32 * nb + c_row(r, g) > a_m ? -INFINITY : s[nb][r];
-      mloc = fmaxf(mloc, s[nb][r]);
+      s[r] = __builtin_amdgcn_exp2f(s[r] - m_i);
+      rsum += s[r];
     }
-  }
-  mloc = half_max(mloc);
-  const bool raise = mloc > m_i + kLazyMaxLog2;
-  if (__any(raise)) {
-    const float m_new = raise ? mloc : m_i, alpha = __builtin_amdgcn_exp2f(m_i - m_new);
-    m_i = m_new;
-    l_i *= alpha;
+    l_i += rsum;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int hh = 0; hh < 2; ++hh) {
+      const u32x4 pb = pack8<Tr>(s, 8 * hh);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) oacc[db][r] *= alpha;
-  }
-  float rsum = 0.f;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[nb][r] = __builtin_amdgcn_exp2f(s[nb][r] - m_i);
-      rsum += s[nb][r];
+      for (int db = 0; db < DB; ++db) oacc[db] = Tr::mfma32(lds_col_operand<D>(v_tile, 32 * nb + 16 * hh, db, lane), pb, oacc[db]);
     }
-  l_i += rsum;
-#pragma unroll
-  for (int sl = 0; sl < BN / 16; ++sl) {
-    const u32x4 pb = pack8<Tr>(s[sl >> 1], 8 * (sl & 1));
-#pragma unroll
-    for (int db = 0; db < DB; ++db) oacc[db] = Tr::mfma32(lds_col_operand<D>(v_tile, 16 * sl, db, lane), pb, oacc[db]);
   }
 }
 
@@ -461,8 +486,8 @@ __device__ __forceinline__ void packed_dq_interior(const char* k_tile, const cha
 
 // `row`: of the query, its log-normaliser taken off
 template <typename Tr, int D>
-__device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, const u32x4 (&qreg)[D / 16],
-                                               const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rows, int n0, int a_m, int a_w0, Pair row,
+__device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, bool strong,
+                                               const u32x4 (&qreg)[D / 16], const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rows, int n0, int a_m, int a_w0, Pair row,
                                                float qk_scale, float delta, int lane) {
   constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
   const int g = lane >> 5;
@@ -471,9 +496,13 @@ __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v
     const int nb0 = n0 + 32 * nb;
     if (nb0 > a_w0 + 31) continue;   // entirely above this wave's rows
     f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
-    add_bias<-1>(s, hi_s, lo_s, 32 * nb, g, row, qk_scale);
+    add_bias(s, hi_s, lo_s, 32 * nb, g, row, qk_scale, strong);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = nb0 + c_row(r, g) > a_m ? 0.f : __builtin_amdgcn_exp2f(s[r]);
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
+    if (nb0 + 31 > a_w0) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = nb0 + c_row(r, g) > a_m ? 0.f : s[r];
+    }
     f32x16 dp = dots<Tr, D>(v_tile, 32 * nb, doreg, splat(-delta), lane);
     float rsum = 0.f;
 #pragma unroll
@@ -491,23 +520,42 @@ __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v
   }
 }
 
-// hi_s, lo_s: of the rows, their log-normalisers taken off; dl_s: -delta
+struct Rows {                          // of a step of dK/dV in LDS, log-normalisers taken off
+  alignas(16) float rc[kKvBM];         // start values of the score accumulators
+  alignas(16) float hi[kKvBM];         // at the diagonal: pairs
+  alignas(16) float lo[kKvBM];
+  alignas(16) float dl[kKvBM];         // -delta
+  alignas(16) int strong[4];           // whether those of a wave need their pairs
+};
+
 template <typename Tr, int D>
-__device__ __forceinline__ void packed_dkdv_step(const char* q_tile, const char* do_tile, const float* hi_s, const float* lo_s, const float* dl_s, const u32x4 (&kreg)[D / 16],
-                                                 const u32x4 (&vreg)[D / 16], f32x16 (&dkacc)[(D + 31) / 32], f32x16 (&dvacc)[(D + 31) / 32], float& csum, int a_s0, int n,
-                                                 int n_w0, Pair col, float qk_scale, int lane) {
+__device__ __forceinline__ void packed_dkdv_step(const char* q_tile, const char* do_tile, const Rows& rows, bool strong, const u32x4 (&kreg)[D / 16], const u32x4 (&vreg)[D / 16],
+                                                 f32x16 (&dkacc)[(D + 31) / 32], f32x16 (&dvacc)[(D + 31) / 32], float& csum, int a_s0, int n, int n_w0, Pair col,
+                                                 float qk_scale, int lane) {
   constexpr int DB = (D + 31) / 32, MB = kKvBM / 32;
   const int g = lane >> 5;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     const int a_b0 = a_s0 + 32 * mb;
     if (a_b0 + 31 < n_w0) continue;   // entirely above the diagonal for this wave
-    f32x16 s = dots<Tr, D>(q_tile, 32 * mb, kreg, splat(0.f), lane);
-    f32x16 dp = dots<Tr, D>(do_tile, 32 * mb, vreg, acc_init(dl_s, 32 * mb, g), lane);
-    add_bias<1>(s, hi_s, lo_s, 32 * mb, g, col, qk_scale);
+    f32x16 s;
+    if (strong) {
+      s = dots<Tr, D>(q_tile, 32 * mb, kreg, splat(0.f), lane);
+      add_pairs<1>(s, rows.hi, rows.lo, 32 * mb, g, col, qk_scale);
+    } else {
+      s = dots<Tr, D>(q_tile, 32 * mb, kreg, acc_init(rows.rc, 32 * mb, g), lane);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], qk_scale, -col.hi);
+    }
+    f32x16 dp = dots<Tr, D>(do_tile, 32 * mb, vreg, acc_init(rows.dl, 32 * mb, g), lane);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
+    if (a_b0 < n_w0 + 31) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = n > a_b0 + c_row(r, g) ? 0.f : s[r];
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s[r] = n > a_b0 + c_row(r, g) ? 0.f : __builtin_amdgcn_exp2f(s[r]);
       dp[r] *= s[r];
       csum += dp[r];
     }
@@ -602,10 +650,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
   __shared__ __align__(16) float cn_s1[BN];
   __shared__ __align__(16) float lo_s0[BN];
   __shared__ __align__(16) float lo_s1[BN];
+  __shared__ int strong_s[2];   // whether a tile's keys need their pairs
   int item, h;
   packed_block(a, a.H, item, h);
+  const PackedItem it = a.plan.q_items[item];   // (next to their count: there is memory for as many as the launch has)
   if (item >= a.plan.counts[0]) return;
-  const PackedItem it = a.plan.q_items[item];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, i = lane & 31;
   const int M = it.m, N = it.n, p_seq = N - M, m0 = it.tile * BM;
   const int hk = h / a.group;
@@ -644,10 +693,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
       }
     };
     // at the diagonal a pair, elsewhere the start value of the score accumulators; keys past the last one get a probability of zero
-    auto store_pair = [&](float* hi, float* lo) {
+    auto store_pair = [&](float* hi, float* lo, int* strong) {   // by the first wave
       const Pair c = pair_of((cn_raw - c_ref) * kLog2eD);
+      const bool any = __any(cn_ok && fabsf(c.hi) > kStrongGates);
       hi[tid] = cn_ok ? c.hi : INFINITY;
       lo[tid] = cn_ok ? c.lo : 0.f;
+      if (tid == 0) *strong = any;
     };
     auto cn_term = [&]() { return cn_ok ? (float)(c_ref - cn_raw) * kLog2e * inv_scale : -INFINITY; };   // (the scale is positive where it is used)
     auto issue = [&](int n0, char* kt, char* vt) {
@@ -657,28 +708,29 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
     };
     issue_cn((n_tiles - 1) * BN);
     const Pair row = pair_of((c_row[min(max(a_m, 0), N - 1)] - c_ref) * kLog2eD);
-    auto compute = [&](int n0, const char* kt, const char* vt, const float* hi, const float* lo) {
+    const bool strong_rows = __any(fabsf(row.hi) > kStrongGates);
+    auto compute = [&](int n0, const char* kt, const char* vt, const float* hi, const float* lo, int strong) {
       if (n0 > a_w0 + 31 || !wave_has_rows) return;   // tile entirely above this wave's rows
-      packed_fwd_tile<Tr, D>(kt, vt, hi, lo, qreg, oacc, m_i, l_i, n0, a_m, row, qk_scale, lane);
+      packed_fwd_tile<Tr, D>(kt, vt, hi, lo, strong_rows || __builtin_amdgcn_readfirstlane(strong), qreg, oacc, m_i, l_i, n0, a_m, a_w0, row, qk_scale, lane);
     };
     // tiles at the diagonal; all of them where the pipelined code, which needs a positive scale and a few tiles, is not entered
     int n_diag = 0;
     while (n_diag < n_tiles - t_begin && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
     if (!(qk_scale > 0.f) || n_tiles - t_begin - n_diag < kMinPipelinedTiles) n_diag = n_tiles - t_begin;
     const int t_stop = n_tiles - n_diag, n_int = t_stop - t_begin;
-    if (n_diag > 0 && tid < BN) store_pair(cn_s0, lo_s0);
+    if (n_diag > 0 && tid < BN) store_pair(cn_s0, lo_s0, strong_s);
     for (int t = n_tiles - 1; t >= t_stop; t -= 2) {
       wait_vmem_all();
       __syncthreads();
       if (t - 1 >= t_stop) issue((t - 1) * BN, k_tile1, v_tile1);
-      compute(t * BN, k_tile0, v_tile0, cn_s0, lo_s0);
+      compute(t * BN, k_tile0, v_tile0, cn_s0, lo_s0, strong_s[0]);
       if (t - 1 < t_stop) break;
-      if (tid < BN) store_pair(cn_s1, lo_s1);
+      if (tid < BN) store_pair(cn_s1, lo_s1, strong_s + 1);
       wait_vmem_all();
       __syncthreads();
       if (t - 2 >= t_stop) issue((t - 2) * BN, k_tile0, v_tile0);
-      compute((t - 1) * BN, k_tile1, v_tile1, cn_s1, lo_s1);
-      if (t - 2 >= t_stop && tid < BN) store_pair(cn_s0, lo_s0);
+      compute((t - 1) * BN, k_tile1, v_tile1, cn_s1, lo_s1, strong_s[1]);
+      if (t - 2 >= t_stop && tid < BN) store_pair(cn_s0, lo_s0, strong_s);
     }
     if (n_int > 0) {   // K runs one tile ahead of V: iteration j computes S(j + 1) and P(j) V(j)
       auto int_n0 = [&](int j) { return (t_stop - 1 - j) * BN; };
@@ -778,10 +830,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
   __shared__ __align__(16) float cn_s1[BN];
   __shared__ __align__(16) float lo_s0[BN];
   __shared__ __align__(16) float lo_s1[BN];
+  __shared__ int strong_s[2];   // whether a tile's keys need their pairs
   int item, h;
   packed_block(a, a.H, item, h);
+  const PackedItem it = a.plan.q_items[item];   // (next to their count: there is memory for as many as the launch has)
   if (item >= a.plan.counts[0]) return;
-  const PackedItem it = a.plan.q_items[item];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, i = lane & 31;
   const int M = it.m, N = it.n, p_seq = N - M, m0 = it.tile * BM;
   const int hk = h / a.group;
@@ -825,10 +878,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
         cn_raw = c_row[min(n0 + tid, N - 1)];
       }
     };
-    auto store_pair = [&](float* hi, float* lo) {
+    auto store_pair = [&](float* hi, float* lo, int* strong) {   // by the first wave
       const Pair c = pair_of((cn_raw - c_ref) * kLog2eD);
+      const bool any = __any(cn_ok && fabsf(c.hi) > kStrongGates);
       hi[tid] = cn_ok ? c.hi : INFINITY;
       lo[tid] = cn_ok ? c.lo : 0.f;
+      if (tid == 0) *strong = any;
     };
     auto cn_term = [&]() { return (float)(c_ref - cn_raw) * kLog2e * inv_scale; };   // (off the diagonal every key is one)
     auto issue = [&](int n0, char* kt, char* vt) {
@@ -841,7 +896,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
     const bool row_ok = m < M && l > -INFINITY;
     Pair row = pair_of((c_m - c_ref) * kLog2eD);
     const float rowc = row_ok ? row.hi - l * kLog2e : -INFINITY;
-    row = row_ok ? Pair{row.hi, row.lo - l * kLog2e} : Pair{-INFINITY, 0.f};
+    const bool strong_rows = __any(row_ok && fabsf(row.hi) > kStrongGates);
+    row = row_ok ? less(row, l * kLog2e) : Pair{-INFINITY, 0.f};
     {
       float part = 0.f;   // each half of the wave holds half of the row
 #pragma unroll
@@ -856,12 +912,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
     n_diag = min(n_diag + (n_diag & 1), n_tiles - t_begin);
     const int t_stop = n_tiles - n_diag;
     if (tid < BN) {
-      if (n_diag > 0) store_pair(cn_s0, lo_s0);
+      if (n_diag > 0) store_pair(cn_s0, lo_s0, strong_s);
       else cn_s0[tid] = cn_term();
     }
-    auto next_terms = [&](int t, float* cn, float* lo) {   // of tile t, which has been requested
+    auto next_terms = [&](int t, float* cn, float* lo, int* strong) {   // of tile t, which has been requested
       if (tid < BN) {
-        if (t >= t_stop) store_pair(cn, lo);
+        if (t >= t_stop) store_pair(cn, lo, strong);
         else cn[tid] = cn_term();
       }
     };
@@ -869,14 +925,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
       wait_vmem_all();
       __syncthreads();
       if (t > t_begin) issue((t - 1) * BN, k_tile1, v_tile1);
-      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, lane);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[0]), qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, lane);
       if (t <= t_begin) break;
-      next_terms(t - 1, cn_s1, lo_s1);
+      next_terms(t - 1, cn_s1, lo_s1, strong_s + 1);
       wait_vmem_all();
       __syncthreads();
       if (t - 1 > t_begin) issue((t - 2) * BN, k_tile0, v_tile0);
-      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, lane);
-      if (t - 1 > t_begin) next_terms(t - 2, cn_s0, lo_s0);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[1]), qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, lane);
+      if (t - 1 > t_begin) next_terms(t - 2, cn_s0, lo_s0, strong_s);
     }
     for (int t = t_stop - 1; t >= t_begin; t -= 2) {
       wait_vmem_all();
@@ -933,16 +989,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
   __shared__ __align__(16) char q_tile1[Tile<D>::bytes(BMQ)];
   __shared__ __align__(16) char do_tile0[Tile<D>::bytes(BMQ)];
   __shared__ __align__(16) char do_tile1[Tile<D>::bytes(BMQ)];
-  __shared__ __align__(16) float rc_s0[BMQ];
-  __shared__ __align__(16) float rc_s1[BMQ];
-  __shared__ __align__(16) float lo_s0[BMQ];
-  __shared__ __align__(16) float lo_s1[BMQ];
-  __shared__ __align__(16) float dl_s0[BMQ];
-  __shared__ __align__(16) float dl_s1[BMQ];
+  __shared__ Rows rows_s0;
+  __shared__ Rows rows_s1;
   int item, hk;
   packed_block(a, a.Hk, item, hk);
-  if (item >= a.plan.counts[1]) return;
   const PackedItem it = a.plan.k_items[item];
+  if (item >= a.plan.counts[1]) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 5, i = lane & 31;
   const int M = it.m, N = it.n, p_seq = N - M, n0 = it.tile * BN;
   const uint16_t* kp = a.k.ptr + (int64_t)it.k0 * a.k.st + hk * a.k.sh;
@@ -1003,19 +1055,22 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       d_raw = a.delta[rows + mc];
     }
   };
-  // at the diagonal a pair, else the start value of the score accumulators; rows past M and those that see no key get a probability of zero
+  // the start values of the score accumulators, at the diagonal pairs as well; rows past M and those that see no key get a probability of zero
   auto on_diagonal = [&](Step s) { return p_seq + s.ms < n0 + BN - 1; };
-  auto store_rows = [&](Step s, float* rc, float* lo, float* dl) {
+  auto store_rows = [&](Step s, Rows& to) {
+    const bool ok = row_ok && l_raw > -INFINITY;
     if (row_lane) {
-      const bool ok = row_ok && l_raw > -INFINITY;
-      if (on_diagonal(s)) {
-        const Pair c = pair_of((c_raw - c_ref) * kLog2eD);
-        rc[row_slot] = ok ? c.hi : -INFINITY;
-        lo[row_slot] = ok ? c.lo - l_raw * kLog2e : 0.f;
-      } else {
-        rc[row_slot] = ok ? ((float)(c_raw - c_ref) - l_raw) * kLog2e * inv_scale : copysignf(INFINITY, -inv_scale);
+      to.rc[row_slot] = ok ? ((float)(c_raw - c_ref) - l_raw) * kLog2e * inv_scale : copysignf(INFINITY, -inv_scale);
+      to.dl[row_slot] = ok ? -d_raw : 0.f;
+    }
+    if (on_diagonal(s)) {
+      const Pair c = pair_of((c_raw - c_ref) * kLog2eD), r = less(c, l_raw * kLog2e);
+      const bool any = __any(row_lane && ok && fabsf(c.hi) > kStrongGates);
+      if (lane == 0) to.strong[wave] = any;
+      if (row_lane) {
+        to.hi[row_slot] = ok ? r.hi : -INFINITY;
+        to.lo[row_slot] = ok ? r.lo : 0.f;
       }
-      dl[row_slot] = ok ? -d_raw : 0.f;
     }
   };
   auto q_at = [&](Step s) { return a.q.ptr + head_of(s.j) * a.q.sh + (int64_t)(it.q0 + s.ms) * a.q.st; };
@@ -1031,9 +1086,15 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     for (int e = 0; e < PER; ++e) dold.issue_one(e, ds, do_bytes, dot);
   };
   Pair col{0.f, 0.f};   // of the lane's key, for the head that is being computed
+  bool strong_col = false;
   auto new_key_term = [&]() {
     col = pair_of((c_key - c_ref) * kLog2eD);
+    strong_col = __any(n < N && fabsf(col.hi) > kStrongGates);
     if (n >= N) col = {INFINITY, 0.f};
+  };
+  auto strong_of = [&](const Rows& rows) {
+    const int4 x = *reinterpret_cast<const int4*>(rows.strong);
+    return strong_col || __builtin_amdgcn_readfirstlane(x.x | x.y | x.z | x.w);
   };
   double csum = 0.0;   // (steps in 32 bits, their sum in 64, as in dQ)
   // dc of a head's keys; `more`: its other steps have left their part there
@@ -1061,7 +1122,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     };
     Step cur{j0, n_diag > 0 ? m_lo : m_top};
     issue(cur, q_tile1, do_tile1);
-    store_rows(cur, rc_s1, lo_s1, dl_s1);
+    store_rows(cur, rows_s1);
     new_key_term();
     wait_vmem_all();
     for (int t = 0;; ++t) {
@@ -1071,14 +1132,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       __syncthreads();
       if (more) issue(nx, odd ? q_tile1 : q_tile0, odd ? do_tile1 : do_tile0);
       const char *qt = odd ? q_tile0 : q_tile1, *dot = odd ? do_tile0 : do_tile1;
-      const float *rc = odd ? rc_s0 : rc_s1, *dl = odd ? dl_s0 : dl_s1;
+      const Rows& rows = odd ? rows_s0 : rows_s1;
       float sum = 0.f;
-      if (on_diagonal(cur)) packed_dkdv_step<Tr, D>(qt, dot, rc, odd ? lo_s0 : lo_s1, dl, kreg, vreg, dkacc, dvacc, sum, p_seq + cur.ms, n, n_w0, col, qk_scale, lane);
-      else dkdv_step<Tr, D>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, sum, p_seq + cur.ms, n, n_w0, qk_scale, col.hi, lane);
+      packed_dkdv_step<Tr, D>(qt, dot, rows, on_diagonal(cur) && strong_of(rows), kreg, vreg, dkacc, dvacc, sum, p_seq + cur.ms, n, n_w0, col, qk_scale, lane);
       csum += (double)sum;
       if (nx.j != cur.j) store_dc(cur.j, false);
       if (!more) break;
-      store_rows(nx, odd ? rc_s1 : rc_s0, odd ? lo_s1 : lo_s0, odd ? dl_s1 : dl_s0);
+      store_rows(nx, odd ? rows_s1 : rows_s0);
       if (nx.j != cur.j) new_key_term();
       wait_vmem_all();
       cur = nx;
@@ -1090,13 +1150,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       const Step s{j, m_lo + d * BMQ};
       if (t > 0) __syncthreads();   // buffers 1 are free again
       issue(s, q_tile1, do_tile1);
-      store_rows(s, rc_s1, lo_s1, dl_s1);
+      store_rows(s, rows_s1);
       new_key_term();
       wait_vmem_all();
       __syncthreads();
       if (t == diag_steps - 1 && n_int > 0) issue(Step{j0, m_top}, q_tile0, do_tile0);
       float sum = 0.f;
-      packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rc_s1, lo_s1, dl_s1, kreg, vreg, dkacc, dvacc, sum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
+      packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rows_s1, strong_of(rows_s1), kreg, vreg, dkacc, dvacc, sum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
       csum += (double)sum;
       if (++d == n_diag) {
         store_dc(j++, false);
@@ -1105,20 +1165,20 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     }
     if (n_int > 0) {
       if (n_diag == 0) issue(Step{j0, m_top}, q_tile0, do_tile0);
-      store_rows(Step{j0, m_top}, rc_s0, lo_s0, dl_s0);
+      store_rows(Step{j0, m_top}, rows_s0);
       new_key_term();
     }
     Step cur{j0, m_top};
     const int m_int = m_lo + n_diag * BMQ;   // first row of the interior steps
     // a step from one set of buffers, the next one's tiles into the other; an empty extent where there is none (zeros into the free buffers)
-    auto interior = [&](const char* qt, const char* dot, const float* rc, const float* dl, char* qf, char* dof, float* rcf, float* dlf, bool more) {
+    auto interior = [&](const char* qt, const char* dot, const Rows& rows, char* qf, char* dof, Rows& to, bool more) {
       const bool last = cur.ms == m_int;   // of its head
       const Step nx = last ? Step{cur.j + 1, m_top} : Step{cur.j, cur.ms - BMQ};
       if (more) issue_rows(nx);
       const uint16_t *qs = q_at(more ? nx : cur), *ds = do_at(more ? nx : cur);
       const int q_bytes = more ? qld.extent(a.q.st, nx.ms, M) : 0, do_bytes = more ? dold.extent(a.d_o.st, nx.ms, M) : 0;
       float sum = 0.f;
-      dkdv_step_interior<Tr, D, 2 * PER>(qt, dot, rc, dl, kreg, vreg, dkacc, dvacc, sum, qk_scale, col.hi, lane, [&](auto k) {
+      dkdv_step_interior<Tr, D, 2 * PER>(qt, dot, rows.rc, rows.dl, kreg, vreg, dkacc, dvacc, sum, qk_scale, col.hi, lane, [&](auto k) {
         constexpr int K = decltype(k)::value;
         if constexpr (K < PER) qld.issue_one(K, qs, q_bytes, qf);
         else dold.issue_one(K - PER, ds, do_bytes, dof);
@@ -1126,7 +1186,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       csum += (double)sum;
       if (last) store_dc(cur.j, n_diag > 0);
       if (more) {
-        store_rows(nx, rcf, nullptr, dlf);   // (off the diagonal)
+        store_rows(nx, to);
         if (last) new_key_term();
       }
       cur = nx;
@@ -1134,11 +1194,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     for (int t = 0; t < int_steps; t += 2) {
       wait_vmem_all();
       __syncthreads();
-      interior(q_tile0, do_tile0, rc_s0, dl_s0, q_tile1, do_tile1, rc_s1, dl_s1, t + 1 < int_steps);
+      interior(q_tile0, do_tile0, rows_s0, q_tile1, do_tile1, rows_s1, t + 1 < int_steps);
       if (t + 1 >= int_steps) break;
       wait_vmem_all();
       __syncthreads();
-      interior(q_tile1, do_tile1, rc_s1, dl_s1, q_tile0, do_tile0, rc_s0, dl_s0, t + 2 < int_steps);
+      interior(q_tile1, do_tile1, rows_s1, q_tile0, do_tile0, rows_s0, t + 2 < int_steps);
     }
     wait_vmem_all();   // (the last interior step requested empty tiles)
   }
@@ -1195,16 +1255,21 @@ int extra_parts(int at_once, int heads, int tiles, int64_t longest, int least) {
 
 }  // namespace
 
+// Groups of a launch over `tokens` of which an XCD reads `bytes` each: the walks of a group share its L2 as far as 8 MiB of them do (fox_kernels.hpp, order_groups).
+static int order_groups_of(int64_t tokens, int64_t bytes) {
+  return (int)std::min<int64_t>(kOrderGroups, std::max<int64_t>(1, tokens * bytes >> 23));
+}
 PackedShape packed_shape(int B, int T, int N, int H, int Hk, int D) {
   PackedShape s;
   s.q_bound = tile_bound(B, T);
   s.k_bound = tile_bound(B, N);
   s.q_extra = extra_parts((D <= 64 ? 3 : 2) * kCus, H, s.q_bound, ((int64_t)N + kFwdBN - 1) / kFwdBN, kQueryShare);
   s.k_extra = extra_parts((D <= 64 ? 2 : 1) * kCus, Hk, s.k_bound, ((int64_t)T + kKvBM - 1) / kKvBM * (H / Hk), kKeyShare);
+  s.q_groups = order_groups_of(N, ((int64_t)Hk + kXcds - 1) / kXcds * D * 4);
+  s.k_groups = order_groups_of(T, ((int64_t)H + kXcds - 1) / kXcds * D * 4);
   s.seqs_at = 256;
   const int64_t seqs = (int64_t)B + kPackedOuter;   // once for the queries, once for the keys
-  s.seq_parts_at = s.seqs_at + up(2 * seqs * sizeof(int4));
-  s.items_at = s.seq_parts_at + up(2 * seqs * sizeof(int32_t));
+  s.items_at = s.seqs_at + up(2 * seqs * sizeof(int4));
   s.plan_bytes = s.items_at + ((int64_t)s.q_bound + s.q_extra + s.k_bound + s.k_extra) * (int64_t)sizeof(PackedItem);
   const int64_t acc = (int64_t)(D + 31) / 32 * 32 * kPackedTile, q_rows = (int64_t)s.q_extra * H, k_rows = (int64_t)s.k_extra * Hk;
   s.q_arrived_at = up(q_rows * (acc + 2 * kPackedTile) * 4);
@@ -1218,10 +1283,11 @@ void packed_memory(PackedK& a, const PackedShape& s, void* plan, void* workspace
   a.q_bound = s.q_bound;
   a.k_bound = s.k_bound;
   a.q_extra = s.q_extra;
+  a.q_groups = s.q_groups;
+  a.k_groups = s.k_groups;
   a.k_extra = s.k_extra;
   a.plan.counts = (int32_t*)at;
   a.plan.seqs = (int4*)(at + s.seqs_at);
-  a.plan.seq_parts = (int32_t*)(at + s.seq_parts_at);
   a.plan.q_items = (PackedItem*)(at + s.items_at);
   a.plan.k_items = a.plan.q_items + s.q_bound + s.q_extra;
   a.q_parts = (float*)ws;
