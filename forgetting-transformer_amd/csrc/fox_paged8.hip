@@ -6,6 +6,8 @@
 // The scales that the append gives are powers of two.  x / scale is exact then, so a code is one rounding of its element (to the nearest, ties to the even one) and a block
 // whose scale has to grow is rounded again from its codes without another error; e4m3 has as many bits at any scale, whole numbers lose half a bit
 // on average against the scale that just fits.  The readers take any scales.
+#include <algorithm>
+
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
 #include "fox_paged_plan.hpp"
@@ -188,10 +190,12 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const Paged8AppendK 
 }
 
 // ---------------------------------------------------------------------------
-// Gather: the first tokens of requests out of their pages, one request after the other, in 16 bits.  A workgroup takes kGatherTokens places: their requests from a search
+// Gather: the first tokens of requests out of their pages, one request after the other, in 16 bits.  A workgroup takes eight places: their requests from a search
 // in the ends, their pages from the table, then rows of eight elements a lane, head by head, so that the codes of neighbouring tokens are read as they lie.
+// Memory bounds it where there are many tokens; few need many workgroups.  In us for 4 / 8 / 16 / 32 places: 1600 tokens, 12 heads, D 64 4.8 / 4.7 / 5.8 / 7.8, 16384 tokens, 4 key heads, D 128
+// 11.3 / 10.3 / 9.5 / 11.6, 80000 of those 40.3 / 37.5 / 37.1 / 36.7.
 // ---------------------------------------------------------------------------
-constexpr int kGatherTokens = 32;
+constexpr int kGatherTokens = 8;
 
 template <typename Tr, int CODES, int D>
 __global__ __launch_bounds__(256) void paged_gather_kernel(const PagedGatherK a, const Divisor by_heads) {
@@ -201,64 +205,65 @@ __global__ __launch_bounds__(256) void paged_gather_kernel(const PagedGatherK a,
   const int tid = threadIdx.x;
   const Pages8K& pg = a.pages;
   for (int i = tid; i <= a.B; i += 256) ends[i] = a.ends[i];
-  __syncthreads();
-  const int64_t t0 = (int64_t)blockIdx.x * TOK;
-  if (tid < TOK) {
-    const int64_t t = t0 + tid;
-    int lo = 0, hi = a.B;   // the first request whose tokens end behind t
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (ends[mid + 1] > t) hi = mid;
-      else lo = mid + 1;
-    }
-    int64_t slot = -1;
-    if (lo < a.B && t >= ends[lo]) {
-      const int64_t pos = t - ends[lo], idx = pos >> pg.shift;
-      const int who = a.requests ? a.requests[lo] : lo;
-      if ((uint32_t)who < (uint32_t)a.R && idx < a.W) {
-        const int page = a.table[who * a.table_sb + idx];
-        if ((uint32_t)page < (uint32_t)pg.P) slot = ((int64_t)page << pg.shift) + (pos & ((1 << pg.shift) - 1));
+  for (int64_t t0 = (int64_t)blockIdx.x * TOK; t0 < a.T; t0 += (int64_t)gridDim.x * TOK) {
+    __syncthreads();
+    if (tid < TOK) {
+      const int64_t t = t0 + tid;
+      int lo = 0, hi = a.B;   // the first request whose tokens end behind t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (ends[mid + 1] > t) hi = mid;
+        else lo = mid + 1;
       }
-    }
-    slot_s[tid] = slot;
-  }
-  __syncthreads();
-  const int count = (int)min((int64_t)TOK, a.T - t0);
-  for (int idx = tid; idx < PER_HEAD * a.Hk; idx += 256) {
-    const int hk = idx / PER_HEAD, in = idx % PER_HEAD, tok = in / LPR, ch = in % LPR;
-    if (tok >= count) continue;
-    const int64_t slot = slot_s[tok], from = slot < 0 ? 0 : slot;
-    const int64_t page = from >> pg.shift;
-    const int at = (int)(from & ((1 << pg.shift) - 1));
-    u32x4 out[2];
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const Pages8K::Codes& c = side ? pg.v : pg.k;
-      if constexpr (CODES == kCodesNone) {
-        out[side] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(c.ptr) + page * c.sp + hk * c.sh + at * c.st + 8 * ch);
-      } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(c.ptr + page * c.sp + hk * c.sh + at * c.st + 8 * ch);
-        const float scale = c.scale[page * c.s_sp + hk * c.s_sh + (at >> pg.block_shift) * c.s_st];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float f[4];
-          if constexpr (CODES == kCodesE4m3) E4m3::decode4(w[i], f);
-          else Int8::decode4(w[i], f);
-          out[side][2 * i] = Tr::pack2(f[0] * scale, f[1] * scale);
-          out[side][2 * i + 1] = Tr::pack2(f[2] * scale, f[3] * scale);
+      int64_t slot = -1;
+      if (lo < a.B && t >= ends[lo]) {
+        const int64_t pos = t - ends[lo], idx = pos >> pg.shift;
+        const int who = a.requests ? a.requests[lo] : lo;
+        if ((uint32_t)who < (uint32_t)a.R && idx < a.W) {
+          const int page = a.table[who * a.table_sb + idx];
+          if ((uint32_t)page < (uint32_t)pg.P) slot = ((int64_t)page << pg.shift) + (pos & ((1 << pg.shift) - 1));
         }
       }
-      if (slot < 0) out[side] = u32x4{0u, 0u, 0u, 0u};
+      slot_s[tid] = slot;
     }
-    const int64_t to = ((t0 + tok) * a.Hk + hk) * D + 8 * ch;
-    *reinterpret_cast<u32x4*>(a.k + to) = out[0];
-    *reinterpret_cast<u32x4*>(a.v + to) = out[1];
-  }
-  for (int idx = tid; idx < count * a.H; idx += 256) {
-    const int tok = divide(idx, by_heads), h = idx - tok * a.H;
-    const int64_t slot = slot_s[tok], from = slot < 0 ? 0 : slot;
-    const float g = pg.g[(from >> pg.shift) * pg.g_sp + h * pg.g_sh + (from & ((1 << pg.shift) - 1)) * pg.g_ss];
-    a.g[t0 * a.H + idx] = slot < 0 ? 0.f : g;
+    __syncthreads();
+    const int count = (int)min((int64_t)TOK, a.T - t0);
+    for (int idx = tid; idx < PER_HEAD * a.Hk; idx += 256) {
+      const int hk = idx / PER_HEAD, in = idx % PER_HEAD, tok = in / LPR, ch = in % LPR;
+      if (tok >= count) continue;
+      const int64_t slot = slot_s[tok], from = slot < 0 ? 0 : slot;
+      const int64_t page = from >> pg.shift;
+      const int at = (int)(from & ((1 << pg.shift) - 1));
+      u32x4 out[2];
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        const Pages8K::Codes& c = side ? pg.v : pg.k;
+        if constexpr (CODES == kCodesNone) {
+          out[side] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(c.ptr) + page * c.sp + hk * c.sh + at * c.st + 8 * ch);
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(c.ptr + page * c.sp + hk * c.sh + at * c.st + 8 * ch);
+          const float scale = c.scale[page * c.s_sp + hk * c.s_sh + (at >> pg.block_shift) * c.s_st];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float f[4];
+            if constexpr (CODES == kCodesE4m3) E4m3::decode4(w[i], f);
+            else Int8::decode4(w[i], f);
+            out[side][2 * i] = Tr::pack2(f[0] * scale, f[1] * scale);
+            out[side][2 * i + 1] = Tr::pack2(f[2] * scale, f[3] * scale);
+          }
+        }
+        if (slot < 0) out[side] = u32x4{0u, 0u, 0u, 0u};
+      }
+      const int64_t to = ((t0 + tok) * a.Hk + hk) * D + 8 * ch;
+      *reinterpret_cast<u32x4*>(a.k + to) = out[0];
+      *reinterpret_cast<u32x4*>(a.v + to) = out[1];
+    }
+    for (int idx = tid; idx < count * a.H; idx += 256) {
+      const int tok = divide(idx, by_heads), h = idx - tok * a.H;
+      const int64_t slot = slot_s[tok], from = slot < 0 ? 0 : slot;
+      const float g = pg.g[(from >> pg.shift) * pg.g_sp + h * pg.g_sh + (from & ((1 << pg.shift) - 1)) * pg.g_ss];
+      a.g[t0 * a.H + idx] = slot < 0 ? 0.f : g;
+    }
   }
 }
 
@@ -674,7 +679,8 @@ static hipError_t decode8_t(const Paged8DecodeK& a, int D, hipStream_t s) {
 }
 template <typename Tr, int CODES, int D>
 static hipError_t gather_d(const PagedGatherK& a, hipStream_t s) {
-  hipLaunchKernelGGL((paged_gather_kernel<Tr, CODES, D>), dim3((unsigned)(((int64_t)a.T + kGatherTokens - 1) / kGatherTokens)), dim3(256), 0, s, a, divisor(a.H));
+  const int64_t groups = ((int64_t)a.T + kGatherTokens - 1) / kGatherTokens;
+  hipLaunchKernelGGL((paged_gather_kernel<Tr, CODES, D>), dim3((unsigned)std::min<int64_t>(groups, 1 << 22)), dim3(256), 0, s, a, divisor(a.H));
   return hipGetLastError();
 }
 template <typename Tr, int CODES>
