@@ -211,15 +211,27 @@ __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
     }
     return r;
   };
-  // parts of a bucket, their first places, and each tile's among them (any order within a bucket); a wave a sequence
-  for (int b = wave; b < S; b += WAVES) {
-    const int4 s = seqs[b];
-    const int tiles = tiles_of(s);
-    for (int t = lane; t < tiles; t += 64) {
-      const Tile x = tile_of(s, t);
-      atomicAdd(&mem.buckets[x.bucket], x.parts);
+  // Every tile of every sequence: a lane takes those of a short one, the lanes of a wave those of a long one.
+  auto each_tile = [&](auto&& f) {
+    for (int b0 = 0; b0 < S; b0 += NT) {
+      const int b = b0 + lane * WAVES + wave;
+      const int4 s = b < S ? seqs[b] : make_int4(0, 0, 0, 0);
+      const int tiles = tiles_of(s);
+      constexpr int SHORT = 4;
+      for (int t = 0; t < (tiles <= SHORT ? tiles : 0); ++t) f(s, t);
+      for (uint64_t left = __ballot(tiles > SHORT); left; left &= left - 1) {
+        const int from = __builtin_ctzll(left);
+        const int4 w = make_int4(__builtin_amdgcn_readlane(s.x, from), __builtin_amdgcn_readlane(s.y, from), __builtin_amdgcn_readlane(s.z, from),
+                                 __builtin_amdgcn_readlane(s.w, from));
+        for (int t = lane, n = tiles_of(w); t < n; t += 64) f(w, t);
+      }
     }
-  }
+  };
+  // parts of a bucket, their first places, and each tile's among them (any order within a bucket)
+  each_tile([&](int4 s, int t) {
+    const Tile x = tile_of(s, t);
+    atomicAdd(&mem.buckets[x.bucket], x.parts);
+  });
   __syncthreads();
   const int own = mem.buckets[tid];
   int end = wave_sum_scan(own, lane);
@@ -227,22 +239,19 @@ __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
   __syncthreads();
   for (int w = 0; w < wave; ++w) end += mem.waves[w];
   mem.buckets[tid] = end - own;
-  if (tid == NT - 1) a.plan.counts[KEYS] = end;
+  if (tid == NT - 1) {
+    a.plan.counts[KEYS] = end;
+    if (!KEYS && !a.lse) a.plan.counts[1] = 0;   // (a backward of it all the same finds no tiles)
+  }
   __syncthreads();
   PackedItem* const items = KEYS ? a.plan.k_items : a.plan.q_items;
-  for (int b = wave; b < S; b += WAVES) {
-    const int4 s = seqs[b];
-    const int tiles = tiles_of(s);
-    PackedItem it{s.x, s.y, s.z, s.w, 0, 0, 0, 0};
-    for (int t = lane; t < tiles; t += 64) {
-      const Tile x = tile_of(s, t);
-      PackedItem* const at = items + atomicAdd(&mem.buckets[x.bucket], x.parts);
-      it.tile = t;
-      it.parts = x.parts;
-      it.slot = x.parts > 1 ? atomicAdd(&mem.slots, x.parts) : 0;
-      for (it.part = 0; it.part < x.parts; ++it.part) at[it.part] = it;
-    }
-  }
+  each_tile([&](int4 s, int t) {
+    const Tile x = tile_of(s, t);
+    PackedItem* const at = items + atomicAdd(&mem.buckets[x.bucket], x.parts);
+    PackedItem it{s.x, s.y, s.z, s.w, t, 0, x.parts, 0};
+    if (x.parts > 1) it.slot = atomicAdd(&mem.slots, x.parts);
+    for (; it.part < x.parts; ++it.part) at[it.part] = it;
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -1296,8 +1305,10 @@ void packed_memory(PackedK& a, const PackedShape& s, void* plan, void* workspace
   a.k_arrived = (uint32_t*)(ws + s.k_arrived_at);
 }
 
-// Whether a row of the scans is a wave's rather than a workgroup's: where there are more rows than workgroups of 1024 at once, and the average row has little for 1024 threads.
-static bool short_rows(int64_t elements, int rows, int heads) { return (int64_t)rows * heads > 2 * kCus && elements <= (int64_t)512 * rows; }
+// Whether a row of the scans is a wave's rather than a workgroup's of 1024.  A wave is done after some 5 + 0.008 us for each of the longest row's elements, workgroups
+// after 6 + 0.01 for each row.  (A wave / a workgroup, 16 heads, us: 64 rows of 100 elements 8.6 / 16.2, 64 of 800 11.2 / 18.6, 256 of 500 12.2 / 57.7, 32 of 500 9.1 / 10.6, 24 of 800
+// 10.2 / 9.2, 32 of 1500 16.2 / 12.9, 20 of 4000 36.2 / 14.4.)
+static bool short_rows(int64_t elements, int64_t rows, int heads) { return 2 * elements <= 3 * rows * rows * heads; }
 
 template <typename Tr, int D>
 static hipError_t packed_fwd_d(const PackedK& args, hipStream_t s) {

@@ -139,7 +139,9 @@ __device__ __forceinline__ void append_rows(const u32x4 (&x)[(16 * (D / 8) + 63)
 
 // A run is what lies in one block of consecutive slots of consecutive tokens; its first token's wave of a key head takes it whole, so that the block's scale is known before
 // a code is written and nobody waits for anybody.  A wave looks at CHUNK tokens of a head for the beginnings of runs: one token each where there are few (the next tokens
-// of a step are runs of their own), sixteen where prompts fill whole blocks.
+// of a step are runs of their own), sixteen where prompts fill whole blocks, so that few waves find nothing to do.  Few tokens are bound by their chain of loads: slots, scale, codes.
+// In us for 1 / 4 / 8 / 16 tokens a wave: runs of one token, 48 of 12 heads, D 64 4.8 / 10.5 / 17.6 / 31.9, 1024 of 4 heads, D 128 8.1 / 13.1 / 22.8 / 43.4, 4096 22.9 / 21.5 / 26.7 / 43.7; whole
+// blocks, 1024 tokens 8.8 / 6.2 / 5.9 / 5.8, 4096 27.2 / 11.4 / 6.3 / 6.3, 16384 95 / 29.5 / 17.4 / 11.4 (51 MB there: 4.5 TB/s).
 template <typename Tr, typename C, int D, int CHUNK>
 __global__ __launch_bounds__(256) void paged8_append_kernel(const Paged8AppendK a) {
   constexpr int LPR = D / 8, R = 64 / LPR, NIT = (16 + R - 1) / R;
@@ -631,7 +633,9 @@ __global__ __launch_bounds__(256, kPaged8Waves<D>) void paged8_decode_kernel(con
 template <typename Tr, typename C, int D>
 static hipError_t append_d(const Paged8AppendK& a, hipStream_t s) {
   const auto grid = [&](int chunk) { return dim3((unsigned)(((int64_t)((a.T + chunk - 1) / chunk) * a.Hk + 3) / 4)); };
-  if ((int64_t)a.T * a.Hk <= 16 * kCus) hipLaunchKernelGGL((paged8_append_kernel<Tr, C, D, 1>), grid(1), dim3(256), 0, s, a);
+  const int64_t rows = (int64_t)a.T * a.Hk;
+  if (rows <= 16 * kCus) hipLaunchKernelGGL((paged8_append_kernel<Tr, C, D, 1>), grid(1), dim3(256), 0, s, a);
+  else if (rows <= 128 * kCus) hipLaunchKernelGGL((paged8_append_kernel<Tr, C, D, 8>), grid(8), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((paged8_append_kernel<Tr, C, D, 16>), grid(16), dim3(256), 0, s, a);
   return hipGetLastError();
 }

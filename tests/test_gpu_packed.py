@@ -134,6 +134,9 @@ CASES = [  # new tokens, tokens in front, H, Hk, D, dtype, more
     ([2, 130], [6000, 10], 2, 2, 32, torch.bfloat16, {}),
     ([1], [9000], 16, 4, 16, torch.float16, {}),
     ([1500, 20], [-700, 0], 1, 1, 128, torch.bfloat16, {}),
+    # many sequences, long ones among them
+    ([3] * 130 + [900, 2, 700], [0] * 131 + [5, 300], 2, 1, 64, torch.bfloat16, dict(pad=4)),
+    ([1, 0, 2] * 400 + [600], [2, 0, 0] * 400 + [0], 2, 2, 16, torch.float16, dict(lead=2)),
 ]
 
 
