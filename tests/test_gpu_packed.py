@@ -137,6 +137,11 @@ CASES = [  # new tokens, tokens in front, H, Hk, D, dtype, more
     # many sequences, long ones among them
     ([3] * 130 + [900, 2, 700], [0] * 131 + [5, 300], 2, 1, 64, torch.bfloat16, dict(pad=4)),
     ([1, 0, 2] * 400 + [600], [2, 0, 0] * 400 + [0], 2, 2, 16, torch.float16, dict(lead=2)),
+    # gates that need their sums in two parts at the diagonal, everywhere and in some tiles
+    ([600, 300], [0, 100], 4, 2, 128, torch.bfloat16, dict(gate=-2.0)),
+    ([900], [50], 3, 1, 64, torch.bfloat16, dict(gate=-3.0)),
+    ([1000, 400], [0, 70], 4, 4, 64, torch.bfloat16, dict(gate=2.2)),
+    ([500, 300], [0, 0], 2, 1, 128, torch.float16, dict(gate=2.2)),
 ]
 
 
