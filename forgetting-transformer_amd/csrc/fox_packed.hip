@@ -495,11 +495,12 @@ __device__ __forceinline__ void packed_dq_interior(const char* k_tile, const cha
   }
 }
 
-// `row`: of the query, its log-normaliser taken off
+// `row`: of the query, its log-normaliser taken off.  `all`: the wave's rows see these 32 keys at most, so that what is missing of delta is known in time for dq too (sequences of 2 tokens,
+// D 64: dq off by 3.7e-3, now 2.4e-3; on longer walks it averages out).
 template <typename Tr, int D>
 __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, bool strong,
                                                const u32x4 (&qreg)[D / 16], const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rows, int n0, int a_m, int a_w0, Pair row,
-                                               float qk_scale, float delta, int lane) {
+                                               float qk_scale, float delta, bool all, int lane) {
   constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
   const int g = lane >> 5;
 #pragma unroll
@@ -522,6 +523,11 @@ __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v
       rsum += dp[r];
     }
     rows += rsum;
+    if (all) {
+      const float missing = half_sum(rsum);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = fmaf(-s[r], missing, dp[r]);
+    }
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       const u32x4 dsb = pack8<Tr>(dp, 8 * hh);
@@ -830,11 +836,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
 
 // ---------------------------------------------------------------------------
 // dQ: the same walk with Q and dO in registers.  It leaves delta in full for the dK/dV kernel, which runs behind it.
-// Bound by the matrix units: 8 sequences of about 3000 tokens, 16 heads, D 128 910 to 1090 TFLOP/s.  dS goes into its product in 16 bits, as P does in the forward: 2.5e-3 of dq next to the
-// 1.7e-3 of its own rounding.
+// Bound by the matrix units: 8 sequences of about 3000 tokens, 16 heads, D 128 910 to 1090 TFLOP/s.  dS goes into its product in 16 bits, as P does in the forward: 2.4e-3 of dq next to the
+// 1.7e-3 of its own rounding, 2.5e-3 with what delta is off on longer walks.
 // ---------------------------------------------------------------------------
 template <typename Tr, int D>
-__global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
+__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const PackedK a) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr int BM = kFwdBM, BN = kFwdBN, KK = D / 16, DB = (D + 31) / 32;
   __shared__ __align__(16) char k_tile0[Tile<D>::bytes(BN)];
@@ -911,7 +917,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
     const bool row_ok = m < M && l > -INFINITY;
     Pair row = pair_of((c_m - c_ref) * kLog2eD);
     const float rowc = row_ok ? row.hi - l * kLog2e : -INFINITY;
-    const bool strong_rows = __any(row_ok && fabsf(row.hi) > kStrongGates);
+    const bool strong_rows = __any(row_ok && fabsf(row.hi) > kStrongGates), few_keys = min(N, a_w0 + 32) <= 32;
     row = row_ok ? less(row, l * kLog2e) : Pair{-INFINITY, 0.f};
     {
       float part = 0.f;   // each half of the wave holds half of the row
@@ -940,13 +946,13 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(const PackedK a) {
       wait_vmem_all();
       __syncthreads();
       if (t > t_begin) issue((t - 1) * BN, k_tile1, v_tile1);
-      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[0]), qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, lane);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[0]), qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, few_keys, lane);
       if (t <= t_begin) break;
       next_terms(t - 1, cn_s1, lo_s1, strong_s + 1);
       wait_vmem_all();
       __syncthreads();
       if (t - 1 > t_begin) issue((t - 2) * BN, k_tile0, v_tile0);
-      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[1]), qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, lane);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[1]), qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, few_keys, lane);
       if (t - 1 > t_begin) next_terms(t - 2, cn_s0, lo_s0, strong_s);
     }
     for (int t = t_stop - 1; t >= t_begin; t -= 2) {

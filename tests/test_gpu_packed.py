@@ -187,6 +187,29 @@ def test_packed_closed_gates(D, dtype):
     check(x, cu_q, cu_k, D ** -0.5, [out.detach(), *torch.autograd.grad(out, leaves, x[4])], dtype)
 
 
+@pytest.mark.parametrize("D,dtype", [(16, torch.bfloat16), (64, torch.float16), (128, torch.bfloat16)])
+def test_packed_dq_of_few_keys(D, dtype):
+    """Rows that see up to 32 keys: dq within its own rounding and that of ds, without the part of the module's bound that comes from the rounded o."""
+    from forgetting_transformer import forgetting_attention_packed
+    new = [2, 1, 3, 32, 7, 2, 20, 100, 2, 31]
+    *x, cu_q, cu_k = inputs(new, [0] * len(new), 4, 2, D, dtype, seed=31)
+    leaves = [t.detach().requires_grad_() for t in x[:4]]
+    got = torch.autograd.grad(forgetting_attention_packed(*leaves, cu_q), leaves, x[4])[0]
+    u, scale, ends = torch.finfo(dtype).eps / 2, D ** -0.5, cu_q.tolist()
+    for at, n in zip(ends, new):
+        r = slice(at, at + min(n, 32))
+        q, k, v, f, do = (t[r] for t in x)
+        want, _, _, small, noise = sequence(q, k, v, f, do, scale)
+        q, do, k, v = (t.double().transpose(0, 1).repeat_interleave(4 // t.shape[1], 0) for t in (q, do, k, v))
+        c = f.double().cumsum(0).t()
+        s = (torch.matmul(q, k.transpose(-1, -2)) * scale + c[..., None] - c[:, None]).masked_fill(~torch.ones(len(c[0]), len(c[0]), dtype=torch.bool, device="cuda").tril(), -math.inf)
+        p, dp = torch.softmax(s, -1), torch.matmul(do, v.transpose(-1, -2))
+        ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+        bound = (u + 2.0 ** -14) * (want[1].abs() + scale * torch.matmul(ds.abs(), k.abs()).transpose(0, 1)) + noise[1] + (small[1] if dtype == torch.float16 else 0.0) + 1e-30
+        err = (got[r].double() - want[1]).abs()
+        assert (err <= bound).all(), (n, (err / bound).max().item())
+
+
 def test_packed_gradients_against_differences():
     """The kernels' gradients along directions against central differences of the forward's formula in 64 bits."""
     from forgetting_transformer import forgetting_attention_packed
