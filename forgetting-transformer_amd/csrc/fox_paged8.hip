@@ -322,8 +322,10 @@ template <int D> constexpr int kPaged8Keys = D >= 64 ? 32 : 64;
 template <int D> constexpr int kPaged8Waves = D >= 128 ? 3 : 4;
 
 // VECTORS: four gates of consecutive tokens are read at once.  (Where the kernel chooses at run time nobody knows how many loads are on their way, and every step waits for all.)
-template <typename Tr, typename C, int D, bool VECTORS>
-__global__ __launch_bounds__(256, kPaged8Waves<D>) void paged8_decode_kernel(const Paged8DecodeK a8) {
+// WAVES: four with runs of whole batches, pieces of a row for several workgroups; or one workgroup for a row, of as many waves as the registers allow, each with its share of the steps.
+template <int D> constexpr int kPaged8RowWaves = D >= 128 ? 8 : 16;
+template <typename Tr, typename C, int D, bool VECTORS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 4 ? kPaged8Waves<D> : WAVES / 4) void paged8_decode_kernel(const Paged8DecodeK a8) {
   constexpr int KEYS = kPaged8Keys<D>, NT = KEYS / 16;   // tiles of sixteen keys
   constexpr int STEPS = paged_batch(D) / 4 / KEYS;       // of a wave's batch
   constexpr int LB = D >= 64 ? 16 : 8;         // codes a lane loads at once
@@ -335,10 +337,10 @@ __global__ __launch_bounds__(256, kPaged8Waves<D>) void paged8_decode_kernel(con
   constexpr int AS = D + 4;                    // floats of a head's accumulator at the merge, where it takes the place of V
   static_assert(16 * AS * 4 <= 32 * RS, "a wave's accumulators fit where its V was");
   constexpr int KRS = D + 16;                  // bytes from one key to the next where K goes through LDS
-  __shared__ __align__(16) char v_s[4][32 * RS];
+  __shared__ __align__(16) char v_s[WAVES][32 * RS];
   static_assert(!LINES || KEYS * KRS <= 32 * RS, "K passes through the place of V, before V");
-  __shared__ float part_m[4][16], part_l[4][16];
-  __shared__ double part_g[4][16];
+  __shared__ float part_m[WAVES][16], part_l[WAVES][16];
+  __shared__ double part_g[WAVES][16];
 
   const PagedDecodeK& a = a8.row;
   const Pages8K& pg = a8.pages;
@@ -360,8 +362,17 @@ __global__ __launch_bounds__(256, kPaged8Waves<D>) void paged8_decode_kernel(con
   const uint32_t ks_sp = (uint32_t)pg.k.s_sp, ks_st = (uint32_t)pg.k.s_st, vs_sp = (uint32_t)pg.v.s_sp, vs_st = (uint32_t)pg.v.s_st;
 
   // run of this wave in steps, from the last
-  const int keys = at.share.keys, all = (keys + KEYS * STEPS - 1) / (KEYS * STEPS), per = at.share.batches;
-  const int b1 = max(all - (at.piece * 4 + wave) * per, 0), s0 = max(b1 - per, 0) * STEPS, s1 = min(b1 * STEPS, (keys + KEYS - 1) / KEYS);
+  const int keys = at.share.keys, steps = (keys + KEYS - 1) / KEYS;
+  int s0, s1;
+  if constexpr (WAVES == 4) {
+    const int all = (keys + KEYS * STEPS - 1) / (KEYS * STEPS), per = at.share.batches, b1 = max(all - (at.piece * 4 + wave) * per, 0);
+    s0 = max(b1 - per, 0) * STEPS;
+    s1 = min(b1 * STEPS, steps);
+  } else {
+    const int per = (steps + WAVES - 1) / WAVES;
+    s1 = max(steps - wave * per, 0);
+    s0 = max(s1 - per, 0);
+  }
 
   // element e of k-step s of a lane is number elem0(s) + e of its row
   auto elem0 = [&](int s) { return D >= 64 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 8 * g; };
@@ -601,12 +612,12 @@ __global__ __launch_bounds__(256, kPaged8Waves<D>) void paged8_decode_kernel(con
   for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(v_tile + (i16 * AS + 16 * d + 4 * g) * 4) = acc[d];
   __syncthreads();
   constexpr int CPH = D / 4;   // threads of a head, four elements each
-  for (int idx = tid; idx < heads * CPH; idx += 256) {
+  for (int idx = tid; idx < heads * CPH; idx += 64 * WAVES) {
     const int j = idx / CPH, d = idx % CPH * 4, h = h0 + j;
-    float mw[4], top = part_m[0][j];
+    float mw[WAVES], top = part_m[0][j];
     double shift = 0.0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       mw[w] = part_m[w][j] + (float)shift * kLog2e;
       shift += part_g[w][j];
       top = fmaxf(top, mw[w]);
@@ -614,7 +625,7 @@ __global__ __launch_bounds__(256, kPaged8Waves<D>) void paged8_decode_kernel(con
     float lt = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float weight = __builtin_amdgcn_exp2f(mw[w] - top);
       lt += part_l[w][j] * weight;
       o += *reinterpret_cast<const f32x4*>(v_s[w] + (j * AS + d) * 4) * weight;
@@ -642,9 +653,24 @@ static hipError_t append_d(const Paged8AppendK& a, hipStream_t s) {
   else hipLaunchKernelGGL((paged8_append_kernel<Tr, C, D, 16>), grid(16), dim3(256), 0, s, a);
   return hipGetLastError();
 }
+// Whether rows stay whole, a large workgroup each and no merge behind.  That takes some 4.7 us and 0.07 us for each 1000 elements of a row's keys, while there are CUs for all rows; in pieces it is
+// 11 us and what the bytes of all rows take.  (Whole / pieces, us: D 64, 12 rows of 500 keys 7.1 / 10.3, of 1500 11.9 / 10.9, 96 of 1500 12.4 / 13.3, 240 of 1500 13.2 / 20.8, 384 23.5 / 27.9, 576
+// 34.4 / 33.4; D 128, 32 rows of 500 9.0 / 11.2, of 1000 12.6 / 11.1, 256 of 1500 20.5 / 28.6.)  What the host knows is the longest a row can be, so very long rows are left to pieces: others may be short.
+static bool whole_rows(const Paged8DecodeK& a, int D) {
+  const int64_t rows = (int64_t)a.row.B * a.row.H, elements = (int64_t)a.row.max_keys * D;
+  return rows <= kCus && elements <= 1 << 18 && elements * (200 - rows) <= 17000000;
+}
 template <typename Tr, typename C, int D>
 static hipError_t decode8_d(const Paged8DecodeK& args, hipStream_t s) {
   Paged8DecodeK a = args;
+  if (whole_rows(a, D)) {
+    a.row.ws_row = nullptr;
+    constexpr int WAVES = kPaged8RowWaves<D>;
+    const dim3 rows((unsigned)(a.row.B * a.row.H));
+    if (a.gates_in_vectors) hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, true, WAVES>), rows, dim3(64 * WAVES), 0, s, a);
+    else hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, false, WAVES>), rows, dim3(64 * WAVES), 0, s, a);
+    return hipGetLastError();
+  }
   a.row.per_piece = 1.0 / kPagedPieces;
   a.row.batch_us = 5.f;
   a.row.planned = plan_ahead(a.row);
@@ -653,8 +679,8 @@ static hipError_t decode8_d(const Paged8DecodeK& args, hipStream_t s) {
     if (e != hipSuccess) return e;
   }
   const dim3 grid((unsigned)paged_decode_workgroups(a.row.B, a.row.H, a.row.max_keys, D));
-  if (a.gates_in_vectors) hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, false>), grid, dim3(256), 0, s, a);
+  if (a.gates_in_vectors) hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, true, 4>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((paged8_decode_kernel<Tr, C, D, false, 4>), grid, dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || most_pieces(a.row.max_keys, D) <= 1) return e;
   PagedDecodeK m = a.row;   // the merge goes by query heads

@@ -273,6 +273,8 @@ CASES = [  # B, H, Hk, D, S, W, lengths, codes, dtype, layout
     (1, 1, 1, 16, 8, 1, [1], "e4m3", torch.bfloat16, "apart"), (3, 2, 2, 32, 8, 4, [0, 1, 32], "int8", torch.float16, "between"),
     (4, 6, 3, 64, 16, 20, [5, 16, 17, 320], "e4m3", torch.bfloat16, "inside"), (2, 12, 12, 64, 16, 100, [1500, 1], "int8", torch.bfloat16, "apart"),
     (2, 8, 4, 128, 64, 40, [2560, 2499], "e4m3", torch.float16, "between"), (5, 4, 1, 16, 16, 200, [3200, 0, 7, 1024, 1025], "int8", torch.float16, "inside"),
+    (5, 4, 1, 16, 16, 1200, [18000, 0, 7, 1024, 1025], "int8", torch.float16, "inside"), (3, 12, 4, 64, 32, 20, [0, 1, 640], "e4m3", torch.float16, "between"),
+    (4, 20, 1, 128, 16, 30, [480, 33, 32, 257], "int8", torch.bfloat16, "apart"), (256, 1, 1, 128, 16, 20, None, "e4m3", torch.bfloat16, "inside"),
     (1, 40, 2, 128, 4096, 3, [9001], "e4m3", torch.bfloat16, "apart"), (70, 2, 1, 32, 32, 30, None, "e4m3", torch.bfloat16, "apart"),
     (130, 1, 1, 64, 8, 90, None, "int8", torch.float16, "between"), (1, 17, 1, 128, 32, 700, [22400], "int8", torch.bfloat16, "apart"),
     (6, 32, 2, 128, 256, 4, None, "e4m3", torch.bfloat16, "inside"), (300, 3, 3, 16, 8, 40, None, "e4m3", torch.float16, "apart"),
