@@ -22,6 +22,7 @@
 // - o.do is off by the rounding of o and of P; what is missing of delta is sum_j P_ij (dP_ij - o.do), which the dQ kernel has at its end.  It stores
 //   the sum of the two for the dK/dV kernel.
 #include <algorithm>
+#include <cmath>
 
 #include "fox_common.hpp"
 #include "fox_kernels.hpp"
@@ -37,6 +38,8 @@ static_assert(kPackedTile == kFwdBM && kPackedTile == kKvBN && kKvBM == kKvBN, "
 constexpr float kLowestGate = -1e6f;
 // Shares below which no walk is cut, in 64 keys and 128 rows of a head.
 constexpr int kQueryShare = 4, kKeyShare = 4, kNoShare = 0x7fffffff;
+// Parts for a share of units, at most, in halves: three from two shares on, four from one on.
+constexpr int kQueryOver = 3, kKeyOver = 4;
 
 // ---------------------------------------------------------------------------
 // Plan
@@ -188,7 +191,7 @@ __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
   // 150 to 2048 tokens 34.8 / 36.0 and 44.1 / 45.9.  dK/dV of those, whose workgroups are fewer and walk in longer steps: 63.6 / 49.0.)
   Share share{kNoShare, 0.f};
   if (extra > 0) {
-    const unsigned long long u = max((2 * mem.units + extra - 1) / extra, (unsigned long long)(KEYS ? kKeyShare : kQueryShare));
+    const unsigned long long u = max(((KEYS ? kKeyOver : kQueryOver) * mem.units / 2 + extra) / extra, (unsigned long long)(KEYS ? kKeyShare : kQueryShare));
     share.whole = (int)min(KEYS ? u : 2 * u, (unsigned long long)kNoShare);
     share.inverse = 1.0f / (float)u;
   }
@@ -1269,10 +1272,12 @@ int tile_bound(int B, int rows) {
   return (int)(rows / kPackedTile + partial);
 }
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-// More parts than tiles, at most: twice as many as workgroups run at once for a head, none where the longest walk there can be stays whole.
-int extra_parts(int at_once, int heads, int tiles, int64_t longest, int least) {
-  const int64_t target = at_once / heads, most = tiles * longest / least * 2;
-  return target < 2 || longest <= least ? 0 : (int)(2 * target < most ? 2 * target : most);
+// Parts of cut walks, at most: `over` halves as many as workgroups run at once for a head (each walk's last part may be a short one), or as come of walks of `longest` units, and of `units` in all, in
+// shares of at least `least`; none where the longest walk there can be stays whole.  Each costs a workgroup that may find nothing to do.
+int extra_parts(int at_once, int heads, int over, int64_t tiles, int64_t longest, double units, int least) {
+  const int64_t target = at_once / heads;
+  if (target < 2 || longest <= least) return 0;
+  return (int)std::min({(double)(over * target / 2), std::floor((double)tiles * std::sqrt((double)longest)), std::floor(over * units / (2.0 * least)) + 1.0});
 }
 
 }  // namespace
@@ -1285,8 +1290,10 @@ PackedShape packed_shape(int B, int T, int N, int H, int Hk, int D) {
   PackedShape s;
   s.q_bound = tile_bound(B, T);
   s.k_bound = tile_bound(B, N);
-  s.q_extra = extra_parts((D <= 64 ? 3 : 2) * kCus, H, s.q_bound, ((int64_t)N + kFwdBN - 1) / kFwdBN, kQueryShare);
-  s.k_extra = extra_parts((D <= 64 ? 2 : 1) * kCus, Hk, s.k_bound, ((int64_t)T + kKvBM - 1) / kKvBM * (H / Hk), kKeyShare);
+  const int64_t q_tiles = ((int64_t)T + kPackedTile - 1) / kPackedTile, k_tiles = ((int64_t)N + kPackedTile - 1) / kPackedTile, k_steps = ((int64_t)N + kFwdBN - 1) / kFwdBN;
+  // (a sequence has at most all whole tiles, and the others' keys add up to all)
+  s.q_extra = extra_parts((D <= 64 ? 3 : 2) * kCus, H, kQueryOver, s.q_bound, k_steps, (double)(q_tiles + 1) * (double)(k_steps + B), kQueryShare);
+  s.k_extra = extra_parts((D <= 64 ? 2 : 1) * kCus, Hk, kKeyOver, s.k_bound, q_tiles * (H / Hk), (double)(k_tiles + 1) * (double)(q_tiles + B) * (H / Hk), kKeyShare);
   s.q_groups = order_groups_of(N, ((int64_t)Hk + kXcds - 1) / kXcds * D * 4);
   s.k_groups = order_groups_of(T, ((int64_t)H + kXcds - 1) / kXcds * D * 4);
   s.seqs_at = 256;
