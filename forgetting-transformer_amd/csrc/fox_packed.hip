@@ -378,15 +378,6 @@ __device__ __forceinline__ Pair pair_of(double x) {
 }
 constexpr double kLog2eD = 1.4426950408889634074;
 
-// x - y, y a number of 32 bits: the upper half's rounding goes to the lower one.
-__device__ __forceinline__ Pair less(Pair x, float y) {
-  const float hi = x.hi - y, b = hi - x.hi;
-  return {hi, x.lo + ((x.hi - (hi - b)) - (y + b))};
-}
-// Sums of gates, in log2 units from the tile's reference on, up to which their upper halves alone are good enough: a bias is off by 2^-19 then.  (A training step of eight documents
-// of 768 tokens, D 64: 124 us with pairs everywhere.)
-constexpr float kStrongGates = 32.f;
-
 // x[r] = s[r] scale + (row - column) with the pairs of rows (or columns) c_row(r, g) in LDS; sign -1: LDS holds the columns.
 template <int SIGN>
 __device__ __forceinline__ void add_pairs(f32x16& s, const float* hi_s, const float* lo_s, int at, int g, Pair own, float scale) {
@@ -399,18 +390,6 @@ __device__ __forceinline__ void add_pairs(f32x16& s, const float* hi_s, const fl
     __builtin_amdgcn_sched_barrier(0);
   }
 }
-// The same; the columns' upper halves alone where no gate is strong.
-__device__ __forceinline__ void add_bias(f32x16& s, const float* hi_s, const float* lo_s, int at, int g, Pair own, float scale, bool strong) {
-  if (strong) return add_pairs<-1>(s, hi_s, lo_s, at, g, own, scale);
-#pragma unroll
-  for (int q4 = 0; q4 < 4; ++q4) {
-    const f32x4 hi = *reinterpret_cast<const f32x4*>(&hi_s[at + 8 * q4 + 4 * g]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[4 * q4 + e] = fmaf(s[4 * q4 + e], scale, own.hi - hi[e]);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-}
-
 template <typename Tr, int D>
 __device__ __forceinline__ f32x16 dots(const char* tile, int row0, const u32x4 (&reg)[D / 16], f32x16 s, int lane) {
   const int g = lane >> 5, i = lane & 31;
@@ -427,7 +406,7 @@ __device__ __forceinline__ f32x16 splat(float x) {
 
 // A running maximum and sum for every 32 keys: those above the rows of the wave cost nothing, and only those at the diagonal are masked.
 template <typename Tr, int D>
-__device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, bool strong, const u32x4 (&qreg)[D / 16],
+__device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, const u32x4 (&qreg)[D / 16],
                                                 f32x16 (&oacc)[(D + 31) / 32], float& m_i, float& l_i, int n0, int a_m, int a_w0, Pair row, float qk_scale, int lane) {
   constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
   const int g = lane >> 5;
@@ -436,7 +415,7 @@ __device__ __forceinline__ void packed_fwd_tile(const char* k_tile, const char* 
     const int nb0 = n0 + 32 * nb;
     if (nb0 > a_w0 + 31) continue;
     f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
-    add_bias(s, hi_s, lo_s, 32 * nb, g, row, qk_scale, strong);
+    add_pairs<-1>(s, hi_s, lo_s, 32 * nb, g, row, qk_scale);
     if (nb0 + 31 > a_w0) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = nb0 + c_row(r, g) > a_m ? -INFINITY : s[r];
@@ -501,7 +480,7 @@ __device__ __forceinline__ void packed_dq_interior(const char* k_tile, const cha
 // `row`: of the query, its log-normaliser taken off.  `all`: the wave's rows see these 32 keys at most, so that what is missing of delta is known in time for dq too (sequences of 2 tokens,
 // D 64: dq off by 3.7e-3, now 2.4e-3; on longer walks it averages out).
 template <typename Tr, int D>
-__device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s, bool strong,
+__device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v_tile, const float* hi_s, const float* lo_s,
                                                const u32x4 (&qreg)[D / 16], const u32x4 (&doreg)[D / 16], f32x16 (&dqacc)[(D + 31) / 32], float& rows, int n0, int a_m, int a_w0, Pair row,
                                                float qk_scale, float delta, bool all, int lane) {
   constexpr int BN = kFwdBN, DB = (D + 31) / 32, NB = BN / 32;
@@ -511,7 +490,7 @@ __device__ __forceinline__ void packed_dq_tile(const char* k_tile, const char* v
     const int nb0 = n0 + 32 * nb;
     if (nb0 > a_w0 + 31) continue;   // entirely above this wave's rows
     f32x16 s = dots<Tr, D>(k_tile, 32 * nb, qreg, splat(0.f), lane);
-    add_bias(s, hi_s, lo_s, 32 * nb, g, row, qk_scale, strong);
+    add_pairs<-1>(s, hi_s, lo_s, 32 * nb, g, row, qk_scale);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r]);
     if (nb0 + 31 > a_w0) {
@@ -545,11 +524,10 @@ struct Rows {                          // of a step of dK/dV in LDS, log-normali
   alignas(16) float hi[kKvBM];         // at the diagonal: pairs
   alignas(16) float lo[kKvBM];
   alignas(16) float dl[kKvBM];         // -delta
-  alignas(16) int strong[4];           // whether those of a wave need their pairs
 };
 
 template <typename Tr, int D>
-__device__ __forceinline__ void packed_dkdv_step(const char* q_tile, const char* do_tile, const Rows& rows, bool strong, const u32x4 (&kreg)[D / 16], const u32x4 (&vreg)[D / 16],
+__device__ __forceinline__ void packed_dkdv_step(const char* q_tile, const char* do_tile, const Rows& rows, bool diagonal, const u32x4 (&kreg)[D / 16], const u32x4 (&vreg)[D / 16],
                                                  f32x16 (&dkacc)[(D + 31) / 32], f32x16 (&dvacc)[(D + 31) / 32], float& csum, int a_s0, int n, int n_w0, Pair col,
                                                  float qk_scale, int lane) {
   constexpr int DB = (D + 31) / 32, MB = kKvBM / 32;
@@ -559,7 +537,7 @@ __device__ __forceinline__ void packed_dkdv_step(const char* q_tile, const char*
     const int a_b0 = a_s0 + 32 * mb;
     if (a_b0 + 31 < n_w0) continue;   // entirely above the diagonal for this wave
     f32x16 s;
-    if (strong) {
+    if (diagonal) {
       s = dots<Tr, D>(q_tile, 32 * mb, kreg, splat(0.f), lane);
       add_pairs<1>(s, rows.hi, rows.lo, 32 * mb, g, col, qk_scale);
     } else {
@@ -672,7 +650,6 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
   __shared__ __align__(16) float cn_s1[BN];
   __shared__ __align__(16) float lo_s0[BN];
   __shared__ __align__(16) float lo_s1[BN];
-  __shared__ int strong_s[2];   // whether a tile's keys need their pairs
   int item, h;
   packed_block(a, a.H, item, h);
   const PackedItem it = a.plan.q_items[item];   // (next to their count: there is memory for as many as the launch has)
@@ -715,12 +692,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
       }
     };
     // at the diagonal a pair, elsewhere the start value of the score accumulators; keys past the last one get a probability of zero
-    auto store_pair = [&](float* hi, float* lo, int* strong) {   // by the first wave
+    auto store_pair = [&](float* hi, float* lo) {
       const Pair c = pair_of((cn_raw - c_ref) * kLog2eD);
-      const bool any = __any(cn_ok && fabsf(c.hi) > kStrongGates);
       hi[tid] = cn_ok ? c.hi : INFINITY;
       lo[tid] = cn_ok ? c.lo : 0.f;
-      if (tid == 0) *strong = any;
     };
     auto cn_term = [&]() { return cn_ok ? (float)(c_ref - cn_raw) * kLog2e * inv_scale : -INFINITY; };   // (the scale is positive where it is used)
     auto issue = [&](int n0, char* kt, char* vt) {
@@ -730,29 +705,28 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_fwd_kernel(const 
     };
     issue_cn((n_tiles - 1) * BN);
     const Pair row = pair_of((c_row[min(max(a_m, 0), N - 1)] - c_ref) * kLog2eD);
-    const bool strong_rows = __any(fabsf(row.hi) > kStrongGates);
-    auto compute = [&](int n0, const char* kt, const char* vt, const float* hi, const float* lo, int strong) {
+    auto compute = [&](int n0, const char* kt, const char* vt, const float* hi, const float* lo) {
       if (n0 > a_w0 + 31 || !wave_has_rows) return;   // tile entirely above this wave's rows
-      packed_fwd_tile<Tr, D>(kt, vt, hi, lo, strong_rows || __builtin_amdgcn_readfirstlane(strong), qreg, oacc, m_i, l_i, n0, a_m, a_w0, row, qk_scale, lane);
+      packed_fwd_tile<Tr, D>(kt, vt, hi, lo, qreg, oacc, m_i, l_i, n0, a_m, a_w0, row, qk_scale, lane);
     };
     // tiles at the diagonal; all of them where the pipelined code, which needs a positive scale and a few tiles, is not entered
     int n_diag = 0;
     while (n_diag < n_tiles - t_begin && (n_tiles - 1 - n_diag) * BN + BN - 1 > a0) ++n_diag;
     if (!(qk_scale > 0.f) || n_tiles - t_begin - n_diag < kMinPipelinedTiles) n_diag = n_tiles - t_begin;
     const int t_stop = n_tiles - n_diag, n_int = t_stop - t_begin;
-    if (n_diag > 0 && tid < BN) store_pair(cn_s0, lo_s0, strong_s);
+    if (n_diag > 0 && tid < BN) store_pair(cn_s0, lo_s0);
     for (int t = n_tiles - 1; t >= t_stop; t -= 2) {
       wait_vmem_all();
       __syncthreads();
       if (t - 1 >= t_stop) issue((t - 1) * BN, k_tile1, v_tile1);
-      compute(t * BN, k_tile0, v_tile0, cn_s0, lo_s0, strong_s[0]);
+      compute(t * BN, k_tile0, v_tile0, cn_s0, lo_s0);
       if (t - 1 < t_stop) break;
-      if (tid < BN) store_pair(cn_s1, lo_s1, strong_s + 1);
+      if (tid < BN) store_pair(cn_s1, lo_s1);
       wait_vmem_all();
       __syncthreads();
       if (t - 2 >= t_stop) issue((t - 2) * BN, k_tile0, v_tile0);
-      compute((t - 1) * BN, k_tile1, v_tile1, cn_s1, lo_s1, strong_s[1]);
-      if (t - 2 >= t_stop && tid < BN) store_pair(cn_s0, lo_s0, strong_s);
+      compute((t - 1) * BN, k_tile1, v_tile1, cn_s1, lo_s1);
+      if (t - 2 >= t_stop && tid < BN) store_pair(cn_s0, lo_s0);
     }
     if (n_int > 0) {   // K runs one tile ahead of V: iteration j computes S(j + 1) and P(j) V(j)
       auto int_n0 = [&](int j) { return (t_stop - 1 - j) * BN; };
@@ -854,7 +828,6 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const P
   __shared__ __align__(16) float cn_s1[BN];
   __shared__ __align__(16) float lo_s0[BN];
   __shared__ __align__(16) float lo_s1[BN];
-  __shared__ int strong_s[2];   // whether a tile's keys need their pairs
   int item, h;
   packed_block(a, a.H, item, h);
   const PackedItem it = a.plan.q_items[item];   // (next to their count: there is memory for as many as the launch has)
@@ -902,12 +875,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const P
         cn_raw = c_row[min(n0 + tid, N - 1)];
       }
     };
-    auto store_pair = [&](float* hi, float* lo, int* strong) {   // by the first wave
+    auto store_pair = [&](float* hi, float* lo) {
       const Pair c = pair_of((cn_raw - c_ref) * kLog2eD);
-      const bool any = __any(cn_ok && fabsf(c.hi) > kStrongGates);
       hi[tid] = cn_ok ? c.hi : INFINITY;
       lo[tid] = cn_ok ? c.lo : 0.f;
-      if (tid == 0) *strong = any;
     };
     auto cn_term = [&]() { return (float)(c_ref - cn_raw) * kLog2e * inv_scale; };   // (off the diagonal every key is one)
     auto issue = [&](int n0, char* kt, char* vt) {
@@ -920,8 +891,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const P
     const bool row_ok = m < M && l > -INFINITY;
     Pair row = pair_of((c_m - c_ref) * kLog2eD);
     const float rowc = row_ok ? row.hi - l * kLog2e : -INFINITY;
-    const bool strong_rows = __any(row_ok && fabsf(row.hi) > kStrongGates), few_keys = min(N, a_w0 + 32) <= 32;
-    row = row_ok ? less(row, l * kLog2e) : Pair{-INFINITY, 0.f};
+    const bool few_keys = min(N, a_w0 + 32) <= 32;
+    row = row_ok ? Pair{row.hi, row.lo - l * kLog2e} : Pair{-INFINITY, 0.f};
     {
       float part = 0.f;   // each half of the wave holds half of the row
 #pragma unroll
@@ -936,12 +907,12 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const P
     n_diag = min(n_diag + (n_diag & 1), n_tiles - t_begin);
     const int t_stop = n_tiles - n_diag;
     if (tid < BN) {
-      if (n_diag > 0) store_pair(cn_s0, lo_s0, strong_s);
+      if (n_diag > 0) store_pair(cn_s0, lo_s0);
       else cn_s0[tid] = cn_term();
     }
-    auto next_terms = [&](int t, float* cn, float* lo, int* strong) {   // of tile t, which has been requested
+    auto next_terms = [&](int t, float* cn, float* lo) {   // of tile t, which has been requested
       if (tid < BN) {
-        if (t >= t_stop) store_pair(cn, lo, strong);
+        if (t >= t_stop) store_pair(cn, lo);
         else cn[tid] = cn_term();
       }
     };
@@ -949,14 +920,14 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const P
       wait_vmem_all();
       __syncthreads();
       if (t > t_begin) issue((t - 1) * BN, k_tile1, v_tile1);
-      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[0]), qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, few_keys, lane);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile0, v_tile0, cn_s0, lo_s0, qreg, doreg, dqacc, rsum, t * BN, a_m, a_w0, row, qk_scale, delta, few_keys, lane);
       if (t <= t_begin) break;
-      next_terms(t - 1, cn_s1, lo_s1, strong_s + 1);
+      next_terms(t - 1, cn_s1, lo_s1);
       wait_vmem_all();
       __syncthreads();
       if (t - 1 > t_begin) issue((t - 2) * BN, k_tile0, v_tile0);
-      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, strong_rows || __builtin_amdgcn_readfirstlane(strong_s[1]), qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, few_keys, lane);
-      if (t - 1 > t_begin) next_terms(t - 2, cn_s0, lo_s0, strong_s);
+      if (wave_has_rows) packed_dq_tile<Tr, D>(k_tile1, v_tile1, cn_s1, lo_s1, qreg, doreg, dqacc, rsum, (t - 1) * BN, a_m, a_w0, row, qk_scale, delta, few_keys, lane);
+      if (t - 1 > t_begin) next_terms(t - 2, cn_s0, lo_s0);
     }
     for (int t = t_stop - 1; t >= t_begin; t -= 2) {
       wait_vmem_all();
@@ -1089,12 +1060,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       to.dl[row_slot] = ok ? -d_raw : 0.f;
     }
     if (on_diagonal(s)) {
-      const Pair c = pair_of((c_raw - c_ref) * kLog2eD), r = less(c, l_raw * kLog2e);
-      const bool any = __any(row_lane && ok && fabsf(c.hi) > kStrongGates);
-      if (lane == 0) to.strong[wave] = any;
+      const Pair c = pair_of((c_raw - c_ref) * kLog2eD);
       if (row_lane) {
-        to.hi[row_slot] = ok ? r.hi : -INFINITY;
-        to.lo[row_slot] = ok ? r.lo : 0.f;
+        to.hi[row_slot] = ok ? c.hi : -INFINITY;
+        to.lo[row_slot] = ok ? c.lo - l_raw * kLog2e : 0.f;
       }
     }
   };
@@ -1111,15 +1080,9 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
     for (int e = 0; e < PER; ++e) dold.issue_one(e, ds, do_bytes, dot);
   };
   Pair col{0.f, 0.f};   // of the lane's key, for the head that is being computed
-  bool strong_col = false;
   auto new_key_term = [&]() {
     col = pair_of((c_key - c_ref) * kLog2eD);
-    strong_col = __any(n < N && fabsf(col.hi) > kStrongGates);
     if (n >= N) col = {INFINITY, 0.f};
-  };
-  auto strong_of = [&](const Rows& rows) {
-    const int4 x = *reinterpret_cast<const int4*>(rows.strong);
-    return strong_col || __builtin_amdgcn_readfirstlane(x.x | x.y | x.z | x.w);
   };
   double csum = 0.0;   // (steps in 32 bits, their sum in 64, as in dQ)
   // dc of a head's keys; `more`: its other steps have left their part there
@@ -1159,7 +1122,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       const char *qt = odd ? q_tile0 : q_tile1, *dot = odd ? do_tile0 : do_tile1;
       const Rows& rows = odd ? rows_s0 : rows_s1;
       float sum = 0.f;
-      packed_dkdv_step<Tr, D>(qt, dot, rows, on_diagonal(cur) && strong_of(rows), kreg, vreg, dkacc, dvacc, sum, p_seq + cur.ms, n, n_w0, col, qk_scale, lane);
+      packed_dkdv_step<Tr, D>(qt, dot, rows, on_diagonal(cur), kreg, vreg, dkacc, dvacc, sum, p_seq + cur.ms, n, n_w0, col, qk_scale, lane);
       csum += (double)sum;
       if (nx.j != cur.j) store_dc(cur.j, false);
       if (!more) break;
@@ -1181,7 +1144,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
       __syncthreads();
       if (t == diag_steps - 1 && n_int > 0) issue(Step{j0, m_top}, q_tile0, do_tile0);
       float sum = 0.f;
-      packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rows_s1, strong_of(rows_s1), kreg, vreg, dkacc, dvacc, sum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
+      packed_dkdv_step<Tr, D>(q_tile1, do_tile1, rows_s1, true, kreg, vreg, dkacc, dvacc, sum, p_seq + s.ms, n, n_w0, col, qk_scale, lane);
       csum += (double)sum;
       if (++d == n_diag) {
         store_dc(j++, false);
