@@ -10,7 +10,8 @@ Tolerances, with u half a step of the 16-bit type (``torch.finfo(t).eps / 2``), 
        of sums in 64 bits, rounded a few times on the way), a probability by as much of itself, dP by 2^-17 |do||v|; a gate's gradient adds
        columns of dS from its key on.  That is the worst case; errors of either sign add up to far less, so the norm of the error is held to 2^-16 of the gradient's too.
 fp16 has no steps below 2^-24, so an entry of p or ds may be off by 2^-25 whatever its size (the largest p of a row is at least 1 before it is divided by the row's sum): n 2^-25 of the largest
-value that it multiplies.  To all of them comes the scores' own error, 2^-14 of the same sums (scores up to 8 in size)."""
+value that it multiplies; and half of such a step, 2^-25, is what an output below 2^-14 may lose by its own rounding (a single key: dk is the 32-bit error of ds times q, some 4e-8, and
+the nearest fp16 are 0 and 6e-8).  To all of them comes the scores' own error, 2^-14 of the same sums (scores up to 8 in size)."""
 import math
 
 import pytest
@@ -79,7 +80,7 @@ def sequence(q, k, v, f, do, scale):
     dk, dv = join(dk), join(dv)
     t = lambda x: x.transpose(0, 1)
     tiny = 2.0 ** -25 * max(m, n) * group                            # of the largest factor: fp16 only
-    small = [tiny * v.abs().max(), tiny * abs(scale) * k.abs().max(), tiny * abs(scale) * q.abs().max(), tiny * do.abs().max()]
+    small = [x + 2.0 ** -25 for x in (tiny * v.abs().max(), tiny * abs(scale) * k.abs().max(), tiny * abs(scale) * q.abs().max(), tiny * do.abs().max())]
     noise = [0.0, t(n_dq), t(n_dk), 0.0]                             # not in steps of the type
     return [t(x) for x in (o, dq, dk, dv, dg)], [t(x) for x in (e_o, e_dq, e_dk + a(dk), e_dv + a(dv))], t(back(e_ds.sum(-2))), small, noise
 
