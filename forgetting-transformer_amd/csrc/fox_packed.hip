@@ -36,7 +36,7 @@ constexpr int kPackedTile = 128;   // rows of a tile of either kind
 static_assert(kPackedTile == kFwdBM && kPackedTile == kKvBN && kKvBM == kKvBN, "a tile is what a workgroup keeps");
 // Log gates below this close like it: -inf itself would make the difference of two sums behind it undefined.
 constexpr float kLowestGate = -1e6f;
-// Shares below which no walk is cut, in 64 keys and 128 rows of a head.
+// Least shares, in 64 keys and 128 rows of a head (2 / 4 / 8, us: six pieces of up to 64 tokens behind up to 900, 12 heads 13.6 / 13.1 / 15.1, longer ones the same).
 constexpr int kQueryShare = 4, kKeyShare = 4, kNoShare = 0x7fffffff;
 // Parts for a share of units, at most, in halves: three from two shares on, four from one on.
 constexpr int kQueryOver = 3, kKeyOver = 4;
@@ -1235,6 +1235,7 @@ int tile_bound(int B, int rows) {
   return (int)(rows / kPackedTile + partial);
 }
 int64_t up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+// (Parts of a half or a third of that length, us: documents of 150 to 2048 tokens, forward 42, 44 for 36, prompts of up to 2048 117, 125 for 110.)
 // Parts of cut walks, at most: `over` halves as many as workgroups run at once for a head (each walk's last part may be a short one), or as come of walks of `longest` units, and of `units` in all, in
 // shares of at least `least`; none where the longest walk there can be stays whole.  Each costs a workgroup that may find nothing to do.
 int extra_parts(int at_once, int heads, int over, int64_t tiles, int64_t longest, double units, int least) {
