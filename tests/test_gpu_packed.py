@@ -351,3 +351,29 @@ def test_packed_refusals():
         torch.autograd.grad(out, leaves, x[4].requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda q: forgetting_attention_packed(q, k, v, f, cu_q))(q[None])
+
+
+def test_packed_of_more_than_four_gi_elements():
+    """Sequences whose elements lie behind 2**32: the same bits as from a call of their own."""
+    from forgetting_transformer import forgetting_attention_packed
+    H, D, n, B = 128, 128, 256, 1026
+    T, tail = B * n, 2 * n
+    g = torch.Generator(device="cuda").manual_seed(41)
+    small = [torch.randn(tail, H, D, generator=g, device="cuda").bfloat16() for _ in range(4)]
+    gates = -torch.rand(tail, H, generator=g, device="cuda")
+    small.insert(3, gates)
+
+    def step(q, k, v, f, do):
+        cu = torch.arange(0, len(q) + 1, n, dtype=torch.int32, device="cuda")
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, f)]
+        out = forgetting_attention_packed(*leaves, cu)
+        return [t[-tail:].clone() for t in (out.detach(), *torch.autograd.grad(out, leaves, do))]
+
+    want = step(*small)
+    large = []
+    for t in small:
+        x = torch.zeros(T, *t.shape[1:], dtype=t.dtype, device="cuda")
+        x[-tail:] = t
+        large.append(x)
+    for a, b in zip(step(*large), want):
+        assert torch.equal(a, b)

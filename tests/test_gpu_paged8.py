@@ -534,3 +534,27 @@ def test_a_captured_step_of_prompts():
         assert torch.equal(out, want[i]), i
         step(eager, [*x[:4], torch.zeros_like(x[4])])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("codes", ["e4m3", "int8"])
+def test_a_pool_of_more_than_four_gibibytes(codes):
+    """Pages whose codes lie behind 2**32: the same bits as from a small pool, for the append, the gather and the attention."""
+    from forgetting_transformer import paged_append_8bit, paged_forgetting_attention_8bit, paged_gather
+    S, Hk, H, D, n = 128, 4, 8, 128, 300
+    far = (1 << 32) // (S * Hk * D)
+    g = torch.Generator(device="cuda").manual_seed(14)
+    k, v = (torch.randn(n, Hk, D, generator=g, device="cuda").bfloat16() for _ in range(2))
+    f, q = -torch.rand(n, H, generator=g, device="cuda"), torch.randn(1, H, D, generator=g, device="cuda").bfloat16()
+    got = []
+    for first, P in ((0, 3), (far, far + 3)):
+        empty = lambda *s, t=CODES[codes][0]: torch.empty(s, dtype=t, device="cuda")
+        kp, vp, fp = empty(P, Hk, S, D), empty(P, Hk, S, D), empty(P, H, S, t=torch.float32)
+        ks, vs = empty(P, Hk, S // 16, t=torch.float32), empty(P, Hk, S // 16, t=torch.float32)
+        pages = [first + 2, first, first + 1]
+        slots = torch.tensor([p * S + i for p in pages for i in range(S)], device="cuda")[:n].contiguous()
+        paged_append_8bit(k, v, f, kp, vp, ks, vs, fp, slots)
+        table, wide = on_gpu([pages]), on_gpu([pages + [-1] * 60])        # (a row whole, and in pieces)
+        out = paged_gather(kp, vp, fp, table, on_gpu([0, n]), max_tokens=n, k_scales=ks, v_scales=vs)
+        got.append([*out, *(paged_forgetting_attention_8bit(q, kp, vp, ks, vs, fp, t, on_gpu([m])) for t, m in ((table, n), (table, 17), (wide, n)))])
+        del kp, vp
+    assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(*got))
