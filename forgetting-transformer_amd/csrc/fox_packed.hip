@@ -34,8 +34,10 @@ namespace {
 
 constexpr int kPackedTile = 128;   // rows of a tile of either kind
 static_assert(kPackedTile == kFwdBM && kPackedTile == kKvBN && kKvBM == kKvBN, "a tile is what a workgroup keeps");
-// Log gates below this close like it: -inf itself would make the difference of two sums behind it undefined.
+// Log gates below this close like it: -inf itself would make the difference of two sums behind it undefined.  NaN stays NaN (fmaxf would drop it): so are the rows behind it then, and the
+// gradients that such a row takes part in.
 constexpr float kLowestGate = -1e6f;
+__device__ __forceinline__ float bounded_gate(float g) { return g < kLowestGate ? kLowestGate : g; }
 // Least shares, in 64 keys and 128 rows of a head (2 / 4 / 8, us: six pieces of up to 64 tokens behind up to 900, 12 heads 13.6 / 13.1 / 15.1, longer ones the same).
 constexpr int kQueryShare = 4, kKeyShare = 4, kNoShare = 0x7fffffff;
 // Parts for a share of units, at most, in halves: three from two shares on, four from one on.
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(1024) void packed_scan_kernel(const PackedK a) {
   const int k0 = min(max(a.cu_k[b], 0), a.N), n = min(max(a.cu_k[b + 1], k0), a.N) - k0;
   const float* g = a.g + (int64_t)k0 * a.g_st + h * a.g_sh;
   double* c = a.c + (int64_t)h * a.N + k0;
-  sum_row<NT, false>(n, [&](int j) { return fmaxf(g[j * a.g_st], kLowestGate); }, [&](int j, double sum) { c[j] = sum; });
+  sum_row<NT, false>(n, [&](int j) { return bounded_gate(g[j * a.g_st]); }, [&](int j, double sum) { c[j] = sum; });
 }
 
 // The backward's counters of arrived parts: its own, since two of one forward may run at once.  (Those of the forward are cleared next to its plan.)
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(256) void packed_clear_kernel(const PackedK a) {
   if (i < a.k_extra * a.Hk) a.k_arrived[i] = 0;
 }
 
-// dg of a (sequence, head) from dc.  The first gate of a sequence moves all its sums alike: an exact zero, as in the rows that belong to none.
+// dg of a (sequence, head) from dc.  The first gate of a sequence moves all its sums alike: an exact zero, as in the rows that belong to none, but NaN where one of the sums is.
 template <int NT>
 __global__ __launch_bounds__(1024) void packed_gate_grad_kernel(const PackedK a) {
   constexpr int THREADS = 1024;
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(1024) void packed_gate_grad_kernel(const PackedK a)
   const float* dc = a.dc + (int64_t)h * a.N + s.z;
   float* dg = a.dg + (int64_t)s.z * a.dg_st + h * a.dg_sh;
   const bool none = b >= a.B;
-  sum_row<NT, true>(s.w, [&](int j) { return dc[j]; }, [&](int j, double sum) { dg[j * a.dg_st] = none || j == 0 ? 0.f : (float)sum; });
+  sum_row<NT, true>(s.w, [&](int j) { return dc[j]; }, [&](int j, double sum) { dg[j * a.dg_st] = none || (j == 0 && sum == sum) ? 0.f : (float)sum; });
 }
 
 namespace {
@@ -888,7 +890,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const P
     };
     issue_cn((n_tiles - 1) * BN);
     // rows past M and rows that see no key (lse = -inf) get -inf
-    const bool row_ok = m < M && l > -INFINITY;
+    const bool row_ok = m < M && l != -INFINITY;   // (NaN stays)
     Pair row = pair_of((c_m - c_ref) * kLog2eD);
     const float rowc = row_ok ? row.hi - l * kLog2e : -INFINITY;
     const bool few_keys = min(N, a_w0 + 32) <= 32;
@@ -1054,7 +1056,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const
   // the start values of the score accumulators, at the diagonal pairs as well; rows past M and those that see no key get a probability of zero
   auto on_diagonal = [&](Step s) { return p_seq + s.ms < n0 + BN - 1; };
   auto store_rows = [&](Step s, Rows& to) {
-    const bool ok = row_ok && l_raw > -INFINITY;
+    const bool ok = row_ok && l_raw != -INFINITY;   // (NaN stays)
     if (row_lane) {
       to.rc[row_slot] = ok ? ((float)(c_raw - c_ref) - l_raw) * kLog2e * inv_scale : copysignf(INFINITY, -inv_scale);
       to.dl[row_slot] = ok ? -d_raw : 0.f;

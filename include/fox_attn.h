@@ -619,7 +619,7 @@ int fox_paged8_decode_workspace_bytes(int32_t B, int32_t H, int32_t Hk, int32_t 
  *   s_ij = sm_scale q_i.k_j + c_i - c_j,  c_j = sum of the sequence's gates up to key j,  o = softmax(s) v.
  * q, o, d_o, dq: (T, H, D); k, v, dk, dv: (N, Hk, D), 16-bit; stride_t is a token's, stride_h a head's, stride_b is not used; token strides are positive and below 2^23.
  * c (H, N) fp64, lse (H, T) and the plan are written by the forward and read by the backward, which takes them in place of g, cu_q and cu_k; lse may be NULL for a forward alone.  The plan and each
- * call's workspace hold the bytes that fox_packed_bytes() gives, 16-byte aligned; calls that may run at once need workspaces of their own.  Log gates below -1e6 count as that.
+ * call's workspace hold the bytes that fox_packed_bytes() gives, 16-byte aligned; calls that may run at once need workspaces of their own.  Log gates below -1e6 count as that; NaN stays NaN.
  */
 typedef struct fox_packed_args {
   int32_t B, T, N, H, Hk, D, dtype;

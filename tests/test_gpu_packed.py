@@ -377,3 +377,36 @@ def test_packed_of_more_than_four_gi_elements():
         large.append(x)
     for a, b in zip(step(*large), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("new,front,H,Hk,D,dtype,at", [   # `at`: the sequence, the key and the head whose gate is NaN
+    ([40, 200, 33], [0, 0, 0], 4, 2, 64, torch.bfloat16, (1, 70, 1)), ([300, 90], [0, 50], 3, 1, 16, torch.float16, (0, 299, 2)),
+    ([600, 20, 5], [0, 0, 0], 4, 4, 128, torch.bfloat16, (0, 130, 3)), ([5, 100], [900, 0], 8, 2, 128, torch.float16, (0, 3, 0)),
+    ([7, 1, 1], [0, 0, 0], 2, 2, 32, torch.bfloat16, (1, 0, 0)), ([1300, 30], [0, 0], 1, 1, 64, torch.bfloat16, (0, 1000, 0)),
+    ([1500, 20], [700, 0], 2, 1, 128, torch.bfloat16, (0, 1900, 1))])
+def test_packed_gate_that_is_nan(new, front, H, Hk, D, dtype, at):
+    """A NaN in one head's gate of a sequence: what the formulas make of it, and nothing else. Rows behind it are NaN, and every key of the sequence is seen from one of them."""
+    from forgetting_transformer import forgetting_attention_packed
+    *x, cu_q, cu_k = inputs(new, front, H, Hk, D, dtype, seed=50 + D, lead=2, pad=3)
+    b, key, h = at
+    r0, rows, k0, keys = cu_q[b].item(), new[b], cu_k[b].item(), new[b] + front[b]
+
+    def step():
+        leaves = [t.detach().clone().requires_grad_() for t in x[:4]]
+        out = forgetting_attention_packed(*leaves, cu_q, cu_k)
+        return [out.detach(), *torch.autograd.grad(out, leaves, x[4])]
+
+    want = step()
+    x[3][k0 + key, h] = float("nan")
+    got = step()
+    first = r0 + max(rows - (keys - key), 0)                # of the rows that see the key
+    hk = h // (H // Hk)
+    is_nan = [torch.zeros_like(y, dtype=torch.bool) for y in want]
+    for i in (0, 1):                                        # o, dq
+        is_nan[i][first:r0 + rows, h] = True
+    for i in (2, 3):                                        # dk, dv of the key head
+        is_nan[i][k0:k0 + keys, hk] = True
+    is_nan[4][k0:k0 + keys, h] = True
+    for name, y, w, n in zip(("o", "dq", "dk", "dv", "dg"), got, want, is_nan):
+        assert torch.equal(torch.isnan(y), n), f"{name}: {torch.isnan(y).sum().item()} NaN, {n.sum().item()} by the formulas"
+        assert torch.equal(y[~n], w[~n]), name
