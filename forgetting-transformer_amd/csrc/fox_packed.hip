@@ -307,6 +307,32 @@ __device__ __forceinline__ void sum_row(int n, Load load, Store store) {
   }
 }
 
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = max(x, __shfl_xor(x, off));
+  return x;
+}
+// Where the keys of sequence b <= B begin: behind every earlier end, as in the plan, so that no two rows have a place in common.  b is a wave's, b0 that of the workgroup's first one.  Every
+// thread of the workgroup of NT calls it.  Ends that do not decrease leave the comparisons alone, without the maxima.
+template <int NT>
+__device__ __forceinline__ int first_key(const PackedK& a, int b0, int b) {
+  __shared__ int tops[NT / 64];
+  const int tid = threadIdx.x, lane = tid & 63, own = b < a.B ? a.cu_k[b] : 0;
+  const int at = a.cu_k[b0];
+  int top = 0;
+  for (int i = tid; i < b0; i += NT) top = max(top, a.cu_k[i]);
+  top = __any(top > at) ? wave_max(top) : 0;
+  if (lane == 0) tops[tid >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) top = max(top, tops[w]);
+  for (int i0 = b0; i0 < b; i0 += 64) {
+    const int x = i0 + lane < b ? a.cu_k[i0 + lane] : 0;
+    if (__any(x > own)) top = max(top, wave_max(x));
+  }
+  return min(max(top, own), a.N);
+}
+
 }  // namespace
 
 // The first workgroups make the plan (that of the keys only where a backward may follow), the others the sums of a (sequence, head) each; with NT = 64 of sixteen.
@@ -317,10 +343,11 @@ __global__ __launch_bounds__(1024) void packed_scan_kernel(const PackedK a) {
   const int plans = a.lse ? 2 : 1;
   if (blockIdx.x == 0) return make_plan<THREADS, false>(a, mem);
   if (blockIdx.x < plans) return make_plan<THREADS, true>(a, mem);
-  const int row = (blockIdx.x - plans) * (THREADS / NT) + threadIdx.x / NT;
-  if (row >= a.B * a.H) return;
+  const int row0 = (blockIdx.x - plans) * (THREADS / NT), row = row0 + threadIdx.x / NT;
   const int b = divide(row, a.by_heads), h = row - b * a.H;
-  const int k0 = min(max(a.cu_k[b], 0), a.N), n = min(max(a.cu_k[b + 1], k0), a.N) - k0;
+  const int k0 = first_key<THREADS>(a, divide(row0, a.by_heads), min(b, a.B));
+  if (row >= a.B * a.H) return;
+  const int n = min(max(a.cu_k[b + 1], k0), a.N) - k0;
   const float* g = a.g + (int64_t)k0 * a.g_st + h * a.g_sh;
   double* c = a.c + (int64_t)h * a.N + k0;
   sum_row<NT, false>(n, [&](int j) { return bounded_gate(g[j * a.g_st]); }, [&](int j, double sum) { c[j] = sum; });

@@ -410,3 +410,22 @@ def test_packed_gate_that_is_nan(new, front, H, Hk, D, dtype, at):
     for name, y, w, n in zip(("o", "dq", "dk", "dv", "dg"), got, want, is_nan):
         assert torch.equal(torch.isnan(y), n), f"{name}: {torch.isnan(y).sum().item()} NaN, {n.sum().item()} by the formulas"
         assert torch.equal(y[~n], w[~n]), name
+
+
+@pytest.mark.parametrize("ends,H,Hk,D", [
+    ([0, 100, 50, 120], 2, 2, 32), ([0, 100, 250, 90, 95, 240, 300], 3, 1, 64), ([30, -5, 300, 20, 10, 280, 299, 7], 4, 2, 16), ([-1, 0, 2 ** 31 - 1, 5, 9], 1, 1, 128),
+    ([0] + [(37 * i) % 301 for i in range(200)], 5, 5, 32), ([0] + [min(i, 299) if i % 50 else 40 for i in range(1500)], 2, 1, 16)])
+def test_packed_ends_that_decrease(ends, H, Hk, D):
+    """Every sequence begins behind all earlier ends and inside the tensors: the same bits as from ends that are in that order."""
+    from forgetting_transformer import forgetting_attention_packed
+    *x, _, _ = inputs([300], [0], H, Hk, D, torch.bfloat16, seed=60)
+    given = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    order = given.clamp(0, 300).cummax(0).values.int()
+
+    def step(*cu):
+        leaves = [t.detach().requires_grad_() for t in x[:4]]
+        out = forgetting_attention_packed(*leaves, *cu)
+        return [out.detach(), *torch.autograd.grad(out, leaves, x[4])]
+
+    for a, b in ((step(given), step(order)), (step(order, given), step(order, order))):
+        assert all(torch.equal(y, z) for y, z in zip(a, b))
