@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <map>
@@ -1226,6 +1227,48 @@ bool overlaps(const Tensor& a, const Tensor& b) {
   };
   return (const char*)a.const_data_ptr() < end(b) && (const char*)b.const_data_ptr() < end(a);
 }
+// Whether two tensors of one shape and type have an element in common; they may lie between each other, as keys and values of one pool do.  An element of both is a solution of
+//   sum_i stride_a[i] x_i - sum_i stride_b[i] y_i = b - a,  0 <= x_i, y_i < size_i,
+// looked for from the largest stride on: what is left has to be within reach of the smaller ones, which for strides that contain each other leaves two values of each.
+// Tensors whose rows lie on each other, and such as are too entangled for kMostSteps, count as having one.
+struct StrideTerm {
+  int64_t stride, lo, hi;   // of the values of one variable
+};
+bool reaches(const StrideTerm* t, const StrideTerm* end, int64_t left, int& steps) {
+  if (t == end) return left == 0;
+  int64_t lo = 0, hi = 0;   // of all that follow
+  for (const StrideTerm* u = t + 1; u != end; ++u) {
+    lo += u->stride * u->lo;
+    hi += u->stride * u->hi;
+  }
+  const auto below = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };   // x / y, rounded down
+  const int64_t first = std::max(t->lo, -below(hi - left, t->stride)), last = std::min(t->hi, below(left - lo, t->stride));
+  for (int64_t x = first; x <= last; ++x) {
+    if (--steps < 0 || reaches(t + 1, end, left - x * t->stride, steps)) return true;
+  }
+  return false;
+}
+bool share_elements(const Tensor& a, const Tensor& b) {
+  constexpr int kMostSteps = 1 << 12;
+  if (!overlaps(a, b)) return false;
+  const int64_t bytes = (const char*)b.const_data_ptr() - (const char*)a.const_data_ptr(), size = a.element_size();
+  if (bytes % size) return true;
+  c10::SmallVector<StrideTerm, 8> terms;
+  for (int64_t i = 0; i < a.dim(); ++i) {
+    const int64_t n = a.size(i) - 1, sa = a.stride(i), sb = b.stride(i);
+    if (n == 0) continue;
+    if (sa < 1 || sb < 1) return true;
+    if (sa == sb) {
+      terms.push_back({sa, -n, n});
+    } else {
+      terms.push_back({sa, 0, n});
+      terms.push_back({sb, -n, 0});
+    }
+  }
+  std::sort(terms.begin(), terms.end(), [](const StrideTerm& x, const StrideTerm& y) { return x.stride > y.stride; });
+  int steps = kMostSteps;
+  return reaches(terms.begin(), terms.end(), bytes / size, steps);
+}
 
 // Pages of S tokens, W of them a request at most: what the kernels take (the Python functions say which limit is passed).
 bool page_size_ok(int64_t S) { return S >= 8 && S <= 4096 && (S & (S - 1)) == 0; }
@@ -1541,9 +1584,9 @@ PyObject* py_paged8_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (!writable(*to[i])) return none();
     for (const Tensor* f : from)
       if (overlaps(*to[i], *f)) return none();
-    for (int j = 0; j < i; ++j) {   // (pages of keys and values, and their scales, may lie between each other, but are not the same)
+    for (int j = 0; j < i; ++j) {   // (pages of keys and values, and their scales, may lie between each other, but not on each other)
       const bool pair = (i == 1 && j == 0) || (i == 3 && j == 2);
-      if (pair ? to[i]->const_data_ptr() == to[j]->const_data_ptr() : overlaps(*to[i], *to[j])) return none();
+      if (pair ? share_elements(*to[i], *to[j]) : overlaps(*to[i], *to[j])) return none();
     }
   }
   if (T > 0) {
@@ -1715,6 +1758,15 @@ PyObject* py_packed_attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// share_elements(a, b): what the appends ask of the pages that they write
+PyObject* py_share_elements(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *a = n == 2 ? tensor_of(o[0]) : nullptr, *b = a ? tensor_of(o[1]) : nullptr;
+  TORCH_CHECK(b && a->sizes() == b->sizes() && a->scalar_type() == b->scalar_type(), "share_elements takes two tensors of one shape and type");
+  return PyBool_FromLong(share_elements(*a, *b));
+  END_HANDLE_TH_ERRORS
+}
+
 // record_bounds(list or None)
 PyObject* py_record_bounds(PyObject*, PyObject* list) {
   if (list != Py_None && !PyList_Check(list)) {
@@ -1745,6 +1797,7 @@ PyMethodDef methods[] = {
     {"paged8_append", (PyCFunction)(void (*)(void))py_paged8_append, METH_FASTCALL, nullptr},
     {"paged_gather", (PyCFunction)(void (*)(void))py_paged_gather, METH_FASTCALL, nullptr},
     {"paged8_attention", (PyCFunction)(void (*)(void))py_paged8_attention, METH_FASTCALL, nullptr},
+    {"share_elements", (PyCFunction)(void (*)(void))py_share_elements, METH_FASTCALL, nullptr},
     {"packed_attention", (PyCFunction)(void (*)(void))py_packed_attention, METH_FASTCALL, nullptr},
     {"token_shift", (PyCFunction)(void (*)(void))py_token_shift, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

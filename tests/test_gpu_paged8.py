@@ -558,3 +558,35 @@ def test_a_pool_of_more_than_four_gibibytes(codes):
         got.append([*out, *(paged_forgetting_attention_8bit(q, kp, vp, ks, vs, fp, t, on_gpu([m])) for t, m in ((table, n), (table, 17), (wide, n)))])
         del kp, vp
     assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("which", ["pages", "heads", "tokens", "scales"])
+def test_append_refuses_pages_that_lie_on_each_other(which):
+    """Keys and values that share memory without beginning at one place; the same pools taken apart are written as separate ones are."""
+    from forgetting_transformer import paged_append_8bit
+    H, Hk, D, S, P, T = 4, 2, 64, 16, 6, 40
+    g = torch.Generator(device="cuda").manual_seed(15)
+    k, v = (torch.randn(T, Hk, D, generator=g, device="cuda").bfloat16() for _ in range(2))
+    f, slots = -torch.rand(T, H, generator=g, device="cuda"), torch.arange(T, device="cuda")
+    zeros = lambda *s, t=torch.int8: torch.zeros(s, dtype=t, device="cuda")
+    pages, scales, fp = [zeros(P, Hk, S, D) for _ in range(2)], [zeros(P, Hk, 1, t=torch.float32) for _ in range(2)], zeros(P, H, S, t=torch.float32)
+    bad_pages, bad_scales = pages, scales
+    if which == "pages":
+        x = zeros(P + 1, Hk, S, D)
+        bad_pages = [x[:-1], x[1:]]
+    elif which == "heads":
+        x = zeros(P, Hk + 1, S, D)
+        bad_pages = [x[:, 1:], x[:, :-1]]
+    elif which == "tokens":
+        x = zeros(P, S + 2, Hk, D).transpose(1, 2)
+        bad_pages = [x[:, :, :S], x[:, :, 2:]]
+    else:
+        x = zeros(P + 3, Hk, 1, t=torch.float32)
+        bad_scales = [x[:-3], x[3:]]
+    with pytest.raises(RuntimeError, match="may not overlap"):
+        paged_append_8bit(k, v, f, *bad_pages, *bad_scales, fp, slots)
+    paged_append_8bit(k, v, f, *pages, *scales, fp, slots)
+    kv, sc = zeros(P, Hk, 2, S, D), zeros(P, 2, Hk, 1, t=torch.float32)
+    between = [kv[:, :, 0], kv[:, :, 1], sc[:, 0], sc[:, 1], torch.zeros_like(fp)]
+    paged_append_8bit(k, v, f, *between, slots)
+    assert all(torch.equal(a, b) for a, b in zip(between, (*pages, *scales, fp)))

@@ -121,3 +121,46 @@ def test_wrapper_refusals():
     assert cache.key_pages[0].shape == (4, 2, 16, 64) and cache.key_scales[0].shape == (4, 2, 1) and cache.log_fgate_pages[0].shape == (4, 4, 16)
     with pytest.raises(AssertionError, match="prompts"):
         cache.attend_prompts(x, 0)
+
+
+def test_pages_that_share_elements():
+    """What the appends ask of the pages of keys and values: random views of one buffer against the sets of their places, and the layouts that pools have."""
+    import random
+    from forgetting_transformer.ops import _native
+    share = _native.load().share_elements
+    rng = random.Random(0)
+    base, buf = torch.arange(4000), torch.zeros(4000, dtype=torch.int8)
+    seen = [0, 0]
+    for _ in range(3000):
+        shape = [rng.choice([1, 2, 3, 4]) for _ in range(4)]
+
+        def strides():
+            s, at = [0] * 4, 1
+            for i in rng.sample(range(4), 4):
+                s[i], at = at, at * shape[i] * rng.choice([1, 1, 2, 3]) + rng.choice([0, 0, 1])
+            return s
+        a = strides()
+        b = a if rng.random() < 0.6 else strides()
+        if rng.random() < 0.1:
+            b[rng.randrange(4)] = rng.randrange(1, 5)        # (rows that may lie on each other)
+        first = [rng.randrange(200) for _ in range(2)]
+        if any(f + sum((n - 1) * st for n, st in zip(shape, s)) >= 4000 for f, s in zip(first, (a, b))):
+            continue
+        places = [set(base.as_strided(shape, s, f).flatten().tolist()) for f, s in zip(first, (a, b))]
+        want = bool(places[0] & places[1])
+        assert share(buf.as_strided(shape, a, first[0]), buf.as_strided(shape, b, first[1])) is want, (shape, a, b, first)
+        seen[want] += 1
+    assert min(seen) > 200
+    P, H, S, D = 64, 4, 16, 64
+    for shape, at in (((P, 2, H, S, D), 1), ((P, H, 2, S, D), 2), ((P, H, S, 2, D), 3), ((2, P, H, S, D), 0)):
+        kv = torch.zeros(shape, dtype=torch.int8)
+        k, v = kv.select(at, 0), kv.select(at, 1)
+        assert not share(k, v) and not share(v, k) and share(k, k)
+        assert share(k[1:], k[:-1]) and share(k[:, 1:], k[:, :-1]) and share(k[:, :, 1:], k[:, :, :-1])
+    kv = torch.zeros(P, 2 * H * S * D, dtype=torch.int8)
+    k, v = kv[:, :H * S * D].view(P, H, S, D), kv[:, H * S * D:].view(P, S, H, D).transpose(1, 2)     # of different orders within a page
+    assert not share(k, v) and share(k, kv[:, D:D + H * S * D].view(P, S, H, D).transpose(1, 2))
+    same = k[:1].expand(P, H, S, D)                                  # (pages that lie on each other)
+    assert not share(k, torch.zeros_like(k)) and share(same, same[:, :, :1].expand(P, H, S, D)) and not share(same, v)
+    with pytest.raises(RuntimeError, match="one shape"):
+        share(k, k[:1])
