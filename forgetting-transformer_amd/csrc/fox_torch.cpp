@@ -1442,8 +1442,8 @@ PyObject* py_paged_append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (needs_graph({k, v, g}) || !writable(*kp) || !writable(*vp) || !writable(*gp)) return none();
   const Tensor* to[3] = {kp, vp, gp};
   const Tensor* from[3] = {k, v, g};
-  // (pages of keys and values may lie between each other, but are not the same)
-  if (kp->const_data_ptr() == vp->const_data_ptr()) return none();
+  // (pages of keys and values may lie between each other, but not on each other)
+  if (share_elements(*kp, *vp)) return none();
   for (int i = 0; i < 3; ++i) {
     if (overlaps(*to[i], *slots)) return none();
     for (int j = 0; j < 3; ++j)

@@ -519,3 +519,17 @@ def test_limits_are_assertions():
             paged_append(x, x, torch.zeros(2, 1, device="cuda"), kp, vp, fp, torch.arange(2, device="cuda"))
         with pytest.raises(AssertionError):
             paged_forgetting_attention(x, kp, vp, fp, on_gpu([[0], [1]]), on_gpu([1, 1]))
+
+
+@pytest.mark.parametrize("which", ["pages", "heads", "tokens"])
+def test_append_refuses_pages_that_lie_on_each_other(which):
+    """Keys and values that share memory without beginning at one place."""
+    from forgetting_transformer import paged_append
+    H, D, S, P, T = 2, 64, 16, 6, 40
+    k, f, slots = torch.ones(T, H, D, device="cuda").bfloat16(), torch.zeros(T, H, device="cuda"), torch.arange(T, device="cuda")
+    zeros = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")
+    x = {"pages": lambda: zeros(P + 1, H, S, D), "heads": lambda: zeros(P, H + 1, S, D), "tokens": lambda: zeros(P, S + 2, H, D).transpose(1, 2)}[which]()
+    kp, vp = {"pages": lambda: (x[:-1], x[1:]), "heads": lambda: (x[:, 1:], x[:, :-1]), "tokens": lambda: (x[:, :, :S], x[:, :, 2:])}[which]()
+    with pytest.raises(RuntimeError, match="may not overlap"):
+        paged_append(k, k, f, kp, vp, torch.zeros(P, H, S, device="cuda"), slots)
+    assert not x.any()
