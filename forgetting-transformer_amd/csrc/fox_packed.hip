@@ -127,7 +127,10 @@ struct PlanMemory {
   int slots, top[2][16], waves[16];
 };
 
-// The list of the tiles of queries, or of those of keys, by one workgroup of NT threads.  Ends that decrease or lie outside the tensors are brought into order, so
+// An end of a sequence among `rows` rows.  One behind them is left out: cut to them, its sequence would be aligned at another key.
+__device__ __forceinline__ int end_within(int end, int rows) { return end > rows ? 0 : max(end, 0); }
+
+// The list of the tiles of queries, or of those of keys, by one workgroup of NT threads.  Ends that decrease are brought into order and those outside the tensors left out, so
 // that no tile leaves them.
 template <int NT, bool KEYS>
 __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
@@ -150,8 +153,10 @@ __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
   for (int b0 = 0; b0 < a.B; b0 += NT) {
     const int b = b0 + tid;
     const bool in = b < a.B;
-    const int sq = in ? a.cu_q[b] : 0, sk = in ? a.cu_k[b] : 0, last_q = in ? a.cu_q[b + 1] : 0, last_k = in ? a.cu_k[b + 1] : 0;
-    int q = wave_max_scan(max(sq, 0), lane), k = wave_max_scan(max(sk, 0), lane);
+    auto q_end = [&](int i) { return in ? end_within(a.cu_q[i], a.T) : 0; };
+    auto k_end = [&](int i) { return in ? end_within(a.cu_k[i], a.N) : 0; };
+    const int sq = q_end(b), sk = k_end(b), last_q = q_end(b + 1), last_k = k_end(b + 1);
+    int q = wave_max_scan(sq, lane), k = wave_max_scan(sk, lane);
     __syncthreads();
     if (lane == 63) {
       mem.top[0][wave] = q;
@@ -162,9 +167,9 @@ __device__ __forceinline__ void make_plan(const PackedK& a, PlanMemory& mem) {
       q = max(q, mem.top[0][w]);
       k = max(k, mem.top[1][w]);
     }
-    q = min(max(q, top_q), a.T);
-    k = min(max(k, top_k), a.N);
-    const int q1 = min(max(q, last_q), a.T), k1 = min(max(k, last_k), a.N);
+    q = max(q, top_q);
+    k = max(k, top_k);
+    const int q1 = max(q, last_q), k1 = max(k, last_k);
     if (in) {
       const int4 s = make_int4(q, q1 - q, k, k1 - k);
       seqs[b] = s;
@@ -317,20 +322,21 @@ __device__ __forceinline__ int wave_max(int x) {
 template <int NT>
 __device__ __forceinline__ int first_key(const PackedK& a, int b0, int b) {
   __shared__ int tops[NT / 64];
-  const int tid = threadIdx.x, lane = tid & 63, own = b < a.B ? a.cu_k[b] : 0;
-  const int at = a.cu_k[b0];
+  const int tid = threadIdx.x, lane = tid & 63;
+  auto end = [&](int i) { return end_within(a.cu_k[i], a.N); };
+  const int at = end(b0), own = b < a.B ? end(b) : 0;
   int top = 0;
-  for (int i = tid; i < b0; i += NT) top = max(top, a.cu_k[i]);
+  for (int i = tid; i < b0; i += NT) top = max(top, end(i));
   top = __any(top > at) ? wave_max(top) : 0;
   if (lane == 0) tops[tid >> 6] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) top = max(top, tops[w]);
   for (int i0 = b0; i0 < b; i0 += 64) {
-    const int x = i0 + lane < b ? a.cu_k[i0 + lane] : 0;
+    const int x = i0 + lane < b ? end(i0 + lane) : 0;
     if (__any(x > own)) top = max(top, wave_max(x));
   }
-  return min(max(top, own), a.N);
+  return max(top, own);
 }
 
 }  // namespace
@@ -347,7 +353,7 @@ __global__ __launch_bounds__(1024) void packed_scan_kernel(const PackedK a) {
   const int b = divide(row, a.by_heads), h = row - b * a.H;
   const int k0 = first_key<THREADS>(a, divide(row0, a.by_heads), min(b, a.B));
   if (row >= a.B * a.H) return;
-  const int n = min(max(a.cu_k[b + 1], k0), a.N) - k0;
+  const int n = max(end_within(a.cu_k[b + 1], a.N), k0) - k0;
   const float* g = a.g + (int64_t)k0 * a.g_st + h * a.g_sh;
   double* c = a.c + (int64_t)h * a.N + k0;
   sum_row<NT, false>(n, [&](int j) { return bounded_gate(g[j * a.g_st]); }, [&](int j, double sum) { c[j] = sum; });

@@ -56,7 +56,8 @@ def forgetting_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     cu_seqlens: ``(B + 1,)`` int32 on the device, 0 and the ends of the sequences' queries, not decreasing; cu_seqlens_k: the same of their keys, which
     are those of the queries where it is not given.  Of a sequence with m queries and n keys, query i sees the keys ``j <= i + n - m``: the keys of a prompt's earlier pieces
     lie in front of those of the piece.  A query that sees no key gives zeros, and so do places that belong to no sequence (as a step with room for more tokens
-    has them behind its last one); no gradient reaches them or comes from them.  ``sm_scale`` defaults to ``1 / sqrt(D)``.
+    has them behind its last one); no gradient reaches them or comes from them.  A sequence whose queries (keys) end behind the last of the tensor has none, and neither have those
+    that follow.  ``sm_scale`` defaults to ``1 / sqrt(D)``.
 
     Gradients for q, k, v and log_fgate.  Nothing waits for the device.
     """

@@ -112,7 +112,8 @@ class PagedFgateCache:
         """What ``attend`` gives, for steps whose requests bring many tokens: the keys of the requests that bring any are read back from the pages, and every request's tokens go
         through ``forgetting_attention_packed`` over them.
 
-        ``max_keys`` promises that those requests hold no more tokens together (more are cut); without it there is room for all that the pool holds.
+        ``max_keys`` promises that those requests hold no more tokens together: one whose tokens end behind them gives zeros, and so do those that follow.  Without it there is room for all
+        that the pool holds.
         """
         assert self._ends is not None, "schedule a step with prompts first"
         assert max_keys is None or max_keys > 0, "max_keys must be positive"

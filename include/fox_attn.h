@@ -615,7 +615,7 @@ int fox_paged8_decode_workspace_bytes(int32_t B, int32_t H, int32_t Hk, int32_t 
 /*
  * Forgetting Attention over packed sequences.  B sequences lie one after the other: queries cu_q[b] .. cu_q[b+1] - 1 and keys cu_k[b] .. cu_k[b+1] - 1 belong to sequence b (int32
  * ends on the device, not decreasing).  Query i of m sees the keys j <= i + n - m of the n of its sequence; one that sees none gives zeros, and so do rows that belong to
- * no sequence, in gradients as well.  Query head h reads key head h / (H / Hk) and has log gates of its own:
+ * no sequence, in gradients as well.  An end behind the tensor is left out: its sequence, and those that follow, have no queries or keys.  Query head h reads key head h / (H / Hk) and has log gates of its own:
  *   s_ij = sm_scale q_i.k_j + c_i - c_j,  c_j = sum of the sequence's gates up to key j,  o = softmax(s) v.
  * q, o, d_o, dq: (T, H, D); k, v, dk, dv: (N, Hk, D), 16-bit; stride_t is a token's, stride_h a head's, stride_b is not used; token strides are positive and below 2^23.
  * c (H, N) fp64, lse (H, T) and the plan are written by the forward and read by the backward, which takes them in place of g, cu_q and cu_k; lse may be NULL for a forward alone.  The plan and each

@@ -416,16 +416,31 @@ def test_packed_gate_that_is_nan(new, front, H, Hk, D, dtype, at):
     ([0, 100, 50, 120], 2, 2, 32), ([0, 100, 250, 90, 95, 240, 300], 3, 1, 64), ([30, -5, 300, 20, 10, 280, 299, 7], 4, 2, 16), ([-1, 0, 2 ** 31 - 1, 5, 9], 1, 1, 128),
     ([0] + [(37 * i) % 301 for i in range(200)], 5, 5, 32), ([0] + [min(i, 299) if i % 50 else 40 for i in range(1500)], 2, 1, 16)])
 def test_packed_ends_that_decrease(ends, H, Hk, D):
-    """Every sequence begins behind all earlier ends and inside the tensors: the same bits as from ends that are in that order."""
+    """Every sequence begins behind all earlier ends, and ends behind the tensors are left out: the same bits as from ends that are in that order."""
     from forgetting_transformer import forgetting_attention_packed
     *x, _, _ = inputs([300], [0], H, Hk, D, torch.bfloat16, seed=60)
     given = torch.tensor(ends, dtype=torch.int32, device="cuda")
-    order = given.clamp(0, 300).cummax(0).values.int()
+    order = torch.where(given > 300, 0, given).clamp(min=0).cummax(0).values.int()
 
     def step(*cu):
         leaves = [t.detach().requires_grad_() for t in x[:4]]
         out = forgetting_attention_packed(*leaves, *cu)
         return [out.detach(), *torch.autograd.grad(out, leaves, x[4])]
 
-    for a, b in ((step(given), step(order)), (step(order, given), step(order, order))):
+    for a, b in ((step(given), step(order)), (step(given, order), step(order, order)), (step(order, given), step(order, order))):
         assert all(torch.equal(y, z) for y, z in zip(a, b))
+
+
+def test_packed_ends_behind_the_tensors():
+    """A sequence that ends behind the keys, or behind the queries, holds none, and neither do those that follow; the ones in front are whole."""
+    from forgetting_transformer import forgetting_attention_packed
+    *x, cu_q, cu_k = inputs([40, 200, 33, 5], [0, 90, 20, 7], 4, 2, 64, torch.bfloat16, seed=61)
+    ends_q, ends_k = cu_q.tolist(), cu_k.tolist()
+    for T, N in ((278, 394), (278, 383), (278, 331), (278, 330), (278, 39), (277, 395), (273, 395), (100, 395), (272, 360), (39, 200)):
+        leaves = [t.detach().requires_grad_() for t in (x[0][:T], *(t[:N] for t in x[1:4]))]
+        out = forgetting_attention_packed(*leaves, cu_q, cu_k)
+        got = [out.detach(), *torch.autograd.grad(out, leaves, x[4][:T])]
+        m = [e if e <= T else max(y for y in ends_q if y <= T) for e in ends_q]        # without the ends behind them
+        n = [e if e <= N else max(y for y in ends_k if y <= N) for e in ends_k]
+        order = [torch.tensor(e, dtype=torch.int32, device="cuda") for e in (m, n)]
+        check([t[:len(y)] for t, y in zip(x, (*leaves, out))], *order, 64 ** -0.5, got, torch.bfloat16)

@@ -590,3 +590,66 @@ def test_append_refuses_pages_that_lie_on_each_other(which):
     between = [kv[:, :, 0], kv[:, :, 1], sc[:, 0], sc[:, 1], torch.zeros_like(fp)]
     paged_append_8bit(k, v, f, *between, slots)
     assert all(torch.equal(a, b) for a, b in zip(between, (*pages, *scales, fp)))
+
+
+def prompts_cache(lengths, codes=None, **more):
+    """A cache of one layer whose requests have just brought `lengths` tokens, and the step's queries."""
+    from forgetting_transformer import PagedFgateCache
+    H, D, B = 4, 64, len(lengths)
+    c = PagedFgateCache(1, H, D, **{**dict(num_pages=40, max_requests=B, max_length=160, page_size=16, cache_dtype=CODES[codes][0] if codes else None), **more})
+    g = torch.Generator(device="cuda").manual_seed(16)
+    room = sum(lengths) + 5
+    q, k, v = (torch.randn(room, H, D, generator=g, device="cuda").bfloat16() for _ in range(3))
+    f = torch.nn.functional.logsigmoid(torch.randn(room, H, generator=g, device="cuda") + 2.0)
+
+    def step(new=None):
+        c.schedule(on_gpu(lengths) if new is None else new, room, prompts=True)
+        c.update(k, v, f, 0)
+    return c, q, step
+
+
+@pytest.mark.parametrize("codes", ["int8", None])
+def test_prompts_past_max_keys_give_zeros(codes):
+    """A request whose keys do not fit gives zeros, and so do those behind it; the ones in front are whole."""
+    lengths = [50, 0, 60, 70, 33]
+    c, q, step = prompts_cache(lengths, codes)
+    step()
+    ks, vs = (x[0] if x is not None else torch.ones(40, 4, 1, device="cuda") for x in (c.key_scales, c.value_scales))
+    s = c.step
+    want, top = attention_reference(q, c.key_pages[0], c.value_pages[0], ks, vs, c.log_fgate_pages[0], c.block_table.tolist(), s.keys.tolist(), s.requests.tolist(), 64 ** -0.5)
+    u = 2.0 ** -8
+    for max_keys, fits in ((213, 213), (212, 180), (500, 213), (109, 50), (110, 110), (179, 110), (50, 50), (49, 0), (1, 0)):
+        out = c.attend_prompts(q, 0, max_keys=max_keys)
+        assert ((out[:fits].double() - want[:fits]).abs() <= u * want[:fits].abs() + (u + 2.0 ** -12) * top).all(), max_keys
+        assert not out[fits:].any(), max_keys
+
+
+def test_a_captured_step_of_prompts_with_max_keys():
+    """The same in a graph, replayed for pieces of other lengths with eager work between; some of them do not fit."""
+    xs = [on_gpu(n) for n in ([20, 1, 0], [5, 30, 29], [0, 0, 3], [40, 2, 2], [1, 1, 1])]
+    make = lambda: prompts_cache([20, 40, 40], "e4m3")
+    eager, q, step = make()
+    want = []
+    for new in xs:
+        step(new)
+        want.append(eager.attend_prompts(q, 0, max_keys=75))
+    assert want[1][:35].any() and not want[1][35:].any() and want[3][:40].any() and not want[3][40:].any()
+    c, q, step = make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other, _, warm = make()
+        warm(xs[0])
+        other.attend_prompts(q, 0, max_keys=75)
+    torch.cuda.current_stream().wait_stream(side)
+    new, graph = xs[0].clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(new)
+        out = c.attend_prompts(q, 0, max_keys=75)
+    for i, x in enumerate(xs):
+        new.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i]), i
+        eager.attend_prompts(q, 0, max_keys=60)
+        torch.cuda.synchronize()
