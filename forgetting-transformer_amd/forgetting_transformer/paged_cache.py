@@ -113,12 +113,15 @@ class PagedFgateCache:
         through ``forgetting_attention_packed`` over them.
 
         ``max_keys`` promises that those requests hold no more tokens together: one whose tokens end behind them gives zeros, and so do those that follow.  Without it there is room for all
-        that the pool holds.
+        that the step's requests can hold, ``max_length`` each or the whole pool if that is less: 16-bit keys and values, and sums of the gates, for so many tokens in every layer.
         """
         assert self._ends is not None, "schedule a step with prompts first"
         assert max_keys is None or max_keys > 0, "max_keys must be positive"
         pages = self.key_pages[layer_idx]
+        if max_keys is None:
+            (requests, width), (num_pages, _, page_size, _) = self.block_table.shape, pages.shape
+            max_keys = min(num_pages, min(requests, self.step.slots.shape[0]) * width) * page_size
         scales = {} if self.key_scales is None else dict(k_scales=self.key_scales[layer_idx], v_scales=self.value_scales[layer_idx], dtype=self.dtype)
         k, v, log_fgate = paged_gather(pages, self.value_pages[layer_idx], self.log_fgate_pages[layer_idx], self.block_table, self._ends[1],
-                                       max_tokens=pages.shape[0] * pages.shape[2] if max_keys is None else max_keys, **scales)
+                                       max_tokens=max_keys, **scales)
         return forgetting_attention_packed(q, k, v, log_fgate, *self._ends, sm_scale=sm_scale)

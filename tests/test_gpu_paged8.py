@@ -653,3 +653,21 @@ def test_a_captured_step_of_prompts_with_max_keys():
         assert torch.equal(out, want[i]), i
         eager.attend_prompts(q, 0, max_keys=60)
         torch.cuda.synchronize()
+
+
+def test_room_of_prompts_without_max_keys():
+    """No more than the step's requests can hold, where the pool is larger."""
+    c, q, step = prompts_cache([50, 60], "e4m3", num_pages=1 << 16, max_length=64)
+    step()
+    want = c.attend_prompts(q, 0, max_keys=128)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = c.attend_prompts(q, 0)
+    assert torch.equal(out, want)
+    keys = 2 * 64                                       # of k, v, gates, their sums; of the queries o; plan and parts as they come
+    assert torch.cuda.max_memory_allocated() - before <= keys * 4 * (2 * 64 * 2 + 4 + 8) + q.numel() * 2 + (8 << 20)
+    few = q[:1].contiguous()
+    c.schedule(on_gpu([0, 1]), 1, prompts=True)
+    c.update(few, few, torch.zeros(1, 4, device="cuda"), 0)
+    assert torch.equal(c.attend_prompts(few, 0), c.attend_prompts(few, 0, max_keys=64))
