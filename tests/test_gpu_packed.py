@@ -444,3 +444,30 @@ def test_packed_ends_behind_the_tensors():
         n = [e if e <= N else max(y for y in ends_k if y <= N) for e in ends_k]
         order = [torch.tensor(e, dtype=torch.int32, device="cuda") for e in (m, n)]
         check([t[:len(y)] for t, y in zip(x, (*leaves, out))], *order, 64 ** -0.5, got, torch.bfloat16)
+
+
+@pytest.mark.parametrize("D,dtype", [(16, torch.float16), (64, torch.bfloat16), (128, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("scale", [-0.2, -1e-3, 0.0, 1e-32, 1e-3, 0.3])
+def test_packed_scales_of_long_walks(D, dtype, scale):
+    """Scales of either sign and next to none where most steps lie off the diagonal, heads and rows in parts among them. A probability's error relative to itself goes with the size of the scores,
+    so the norm of dg is held to 2^-16 for scores of size one and to as much more as they are larger."""
+    from forgetting_transformer import forgetting_attention_packed
+    *x, cu_q, cu_k = inputs([900, 1, 260], [0, 300, 700], 4, 2, D, dtype, seed=70 + D)
+    leaves = [t.detach().requires_grad_() for t in x[:4]]
+    out = forgetting_attention_packed(*leaves, cu_q, cu_k, sm_scale=scale)
+    wrong, size = check(x, cu_q, cu_k, scale, [out.detach(), *torch.autograd.grad(out, leaves, x[4])], dtype)
+    assert wrong <= 2.0 ** -16 * max(1.0, abs(scale) * D ** 0.5) * size
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16), (128, torch.float16)])
+def test_packed_closed_gates_of_long_walks(D, dtype):
+    """Closed gates in interior tiles and at the diagonal; the norm of dg is held too."""
+    from forgetting_transformer import forgetting_attention_packed
+    *x, cu_q, cu_k = inputs([800, 130], [100, 500], 4, 2, D, dtype, seed=80 + D)
+    f = x[3]
+    f[60], f[300], f[301, 1], f[700] = -math.inf, torch.finfo(torch.float32).min, -math.inf, -math.inf
+    f[900], f[1200:1203, 2] = -math.inf, -math.inf                 # the first gate of a sequence, several in a row
+    leaves = [t.detach().requires_grad_() for t in x[:4]]
+    out = forgetting_attention_packed(*leaves, cu_q, cu_k)
+    wrong, size = check(x, cu_q, cu_k, D ** -0.5, [out.detach(), *torch.autograd.grad(out, leaves, x[4])], dtype)
+    assert wrong <= 2.0 ** -16 * size
