@@ -983,7 +983,7 @@ int fox_paged_gather(const fox_paged_gather_args* a, void* stream) {
   if (!a->requests && a->B > a->requests_in_table) return fail(FOX_E_ARG, "%d rows but %d requests in the table", a->B, a->requests_in_table);
   if (!a->block_table || !a->ends || !a->k || !a->v || !a->g) return fail(FOX_E_ARG, "block_table, ends, k, v and g must not be NULL");
   if (((uintptr_t)a->k | (uintptr_t)a->v) & 15) return fail(FOX_E_ALIGN, "k and v must be 16-byte aligned");
-  if (a->T > 1 << 30 || a->pages.H > 1 << 20) return fail(FOX_E_ARG, "too many tokens or heads for one call");   // (32 tokens of all heads are counted in 32 bits)
+  if (a->T > 1 << 30 || a->pages.H > 1 << 20) return fail(FOX_E_ARG, "too many tokens or heads for one call");   // (a workgroup counts the heads of its eight tokens in 32 bits)
   k.table = a->block_table; k.table_sb = a->block_table_stride;
   k.requests = a->requests; k.ends = a->ends;
   k.k = (uint16_t*)a->k; k.v = (uint16_t*)a->v; k.g = a->g;

@@ -17,7 +17,8 @@
 // live with the 16 bits of its operands:
 // - c is kept in 64 bits; the kernels subtract a reference near their tile before they round.  Off the diagonal the reference lies between a tile's queries and its
 //   keys, so that a bias is a sum of two terms of one sign and off by its own rounding.  On the diagonal two terms as large as the gates of 128 keys would cancel: there every
-//   bias is the difference of two pairs of 32-bit numbers.  (One reference for all tiles and 32 bits: dg at gates of -2.1 off by 2e-4 of itself, now below 2e-6.)
+//   bias is the difference of two pairs of 32-bit numbers.  (One reference for all tiles and 32 bits: dg at gates of -2.1 off by 2e-4 of itself;
+//   now sequences of 600 and 700 tokens, D 128 and 32, by 4e-6 and 5e-6 of its norm, gates of -3 by 1.3e-5, gates near 0 by 2e-6.)
 // - The row sum of the forward adds the probabilities before they are rounded for the matrix instruction.
 // - o.do is off by the rounding of o and of P; what is missing of delta is sum_j P_ij (dP_ij - o.do), which the dQ kernel has at its end.  It stores
 //   the sum of the two for the dK/dV kernel.
@@ -1010,7 +1011,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void packed_dq_kernel(const P
 // ---------------------------------------------------------------------------
 // dK/dV: one workgroup keeps 128 keys of a key head (K, V and the accumulators in registers) and walks the query rows that see them in steps of 128, for
 // one query head of the group after the other: the sums over the group never leave the registers.
-// Bound by the matrix units: 8 sequences of about 3000 tokens, 16 heads on 4, D 128 827 to 1000 TFLOP/s, one workgroup a CU whose waves have no other to hide behind.
+// Bound by the matrix units: 8 sequences of about 3000 tokens, 16 heads on 4, D 128 827 to 1000 TFLOP/s, one workgroup a CU whose waves have no other to hide behind.  (There 56 scalar
+// registers are kept in a vector register; none goes to memory.)
 // ---------------------------------------------------------------------------
 template <typename Tr, int D>
 __global__ __launch_bounds__(256, D <= 64 ? 2 : 1) void packed_dkdv_kernel(const PackedK a) {
@@ -1326,7 +1328,8 @@ void packed_memory(PackedK& a, const PackedShape& s, void* plan, void* workspace
 
 // Whether a row of the scans is a wave's rather than a workgroup's of 1024.  A wave is done after some 5 + 0.008 us for each of the longest row's elements, workgroups
 // after 6 + 0.01 for each row.  (A wave / a workgroup, 16 heads, us: 64 rows of 100 elements 8.6 / 16.2, 64 of 800 11.2 / 18.6, 256 of 500 12.2 / 57.7, 32 of 500 9.1 / 10.6, 24 of 800
-// 10.2 / 9.2, 32 of 1500 16.2 / 12.9, 20 of 4000 36.2 / 14.4.)
+// 10.2 / 9.2, 32 of 1500 16.2 / 12.9, 20 of 4000 36.2 / 14.4.)  The host knows the rows and all their elements, not the longest of them, so the rule takes rows to be alike.  Where they are not, one
+// long row makes its wave the last by far: 63 of 100 and one of 16384 136 / 28 and, in the gradient, 152 / 24; 31 of 401 and one of 8512 73 / 18 and 80 / 15; 255 of 301 and one of 4064, 8 heads, 22 / 33.
 static bool short_rows(int64_t elements, int64_t rows, int heads) { return 2 * elements <= 3 * rows * rows * heads; }
 
 template <typename Tr, int D>

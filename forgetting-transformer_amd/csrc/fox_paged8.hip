@@ -3,9 +3,10 @@
 // A page of S tokens holds the codes of every key head's keys and values (P, Hk, S, D) and one fp32 scale for each block of G = min(S, 16) tokens and head; an
 // element stands for code * scale.  The log gates, one for every query head, stay in 32 bits.  Codes are e4m3 (largest 448) or whole numbers (largest 127).
 //
-// The scales that the append gives are powers of two.  x / scale is exact then, so a code is one rounding of its element (to the nearest, ties to the even one) and a block
-// whose scale has to grow is rounded again from its codes without another error; e4m3 has as many bits at any scale, whole numbers lose half a bit
-// on average against the scale that just fits.  The readers take any scales.
+// The scales that the append gives are powers of two.  x / scale is exact then, so the code of a new element is one rounding of it (to the nearest, ties to the even one).  A block
+// whose scale has to grow is rounded again from its codes: e4m3 keeps a code's bits at any scale down to its subnormals; those, and whole numbers, lose up to half a step of the new scale each time, and with
+// the steps in front of it half as large or less, an element is off by less than one step of the last scale in all, where one rounding takes half of it.  Whole numbers lose half a bit on average against
+// the scale that just fits.  The readers take any scales.
 #include <algorithm>
 
 #include "fox_common.hpp"
@@ -141,7 +142,8 @@ __device__ __forceinline__ void append_rows(const u32x4 (&x)[(16 * (D / 8) + 63)
 // a code is written and nobody waits for anybody.  A wave looks at CHUNK tokens of a head for the beginnings of runs: one token each where there are few (the next tokens
 // of a step are runs of their own), sixteen where prompts fill whole blocks, so that few waves find nothing to do.  Few tokens are bound by their chain of loads: slots, scale, codes.
 // In us for 1 / 4 / 8 / 16 tokens a wave: runs of one token, 48 of 12 heads, D 64 4.8 / 10.5 / 17.6 / 31.9, 1024 of 4 heads, D 128 8.1 / 13.1 / 22.8 / 43.4, 4096 22.9 / 21.5 / 26.7 / 43.7; whole
-// blocks, 1024 tokens 8.8 / 6.2 / 5.9 / 5.8, 4096 27.2 / 11.4 / 6.3 / 6.3, 16384 95 / 29.5 / 17.4 / 11.4 (51 MB there: 4.5 TB/s).
+// blocks, 1024 tokens 8.8 / 6.2 / 5.9 / 5.8, 4096 27.2 / 11.4 / 6.3 / 6.3, 16384 95 / 29.5 / 17.4 / 11.4: repeated, its 52 MB in the last-level cache.
+// Inputs that no cache holds take 18.8 us there, 2.8 TB/s.
 template <typename Tr, typename C, int D, int CHUNK>
 __global__ __launch_bounds__(256) void paged8_append_kernel(const Paged8AppendK a) {
   constexpr int LPR = D / 8, R = 64 / LPR, NIT = (16 + R - 1) / R;
@@ -195,7 +197,8 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const Paged8AppendK 
 // Gather: the first tokens of requests out of their pages, one request after the other, in 16 bits.  A workgroup takes eight places: their requests from a search
 // in the ends, their pages from the table, then rows of eight elements a lane, head by head, so that the codes of neighbouring tokens are read as they lie.
 // Memory bounds it where there are many tokens; few need many workgroups.  In us for 4 / 8 / 16 / 32 places: 1600 tokens, 12 heads, D 64 4.8 / 4.7 / 5.8 / 7.8, 16384 tokens, 4 key heads, D 128
-// 11.3 / 10.3 / 9.5 / 11.6, 80000 of those 40.3 / 37.5 / 37.1 / 36.7.
+// 11.3 / 10.3 / 9.5 / 11.6, 80000 of those 40.3 / 37.5 / 37.1 / 36.7 (repeated; 40.9 for 37.5, 5.5 TB/s, on inputs that no cache holds).  Every workgroup reads all ends: 32768 tokens of 12 heads, D 64, of 64 requests
+// 19.4, of 1024 22.4, of 4096 29.2.
 // ---------------------------------------------------------------------------
 constexpr int kGatherTokens = 8;
 

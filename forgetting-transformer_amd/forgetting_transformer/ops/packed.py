@@ -59,7 +59,8 @@ def forgetting_attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tenso
     has them behind its last one); no gradient reaches them or comes from them.  A sequence whose queries (keys) end behind the last of the tensor has none, and neither have those
     that follow.  ``sm_scale`` defaults to ``1 / sqrt(D)``.
 
-    Gradients for q, k, v and log_fgate.  Nothing waits for the device.
+    Gradients for q, k, v and log_fgate.  Nothing waits for the device.  There is no ``adaptive_threshold`` here: where strong gates prune most of a long batch, the dense operator on padded rows
+    may be the faster one.
     """
     ext = _native.load()
     out = ext.packed_attention(q, k, v, log_fgate, cu_seqlens, cu_seqlens_k, sm_scale)
