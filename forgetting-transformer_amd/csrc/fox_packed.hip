@@ -319,7 +319,8 @@ __device__ __forceinline__ int wave_max(int x) {
   return x;
 }
 // Where the keys of sequence b <= B begin: behind every earlier end, as in the plan, so that no two rows have a place in common.  b is a wave's, b0 that of the workgroup's first one.  Every
-// thread of the workgroup of NT calls it.  Ends that do not decrease leave the comparisons alone, without the maxima.
+// thread of the workgroup of NT calls it.  Ends that do not decrease cost the comparisons alone, without the maxima (the launch without / with them, us: 64 sequences
+// of 100 tokens, 16 heads, 8.2 / 9.2, 4096 of 8, 12 heads, 25 / 31, up to 24 sequences the same).
 template <int NT>
 __device__ __forceinline__ int first_key(const PackedK& a, int b0, int b) {
   __shared__ int tops[NT / 64];
